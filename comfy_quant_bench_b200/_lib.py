@@ -40,6 +40,10 @@ CQ_GEMM_AUTO = 0
 CQ_GEMM_ONE_SM = 1
 CQ_GEMM_PAIR = 2
 
+CQ_DT_BF16 = 0
+CQ_DT_F16 = 1
+CQ_DT_FP8_E4M3 = 2
+
 CQ_OUT_PLAIN = 0
 CQ_OUT_GELU_TANH = 1
 CQ_OUT_GATED_RESIDUAL = 2
@@ -103,6 +107,18 @@ SIGNATURES = {
                                           _vp]),
     "cq_heads_to_rows": (_int, [_vp, _i64, _int, _int, _vp, _int, _i64, _i64, _vp]),
     "cq_gemm_rowcol_swiglu": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
+    "cq_w4a16_linear": (_int, [_vp, _i64, _int, _i64, _i64, _i64, _vp, _vp, _vp, _int, _vp, _vp, _vp]),
+    "cq_paged_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
+    "cq_paged_attention": (_int, [_vp, _i64, _i64, _int, _i64, _i64, _i64, _i64, _vp, _vp, _int, _i64, _i64, _i64, _i64,
+                                  _i64, _vp, _i64, _i64, _i64, _vp, _vp, _f32, _i64, _i64, _vp, _vp, _vp, _vp, _vp,
+                                  _i64, _vp]),
+    "cq_kv_append": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _int, _i64, _i64, _i64, _i64, _vp, _vp, _int,
+                            _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "cq_pages_workspace_bytes": (_i64, [_i64, _i64]),
+    "cq_pages_update": (_int, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp,
+                               _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp]),
+    "cq_pages_compact": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _vp,
+                                _i64, _vp]),
     "cq_linear_convrot_w4a4_swiglu": (_int, [_vp, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
 }
 

@@ -1,5 +1,8 @@
 // Declarations shared by the kernel files and the C ABI layer (one translation unit: libcq.cu).
 #pragma once
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
 #include "cq_common.cuh"
 
 namespace cq {
@@ -124,5 +127,97 @@ cudaError_t launch_selftest_wait(cudaStream_t st);
 bool gemv_affine_fits(int M, int a_kperm);
 cudaError_t launch_gemv_affine(const int8_t* a, const float* sa, const void* b, const void* s, const void* zt,
                                const void* bias, void* out, int M, int N, int K, cudaStream_t st, bool pdl = false);
+
+// W4A16 linear: 16-bit activations, packed uint4 weights, a scale and a zero per group (awq_w4a16)
+struct W4A16Args {
+  const void* x;              // [M, K] bf16 or f16, rows ldx elements apart
+  const uint8_t* b;           // [N, K/2] packed uint4, low nibble = even column
+  const __nv_bfloat16* s;     // [K/group, N]
+  const __nv_bfloat16* z;     // [K/group, N]
+  const void* bias;           // [N] of x's type, or null
+  void* out;                  // [M, N] of x's type
+  int64_t ldx;
+  int M, N, K, group, f16;
+};
+cudaError_t launch_w4a16(const W4A16Args& a, cudaStream_t st);
+
+// attention of one new token per sequence over a paged cache
+struct PagedAttnArgs {
+  const void* q;              // [B, Hq, D], strides q_sb, q_sh (elements)
+  int64_t q_sb, q_sh;
+  const void* k;              // key cache; page, kv head and token strides in elements, D contiguous
+  const void* v;              // value cache, the same strides
+  int64_t page_stride, head_stride, tok_stride;
+  const int* table;           // [table_rows, table_width] page indexes, rows table_stride apart
+  int64_t table_stride;
+  const int* rows;            // [B] table row of each query, or null: row b
+  const int* lens;            // [table_rows] tokens of each row
+  const float* k_scale;       // [Hkv] or null: 1
+  const float* v_scale;
+  void* out;                  // [B, Hq, D]
+  float* lse;                 // [B, Hq] log of the softmax's sum, or null
+  void* ws;
+  int B, Hq, Hkv, D, num_pages, page_size, table_rows, table_width, dtype, cache_dtype, window, sinks;
+  float scale;
+};
+int64_t paged_attention_workspace(int64_t batch, int Hq, int Hkv, int D);
+cudaError_t launch_paged_attention(const PagedAttnArgs& a, cudaStream_t st);
+
+// free, fork and reserve rows of a paged cache
+struct PagesArgs {
+  int* table;                 // [table_rows, table_width]
+  int64_t table_stride;
+  int* lens;                  // [table_rows]
+  int* refs;                  // [num_pages]
+  const int* free_rows;       // [n_free]
+  const int* src;             // [n_fork]
+  const int* dst;             // [n_fork]
+  const int* res_rows;        // [n_res]
+  const int* counts;          // [n_res] new tokens of each row, or null: count
+  int* start;                 // [n_res] tokens before, -1 where refused
+  int* copies;                // [n_res, 2] (source, destination) page of a copy on write, -1 where none
+  int* ws;                    // 2 * n_res + num_pages
+  int table_rows, table_width, num_pages, page_size, n_free, n_fork, n_res, count;
+};
+int64_t pages_branch_shared(int table_rows, int num_pages);   // bytes of shared memory
+cudaError_t launch_pages_branch(const PagesArgs& a, cudaStream_t st);
+
+struct PagesCopyArgs {
+  const int* moves;           // [n, 2]
+  void* k;                    // [layers, num_pages, page_bytes], layers layer_bytes apart
+  void* v;
+  int64_t layer_bytes, page_bytes;
+  int n, layers, num_pages;
+};
+cudaError_t launch_pages_copy(const PagesCopyArgs& a, cudaStream_t st);
+
+struct CompactArgs {
+  const int* table;           // [table_rows, table_width]
+  int* table_out;
+  int64_t table_stride, out_stride;
+  const int* refs;            // [num_pages]
+  int* refs_out;
+  int* moves;                 // [num_pages / 2, 2], -1 past the last move
+  int* map;                   // [num_pages] workspace
+  int table_rows, table_width, num_pages;
+};
+cudaError_t launch_pages_compact(const CompactArgs& a, cudaStream_t st);
+
+struct AppendArgs {
+  const void* k_new;          // [layers, T, Hkv, D] bf16 or f16; layer, token and head strides in elements
+  const void* v_new;
+  int64_t kn_sl, kn_st, kn_sh, vn_sl, vn_st, vn_sh;
+  void* k;                    // caches, strides in elements
+  void* v;
+  int64_t layer_stride, page_stride, head_stride, tok_stride;
+  const int* table;
+  int64_t table_stride;
+  const int* rows;            // [T]
+  const int* positions;       // [T]
+  const float* k_scale;       // [Hkv] or null: 1 (8-bit caches)
+  const float* v_scale;
+  int layers, T, Hkv, D, num_pages, page_size, table_rows, table_width, dtype, cache_dtype;
+};
+cudaError_t launch_kv_append(const AppendArgs& a, cudaStream_t st);
 
 }  // namespace cq

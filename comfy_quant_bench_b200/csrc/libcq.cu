@@ -5,6 +5,10 @@
 #include "gemm_pair.cu"
 #include "gemv.cu"
 #include "dit.cu"
+#include "w4a16.cu"
+#include "paged_attention.cu"
+#include "kvpages.cu"
 #include "selftest.cu"
 #include "capi.cu"
+#include "capi_decode.cu"
 #include "noalloc.cu"

@@ -475,6 +475,50 @@ def w4a8_affine_linear(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tens
     return out if dt == torch.bfloat16 else out.to(dt)
 
 
+def w4a16_linear(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor, zeros: torch.Tensor,
+                 bias: torch.Tensor | None = None, *, group_size: int = 128,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+    """Linear of 16-bit activations with awq-layout weights: W = (q - 8) * scale + zeros, y = x W^T + bias.
+
+    x [..., K] bf16 or f16 (its rows may be strided), qweight int8 or uint8 [N, K/2] (low nibble = even column),
+    scale and zeros bf16 [K/group_size, N] (group_size 32, 64 or 128), bias [N].  Products and sums are fp32, rounded
+    once to the type of x.  For the few tokens of a decode step; ``w4a8_affine_linear`` takes many tokens."""
+    k = x.shape[-1]
+    n = qweight.shape[0]
+    dt = x.dtype
+    if dt != torch.bfloat16 and dt != torch.float16:
+        raise ValueError(f"x must be bf16 or f16, got {dt}")
+    if k != qweight.shape[-1] * 2:
+        raise ValueError(f"Input K={k} does not match qweight K={qweight.shape[-1] * 2}")
+    if group_size not in (32, 64, 128) or k % group_size:
+        raise ValueError(f"group_size must be 32, 64 or 128 and divide K={k}, got {group_size}")
+    shape = (k // group_size, n)
+    if scale.dtype != torch.bfloat16 or zeros.dtype != torch.bfloat16 or scale.shape != shape or zeros.shape != shape:
+        raise ValueError(f"scale and zeros must be bf16 [{shape[0]}, {n}]")
+    if qweight.dtype not in (torch.int8, torch.uint8) or qweight.dim() != 2:
+        raise ValueError("qweight must be int8 or uint8 [N, K/2]")
+    if not (qweight.is_contiguous() and scale.is_contiguous() and zeros.is_contiguous()):
+        raise ValueError("qweight, scale and zeros must be contiguous")
+    dev = _require_cuda(x, qweight, scale, zeros, bias, out)
+    x2 = x if x.dim() == 2 else x.reshape(-1, k)
+    ldx = x2.stride(0)
+    if x2.stride(1) != 1 or ldx % 8 or ldx < k or x2.data_ptr() % 16:
+        x2 = x2.contiguous() if x2.data_ptr() % 16 == 0 else x2.clone(memory_format=torch.contiguous_format)
+        ldx = k
+    m = x2.shape[0]
+    if bias is not None and (bias.dtype != dt or bias.shape != (n,) or not bias.is_contiguous()):
+        if bias.numel() != n:
+            raise ValueError(f"bias must have {n} elements")
+        bias = bias.reshape(n).to(dt).contiguous()
+    if out is None:
+        out = torch.empty(*x.shape[:-1], n, dtype=dt, device=dev)
+    elif out.dtype != dt or out.shape != (*x.shape[:-1], n) or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous {dt} of shape {(*x.shape[:-1], n)}")
+    _lib.call("cq_w4a16_linear", x2.data_ptr(), ldx, 0 if dt == torch.bfloat16 else 1, m, k, n, qweight.data_ptr(),
+              scale.data_ptr(), zeros.data_ptr(), int(group_size), _ptr(bias), out.data_ptr(), _stream(dev))
+    return out
+
+
 def w4a8_affine_linear_into(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor, zeros_prepared: torch.Tensor,
                             bias: torch.Tensor | None, outs, col0: int, ldo: int, group_size: int = 128,
                             convrot_groupsize: int = 0) -> None:

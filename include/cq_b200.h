@@ -453,6 +453,110 @@ CQ_API int cq_qkv_rmsnorm_rope_layout(const void* y, int64_t S, int H, int D, co
                                       const void* k_norm, float eps, const float* rope, void* q, void* k, void* v,
                                       int64_t s_all, int64_t s0, int token_major, void* stream);
 
+/* ------------------------------------------------------------------------------------------------------------
+ * Decode side: the W4A16 linear and a paged key-value cache (language models beside the DiT: text encoders and
+ * prompt writers in the awq_w4a16 format).  No counterpart in the reference, whose A16 path dequantizes the weight
+ * and calls a library product (patches/comfyui_awq_w4a16_format.patch:79-80).
+ * ---------------------------------------------------------------------------------------------------------- */
+
+/* Element types of the decode-side operators. */
+typedef enum {
+  CQ_DT_BF16 = 0,
+  CQ_DT_F16 = 1,
+  CQ_DT_FP8_E4M3 = 2  /* caches only: a value is its 8-bit code times the scale of its key-value head */
+} cq_dtype;
+
+/*
+ * cq_w4a16_linear: out[m, n] = sum_k x[m, k] ((q[n, k] - 8) scale[k / group, n] + zeros[k / group, n]) + bias[n],
+ * products and sums in fp32, rounded once to the type of x.
+ *   x        [M, K] of `dtype` (bf16 or f16), rows ldx elements apart; 16-byte aligned, ldx % 8 == 0
+ *   qweight  packed uint4 [N, K/2], low nibble = even column, 16-byte aligned
+ *   scale, zeros  bf16 [K/group, N];  bias  [N] of `dtype` or NULL;  out  [M, N] of `dtype`
+ * group 32, 64 or 128, K a multiple of it and at most 32768; any N; M up to 524280.  Built for the few tokens of a
+ * decode step (it reads the weights once per 64 tokens); cq_linear_w4a8_affine is the linear for many tokens.
+ */
+CQ_API int cq_w4a16_linear(const void* x, int64_t ldx, int dtype, int64_t M, int64_t K, int64_t N,
+                           const void* qweight, const void* scale, const void* zeros, int group, const void* bias,
+                           void* out, void* stream);
+
+/*
+ * Paged cache: keys and values of a layer in pages of `page_size` tokens (a power of two, 8 to 1024), addressed as
+ * cache[page * page_stride + head * head_stride + token * token_stride + d] (elements; keys and values alike, each
+ * its own base).  A table row lists a sequence's pages, int32, -1 where it has none; seq_lens int32 [table_rows] is
+ * the number of its tokens; ref_counts int32 [num_pages] the number of table rows that hold a page (0: free).
+ * A table entry outside [0, num_pages) is never followed.  table_width * page_size < 2^31.
+ *
+ * cq_paged_attention: out[b, h] = sum_j p_j v_j / sum_j p_j with p_j = exp(scale q[b, h] . k_j - max) over the visible
+ * tokens j of table row rows[b] (NULL: row b): j < seq_lens[row] and, with window > 0, j >= seq_lens[row] - window or
+ * j < sinks.  Query head h reads key-value head h / (q_heads / kv_heads).  A row that sees nothing (no tokens, no
+ * page, a row out of range) gives zeros.
+ *   q    [batch, q_heads, head_dim] of `dtype` (bf16 or f16) with strides in elements; out the same, contiguous
+ *   lse  f32 [batch, q_heads] or NULL: log sum_j exp(scale q . k_j) (-inf for a row that sees nothing)
+ *   cache_dtype  dtype, or CQ_DT_FP8_E4M3 with k_scale / v_scale f32 [kv_heads] (NULL: 1)
+ *   head_dim 64, 128 or 256; workspace of cq_paged_attention_workspace_bytes, 16-byte aligned, of this call alone
+ * 16-byte aligned bases and strides.
+ */
+CQ_API int64_t cq_paged_attention_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim);
+CQ_API int cq_paged_attention(const void* q, int64_t q_batch_stride, int64_t q_head_stride, int dtype, int64_t batch,
+                              int64_t q_heads, int64_t kv_heads, int64_t head_dim, const void* k_cache,
+                              const void* v_cache, int cache_dtype, int64_t num_pages, int64_t page_size,
+                              int64_t page_stride, int64_t head_stride, int64_t token_stride,
+                              const int32_t* block_table, int64_t table_rows, int64_t table_width,
+                              int64_t table_stride, const int32_t* rows, const int32_t* seq_lens, float scale,
+                              int64_t window, int64_t sinks, const float* k_scale, const float* v_scale, void* out,
+                              float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * cq_kv_append: the new keys and values of `tokens` tokens into the pages of their rows: token t goes to position
+ * positions[t] of table row rows[t], in each of `layers` layers (k_new, v_new [layers, tokens, kv_heads, head_dim]
+ * of `dtype` with strides in elements).  A token whose row, position or page is out of range is skipped, as the
+ * positions of a refused reservation (-1) are.  Two tokens must not share a position.  A CQ_DT_FP8_E4M3 cache
+ * receives x / scale rounded to nearest even, kept inside +-448 (NaN stays NaN).
+ */
+CQ_API int cq_kv_append(const void* k_new, int64_t k_layer_stride, int64_t k_token_stride, int64_t k_head_stride,
+                        const void* v_new, int64_t v_layer_stride, int64_t v_token_stride, int64_t v_head_stride,
+                        int dtype, int64_t layers, int64_t tokens, int64_t kv_heads, int64_t head_dim, void* k_cache,
+                        void* v_cache, int cache_dtype, int64_t num_pages, int64_t page_size, int64_t layer_stride,
+                        int64_t page_stride, int64_t head_stride, int64_t token_stride, const int32_t* block_table,
+                        int64_t table_rows, int64_t table_width, int64_t table_stride, const int32_t* rows,
+                        const int32_t* positions, const float* k_scale, const float* v_scale, void* stream);
+
+/*
+ * cq_pages_update: the bookkeeping of a paged cache on the device, in up to three phases, each on a list of distinct
+ * table rows (int32, device memory):
+ *   free     free_rows [n_free] give up their pages and become empty;
+ *   fork     dst_rows [n_fork], empty, take the pages and length of src_rows [n_fork] (a source may repeat and is no
+ *            destination); every page is held by one row more;
+ *   reserve  reserve_rows [n_reserve] grow by counts[i] (or `count`) tokens.  A row whose last page is partly filled
+ *            and held by another row when the phase begins gets a copy of its own (copies[i] = source and
+ *            destination page, else -1, -1), copied in every layer of k_cache and v_cache (layers of layer_bytes, a
+ *            page contiguous in page_bytes; layers == 0: not copied).  Free pages are taken lowest index first, for
+ *            the rows in order; a page given up in this phase is free only after it.  start[i]: tokens before.
+ * A phase that cannot be done whole is refused: it and the phases after it change nothing, start and copies are -1,
+ * and the device status word (cq_take_device_status) gets CQ_ERR_ARG (rows out of range, repeated, a destination
+ * that is not empty) or CQ_ERR_CAPACITY (too few free pages or too narrow a table) with site 101 (free), 102 (fork)
+ * or 103 (reserve).  workspace: cq_pages_workspace_bytes(num_pages, n_reserve).
+ */
+CQ_API int64_t cq_pages_workspace_bytes(int64_t num_pages, int64_t reserved_rows);
+CQ_API int cq_pages_update(int32_t* block_table, int64_t table_rows, int64_t table_width, int64_t table_stride,
+                           int32_t* seq_lens, int32_t* ref_counts, int64_t num_pages, int64_t page_size,
+                           const int32_t* free_rows, int64_t n_free, const int32_t* src_rows, const int32_t* dst_rows,
+                           int64_t n_fork, const int32_t* reserve_rows, int64_t n_reserve, const int32_t* counts,
+                           int64_t count, int32_t* start, int32_t* copies, void* k_cache, void* v_cache,
+                           int64_t layers, int64_t layer_bytes, int64_t page_bytes, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
+/*
+ * cq_pages_compact: with L pages held by some row, the held pages with index >= L move, in order, to the free pages
+ * below L, in order, in every layer of both caches; table_out and refs_out (which may be the inputs) get the tables
+ * and counts after it; moves int32 [num_pages / 2, 2] lists (from, to), then -1.  workspace: 4 * num_pages bytes.
+ */
+CQ_API int cq_pages_compact(const int32_t* block_table, int64_t table_rows, int64_t table_width, int64_t table_stride,
+                            int32_t* table_out, int64_t out_stride, const int32_t* ref_counts, int32_t* refs_out,
+                            int64_t num_pages, int32_t* moves, void* k_cache, void* v_cache, int64_t layers,
+                            int64_t layer_bytes, int64_t page_bytes, void* workspace, int64_t workspace_bytes,
+                            void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,99 @@
+"""CPU-side checks of the decode-side operators: the C ABI rejects bad arguments on the host before touching a device,
+and the Python operators reject CPU tensors."""
+import ctypes
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from comfy_quant_bench_b200 import _lib
+    return _lib.load()
+
+
+VP = ctypes.c_void_p(256)
+
+
+def test_linear_argument_checks_need_no_device(lib):
+    from comfy_quant_bench_b200 import _lib as L
+
+    def call(x=VP, ldx=256, dtype=0, m=2, k=256, n=16, w=VP, s=VP, z=VP, g=64, b=None, out=VP):
+        return lib.cq_w4a16_linear(x, ldx, dtype, m, k, n, w, s, z, g, b, out, None)
+    assert call(dtype=2) == L.CQ_ERR_ARG and call(g=16) == L.CQ_ERR_ARG and call(g=0) == L.CQ_ERR_ARG
+    assert call(k=96) == L.CQ_ERR_SHAPE and call(k=0) == L.CQ_ERR_SHAPE and call(ldx=128) == L.CQ_ERR_SHAPE
+    assert call(m=-1) == L.CQ_ERR_SHAPE and call(n=-1) == L.CQ_ERR_SHAPE and call(k=1 << 20, ldx=1 << 20) == L.CQ_ERR_SHAPE
+    assert call(x=None) == L.CQ_ERR_ARG and call(w=None) == L.CQ_ERR_ARG and call(out=None) == L.CQ_ERR_ARG
+    assert call(x=ctypes.c_void_p(264)) == L.CQ_ERR_ALIGN and call(ldx=257) == L.CQ_ERR_ALIGN
+    assert call(w=ctypes.c_void_p(260)) == L.CQ_ERR_ALIGN
+    assert call(m=0, x=None, w=None, s=None, z=None, out=None) == L.CQ_OK
+    assert call(n=0) == L.CQ_OK
+
+
+def test_attention_argument_checks_need_no_device(lib):
+    from comfy_quant_bench_b200 import _lib as L
+    size = lib.cq_paged_attention_workspace_bytes(2, 8, 2, 128)
+    assert size >= 0
+    assert lib.cq_paged_attention_workspace_bytes(2, 8, 3, 128) == -1
+    assert lib.cq_paged_attention_workspace_bytes(2, 8, 2, 96) == -1
+    assert lib.cq_paged_attention_workspace_bytes(-1, 8, 2, 64) == -1
+
+    def call(q=VP, sb=1024, sh=128, dt=0, b=2, hq=8, hk=2, d=128, k=VP, v=VP, cdt=0, pages=10, page=16, sp=4096, shd=2048,
+             st=128, table=VP, rows=2, width=4, ts=4, lens=VP, window=0, sinks=0, out=VP, ws=VP, wsn=1 << 40):
+        return lib.cq_paged_attention(q, sb, sh, dt, b, hq, hk, d, k, v, cdt, pages, page, sp, shd, st, table, rows, width,
+                                      ts, None, lens, 1.0, window, sinks, None, None, out, None, ws, wsn, None)
+    assert call(dt=2) == L.CQ_ERR_ARG and call(dt=0, cdt=1) == L.CQ_ERR_ARG and call(cdt=9) == L.CQ_ERR_ARG
+    assert call(window=-1) == L.CQ_ERR_ARG and call(sinks=-1) == L.CQ_ERR_ARG
+    assert call(page=12) == L.CQ_ERR_SHAPE and call(page=4) == L.CQ_ERR_SHAPE and call(pages=0) == L.CQ_ERR_SHAPE
+    assert call(ts=3) == L.CQ_ERR_SHAPE and call(hq=7) == L.CQ_ERR_SHAPE and call(d=96) == L.CQ_ERR_SHAPE
+    assert call(b=70000) == L.CQ_ERR_SHAPE and call(wsn=-1) == L.CQ_ERR_SHAPE
+    assert call(q=None) == L.CQ_ERR_ARG and call(lens=None) == L.CQ_ERR_ARG and call(table=None) == L.CQ_ERR_ARG
+    assert call(q=ctypes.c_void_p(8)) == L.CQ_ERR_ALIGN and call(st=129) == L.CQ_ERR_ALIGN
+    assert call(cdt=2, st=8) == L.CQ_ERR_ALIGN
+    assert call(b=0, q=None, k=None, v=None, lens=None, out=None) == L.CQ_OK
+
+
+def test_page_argument_checks_need_no_device(lib):
+    from comfy_quant_bench_b200 import _lib as L
+
+    def update(rows=4, width=8, ts=8, pages=10, page=16, nf=1, nk=0, nr=0, count=1, layers=0, lb=0, pb=0, wsn=1 << 20,
+               table=VP, start=VP, k=None):
+        return lib.cq_pages_update(table, rows, width, ts, VP, VP, pages, page, VP, nf, VP, VP, nk, VP, nr, None, count,
+                                   start, VP, k, k, layers, lb, pb, VP, wsn, None)
+    assert update(page=10) == L.CQ_ERR_SHAPE and update(ts=7) == L.CQ_ERR_SHAPE and update(nf=5) == L.CQ_ERR_SHAPE
+    assert update(nr=1, count=-1) == L.CQ_ERR_SHAPE and update(nr=1, wsn=8) == L.CQ_ERR_SHAPE
+    assert update(nr=1, layers=2, lb=64, pb=8, k=VP) == L.CQ_ERR_SHAPE
+    assert update(nr=1, layers=2, lb=64, pb=32, k=None) == L.CQ_ERR_ARG
+    assert update(table=None) == L.CQ_ERR_ARG and update(nr=1, start=None) == L.CQ_ERR_ARG
+    assert update(pages=1 << 22) == L.CQ_ERR_CAPACITY
+    assert update(nf=0) == L.CQ_OK
+    assert lib.cq_pages_workspace_bytes(100, 7) >= 4 * 114 and lib.cq_pages_workspace_bytes(-1, 0) == -1
+    assert lib.cq_pages_compact(VP, 4, 8, 8, VP, 8, VP, VP, 10, VP, None, None, 0, 0, 0, VP, 8, None) == L.CQ_ERR_SHAPE
+    assert lib.cq_pages_compact(VP, 4, 8, 8, VP, 7, VP, VP, 10, VP, None, None, 0, 0, 0, VP, 40, None) == L.CQ_ERR_SHAPE
+    assert lib.cq_pages_compact(VP, 4, 8, 8, VP, 8, None, VP, 10, VP, None, None, 0, 0, 0, VP, 40, None) == L.CQ_ERR_ARG
+    assert lib.cq_pages_compact(VP, 4, 8, 8, VP, 8, VP, VP, 1 << 22, VP, None, None, 0, 0, 0, VP, 1 << 30, None) == \
+        L.CQ_ERR_CAPACITY
+
+    def append(dt=0, cdt=0, t=1, hk=2, d=64, page=16, pos=VP, k=VP, sl=0):
+        return lib.cq_kv_append(k, sl, 128, 64, VP, 0, 128, 64, dt, 1, t, hk, d, VP, VP, cdt, 10, page, 0, 2048, 1024, 64,
+                                VP, 4, 8, 8, VP, pos, None, None, None)
+    assert append(dt=2) == L.CQ_ERR_ARG and append(cdt=1) == L.CQ_ERR_ARG and append(pos=None) == L.CQ_ERR_ARG
+    assert append(page=3) == L.CQ_ERR_SHAPE and append(d=12) == L.CQ_ERR_SHAPE and append(t=-1) == L.CQ_ERR_SHAPE
+    assert append(k=ctypes.c_void_p(258)) == L.CQ_ERR_ALIGN and append(sl=4) == L.CQ_ERR_ALIGN
+    assert append(t=0, k=None) == L.CQ_OK
+
+
+def test_operators_reject_cpu_tensors():
+    from comfy_quant_bench_b200 import kvcache, ops
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.w4a16_linear(torch.zeros(1, 128, dtype=torch.bfloat16), torch.zeros(8, 64, dtype=torch.int8),
+                         torch.zeros(1, 8, dtype=torch.bfloat16), torch.zeros(1, 8, dtype=torch.bfloat16))
+    c = kvcache.PagedKVCache(1, 4, 2, 64, 2, 40, device="cpu")
+    assert c.block_table.shape == (2, 3) and int(c.block_table.max()) == -1
+    one = torch.zeros(1, dtype=torch.int32)
+    new = torch.zeros(1, 2, 64, dtype=torch.bfloat16)
+    for bad in (lambda: c.reserve(one, 1), lambda: c.free(one), lambda: c.fork(one, one), lambda: c.compact(),
+                lambda: c.branch(one, one + 1, 1), lambda: c.append(0, new, new, one, one),
+                lambda: c.attend(0, new, rows=one)):
+        with pytest.raises(ValueError, match="CUDA"):
+            bad()
