@@ -17,7 +17,7 @@ bool fits_int(int64_t v) { return v >= 0 && v <= 0x7FFFFFFF; }
 int check_tables(int64_t table_rows, int64_t table_width, int64_t table_stride, int64_t num_pages, int64_t page_size) {
   if (!fits_int(table_rows) || table_rows > (1 << 24) || !fits_int(table_width) || table_width > (1 << 20) ||
       table_stride < table_width || num_pages < 1 || !fits_int(num_pages) || !valid_page_size(page_size) ||
-      !fits_int(table_width * page_size))
+      table_width * page_size > 0x7FFFFFFF - 1024)      // room for a tile's key index past the row's end
     return CQ_ERR_SHAPE;
   return CQ_OK;
 }

@@ -3,62 +3,713 @@
 //   o[b, h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q[b, h] . k_j - max),  j over the visible keys of row b:
 //   j < len, and with a window: j >= len - window or j < sinks.  A row without visible keys gives zeros.
 //
-// Simple form: one warp per query head, one key at a time, the running maximum and sum in fp32.
+// Bound by reading the visible keys and values once.  The query heads of a key-value head share its tiles, so the
+// products run on tensor cores with the keys as rows and the heads as columns:
+//   S^T [16 keys x 8 heads] = K Q^T,  O^T [D x 8 heads] += V^T P^T.
+// At decode there are at most 16 heads per key-value head: mma.sync with its operands in registers does a tile in
+// tens of instructions, while a tcgen05 tile would be filled to an eighth; HBM, not the tensor pipe, is the limit.
+//
+// Work: a unit is 64 visible keys of one (row, head tile), 16 for each of the CTA's four warps.  Every CTA of a
+// resident grid takes an equal run of units, through as many rows and heads as that covers, so ragged lengths
+// balance and one long row uses every SM.  Each warp keeps its own ring of asynchronous 16-byte copies in flight and
+// never waits for the others inside a run; the ring runs on across rows.  Where a row ends (or the CTA's run does)
+// the warps' running maxima, sums and outputs are joined in shared memory; a row that several CTAs share is joined
+// by a second small kernel in the order of its parts.  Both orders are fixed, so equal calls give equal bits.
+//
+// Softmax statistics, scores and outputs are fp32.  The weights p enter the second product as two 16-bit parts,
+// p = hi + lo (relative error 2^-16), since one part alone would add as much error as rounding the output does.
+// 8-bit caches are widened exactly to f16; a bf16 query is scaled by a power of two per head so that f16 holds it to
+// 2^-24 of its largest element.
 #include "kernels.cuh"
 
 namespace cq {
 
-__device__ __forceinline__ float load_cache(const void* p, int64_t i, int dt) {
-  if (dt == CQ_DT_FP8_E4M3) {
-    const __half_raw h = __nv_cvt_fp8_to_halfraw(static_cast<const __nv_fp8_storage_t*>(p)[i], __NV_E4M3);
-    return __half2float(__half(h));
+namespace pattn {
+constexpr int kWarps = 4;
+constexpr int kTile = 16;                    // keys per warp and step
+constexpr int kUnit = kWarps * kTile;
+// A row is split no finer than this: a part costs its CTA a start and an end (about two units' time), and the join.
+constexpr int kMinUnits = 4;
+// Rows of at most this many units are never split: one launch, no join.
+constexpr int kWholeUnits = 12;
+
+// shared memory: ring, query fragments, joined output, per-warp statistics
+template <int D, int ES, int NT>
+struct Cfg {
+  static constexpr int kRow = D * ES;                          // bytes of one key
+  static constexpr int kTileBytes = kTile * kRow;              // one operand's tile
+  static constexpr int kStageBytes = 2 * kTileBytes;
+  static constexpr int kQ = D / 16 * NT * 256;
+  static constexpr int kO = 8 * NT * D * 4;
+  static constexpr int kMisc = 8 * NT * 4 * (2 * kWarps + 1) + 16;
+  static constexpr int kFixed = kQ + kO + kMisc;
+  static constexpr int kCtas = 3 * kWarps * kStageBytes + kFixed <= 112 * 1024 ? 2 : 1;
+  static constexpr int kFit = ((kCtas == 2 ? 112 : 224) * 1024 - kFixed) / (kWarps * kStageBytes);
+  static constexpr int kStages = kFit < 8 ? kFit : 8;
+  static constexpr int kMaskBytes = kWarps * kStages * 4;
+  static constexpr int kSmem = kWarps * kStages * kStageBytes + kFixed + kMaskBytes;
+  static_assert(kStages >= 3, "ring of three stages");
+};
+
+struct Meta {          // one CTA's run, for the join: its first part's segment, first unit there, the segment's units
+  int seg, unit0, units, count;
+};
+}  // namespace pattn
+
+// ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
+  // src-size 0: nothing is read and 16 zero bytes are written
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <bool F16>
+__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (F16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t movmatrix_t(uint32_t x) {   // transpose of the warp's 8 x 8 matrix of 16-bit values
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
+  return d;
+}
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t pair) {   // exact; NaN stays NaN
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(pair), __NV_E4M3);
+  return static_cast<uint32_t>(h.x) | static_cast<uint32_t>(h.y) << 16;
+}
+// two fp32 values as 16-bit pairs: hi = the nearest, lo = the nearest of what is left
+template <bool F16>
+__device__ __forceinline__ void split16(float x, float y, uint32_t& hi, uint32_t& lo) {
+  if constexpr (F16) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    const float2 f = __bfloat1622float2(h);
+    const __nv_bfloat162 l = __floats2bfloat162_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
   }
-  return dt == CQ_DT_F16 ? __half2float(static_cast<const __half*>(p)[i])
-                         : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+// 16-byte chunk c of row r of a tile whose rows are kRow bytes: the chunks a matrix load reads from eight rows at one
+// c fall on different banks
+template <int kRow>
+__device__ __forceinline__ int swz(int r, int c) {
+  if constexpr (kRow >= 128) return r * kRow + ((c ^ (r & 7)) << 4);
+  return r * kRow + ((c ^ ((r >> 1) & 3)) << 4);
 }
 
-__global__ void __launch_bounds__(128) paged_attention_kernel(const PagedAttnArgs a) {
-  const int lane = threadIdx.x & 31;
-  const int h = blockIdx.x * 4 + (threadIdx.x >> 5), b = blockIdx.y;
-  if (h >= a.Hq) return;
-  const int hk = h / (a.Hq / a.Hkv);
-  const int row = a.rows != nullptr ? a.rows[b] : b;
-  int64_t len = (row >= 0 && row < a.table_rows) ? a.lens[row] : 0;
-  if (len > static_cast<int64_t>(a.table_width) * a.page_size) len = static_cast<int64_t>(a.table_width) * a.page_size;
-  const float ks = a.k_scale != nullptr ? a.k_scale[hk] : 1.0f, vs = a.v_scale != nullptr ? a.v_scale[hk] : 1.0f;
-  float q[8], o[8] = {};
-  const int per = a.D / 32;
-  for (int i = 0; i < per; ++i) q[i] = load_cache(a.q, b * a.q_sb + h * a.q_sh + lane + 32 * i, a.dtype) * a.scale * ks;
-  float m = -INFINITY, l = 0.0f;
-  for (int64_t j = 0; j < len; ++j) {
-    if (a.window > 0 && j < len - a.window && j >= a.sinks) continue;
-    const int page = a.table[row * a.table_stride + j / a.page_size];
-    if (page < 0 || page >= a.num_pages) continue;
-    const int64_t at = page * a.page_stride + hk * a.head_stride + (j % a.page_size) * a.tok_stride + lane;
-    float s = 0.0f;
-    for (int i = 0; i < per; ++i) s = fmaf(q[i], load_cache(a.k, at + 32 * i, a.cache_dtype), s);
-    for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-    const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.0f : mn;   // every score so far may be -inf
-    const float f = expf(m - base), p = expf(s - base);
-    m = mn;
-    l = l * f + p;
-    for (int i = 0; i < per; ++i) o[i] = o[i] * f + p * load_cache(a.v, at + 32 * i, a.cache_dtype);
+// the visible keys of a row: vis of them, the i-th at position i below nsink and at n - vis + i from there on
+struct RowView {
+  int row, n, vis, nsink, units;
+};
+__device__ __forceinline__ RowView row_view(const PagedAttnArgs& a, int b) {
+  RowView v;
+  v.row = a.rows != nullptr ? __ldg(a.rows + b) : b;
+  int n = v.row >= 0 && v.row < a.table_rows ? __ldg(a.lens + v.row) : 0;
+  n = min(max(n, 0), a.table_width * a.page_size);
+  v.n = n;
+  v.vis = n;
+  v.nsink = 0;
+  if (a.window > 0 && n > a.window) {
+    v.nsink = min(a.sinks, n - a.window);
+    v.vis = a.window + v.nsink;
   }
-  for (int i = 0; i < per; ++i) {
-    const float y = l > 0.0f ? o[i] / l * vs : l;
-    const int64_t at = (static_cast<int64_t>(b) * a.Hq + h) * a.D + lane + 32 * i;
-    if (a.dtype == CQ_DT_F16) static_cast<__half*>(a.out)[at] = __float2half_rn(y);
-    else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(y);
-  }
-  if (a.lse != nullptr && lane == 0) a.lse[static_cast<int64_t>(b) * a.Hq + h] = l > 0.0f ? m + logf(l) : -INFINITY;
+  v.units = (v.vis + pattn::kUnit - 1) / pattn::kUnit;
+  return v;
 }
 
-int64_t paged_attention_workspace(int64_t batch, int Hq, int Hkv, int D) { return 0; }
+// a place in the sequence of units: row b, head tile, unit of that segment
+struct UnitIter {
+  int b, head, unit;
+  RowView v;
+  __device__ __forceinline__ void next(const PagedAttnArgs& a, int heads) {
+    if (++unit < v.units) return;
+    unit = 0;
+    if (++head < heads) return;
+    head = 0;
+    while (++b < a.B) {
+      v = row_view(a, b);
+      if (v.units > 0) break;
+    }
+  }
+};
+
+template <bool F16, bool FP8, int D, int NT>
+__global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2, NT>::kCtas)
+    paged_attention_kernel(const PagedAttnArgs a, const int head_tiles, const int whole) {
+  using C = pattn::Cfg<D, FP8 ? 1 : 2, NT>;
+  constexpr int ES = FP8 ? 1 : 2, kRow = C::kRow, kStages = C::kStages;
+  constexpr bool kF16Math = F16 || FP8;
+  constexpr int kHeads = 8 * NT;                        // heads of a tile
+  constexpr int kMt = D / 16;                           // 16-wide slices of the head dim
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint8_t* ring = smem;
+  uint2* qfrag = reinterpret_cast<uint2*>(smem + pattn::kWarps * kStages * C::kStageBytes);
+  float* obuf = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(qfrag) + C::kQ);   // [D][kHeads]
+  float* sm_m = obuf + kHeads * D;                      // [kWarps][kHeads]
+  float* sm_l = sm_m + pattn::kWarps * kHeads;
+  float* qmul = sm_l + pattn::kWarps * kHeads;          // [kHeads] score multiplier
+  int* start = reinterpret_cast<int*>(qmul + kHeads);   // the run's first (b, head, unit)
+  uint32_t* masks = reinterpret_cast<uint32_t*>(start + 4);   // [kWarps][kStages] valid keys of a tile
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
+  const int group = a.Hq / a.Hkv, heads = a.Hkv * head_tiles;
+  if (!whole) grid_dep_launch();                        // the join may be set up while this grid runs
+
+  // ---- this CTA's run of units --------------------------------------------------------------
+  int64_t count = 0;
+  UnitIter it;
+  if (whole) {                                          // runs of whole segments
+    const int64_t segs = static_cast<int64_t>(a.B) * heads;
+    const int64_t s0 = blockIdx.x * segs / gridDim.x, s1 = (blockIdx.x + 1) * segs / gridDim.x;
+    int b0 = static_cast<int>(s0 / heads), h0 = static_cast<int>(s0 % heads);
+    for (int64_t s = s0; s < s1;) {
+      const int b = static_cast<int>(s / heads);
+      const int64_t upto = min(s1, static_cast<int64_t>(b + 1) * heads);
+      const int u = row_view(a, b).units;
+      if (count == 0 && u > 0) { b0 = b; h0 = static_cast<int>(s % heads); }
+      count += u * (upto - s);
+      s = upto;
+    }
+    it.b = b0;
+    it.head = h0;
+    it.unit = 0;
+  } else {                                              // equal runs of units
+    __shared__ int64_t wsum[pattn::kWarps];
+    const int each = (a.B + blockDim.x - 1) / blockDim.x, first = tid * each, last = min(a.B, first + each);
+    int64_t mine = 0;
+    for (int b = first; b < last; ++b) mine += row_view(a, b).units;
+    int64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t u = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += u;
+    }
+    if (lane == 31) wsum[warp] = incl;
+    __syncthreads();
+    int64_t total = 0;
+#pragma unroll
+    for (int w = 0; w < pattn::kWarps; ++w) {
+      if (w == warp) incl += total;
+      total += wsum[w];
+    }
+    total *= heads;
+    const int64_t runs = max(static_cast<int64_t>(1), min(static_cast<int64_t>(gridDim.x), total / pattn::kMinUnits));
+    const int64_t u0 = min(static_cast<int64_t>(blockIdx.x), runs) * total / runs;
+    const int64_t u1 = min(static_cast<int64_t>(blockIdx.x) + 1, runs) * total / runs;
+    count = u1 - u0;
+    const int64_t from = (incl - mine) * heads, to = incl * heads;
+    if (count > 0 && u0 >= from && u0 < to) {
+      int64_t left = u0 - from;
+      for (int b = first; b < last; ++b) {
+        const int u = row_view(a, b).units;
+        if (left < static_cast<int64_t>(u) * heads) {
+          start[0] = b;
+          start[1] = static_cast<int>(left / u);
+          start[2] = static_cast<int>(left % u);
+          break;
+        }
+        left -= static_cast<int64_t>(u) * heads;
+      }
+    }
+    __syncthreads();
+    it.b = count > 0 ? start[0] : 0;
+    it.head = count > 0 ? start[1] : 0;
+    it.unit = count > 0 ? start[2] : 0;
+  }
+  // rows that see nothing belong to no unit: their zeros
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+    if (row_view(a, b).units > 0) continue;
+    uint32_t* o = static_cast<uint32_t*>(a.out) + static_cast<int64_t>(b) * a.Hq * (D / 2);
+    for (int i = tid; i < a.Hq * (D / 2); i += blockDim.x) o[i] = 0;
+    if (a.lse != nullptr)
+      for (int i = tid; i < a.Hq; i += blockDim.x) a.lse[static_cast<int64_t>(b) * a.Hq + i] = -INFINITY;
+  }
+  float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) + gridDim.x * sizeof(pattn::Meta));
+  if (!whole && tid == 0) {
+    pattn::Meta m{0, 0, 0, static_cast<int>(count)};
+    if (count > 0) m = {it.b * heads + it.head, it.unit, row_view(a, it.b).units, static_cast<int>(count)};
+    static_cast<pattn::Meta*>(a.ws)[blockIdx.x] = m;
+  }
+  if (count == 0) return;
+  it.v = row_view(a, it.b);
+
+  // ---- the warp's ring ----------------------------------------------------------------------
+  uint8_t* my_ring = ring + warp * kStages * C::kStageBytes;
+  const uint32_t my_ring_u = smem_u32(my_ring);
+  uint32_t* my_masks = masks + warp * kStages;
+  const int page_shift = 31 - __clz(a.page_size), page_mask = a.page_size - 1;
+  // lane r < 16 looks after key r of the tile; its page index is loaded one step before the copies need it
+  UnitIter ahead = it;
+  int page = -1;
+  int64_t inner = 0;
+  auto look_up = [&]() {
+    const int i = ahead.unit * pattn::kUnit + warp * pattn::kTile + (lane & 15);
+    page = -1;
+    if (i < ahead.v.vis) {
+      const int j = i < ahead.v.nsink ? i : ahead.v.n - ahead.v.vis + i;
+      page = __ldg(a.table + ahead.v.row * a.table_stride + (j >> page_shift));
+      inner = (ahead.head / head_tiles) * a.head_stride + (j & page_mask) * a.tok_stride;
+    }
+  };
+  int64_t looked = 0;                                   // units looked up
+  auto issue = [&](int stage) {                         // copies of the tile looked up last, and the next look-up
+    if (looked <= count) {
+      const bool ok = page >= 0 && page < a.num_pages;
+      const uint32_t mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+      if (lane == 0) my_masks[stage] = mask;
+      if (mask != 0) {
+        const int64_t off = ok ? (page * a.page_stride + inner) * ES : 0;
+        const uint32_t dst = my_ring_u + stage * C::kStageBytes;
+        constexpr int kChunks = kRow / 16;              // 16-byte chunks of a row: 4 to 32
+        constexpr int kRows = 32 / kChunks;             // rows of one copy instruction
+#pragma unroll
+        for (int r0 = 0; r0 < pattn::kTile; r0 += kRows) {
+          const int r = r0 + lane / kChunks, ch = lane % kChunks;
+          const int64_t o = __shfl_sync(0xffffffffu, off, r);
+          const bool valid = mask >> r & 1u;
+          const uint32_t to = dst + swz<kRow>(r, ch);
+          cp_async16(to, static_cast<const uint8_t*>(a.k) + o + 16 * ch, valid);
+          cp_async16(to + C::kTileBytes, static_cast<const uint8_t*>(a.v) + o + 16 * ch, valid);
+        }
+      }
+    }
+    cp_async_commit();
+    if (looked < count) {
+      ahead.next(a, heads);
+      look_up();
+    }
+    ++looked;
+  };
+  look_up();
+  ++looked;
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) issue(s);
+
+  // ---- units --------------------------------------------------------------------------------
+  const float log2e = 1.4426950408889634f;
+  float o[kMt][NT][4], m[NT][2], l[NT][2], mul[NT][2];
+  int part = 0, part_begin = 0;
+  bool fresh = true;
+  int stage = 0;
+  for (int64_t t = 0; t < count; ++t) {
+    const int hk = it.head / head_tiles, h0 = hk * group + (it.head - hk * head_tiles) * kHeads;
+    const int nh = min(kHeads, (hk + 1) * group - h0);
+    if (fresh) {
+      fresh = false;
+      part_begin = it.unit;
+      // the tile's query heads as the second operand's fragments, one warp per head
+      for (int h = warp; h < kHeads; h += pattn::kWarps) {
+        const uint16_t* src = static_cast<const uint16_t*>(a.q) + it.b * a.q_sb + (h0 + h) * a.q_sh;
+        uint2 w[(D / 4 + 31) / 32];
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < (D / 4 + 31) / 32; ++i) {
+          const int e = lane + 32 * i;                  // slice e / 4, column pair e % 4
+          w[i] = make_uint2(0, 0);
+          if (h < nh && e < D / 4) {
+            const uint32_t* p = reinterpret_cast<const uint32_t*>(src + 16 * (e >> 2));
+            w[i] = FP8 ? make_uint2(__ldg(p + 2 * (e & 3)), __ldg(p + 2 * (e & 3) + 1))
+                       : make_uint2(__ldg(p + (e & 3)), __ldg(p + (e & 3) + 4));
+          }
+          if constexpr (FP8 && !F16) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t word = j < 2 ? w[i].x : w[i].y;
+              top = fmaxf(top, fabsf(__uint_as_float((j & 1 ? word >> 16 : word & 0xffffu) << 16)));
+            }
+          }
+        }
+        float factor = 1.0f;
+        if constexpr (FP8 && !F16) {
+#pragma unroll
+          for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+          // 2^e with top in [2^e', 2^(e'+1)) taken to [2^13, 2^14); both powers are normal numbers
+          const int ex = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+          const int by = top > 0.0f && ex < 128 ? min(max(ex - 13, -100), 100) : 0;
+          factor = __uint_as_float(static_cast<uint32_t>(127 + by) << 23);
+          const float down = __uint_as_float(static_cast<uint32_t>(127 - by) << 23);
+#pragma unroll
+          for (int i = 0; i < (D / 4 + 31) / 32; ++i) {
+            uint32_t* u = &w[i].x;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const __half2 x = __floats2half2_rn(__uint_as_float(u[j] << 16) * down,
+                                                  __uint_as_float(u[j] & 0xffff0000u) * down);
+              u[j] = *reinterpret_cast<const uint32_t*>(&x);
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < (D / 4 + 31) / 32; ++i) {
+          const int e = lane + 32 * i;
+          if (e < D / 4) qfrag[((e >> 2) * NT + (h >> 3)) * 32 + (h & 7) * 4 + (e & 3)] = w[i];
+        }
+        if (lane == 0)
+          qmul[h] = a.scale * log2e * factor * (FP8 && a.k_scale != nullptr ? __ldg(a.k_scale + hk) : 1.0f);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        m[n][0] = m[n][1] = -INFINITY;
+        l[n][0] = l[n][1] = 0.0f;
+        mul[n][0] = qmul[8 * n + 2 * c];
+        mul[n][1] = qmul[8 * n + 2 * c + 1];
+#pragma unroll
+        for (int i = 0; i < kMt; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[i][n][j] = 0.0f;
+      }
+    }
+    cp_async_wait<kStages - 2>();
+    __syncwarp();
+    const uint32_t mask = my_masks[stage];
+    if (mask != 0) {
+      const uint32_t kt = my_ring_u + stage * C::kStageBytes, vt = kt + C::kTileBytes;
+      float s[NT][4], s2[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][j] = s2[n][j] = 0.0f;
+      const int kr = (lane & 7) + (lane >> 3 & 1) * 8, kc = lane >> 4;
+      if constexpr (!FP8) {
+#pragma unroll
+        for (int ks = 0; ks < kMt; ++ks) {
+          uint32_t ka[4];
+          ldsm_x4(ka, kt + swz<kRow>(kr, 2 * ks + kc));
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const uint2 q = qfrag[(ks * NT + n) * 32 + lane];
+            mma_16816<kF16Math>(ks & 1 ? s2[n] : s[n], ka, q.x, q.y);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int kp = 0; kp < kMt / 2; ++kp) {
+          uint32_t raw[4];
+          ldsm_x4(raw, kt + swz<kRow>(kr, 2 * kp + kc));
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t r0 = raw[2 * half], r1 = raw[2 * half + 1];
+            const uint32_t ka[4] = {e4m3x2_to_f16x2(r0 & 0xffffu), e4m3x2_to_f16x2(r1 & 0xffffu),
+                                    e4m3x2_to_f16x2(r0 >> 16), e4m3x2_to_f16x2(r1 >> 16)};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const uint2 q = qfrag[((2 * kp + half) * NT + n) * 32 + lane];
+              mma_16816<true>(half ? s2[n] : s[n], ka, q.x, q.y);
+            }
+          }
+        }
+      }
+      // s[n][0..1]: key g, heads 2c, 2c + 1 of the tile's n-th eight; s[n][2..3]: key g + 8
+      const bool ok0 = mask >> g & 1u, ok1 = mask >> (g + 8) & 1u;
+      uint32_t ph[NT][2], pl[NT][2];
+      bool grew = false;
+      float f[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float x0 = ok0 ? (s[n][j] + s2[n][j]) * mul[n][j] : -INFINITY;
+          const float x1 = ok1 ? (s[n][2 + j] + s2[n][2 + j]) * mul[n][j] : -INFINITY;
+          float top = fmaxf(x0, x1);
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+          const float mn = fmaxf(m[n][j], top), base = mn == -INFINITY ? 0.0f : mn;   // all may be -inf so far
+          f[n][j] = exp2f(m[n][j] - base);
+          grew |= mn != m[n][j];
+          m[n][j] = mn;
+          s[n][j] = exp2f(x0 - base);
+          s[n][2 + j] = exp2f(x1 - base);
+          l[n][j] = l[n][j] * f[n][j] + (s[n][j] + s[n][2 + j]);
+        }
+        split16<kF16Math>(s[n][0], s[n][1], ph[n][0], pl[n][0]);
+        split16<kF16Math>(s[n][2], s[n][3], ph[n][1], pl[n][1]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          ph[n][j] = movmatrix_t(ph[n][j]);
+          pl[n][j] = movmatrix_t(pl[n][j]);
+        }
+      }
+      if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+        for (int i = 0; i < kMt; ++i)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][n][j] *= f[n][j & 1];
+      }
+      if constexpr (!FP8) {
+        const int vr = (lane & 7) + (lane >> 4) * 8, vc = lane >> 3 & 1;
+#pragma unroll
+        for (int i = 0; i < kMt; ++i) {
+          uint32_t va[4];
+          ldsm_x4_t(va, vt + swz<kRow>(vr, 2 * i + vc));
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma_16816<kF16Math>(o[i][n], va, ph[n][0], ph[n][1]);
+            mma_16816<kF16Math>(o[i][n], va, pl[n][0], pl[n][1]);
+          }
+        }
+      } else {
+        // a transposed load gives the columns in pairs: row g of slice i is column 2g, row g + 8 column 2g + 1
+#pragma unroll
+        for (int ip = 0; ip < kMt / 2; ++ip) {
+          uint32_t raw[4];
+          ldsm_x4_t(raw, vt + swz<kRow>(kr, 2 * ip + kc));
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t r0 = __byte_perm(raw[2 * half], 0, 0x3120), r1 = __byte_perm(raw[2 * half + 1], 0, 0x3120);
+            const uint32_t va[4] = {e4m3x2_to_f16x2(r0 & 0xffffu), e4m3x2_to_f16x2(r0 >> 16),
+                                    e4m3x2_to_f16x2(r1 & 0xffffu), e4m3x2_to_f16x2(r1 >> 16)};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              mma_16816<true>(o[2 * ip + half][n], va, ph[n][0], ph[n][1]);
+              mma_16816<true>(o[2 * ip + half][n], va, pl[n][0], pl[n][1]);
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
+    issue(stage == 0 ? kStages - 1 : stage - 1);
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+
+    const bool seg_end = it.unit + 1 == it.v.units;
+    if (!seg_end && t + 1 < count) { ++it.unit; continue; }
+
+    // ---- the end of this CTA's part of the segment: join the warps ------------------------------
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], x);
+        if (g == 0) {
+          sm_m[warp * kHeads + 8 * n + 2 * c + j] = m[n][j];
+          sm_l[warp * kHeads + 8 * n + 2 * c + j] = l[n][j];
+        }
+      }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int h = 8 * n + 2 * c + j;
+        float top = sm_m[h];
+#pragma unroll
+        for (int w = 1; w < pattn::kWarps; ++w) top = fmaxf(top, sm_m[w * kHeads + h]);
+        const float f = m[n][j] == -INFINITY ? 0.0f : exp2f(m[n][j] - top);
+#pragma unroll
+        for (int i = 0; i < kMt; ++i) {
+          o[i][n][j] *= f;
+          o[i][n][2 + j] *= f;
+        }
+      }
+    for (int w = 0; w < pattn::kWarps; ++w) {
+      if (w == warp) {
+#pragma unroll
+        for (int i = 0; i < kMt; ++i)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const int d = FP8 ? 16 * i + 2 * g + r : 16 * i + g + 8 * r;
+              float2* to = reinterpret_cast<float2*>(obuf + d * kHeads + 8 * n + 2 * c);
+              float2 v = make_float2(o[i][n][2 * r], o[i][n][2 * r + 1]);
+              if (w > 0) { const float2 u = *to; v.x += u.x; v.y += u.y; }
+              *to = v;
+            }
+      }
+      __syncthreads();
+    }
+    const bool complete = seg_end && part_begin == 0;
+    const float vs = FP8 && a.v_scale != nullptr ? __ldg(a.v_scale + hk) : 1.0f;
+    for (int i = tid; i < nh * (D / 2); i += blockDim.x) {
+      const int h = i / (D / 2), d = 2 * (i - h * (D / 2));
+      float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < pattn::kWarps; ++w) top = fmaxf(top, sm_m[w * kHeads + h]);
+#pragma unroll
+      for (int w = 0; w < pattn::kWarps; ++w)
+        if (sm_m[w * kHeads + h] != -INFINITY) sum += sm_l[w * kHeads + h] * exp2f(sm_m[w * kHeads + h] - top);
+        else sum += sm_l[w * kHeads + h];                 // zero, or NaN where a score was NaN
+      float2 v = make_float2(obuf[d * kHeads + h], obuf[(d + 1) * kHeads + h]);
+      if (complete) {
+        const float inv = sum == 0.0f ? 0.0f : vs / sum;
+        const int64_t at = (static_cast<int64_t>(it.b) * a.Hq + h0 + h) * D + d;
+        if constexpr (F16)
+          *reinterpret_cast<__half2*>(static_cast<__half*>(a.out) + at) = __floats2half2_rn(v.x * inv, v.y * inv);
+        else
+          *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.out) + at) =
+              __floats2bfloat162_rn(v.x * inv, v.y * inv);
+        if (d == 0 && a.lse != nullptr)
+          a.lse[static_cast<int64_t>(it.b) * a.Hq + h0 + h] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) / log2e;
+      } else {
+        float* p = parts + (static_cast<int64_t>(blockIdx.x) * 2 + min(part, 1)) * kHeads * (D + 2);
+        *reinterpret_cast<float2*>(p + h * D + d) = v;
+        if (d == 0) {
+          p[kHeads * D + h] = top;
+          p[kHeads * D + kHeads + h] = sum;
+        }
+      }
+    }
+    __syncthreads();                                      // obuf and the statistics are read
+    ++part;
+    fresh = true;
+    it.next(a, heads);
+  }
+  cp_async_wait<0>();
+}
+
+// Joins the parts of a row that several CTAs shared, in their order.  CTA (r, h): the segment whose first boundary
+// between two runs lies before run r, head h of its tile; most have nothing to do.  Warps take every fourth part.
+template <bool F16, int D, int NT>
+__global__ void __launch_bounds__(128) paged_attention_join_kernel(const PagedAttnArgs a, const int runs, const int head_tiles) {
+  constexpr int kHeads = 8 * NT, kPer = D / 32;           // columns per lane
+  __shared__ float sum_o[4][D];
+  grid_dep_wait();
+  const int r = blockIdx.x + 1, h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const pattn::Meta* metas = static_cast<const pattn::Meta*>(a.ws);
+  const pattn::Meta me = metas[r];
+  if (me.count == 0 || me.unit0 == 0) return;             // no run, or it begins with a segment of its own
+  const int before = metas[r - 1].count;
+  if (before < me.unit0) return;                          // the segment's first boundary is an earlier one
+  const int heads = a.Hkv * head_tiles, group = a.Hq / a.Hkv;
+  const int b = me.seg / heads, head = me.seg - b * heads, hk = head / head_tiles;
+  const int h0 = hk * group + (head - hk * head_tiles) * kHeads;
+  if (h >= min(kHeads, (hk + 1) * group - h0)) return;
+  const float* parts = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.ws) + runs * sizeof(pattn::Meta));
+  // part 0 is run r - 1's last one (its only one where that run begins with this segment), part i run r - 1 + i's first
+  auto at = [&](int i) {
+    const int slot = i == 0 && before > me.unit0 ? 1 : 0;
+    return parts + (static_cast<int64_t>(r - 1 + i) * 2 + slot) * kHeads * (D + 2);
+  };
+  int n = 1;
+  for (int left = me.units - me.unit0; left > 0; ++n) left -= metas[r - 1 + n].count;
+  float top = -INFINITY;
+  for (int i = lane; i < n; i += 32) top = fmaxf(top, at(i)[kHeads * D + h]);
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+  float o[kPer] = {}, l = 0.0f;
+#pragma unroll 4
+  for (int i = warp; i < n; i += 4) {
+    const float* p = at(i);
+    const float m = p[kHeads * D + h], f = m == -INFINITY ? 0.0f : exp2f(m - top);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) o[j] = fmaf(p[h * D + lane + 32 * j], f, o[j]);
+  }
+  for (int i = lane; i < n; i += 32) {
+    const float m = at(i)[kHeads * D + h], s = at(i)[kHeads * D + kHeads + h];
+    l += m == -INFINITY ? s : s * exp2f(m - top);
+  }
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) sum_o[warp][lane + 32 * j] = o[j];
+  __syncthreads();
+  const float vs = a.cache_dtype == CQ_DT_FP8_E4M3 && a.v_scale != nullptr ? __ldg(a.v_scale + hk) : 1.0f;
+  const float inv = l == 0.0f ? 0.0f : vs / l;
+  const int64_t to = (static_cast<int64_t>(b) * a.Hq + h0 + h) * D;
+  for (int d = threadIdx.x; d < D; d += 128) {
+    const float y = ((sum_o[0][d] + sum_o[1][d]) + (sum_o[2][d] + sum_o[3][d])) * inv;
+    if constexpr (F16) static_cast<__half*>(a.out)[to + d] = __float2half_rn(y);
+    else static_cast<__nv_bfloat16*>(a.out)[to + d] = __float2bfloat16_rn(y);
+  }
+  if (threadIdx.x == 0 && a.lse != nullptr)
+    a.lse[static_cast<int64_t>(b) * a.Hq + h0 + h] = l == 0.0f ? -INFINITY : (top + log2f(l)) / 1.4426950408889634f;
+}
+
+namespace {
+int sm_count() {
+  static int cached = 0;
+  if (cached == 0) {
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess)
+      cached = n;
+  }
+  return cached > 0 ? cached : 148;
+}
+constexpr int kMaxRuns = 2 * 148;
+}  // namespace
+
+int64_t paged_attention_workspace(int64_t batch, int Hq, int Hkv, int D) {
+  const int heads = Hq / Hkv <= 8 ? 8 : 16;
+  return batch == 0 ? 0 : kMaxRuns * static_cast<int64_t>(sizeof(pattn::Meta) + 2 * heads * (D + 2) * sizeof(float));
+}
+
+template <bool F16, bool FP8, int D, int NT>
+cudaError_t run_paged_attention(const PagedAttnArgs& a, cudaStream_t st) {
+  using C = pattn::Cfg<D, FP8 ? 1 : 2, NT>;
+  auto kern = paged_attention_kernel<F16, FP8, D, NT>;
+  static bool ready = false;                              // set once per process and kernel; setting it twice is harmless
+  if (!ready) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e != cudaSuccess) return e;
+    ready = true;
+  }
+  const int group = a.Hq / a.Hkv, tiles = (group + 8 * NT - 1) / (8 * NT);
+  int64_t most = static_cast<int64_t>(a.table_width) * a.page_size;    // visible keys of any row
+  if (a.window > 0) most = most < static_cast<int64_t>(a.window) + a.sinks ? most : static_cast<int64_t>(a.window) + a.sinks;
+  const int64_t units = (most + pattn::kUnit - 1) / pattn::kUnit, segs = static_cast<int64_t>(a.B) * a.Hkv * tiles;
+  int grid = sm_count() * C::kCtas;
+  if (grid > kMaxRuns) grid = kMaxRuns;
+  const bool whole = units <= pattn::kWholeUnits;
+  if (whole) {
+    if (segs < grid) grid = static_cast<int>(segs);
+  } else if (segs * ((units + pattn::kMinUnits - 1) / pattn::kMinUnits) < grid) {
+    grid = static_cast<int>(segs * ((units + pattn::kMinUnits - 1) / pattn::kMinUnits));
+  }
+  kern<<<grid, pattn::kWarps * 32, C::kSmem, st>>>(a, tiles, whole ? 1 : 0);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || whole || grid == 1) return e;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(grid - 1, group < 8 * NT ? group : 8 * NT);
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<F16, D, NT>, a, grid, tiles);
+}
+
+template <bool F16, bool FP8>
+cudaError_t pick_paged_attention(const PagedAttnArgs& a, cudaStream_t st) {
+  const bool wide = a.Hq / a.Hkv > 8;                     // heads of a tile: 16, or 8
+  switch (a.D) {
+    case 64: return wide ? run_paged_attention<F16, FP8, 64, 2>(a, st) : run_paged_attention<F16, FP8, 64, 1>(a, st);
+    case 128: return wide ? run_paged_attention<F16, FP8, 128, 2>(a, st) : run_paged_attention<F16, FP8, 128, 1>(a, st);
+    default: return wide ? run_paged_attention<F16, FP8, 256, 2>(a, st) : run_paged_attention<F16, FP8, 256, 1>(a, st);
+  }
+}
 
 cudaError_t launch_paged_attention(const PagedAttnArgs& a, cudaStream_t st) {
-  const dim3 grid((a.Hq + 3) / 4, a.B);
-  paged_attention_kernel<<<grid, 128, 0, st>>>(a);
-  return cudaGetLastError();
+  const bool fp8 = a.cache_dtype == CQ_DT_FP8_E4M3;
+  if (a.dtype == CQ_DT_F16) return fp8 ? pick_paged_attention<true, true>(a, st) : pick_paged_attention<true, false>(a, st);
+  return fp8 ? pick_paged_attention<false, true>(a, st) : pick_paged_attention<false, false>(a, st);
 }
 
 }  // namespace cq
