@@ -107,7 +107,8 @@ SIGNATURES = {
                                           _vp]),
     "cq_heads_to_rows": (_int, [_vp, _i64, _int, _int, _vp, _int, _i64, _i64, _vp]),
     "cq_gemm_rowcol_swiglu": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
-    "cq_w4a16_linear": (_int, [_vp, _i64, _int, _i64, _i64, _i64, _vp, _vp, _vp, _int, _vp, _vp, _vp]),
+    "cq_w4a16_workspace_bytes": (_i64, [_i64, _i64, _int]),
+    "cq_w4a16_linear": (_int, [_vp, _i64, _int, _i64, _i64, _i64, _vp, _vp, _vp, _int, _vp, _vp, _vp, _i64, _vp]),
     "cq_paged_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
     "cq_paged_attention": (_int, [_vp, _i64, _i64, _int, _i64, _i64, _i64, _i64, _vp, _vp, _int, _i64, _i64, _i64, _i64,
                                   _i64, _vp, _i64, _i64, _i64, _vp, _vp, _f32, _i64, _i64, _vp, _vp, _vp, _vp, _vp,

@@ -6,6 +6,7 @@
 
 namespace {
 
+constexpr int64_t kMaxTokens = 1 << 20;          // of a W4A16 linear
 constexpr int64_t kMaxSharedBits = 200 * 1024;   // bytes of the page and row bitmaps in one CTA's shared memory
 
 bool valid16(int dtype) { return dtype == CQ_DT_BF16 || dtype == CQ_DT_F16; }
@@ -26,21 +27,32 @@ int check_tables(int64_t table_rows, int64_t table_width, int64_t table_stride, 
 
 extern "C" {
 
+int64_t cq_w4a16_workspace_bytes(int64_t M, int64_t K, int group) {
+  if (M < 0 || M > kMaxTokens || (group != 32 && group != 64 && group != 128) || K < group || K % group != 0 || K > kMaxK)
+    return -1;
+  return cq::w4a16_workspace(static_cast<int>(M), static_cast<int>(K), group);
+}
+
 int cq_w4a16_linear(const void* x, int64_t ldx, int dtype, int64_t M, int64_t K, int64_t N, const void* qweight,
-                    const void* scale, const void* zeros, int group, const void* bias, void* out, void* stream) {
+                    const void* scale, const void* zeros, int group, const void* bias, void* out, void* workspace,
+                    int64_t workspace_bytes, void* stream) {
   if (!valid16(dtype) || (group != 32 && group != 64 && group != 128)) return CQ_ERR_ARG;
-  if (M < 0 || M > 8 * 65535ll || N < 0 || N > kMaxRows || K < group || K % group != 0 || K > kMaxK || ldx < K)
+  if (M < 0 || M > kMaxTokens || N < 0 || N > kMaxRows || K < group || K % group != 0 || K > kMaxK || ldx < K)
     return CQ_ERR_SHAPE;
+  const int64_t need = cq_w4a16_workspace_bytes(M, K, group);
+  if (workspace_bytes < need) return CQ_ERR_SHAPE;
   if (M == 0 || N == 0) return CQ_OK;
-  if (x == nullptr || qweight == nullptr || scale == nullptr || zeros == nullptr || out == nullptr) return CQ_ERR_ARG;
+  if (x == nullptr || qweight == nullptr || scale == nullptr || zeros == nullptr || out == nullptr ||
+      (workspace == nullptr && need > 0))
+    return CQ_ERR_ARG;
   if (!aligned(x, 16) || ldx % 8 != 0 || !aligned(qweight, 16) || !aligned(scale, 2) || !aligned(zeros, 2) ||
-      !aligned(bias, 2) || !aligned(out, 2))
+      !aligned(bias, 2) || !aligned(out, 2) || !aligned(workspace, 256))
     return CQ_ERR_ALIGN;
   if (int dv = check_device()) return dv;
   const cq::W4A16Args a{x, static_cast<const uint8_t*>(qweight), static_cast<const __nv_bfloat16*>(scale),
                         static_cast<const __nv_bfloat16*>(zeros), bias, out, ldx, static_cast<int>(M),
                         static_cast<int>(N), static_cast<int>(K), group, dtype == CQ_DT_F16 ? 1 : 0};
-  return cuda_status(cq::launch_w4a16(a, static_cast<cudaStream_t>(stream)));
+  return cuda_status(cq::launch_w4a16(a, workspace, static_cast<cudaStream_t>(stream)));
 }
 
 int64_t cq_paged_attention_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim) {

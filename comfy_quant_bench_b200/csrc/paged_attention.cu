@@ -613,15 +613,6 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(const PagedAt
 }
 
 namespace {
-int sm_count() {
-  static int cached = 0;
-  if (cached == 0) {
-    int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess)
-      cached = n;
-  }
-  return cached > 0 ? cached : 148;
-}
 constexpr int kMaxRuns = 2 * 148;
 }  // namespace
 
@@ -644,7 +635,7 @@ cudaError_t run_paged_attention(const PagedAttnArgs& a, cudaStream_t st) {
   int64_t most = static_cast<int64_t>(a.table_width) * a.page_size;    // visible keys of any row
   if (a.window > 0) most = most < static_cast<int64_t>(a.window) + a.sinks ? most : static_cast<int64_t>(a.window) + a.sinks;
   const int64_t units = (most + pattn::kUnit - 1) / pattn::kUnit, segs = static_cast<int64_t>(a.B) * a.Hkv * tiles;
-  int grid = sm_count() * C::kCtas;
+  int grid = num_sms() * C::kCtas;
   if (grid > kMaxRuns) grid = kMaxRuns;
   const bool whole = units <= pattn::kWholeUnits;
   if (whole) {

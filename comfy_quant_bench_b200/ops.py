@@ -514,8 +514,11 @@ def w4a16_linear(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor, ze
         out = torch.empty(*x.shape[:-1], n, dtype=dt, device=dev)
     elif out.dtype != dt or out.shape != (*x.shape[:-1], n) or not out.is_contiguous():
         raise ValueError(f"out must be contiguous {dt} of shape {(*x.shape[:-1], n)}")
+    nbytes = _lib.load().cq_w4a16_workspace_bytes(m, k, group_size)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
     _lib.call("cq_w4a16_linear", x2.data_ptr(), ldx, 0 if dt == torch.bfloat16 else 1, m, k, n, qweight.data_ptr(),
-              scale.data_ptr(), zeros.data_ptr(), int(group_size), _ptr(bias), out.data_ptr(), _stream(dev))
+              scale.data_ptr(), zeros.data_ptr(), int(group_size), _ptr(bias), out.data_ptr(), _ptr(ws), nbytes,
+              _stream(dev))
     return out
 
 

@@ -472,12 +472,15 @@ typedef enum {
  *   x        [M, K] of `dtype` (bf16 or f16), rows ldx elements apart; 16-byte aligned, ldx % 8 == 0
  *   qweight  packed uint4 [N, K/2], low nibble = even column, 16-byte aligned
  *   scale, zeros  bf16 [K/group, N];  bias  [N] of `dtype` or NULL;  out  [M, N] of `dtype`
- * group 32, 64 or 128, K a multiple of it and at most 32768; any N; M up to 524280.  Built for the few tokens of a
- * decode step (it reads the weights once per 64 tokens); cq_linear_w4a8_affine is the linear for many tokens.
+ *   workspace  cq_w4a16_workspace_bytes (0 for M <= 8), 256-byte aligned, of this call alone
+ * group 32, 64 or 128, K a multiple of it and at most 32768; any N; M up to 1048576.  Built for the few tokens of a
+ * decode step (it reads the weights once per 64 tokens); cq_linear_w4a8_affine is the linear for many tokens.  A
+ * token with an infinite or NaN activation gets outputs that are not finite.
  */
+CQ_API int64_t cq_w4a16_workspace_bytes(int64_t M, int64_t K, int group);
 CQ_API int cq_w4a16_linear(const void* x, int64_t ldx, int dtype, int64_t M, int64_t K, int64_t N,
                            const void* qweight, const void* scale, const void* zeros, int group, const void* bias,
-                           void* out, void* stream);
+                           void* out, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Paged cache: keys and values of a layer in pages of `page_size` tokens (a power of two, 8 to 1024), addressed as

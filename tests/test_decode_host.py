@@ -18,14 +18,19 @@ VP = ctypes.c_void_p(256)
 def test_linear_argument_checks_need_no_device(lib):
     from comfy_quant_bench_b200 import _lib as L
 
-    def call(x=VP, ldx=256, dtype=0, m=2, k=256, n=16, w=VP, s=VP, z=VP, g=64, b=None, out=VP):
-        return lib.cq_w4a16_linear(x, ldx, dtype, m, k, n, w, s, z, g, b, out, None)
+    def call(x=VP, ldx=256, dtype=0, m=2, k=256, n=16, w=VP, s=VP, z=VP, g=64, b=None, out=VP, ws=VP, wsn=1 << 30):
+        return lib.cq_w4a16_linear(x, ldx, dtype, m, k, n, w, s, z, g, b, out, ws, wsn, None)
     assert call(dtype=2) == L.CQ_ERR_ARG and call(g=16) == L.CQ_ERR_ARG and call(g=0) == L.CQ_ERR_ARG
     assert call(k=96) == L.CQ_ERR_SHAPE and call(k=0) == L.CQ_ERR_SHAPE and call(ldx=128) == L.CQ_ERR_SHAPE
     assert call(m=-1) == L.CQ_ERR_SHAPE and call(n=-1) == L.CQ_ERR_SHAPE and call(k=1 << 20, ldx=1 << 20) == L.CQ_ERR_SHAPE
     assert call(x=None) == L.CQ_ERR_ARG and call(w=None) == L.CQ_ERR_ARG and call(out=None) == L.CQ_ERR_ARG
     assert call(x=ctypes.c_void_p(264)) == L.CQ_ERR_ALIGN and call(ldx=257) == L.CQ_ERR_ALIGN
     assert call(w=ctypes.c_void_p(260)) == L.CQ_ERR_ALIGN
+    need = lib.cq_w4a16_workspace_bytes(20, 256, 64)
+    assert need >= 20 * 256 * 2 and lib.cq_w4a16_workspace_bytes(4, 256, 64) == 0
+    assert lib.cq_w4a16_workspace_bytes(4, 200, 64) == -1 and lib.cq_w4a16_workspace_bytes(-1, 256, 64) == -1
+    assert call(m=20, wsn=need - 1) == L.CQ_ERR_SHAPE and call(m=20, ws=None) == L.CQ_ERR_ARG
+    assert call(m=20, ws=ctypes.c_void_p(128)) == L.CQ_ERR_ALIGN
     assert call(m=0, x=None, w=None, s=None, z=None, out=None) == L.CQ_OK
     assert call(n=0) == L.CQ_OK
 
