@@ -109,7 +109,7 @@ SIGNATURES = {
     "cq_gemm_rowcol_swiglu": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     "cq_w4a16_workspace_bytes": (_i64, [_i64, _i64, _int]),
     "cq_w4a16_linear": (_int, [_vp, _i64, _int, _i64, _i64, _i64, _vp, _vp, _vp, _int, _vp, _vp, _vp, _i64, _vp]),
-    "cq_paged_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
+    "cq_paged_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i64]),
     "cq_paged_attention": (_int, [_vp, _i64, _i64, _int, _i64, _i64, _i64, _i64, _vp, _vp, _int, _i64, _i64, _i64, _i64,
                                   _i64, _vp, _i64, _i64, _i64, _vp, _vp, _f32, _i64, _i64, _vp, _vp, _vp, _vp, _vp,
                                   _i64, _vp]),
@@ -173,7 +173,9 @@ def check(fn: str, status: int) -> None:
 
 
 def call(name: str, *args) -> None:
-    check(name, getattr(load(), name)(*args))
+    status = getattr(_lib or load(), name)(*args)
+    if status != CQ_OK:
+        check(name, status)
 
 
 def exported_symbols() -> list[str]:

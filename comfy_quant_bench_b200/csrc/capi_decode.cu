@@ -55,11 +55,13 @@ int cq_w4a16_linear(const void* x, int64_t ldx, int dtype, int64_t M, int64_t K,
   return cuda_status(cq::launch_w4a16(a, workspace, static_cast<cudaStream_t>(stream)));
 }
 
-int64_t cq_paged_attention_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim) {
-  if (!fits_int(batch) || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads != 0 || !valid_head_dim(head_dim))
+int64_t cq_paged_attention_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                           int64_t span, int64_t window, int64_t sinks) {
+  if (!fits_int(batch) || q_heads < 1 || kv_heads < 1 || q_heads > 4096 || q_heads % kv_heads != 0 ||
+      !valid_head_dim(head_dim) || !fits_int(span) || window < 0 || sinks < 0)
     return -1;
   return cq::paged_attention_workspace(batch, static_cast<int>(q_heads), static_cast<int>(kv_heads),
-                                       static_cast<int>(head_dim));
+                                       static_cast<int>(head_dim), span, window, sinks);
 }
 
 int cq_paged_attention(const void* q, int64_t q_batch_stride, int64_t q_head_stride, int dtype, int64_t batch,
@@ -75,7 +77,8 @@ int cq_paged_attention(const void* q, int64_t q_batch_stride, int64_t q_head_str
   if (!fits_int(batch) || batch > 65535 || q_heads < 1 || kv_heads < 1 || q_heads > 4096 || q_heads % kv_heads != 0 ||
       !valid_head_dim(head_dim))
     return CQ_ERR_SHAPE;
-  const int64_t need = cq_paged_attention_workspace_bytes(batch, q_heads, kv_heads, head_dim);
+  const int64_t need = cq_paged_attention_workspace_bytes(batch, q_heads, kv_heads, head_dim, table_width * page_size,
+                                                          window, sinks);
   if (workspace_bytes < need) return CQ_ERR_SHAPE;
   if (batch == 0) return CQ_OK;
   if (q == nullptr || k_cache == nullptr || v_cache == nullptr || seq_lens == nullptr || out == nullptr ||

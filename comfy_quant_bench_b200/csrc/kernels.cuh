@@ -163,7 +163,8 @@ struct PagedAttnArgs {
   int B, Hq, Hkv, D, num_pages, page_size, table_rows, table_width, dtype, cache_dtype, window, sinks;
   float scale;
 };
-int64_t paged_attention_workspace(int64_t batch, int Hq, int Hkv, int D);
+// span: keys a table row can hold; 0 bytes where no row is split
+int64_t paged_attention_workspace(int64_t batch, int Hq, int Hkv, int D, int64_t span, int64_t window, int64_t sinks);
 cudaError_t launch_paged_attention(const PagedAttnArgs& a, cudaStream_t st);
 
 // free, fork and reserve rows of a paged cache

@@ -616,9 +616,15 @@ namespace {
 constexpr int kMaxRuns = 2 * 148;
 }  // namespace
 
-int64_t paged_attention_workspace(int64_t batch, int Hq, int Hkv, int D) {
+// units of the row with the most visible keys
+static int64_t most_units(int64_t span, int64_t window, int64_t sinks) {
+  if (window > 0 && window < span) span = sinks < span - window ? window + sinks : span;
+  return (span + pattn::kUnit - 1) / pattn::kUnit;
+}
+
+int64_t paged_attention_workspace(int64_t batch, int Hq, int Hkv, int D, int64_t span, int64_t window, int64_t sinks) {
   const int heads = Hq / Hkv <= 8 ? 8 : 16;
-  return batch == 0 ? 0 : kMaxRuns * static_cast<int64_t>(sizeof(pattn::Meta) + 2 * heads * (D + 2) * sizeof(float));
+  return batch == 0 || most_units(span, window, sinks) <= pattn::kWholeUnits ? 0 : kMaxRuns * static_cast<int64_t>(sizeof(pattn::Meta) + 2 * heads * (D + 2) * sizeof(float));
 }
 
 template <bool F16, bool FP8, int D, int NT>
@@ -632,9 +638,8 @@ cudaError_t run_paged_attention(const PagedAttnArgs& a, cudaStream_t st) {
     ready = true;
   }
   const int group = a.Hq / a.Hkv, tiles = (group + 8 * NT - 1) / (8 * NT);
-  int64_t most = static_cast<int64_t>(a.table_width) * a.page_size;    // visible keys of any row
-  if (a.window > 0) most = most < static_cast<int64_t>(a.window) + a.sinks ? most : static_cast<int64_t>(a.window) + a.sinks;
-  const int64_t units = (most + pattn::kUnit - 1) / pattn::kUnit, segs = static_cast<int64_t>(a.B) * a.Hkv * tiles;
+  const int64_t units = most_units(static_cast<int64_t>(a.table_width) * a.page_size, a.window, a.sinks);
+  const int64_t segs = static_cast<int64_t>(a.B) * a.Hkv * tiles;
   int grid = num_sms() * C::kCtas;
   if (grid > kMaxRuns) grid = kMaxRuns;
   const bool whole = units <= pattn::kWholeUnits;

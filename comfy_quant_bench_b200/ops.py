@@ -17,6 +17,7 @@ on the CPU or on a non-sm_100 device are rejected: there is no eager fallback.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -475,6 +476,38 @@ def w4a8_affine_linear(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tens
     return out if dt == torch.bfloat16 else out.to(dt)
 
 
+# Decode-side operators run in a few microseconds, so their host side is kept to plain checks and one native call.
+
+def _cuda_index(*ts: torch.Tensor | None) -> int:
+    """The CUDA device index that all the tensors are on."""
+    idx = None
+    for t in ts:
+        if t is None:
+            continue
+        i = t.get_device() if t.is_cuda else -1
+        if i != idx:
+            if i < 0:
+                raise ValueError("comfy_quant_bench_b200 ops run on CUDA tensors only (no CPU fallback)")
+            if idx is not None:
+                raise ValueError(f"tensors on different devices: cuda:{idx} and cuda:{i}")
+            idx = i
+    return idx
+
+
+def _launch(name: str, idx: int, *args) -> None:
+    """One native call on the tensors' device and its current stream (the call's last argument)."""
+    if idx == torch.cuda.current_device():
+        _lib.call(name, *args, torch.cuda.current_stream(idx).cuda_stream)
+    else:
+        with torch.cuda.device(idx):
+            _lib.call(name, *args, torch.cuda.current_stream(idx).cuda_stream)
+
+
+@functools.lru_cache(maxsize=1024)
+def _w4a16_workspace(m: int, k: int, group: int) -> int:
+    return _lib.load().cq_w4a16_workspace_bytes(m, k, group)
+
+
 def w4a16_linear(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor, zeros: torch.Tensor,
                  bias: torch.Tensor | None = None, *, group_size: int = 128,
                  out: torch.Tensor | None = None) -> torch.Tensor:
@@ -483,42 +516,47 @@ def w4a16_linear(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor, ze
     x [..., K] bf16 or f16 (its rows may be strided), qweight int8 or uint8 [N, K/2] (low nibble = even column),
     scale and zeros bf16 [K/group_size, N] (group_size 32, 64 or 128), bias [N].  Products and sums are fp32, rounded
     once to the type of x.  For the few tokens of a decode step; ``w4a8_affine_linear`` takes many tokens."""
-    k = x.shape[-1]
+    lead, k = x.shape[:-1], x.shape[-1]
     n = qweight.shape[0]
     dt = x.dtype
-    if dt != torch.bfloat16 and dt != torch.float16:
+    if dt is not torch.bfloat16 and dt is not torch.float16:
         raise ValueError(f"x must be bf16 or f16, got {dt}")
     if k != qweight.shape[-1] * 2:
         raise ValueError(f"Input K={k} does not match qweight K={qweight.shape[-1] * 2}")
     if group_size not in (32, 64, 128) or k % group_size:
         raise ValueError(f"group_size must be 32, 64 or 128 and divide K={k}, got {group_size}")
-    shape = (k // group_size, n)
-    if scale.dtype != torch.bfloat16 or zeros.dtype != torch.bfloat16 or scale.shape != shape or zeros.shape != shape:
-        raise ValueError(f"scale and zeros must be bf16 [{shape[0]}, {n}]")
-    if qweight.dtype not in (torch.int8, torch.uint8) or qweight.dim() != 2:
+    groups = (k // group_size, n)
+    if (scale.dtype is not torch.bfloat16 or zeros.dtype is not torch.bfloat16 or scale.shape != groups
+            or zeros.shape != groups):
+        raise ValueError(f"scale and zeros must be bf16 [{groups[0]}, {n}]")
+    if (qweight.dtype is not torch.int8 and qweight.dtype is not torch.uint8) or qweight.dim() != 2:
         raise ValueError("qweight must be int8 or uint8 [N, K/2]")
     if not (qweight.is_contiguous() and scale.is_contiguous() and zeros.is_contiguous()):
         raise ValueError("qweight, scale and zeros must be contiguous")
-    dev = _require_cuda(x, qweight, scale, zeros, bias, out)
-    x2 = x if x.dim() == 2 else x.reshape(-1, k)
-    ldx = x2.stride(0)
-    if x2.stride(1) != 1 or ldx % 8 or ldx < k or x2.data_ptr() % 16:
-        x2 = x2.contiguous() if x2.data_ptr() % 16 == 0 else x2.clone(memory_format=torch.contiguous_format)
-        ldx = k
-    m = x2.shape[0]
-    if bias is not None and (bias.dtype != dt or bias.shape != (n,) or not bias.is_contiguous()):
-        if bias.numel() != n:
-            raise ValueError(f"bias must have {n} elements")
-        bias = bias.reshape(n).to(dt).contiguous()
+    idx = _cuda_index(x, qweight, scale, zeros, bias, out)
+    x2 = x if len(lead) == 1 else x.reshape(-1, k)
+    m, ldx = x2.shape[0], k
+    xp = x2.data_ptr()
+    if xp % 16 or not x2.is_contiguous():
+        ldx = x2.stride(0)
+        if xp % 16 or x2.stride(1) != 1 or ldx % 8 or ldx < k:
+            x2, ldx = x2.clone(memory_format=torch.contiguous_format), k
+            xp = x2.data_ptr()
+    bp = None
+    if bias is not None:
+        if bias.dtype is not dt or bias.shape != (n,) or not bias.is_contiguous():
+            if bias.numel() != n:
+                raise ValueError(f"bias must have {n} elements")
+            bias = bias.reshape(n).to(dt).contiguous()
+        bp = bias.data_ptr()
     if out is None:
-        out = torch.empty(*x.shape[:-1], n, dtype=dt, device=dev)
-    elif out.dtype != dt or out.shape != (*x.shape[:-1], n) or not out.is_contiguous():
-        raise ValueError(f"out must be contiguous {dt} of shape {(*x.shape[:-1], n)}")
-    nbytes = _lib.load().cq_w4a16_workspace_bytes(m, k, group_size)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
-    _lib.call("cq_w4a16_linear", x2.data_ptr(), ldx, 0 if dt == torch.bfloat16 else 1, m, k, n, qweight.data_ptr(),
-              scale.data_ptr(), zeros.data_ptr(), int(group_size), _ptr(bias), out.data_ptr(), _ptr(ws), nbytes,
-              _stream(dev))
+        out = x.new_empty((*lead, n))
+    elif out.dtype is not dt or out.shape != (*lead, n) or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous {dt} of shape {(*lead, n)}")
+    nbytes = _w4a16_workspace(m, k, group_size)
+    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes > 0 else None
+    _launch("cq_w4a16_linear", idx, xp, ldx, 0 if dt is torch.bfloat16 else 1, m, k, n, qweight.data_ptr(),
+            scale.data_ptr(), zeros.data_ptr(), group_size, bp, out.data_ptr(), _ptr(ws), nbytes)
     return out
 
 

@@ -496,10 +496,13 @@ CQ_API int cq_w4a16_linear(const void* x, int64_t ldx, int dtype, int64_t M, int
  *   q    [batch, q_heads, head_dim] of `dtype` (bf16 or f16) with strides in elements; out the same, contiguous
  *   lse  f32 [batch, q_heads] or NULL: log sum_j exp(scale q . k_j) (-inf for a row that sees nothing)
  *   cache_dtype  dtype, or CQ_DT_FP8_E4M3 with k_scale / v_scale f32 [kv_heads] (NULL: 1)
- *   head_dim 64, 128 or 256; workspace of cq_paged_attention_workspace_bytes, 16-byte aligned, of this call alone
+ *   head_dim 64, 128 or 256
+ *   workspace of cq_paged_attention_workspace_bytes (span = table_width * page_size; 0 where no row is split), 16-byte
+ *   aligned, of this call alone
  * 16-byte aligned bases and strides.
  */
-CQ_API int64_t cq_paged_attention_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim);
+CQ_API int64_t cq_paged_attention_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                                  int64_t span, int64_t window, int64_t sinks);
 CQ_API int cq_paged_attention(const void* q, int64_t q_batch_stride, int64_t q_head_stride, int dtype, int64_t batch,
                               int64_t q_heads, int64_t kv_heads, int64_t head_dim, const void* k_cache,
                               const void* v_cache, int cache_dtype, int64_t num_pages, int64_t page_size,

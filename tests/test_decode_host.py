@@ -37,11 +37,10 @@ def test_linear_argument_checks_need_no_device(lib):
 
 def test_attention_argument_checks_need_no_device(lib):
     from comfy_quant_bench_b200 import _lib as L
-    size = lib.cq_paged_attention_workspace_bytes(2, 8, 2, 128)
-    assert size >= 0
-    assert lib.cq_paged_attention_workspace_bytes(2, 8, 3, 128) == -1
-    assert lib.cq_paged_attention_workspace_bytes(2, 8, 2, 96) == -1
-    assert lib.cq_paged_attention_workspace_bytes(-1, 8, 2, 64) == -1
+    size = lib.cq_paged_attention_workspace_bytes
+    assert size(2, 8, 2, 128, 100000, 0, 0) > 0 and size(0, 8, 2, 128, 100000, 0, 0) == 0
+    assert size(2, 8, 2, 128, 64, 0, 0) == 0 and size(2, 8, 2, 128, 100000, 50, 4) == 0      # no row is split
+    assert size(2, 8, 3, 128, 64, 0, 0) == -1 and size(2, 8, 2, 96, 64, 0, 0) == -1 and size(-1, 8, 2, 64, 64, 0, 0) == -1
 
     def call(q=VP, sb=1024, sh=128, dt=0, b=2, hq=8, hk=2, d=128, k=VP, v=VP, cdt=0, pages=10, page=16, sp=4096, shd=2048,
              st=128, table=VP, rows=2, width=4, ts=4, lens=VP, window=0, sinks=0, out=VP, ws=VP, wsn=1 << 40):
