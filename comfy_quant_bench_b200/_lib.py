@@ -173,9 +173,7 @@ def check(fn: str, status: int) -> None:
 
 
 def call(name: str, *args) -> None:
-    status = getattr(_lib or load(), name)(*args)
-    if status != CQ_OK:
-        check(name, status)
+    check(name, getattr(load(), name)(*args))
 
 
 def exported_symbols() -> list[str]:

@@ -48,6 +48,18 @@ __device__ __forceinline__ void cp_async_halves(uint32_t dst, const unsigned sho
   }
 }
 
+// Lets a kernel use `bytes` of dynamic shared memory, once per device (`devices`: a static of the caller's, one bit each;
+// two threads that both set the attribute do no harm).
+template <typename Kernel>
+inline cudaError_t allow_shared(Kernel kernel, int bytes, unsigned long long& devices) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && (devices >> dev & 1))) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) devices |= 1ull << dev;
+  return e;
+}
+
 // (v & mask) | bits in one instruction
 __device__ __forceinline__ uint32_t and_or(uint32_t v, uint32_t mask, uint32_t bits) {
   uint32_t d;

@@ -8,12 +8,13 @@
 // reference to each), then make room for new tokens: a row whose last page is partly filled and held by another row
 // too gets its own copy of it (copy on write), and pages are taken for what does not fit.  One CTA: each phase is
 // short, needs the one before it, and a list of rows is checked whole before any of it is applied.
-#include "kernels.cuh"
+#include "decode_common.cuh"
 
 namespace cq {
 
 namespace pages {
 constexpr int kThreads = 1024;
+constexpr int kMaxShared = 200 * 1024;   // bytes of the row and page bitmaps
 constexpr int kSiteFree = 101, kSiteFork = 102, kSiteReserve = 103;   // device status sites
 }  // namespace pages
 
@@ -210,8 +211,8 @@ int64_t pages_branch_shared(int table_rows, int num_pages) {
 cudaError_t launch_pages_branch(const PagesArgs& a, cudaStream_t st) {
   const int64_t smem = pages_branch_shared(a.table_rows, a.num_pages);
   if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(pages_branch_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               static_cast<int>(smem));
+    static unsigned long long devices = 0;
+    const cudaError_t e = allow_shared(pages_branch_kernel, pages::kMaxShared, devices);
     if (e != cudaSuccess) return e;
   }
   pages_branch_kernel<<<1, pages::kThreads, smem, st>>>(a);
@@ -295,7 +296,8 @@ __global__ void __launch_bounds__(256) pages_remap_kernel(const CompactArgs a) {
 cudaError_t launch_pages_compact(const CompactArgs& a, cudaStream_t st) {
   const int smem = (a.num_pages + 31) / 32 * 4;
   if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(pages_compact_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static unsigned long long devices = 0;
+    const cudaError_t e = allow_shared(pages_compact_kernel, pages::kMaxShared, devices);
     if (e != cudaSuccess) return e;
   }
   pages_compact_kernel<<<1, pages::kThreads, smem, st>>>(a);

@@ -631,12 +631,9 @@ template <bool F16, bool FP8, int D, int NT>
 cudaError_t run_paged_attention(const PagedAttnArgs& a, cudaStream_t st) {
   using C = pattn::Cfg<D, FP8 ? 1 : 2, NT>;
   auto kern = paged_attention_kernel<F16, FP8, D, NT>;
-  static bool ready = false;                              // set once per process and kernel; setting it twice is harmless
-  if (!ready) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
-    if (e != cudaSuccess) return e;
-    ready = true;
-  }
+  static unsigned long long devices = 0;
+  cudaError_t e = allow_shared(kern, C::kSmem, devices);
+  if (e != cudaSuccess) return e;
   const int group = a.Hq / a.Hkv, tiles = (group + 8 * NT - 1) / (8 * NT);
   const int64_t units = most_units(static_cast<int64_t>(a.table_width) * a.page_size, a.window, a.sinks);
   const int64_t segs = static_cast<int64_t>(a.B) * a.Hkv * tiles;
@@ -649,7 +646,7 @@ cudaError_t run_paged_attention(const PagedAttnArgs& a, cudaStream_t st) {
     grid = static_cast<int>(segs * ((units + pattn::kMinUnits - 1) / pattn::kMinUnits));
   }
   kern<<<grid, pattn::kWarps * 32, C::kSmem, st>>>(a, tiles, whole ? 1 : 0);
-  cudaError_t e = cudaGetLastError();
+  e = cudaGetLastError();
   if (e != cudaSuccess || whole || grid == 1) return e;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];

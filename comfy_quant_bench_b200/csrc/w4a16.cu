@@ -23,7 +23,7 @@ constexpr int kRows = 16 * kRt;
 constexpr int kChunk = 128;                // columns of a ring stage
 constexpr int kStages = 3;
 constexpr int kWBytes = kRows * kChunk / 2;
-constexpr int kSBytes = 80;                // scales (or zeros) of a group's 32 rows, and room for a shift
+constexpr int kSBytes = 128;               // scales (or zeros) of a group's 32 rows, and room for a shift
 constexpr int kRedStride = kRows + 4;      // floats between tokens of a partial tile: no bank conflicts
 }  // namespace w4a16
 
@@ -37,43 +37,67 @@ __global__ void __launch_bounds__(w4a16::kWarps * 32, 1) w4a16_kernel(const W4A1
   const int n0 = blockIdx.x * kRows, m0 = blockIdx.y * tokens;
   const int mt = min(tokens, a.M - m0);                       // tokens of this tile
   const int stage_bytes = kXAt + tokens * 2 * kChunk;
-  const unsigned short* sp = reinterpret_cast<const unsigned short*>(a.s) + n0;
-  const unsigned short* zp = reinterpret_cast<const unsigned short*>(a.z) + n0;
   uint8_t* ring = smem + warp * kStages * stage_bytes;
   const uint32_t ring_u = smem_u32(ring);
   const int chunks = (a.K + kChunk - 1) / kChunk;
-  const int w_at = g * (kChunk / 2) + 4 * c, w_swz = g >> 1 & 3;   // rows g, g + 8, ... share their chunks' swizzle
 
-  auto issue = [&](int ch, int stage) {
-    if (ch < chunks) {
+  // What a lane copies into every stage, as addresses in the next chunk to copy.  Rows past the last are copies of it
+  // (nothing of them is stored); columns past the last are zeros, in the tokens too.
+  const int row_bytes = a.K >> 1;
+  const uint8_t* w_src[kRt * 2];                              // 16 bytes of rows g, g + 8, ...
+#pragma unroll
+  for (int i = 0; i < kRt * 2; ++i)
+    w_src[i] = a.b + static_cast<int64_t>(min(n0 + 8 * i + g, a.N - 1)) * row_bytes + warp * (kChunk / 2) + 16 * c;
+  const uint16_t* x_src = static_cast<const uint16_t*>(a.x) + (m0 + (lane >> 4)) * a.ldx + warp * kChunk + 8 * (lane & 15);
+  uintptr_t s_src = reinterpret_cast<uintptr_t>(a.s + static_cast<int64_t>(warp) * kGroups * a.N + n0);
+  uintptr_t z_src = reinterpret_cast<uintptr_t>(a.z + static_cast<int64_t>(warp) * kGroups * a.N + n0);
+  const int s_ends = 2 * min(kRows, a.N - n0) - 4 * lane;     // bytes of a group's scales from this lane's word on
+  const uint32_t w_dst = g * (kChunk / 2) + ((c ^ (g >> 1 & 3)) << 4);
+  const uint32_t x_dst = kXAt + (lane >> 4) * (2 * kChunk) + (((lane & 15) ^ ((lane >> 4) << 2)) << 4);
+  int left = a.K - warp * kChunk;                             // columns from the next chunk to copy on
+
+  // the aligned word of 16-bit values that this lane copies from `src` on; its bytes past the last value are not read
+  auto copy_halves = [&](uint32_t dst, uintptr_t src) {
+    const int bytes = min(4, s_ends + static_cast<int>(src & 2));
+    if (bytes > 0)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + 4 * lane),
+                   "l"((src & ~static_cast<uintptr_t>(3)) + 4 * lane), "r"(bytes) : "memory");
+  };
+  auto issue = [&](int stage) {
+    if (left > 0) {
       const uint32_t dst = ring_u + stage * stage_bytes;
+      const bool w_ok = left > 32 * c;
 #pragma unroll
       for (int i = 0; i < kRt * 2; ++i) {
-        const int r = 8 * i + (lane >> 2);
-        const bool ok = n0 + r < a.N && ch * kChunk + 32 * c < a.K;
-        const uint8_t* src = a.b + (ok ? static_cast<int64_t>(n0 + r) * (a.K >> 1) + ch * (kChunk / 2) + 16 * c : 0);
-        cp_async16(dst + r * (kChunk / 2) + ((c ^ (r >> 1 & 3)) << 4), src, ok);
+        cp_async16(dst + w_dst + i * (8 * kChunk / 2), w_ok ? w_src[i] : a.b, w_ok);
+        w_src[i] += kWarps * (kChunk / 2);
       }
 #pragma unroll
       for (int i = 0; i < kGroups; ++i) {
-        const int64_t at = static_cast<int64_t>(ch * kGroups + i) * a.N;
-        if ((ch * kGroups + i) * G < a.K) {
-          cp_async_halves(dst + kWBytes + 2 * i * kSBytes, sp + at, min(kRows, a.N - n0), lane);
-          cp_async_halves(dst + kWBytes + (2 * i + 1) * kSBytes, zp + at, min(kRows, a.N - n0), lane);
+        if (i == 0 || left > i * G) {
+          copy_halves(dst + kWBytes + 2 * i * kSBytes, s_src + i * 2 * static_cast<int64_t>(a.N));
+          copy_halves(dst + kWBytes + (2 * i + 1) * kSBytes, z_src + i * 2 * static_cast<int64_t>(a.N));
         }
       }
-      for (int t = lane >> 4; t < mt; t += 2) {
-        const int q = lane & 15;
-        const bool ok = ch * kChunk + 8 * q < a.K;
-        const uint16_t* src = static_cast<const uint16_t*>(a.x) + (ok ? (m0 + t) * a.ldx + ch * kChunk + 8 * q : 0);
-        cp_async16(dst + kXAt + t * (2 * kChunk) + ((q ^ ((t & 1) << 2)) << 4), src, ok);
-      }
+      const bool x_ok = left > 8 * (lane & 15);
+      for (int t = lane >> 4; t < mt; t += 2)
+        cp_async16(dst + x_dst + (t >> 1) * (4 * kChunk), x_ok ? x_src + (t >> 1) * 2 * a.ldx : a.x, x_ok);
+      x_src += kWarps * kChunk;
+      s_src += 2 * kWarps * kGroups * static_cast<int64_t>(a.N);
+      z_src += 2 * kWarps * kGroups * static_cast<int64_t>(a.N);
+      left -= kWarps * kChunk;
     }
     cp_async_commit();
   };
+
   float acc[kRt][NT][4] = {};
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) issue(warp + s * kWarps, s);
+  for (int s = 0; s < kStages - 1; ++s) issue(s);
+  // where the row's scale and zero lie in a group's words: at an odd half where the group's address is one
+  const int s_odd = half_shift(reinterpret_cast<const unsigned short*>(a.s) + n0);
+  const int z_odd = half_shift(reinterpret_cast<const unsigned short*>(a.z) + n0);
+  const int w_at = g * (kChunk / 2) + 4 * c, w_swz = g >> 1 & 3;   // rows g, g + 8, ... share their chunks' swizzle
+  const int x_at = kXAt + g * (2 * kChunk) + ((c ^ ((g & 1) << 2)) << 4);
   const uint32_t one = F16 ? 0x3C003C00u : 0x3F803F80u;
   const uint32_t ones[4] = {one, one, one, one};
   int stage = 0;
@@ -97,9 +121,8 @@ __global__ void __launch_bounds__(w4a16::kWarps * 32, 1) w4a16_kernel(const W4A1
       uint32_t xb[NT][4];                                     // token g's columns j and j + 4 as pairs
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const int t = 8 * n + g;
         uint4 v = make_uint4(0, 0, 0, 0);
-        if (t < mt) v = *reinterpret_cast<const uint4*>(st + kXAt + t * (2 * kChunk) + (((4 * b + c) ^ ((t & 1) << 2)) << 4));
+        if (8 * n + g < mt) v = *reinterpret_cast<const uint4*>(st + (x_at ^ (b << 6)) + n * (16 * kChunk));
         xb[n][0] = __byte_perm(v.x, v.z, 0x5410);
         xb[n][1] = __byte_perm(v.x, v.z, 0x7632);
         xb[n][2] = __byte_perm(v.y, v.w, 0x5410);
@@ -122,12 +145,11 @@ __global__ void __launch_bounds__(w4a16::kWarps * 32, 1) w4a16_kernel(const W4A1
       }
       if ((b + 1) % (G / 32) == 0) {                          // the group's end
         // scale and zero of row `lane`; past the last group there are none, and the tokens there are zeros
-        const int grp = ch * kGroups + b / (G / 32);
-        const int64_t at = static_cast<int64_t>(grp) * a.N;
+        const int grp = ch * kGroups + b / (G / 32), odd = grp & a.N & 1;
         uint32_t mine = 0;
-        if (grp * G < a.K) {
-          const unsigned short* sz = reinterpret_cast<const unsigned short*>(st + kWBytes + 2 * (b / (G / 32)) * kSBytes) + lane;
-          mine = sz[half_shift(sp + at)] | static_cast<uint32_t>(sz[kSBytes / 2 + half_shift(zp + at)]) << 16;
+        if (b / (G / 32) == 0 || grp * G < a.K) {
+          const unsigned short* sz = reinterpret_cast<const unsigned short*>(st + kWBytes + 2 * (b / (G / 32)) * kSBytes);
+          mine = sz[(s_odd ^ odd) + lane] | static_cast<uint32_t>(sz[kSBytes / 2 + (z_odd ^ odd) + lane]) << 16;
         }
 #pragma unroll
         for (int t = 0; t < kRt; ++t)
@@ -144,7 +166,7 @@ __global__ void __launch_bounds__(w4a16::kWarps * 32, 1) w4a16_kernel(const W4A1
       }
     }
     __syncwarp();
-    issue(ch + (kStages - 1) * kWarps, stage == 0 ? kStages - 1 : stage - 1);
+    issue(stage == 0 ? kStages - 1 : stage - 1);
     stage = stage + 1 == kStages ? 0 : stage + 1;
   }
   cp_async_wait<0>();
@@ -182,12 +204,9 @@ cudaError_t run_w4a16(const W4A16Args& a, cudaStream_t st) {
   const int ring = kWarps * kStages * (kWBytes + 2 * (kChunk / G) * kSBytes + tokens * 2 * kChunk), red = kWarps * 8 * NT * kRedStride * 4;
   const int smem = ring > red ? ring : red;
   constexpr int kMost = kWarps * kStages * (kWBytes + 2 * (kChunk / G) * kSBytes + 8 * NT * 2 * kChunk);
-  static bool ready = false;                                  // set once; setting it twice is harmless
-  if (!ready) {
-    const cudaError_t e = cudaFuncSetAttribute(w4a16_kernel<F16, G, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
-    if (e != cudaSuccess) return e;
-    ready = true;
-  }
+  static unsigned long long devices = 0;
+  const cudaError_t e = allow_shared(w4a16_kernel<F16, G, NT>, kMost, devices);
+  if (e != cudaSuccess) return e;
   const dim3 grid((a.N + kRows - 1) / kRows, (a.M + tokens - 1) / tokens);
   w4a16_kernel<F16, G, NT><<<grid, kWarps * 32, smem, st>>>(a, tokens);
   return cudaGetLastError();

@@ -462,12 +462,9 @@ template <bool F16, int G, int NTOK>
 cudaError_t run_w4a16_tc(const W4A16Args& a, void* ws, cudaStream_t st) {
   using P = w4tc::Plan<G, NTOK>;
   auto kern = w4a16_tc_kernel<F16, G, NTOK>;
-  static bool ready = false;                                  // set once; setting it twice is harmless
-  if (!ready) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, P::kSmem);
-    if (e != cudaSuccess) return e;
-    ready = true;
-  }
+  static unsigned long long devices = 0;
+  cudaError_t e = allow_shared(kern, P::kSmem, devices);
+  if (e != cudaSuccess) return e;
   const int tiles = (a.M + NTOK - 1) / NTOK, chunks = (a.K + w4tc::kChunk - 1) / w4tc::kChunk;
   const int groups = static_cast<int>(w4a16_groups_padded(a.K, G));
   uint4* xp = static_cast<uint4*>(ws);
@@ -478,7 +475,7 @@ cudaError_t run_w4a16_tc(const W4A16Args& a, void* ws, cudaStream_t st) {
       !w4a16_map(&tm_x, xp, a.M, static_cast<int64_t>(a.K) * 2, 128, NTOK, CU_TENSOR_MAP_SWIZZLE_128B))
     return cudaErrorInvalidValue;
   w4a16_tokens_kernel<F16><<<tiles * NTOK, 256, 0, st>>>(a.x, a.ldx, a.M, a.K, G, NTOK, groups, xp, r, factor);
-  cudaError_t e = cudaGetLastError();
+  e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   const int row_tiles = (a.N + w4tc::kRows - 1) / w4tc::kRows;
   // K split over a cluster while the grid leaves half of the resident CTAs (two per SM) idle and each still has four

@@ -16,7 +16,7 @@ import functools
 import torch
 
 from . import _lib
-from .ops import _cuda_index, _launch, _ptr
+from .ops import _cuda_index, _ptr, _raw_stream
 
 _DTYPES = {torch.bfloat16: _lib.CQ_DT_BF16, torch.float16: _lib.CQ_DT_F16, torch.float8_e4m3fn: _lib.CQ_DT_FP8_E4M3}
 _SITES = {101: "free", 102: "fork", 103: "reserve"}
@@ -90,6 +90,10 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     elif _i32(rows, 1, "rows").shape[0] != b:
         raise ValueError(f"rows must have {b} entries")
     idx = _cuda_index(q, k_cache, v_cache, block_table, seq_lens, rows, k_scale, v_scale, out)
+    if idx != torch.cuda.current_device():
+        with torch.cuda.device(idx):
+            return paged_attention(q, k_cache, v_cache, block_table, seq_lens, rows=rows, scale=scale, window=window,
+                                   sinks=sinks, k_scale=k_scale, v_scale=v_scale, out=out, return_lse=return_lse)
     ks, vs = _head_scale(k_scale, hk, ct, "k_scale"), _head_scale(v_scale, hk, ct, "v_scale")
     qb, qh, qd = q.stride()
     qp = q.data_ptr()
@@ -103,10 +107,13 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     lse = q.new_empty((b, hq), dtype=torch.float32) if return_lse else None
     nbytes = _attention_workspace(b, hq, hk, d, width * page, window, sinks)
     ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes > 0 else None
-    _launch("cq_paged_attention", idx, qp, qb, qh, _DTYPES[dt], b, hq, hk, d, k_cache.data_ptr(), v_cache.data_ptr(),
-            _DTYPES[ct], pages, page, sp, sh, st, block_table.data_ptr(), table_rows, width,
-            max(block_table.stride(0), width), _ptr(rows), seq_lens.data_ptr(),
-            d ** -0.5 if scale is None else scale, window, sinks, ks, vs, out.data_ptr(), _ptr(lse), _ptr(ws), nbytes)
+    status = _lib.load().cq_paged_attention(
+        qp, qb, qh, _DTYPES[dt], b, hq, hk, d, k_cache.data_ptr(), v_cache.data_ptr(), _DTYPES[ct], pages, page, sp, sh, st,
+        block_table.data_ptr(), table_rows, width, max(block_table.stride(0), width), _ptr(rows), seq_lens.data_ptr(),
+        d ** -0.5 if scale is None else scale, window, sinks, ks, vs, out.data_ptr(), _ptr(lse), _ptr(ws), nbytes,
+        _raw_stream(idx))
+    if status:
+        _lib.check("cq_paged_attention", status)
     return (out, lse) if return_lse else out
 
 
@@ -130,13 +137,19 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     if _i32(rows, 1, "rows").shape[0] != t or _i32(positions, 1, "positions").shape[0] != t:
         raise ValueError(f"rows and positions must have one entry per token ({t})")
     idx = _cuda_index(k, v, k_cache, v_cache, block_table, rows, positions, k_scale, v_scale)
+    if idx != torch.cuda.current_device():
+        with torch.cuda.device(idx):
+            return append_kv(k, v, k_cache, v_cache, block_table, rows, positions, k_scale=k_scale, v_scale=v_scale)
     ks, vs = _head_scale(k_scale, hk, k_cache.dtype, "k_scale"), _head_scale(v_scale, hk, k_cache.dtype, "v_scale")
     (kp, ksl, kst, ksh), (vp, vsl, vst, vsh) = _new_rows(k, k.dim()), _new_rows(v, k.dim())
     table_rows, width = block_table.shape
-    _launch("cq_kv_append", idx, kp.data_ptr(), ksl, kst, ksh, vp.data_ptr(), vsl, vst, vsh, _DTYPES[k.dtype], layers, t,
-            hk, d, k_cache.data_ptr(), v_cache.data_ptr(), _DTYPES[k_cache.dtype], shape[-4], shape[-2],
-            cs[0] if len(cs) == 5 else 0, cs[-4], cs[-3], cs[-2], block_table.data_ptr(), table_rows, width,
-            max(block_table.stride(0), width), rows.data_ptr(), positions.data_ptr(), ks, vs)
+    status = _lib.load().cq_kv_append(
+        kp.data_ptr(), ksl, kst, ksh, vp.data_ptr(), vsl, vst, vsh, _DTYPES[k.dtype], layers, t, hk, d,
+        k_cache.data_ptr(), v_cache.data_ptr(), _DTYPES[k_cache.dtype], shape[-4], shape[-2],
+        cs[0] if len(cs) == 5 else 0, cs[-4], cs[-3], cs[-2], block_table.data_ptr(), table_rows, width,
+        max(block_table.stride(0), width), rows.data_ptr(), positions.data_ptr(), ks, vs, _raw_stream(idx))
+    if status:
+        _lib.check("cq_kv_append", status)
 
 
 def _new_rows(x: torch.Tensor, dim: int):
@@ -184,6 +197,10 @@ def _update(block_table, seq_lens, ref_counts, page_size, free=None, src=None, d
     elif count < 0:
         raise ValueError("count must not be negative")
     idx = _cuda_index(block_table, seq_lens, ref_counts, free, src, dst, reserve, counts, k_cache, v_cache)
+    if idx != torch.cuda.current_device():
+        with torch.cuda.device(idx):
+            return _update(block_table, seq_lens, ref_counts, page_size, free, src, dst, reserve,
+                           count if counts is None else counts, k_cache, v_cache)
     pages = ref_counts.shape[0]
     layers = layer_bytes = page_bytes = n = nbytes = 0
     start = copies = ws = None
@@ -195,11 +212,13 @@ def _update(block_table, seq_lens, ref_counts, page_size, free=None, src=None, d
         nbytes = 4 * (2 * n + pages)
         ws = seq_lens.new_empty(2 * n + pages)
     rows, width = block_table.shape
-    _launch("cq_pages_update", idx, block_table.data_ptr(), rows, width, max(block_table.stride(0), width),
-              seq_lens.data_ptr(), ref_counts.data_ptr(), pages, int(page_size), _ptr(free),
-              0 if free is None else free.shape[0], _ptr(src), _ptr(dst), 0 if dst is None else dst.shape[0],
-              _ptr(reserve), n, _ptr(counts), int(count), _ptr(start), _ptr(copies), _ptr(k_cache), _ptr(v_cache),
-              layers, layer_bytes, page_bytes, _ptr(ws), nbytes)
+    status = _lib.load().cq_pages_update(
+        block_table.data_ptr(), rows, width, max(block_table.stride(0), width), seq_lens.data_ptr(),
+        ref_counts.data_ptr(), pages, page_size, _ptr(free), 0 if free is None else free.shape[0], _ptr(src), _ptr(dst),
+        0 if dst is None else dst.shape[0], _ptr(reserve), n, _ptr(counts), count, _ptr(start), _ptr(copies),
+        _ptr(k_cache), _ptr(v_cache), layers, layer_bytes, page_bytes, _ptr(ws), nbytes, _raw_stream(idx))
+    if status:
+        _lib.check("cq_pages_update", status)
     return start, copies
 
 
@@ -240,6 +259,9 @@ def compact_pages(block_table, ref_counts, k_cache, v_cache, *, out_table: torch
     _i32(block_table, 2, "block_table")
     _i32(ref_counts, 1, "ref_counts")
     idx = _cuda_index(block_table, ref_counts, k_cache, v_cache, out_table, out_refs)
+    if idx != torch.cuda.current_device():
+        with torch.cuda.device(idx):
+            return compact_pages(block_table, ref_counts, k_cache, v_cache, out_table=out_table, out_refs=out_refs)
     pages = ref_counts.shape[0]
     layers, layer_bytes, page_bytes = _page_layout(k_cache, v_cache, pages)
     rows, width = block_table.shape
@@ -253,10 +275,13 @@ def compact_pages(block_table, ref_counts, k_cache, v_cache, *, out_table: torch
         raise ValueError("out_refs must have the shape of ref_counts")
     moves = ref_counts.new_empty((pages // 2, 2))
     ws = ref_counts.new_empty(pages)
-    _launch("cq_pages_compact", idx, block_table.data_ptr(), rows, width, max(block_table.stride(0), width),
-              out_table.data_ptr(), max(out_table.stride(0), width), ref_counts.data_ptr(), out_refs.data_ptr(), pages,
-              moves.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), layers, layer_bytes, page_bytes,
-              ws.data_ptr(), 4 * pages)
+    status = _lib.load().cq_pages_compact(
+        block_table.data_ptr(), rows, width, max(block_table.stride(0), width), out_table.data_ptr(),
+        max(out_table.stride(0), width), ref_counts.data_ptr(), out_refs.data_ptr(), pages, moves.data_ptr(),
+        k_cache.data_ptr(), v_cache.data_ptr(), layers, layer_bytes, page_bytes, ws.data_ptr(), 4 * pages,
+        _raw_stream(idx))
+    if status:
+        _lib.check("cq_pages_compact", status)
     return out_table, out_refs, moves
 
 
