@@ -60,6 +60,16 @@ inline cudaError_t allow_shared(Kernel kernel, int bytes, unsigned long long& de
   return e;
 }
 
+// (a.x, a.y) * (b.x, b.y) + (c.x, c.y) in one instruction, each rounded once
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)),
+        "l"(reinterpret_cast<const uint64_t&>(c)));
+  return d;
+}
+
 // (v & mask) | bits in one instruction
 __device__ __forceinline__ uint32_t and_or(uint32_t v, uint32_t mask, uint32_t bits) {
   uint32_t d;

@@ -18,25 +18,36 @@ namespace cq {
 
 namespace w4a16 {
 constexpr int kWarps = 8;
-constexpr int kRt = 2;                     // 16-row tiles of a CTA
-constexpr int kRows = 16 * kRt;
 constexpr int kChunk = 128;                // columns of a ring stage
-constexpr int kStages = 3;
-constexpr int kWBytes = kRows * kChunk / 2;
-constexpr int kSBytes = 128;               // scales (or zeros) of a group's 32 rows, and room for a shift
-constexpr int kRedStride = kRows + 4;      // floats between tokens of a partial tile: no bank conflicts
+
+// a CTA of RT tiles of 16 weight rows, eight tokens and a ring of S chunks per warp
+template <int G, int RT, int S>
+struct Plan {
+  static constexpr int kRows = 16 * RT;
+  static constexpr int kWBytes = kRows * kChunk / 2;
+  static constexpr int kGroups = kChunk / G;             // scale groups of a chunk
+  static constexpr int kSBytes = RT <= 2 ? 128 : 256;    // scales (or zeros) of a group's rows, and room for a shift
+  static constexpr int kXAt = kWBytes + 2 * kGroups * kSBytes;
+  static constexpr int kRedStride = kRows + 4;           // floats between tokens of a partial tile: no bank conflicts
+  static constexpr int stage(int tokens) { return kXAt + tokens * 2 * kChunk; }
+  static constexpr int shared(int tokens) {
+    const int ring = kWarps * S * stage(tokens), red = kWarps * 8 * kRedStride * 4;
+    return ring > red ? ring : red;
+  }
+};
 }  // namespace w4a16
 
-template <bool F16, int G, int NT>
+template <bool F16, int G, int RT, int S>
 __global__ void __launch_bounds__(w4a16::kWarps * 32, 1) w4a16_kernel(const W4A16Args a, const int tokens) {
   using namespace w4a16;
-  constexpr int kGroups = kChunk / G;      // scale groups of a chunk
-  constexpr int kXAt = kWBytes + 2 * kGroups * kSBytes;
+  using P = Plan<G, RT, S>;
+  constexpr int kRt = RT, kRows = P::kRows, kStages = S, kWBytes = P::kWBytes, kGroups = P::kGroups, kSBytes = P::kSBytes;
+  constexpr int kXAt = P::kXAt, kRedStride = P::kRedStride;
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int n0 = blockIdx.x * kRows, m0 = blockIdx.y * tokens;
   const int mt = min(tokens, a.M - m0);                       // tokens of this tile
-  const int stage_bytes = kXAt + tokens * 2 * kChunk;
+  const int stage_bytes = P::stage(tokens);
   uint8_t* ring = smem + warp * kStages * stage_bytes;
   const uint32_t ring_u = smem_u32(ring);
   const int chunks = (a.K + kChunk - 1) / kChunk;
@@ -56,12 +67,15 @@ __global__ void __launch_bounds__(w4a16::kWarps * 32, 1) w4a16_kernel(const W4A1
   const uint32_t x_dst = kXAt + (lane >> 4) * (2 * kChunk) + (((lane & 15) ^ ((lane >> 4) << 2)) << 4);
   int left = a.K - warp * kChunk;                             // columns from the next chunk to copy on
 
-  // the aligned word of 16-bit values that this lane copies from `src` on; its bytes past the last value are not read
+  // the aligned words of 16-bit values that this lane copies from `src` on; bytes past the last value are not read
   auto copy_halves = [&](uint32_t dst, uintptr_t src) {
-    const int bytes = min(4, s_ends + static_cast<int>(src & 2));
-    if (bytes > 0)
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + 4 * lane),
-                   "l"((src & ~static_cast<uintptr_t>(3)) + 4 * lane), "r"(bytes) : "memory");
+#pragma unroll
+    for (int q = 0; q <= kRows / 2; q += 32) {
+      const int bytes = min(4, s_ends - 4 * q + static_cast<int>(src & 2));
+      if (bytes > 0)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + 4 * (lane + q)),
+                     "l"((src & ~static_cast<uintptr_t>(3)) + 4 * (lane + q)), "r"(bytes) : "memory");
+    }
   };
   auto issue = [&](int stage) {
     if (left > 0) {
@@ -90,7 +104,7 @@ __global__ void __launch_bounds__(w4a16::kWarps * 32, 1) w4a16_kernel(const W4A1
     cp_async_commit();
   };
 
-  float acc[kRt][NT][4] = {};
+  float acc[kRt][4] = {};
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) issue(s);
   // where the row's scale and zero lie in a group's words: at an odd half where the group's address is one
@@ -105,31 +119,24 @@ __global__ void __launch_bounds__(w4a16::kWarps * 32, 1) w4a16_kernel(const W4A1
     cp_async_wait<kStages - 2>();
     __syncwarp();
     const uint8_t* st = ring + stage * stage_bytes;
-    float p[kRt][NT][4], r[NT][4];
+    float p[kRt][4], r[4];
 #pragma unroll
     for (int b = 0; b < 4; ++b) {                             // blocks of 32 columns: lane c holds columns 8c .. 8c + 7
       if (b % (G / 32) == 0) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int j = 0; j < 4; ++j) {
+          r[j] = 0.0f;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            r[n][j] = 0.0f;
-#pragma unroll
-            for (int t = 0; t < kRt; ++t) p[t][n][j] = 0.0f;
-          }
+          for (int t = 0; t < kRt; ++t) p[t][j] = 0.0f;
+        }
       }
-      uint32_t xb[NT][4];                                     // token g's columns j and j + 4 as pairs
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (8 * n + g < mt) v = *reinterpret_cast<const uint4*>(st + (x_at ^ (b << 6)) + n * (16 * kChunk));
-        xb[n][0] = __byte_perm(v.x, v.z, 0x5410);
-        xb[n][1] = __byte_perm(v.x, v.z, 0x7632);
-        xb[n][2] = __byte_perm(v.y, v.w, 0x5410);
-        xb[n][3] = __byte_perm(v.y, v.w, 0x7632);
-        mma_16816<F16>(r[n], ones, xb[n][0], xb[n][1]);
-        mma_16816<F16>(r[n], ones, xb[n][2], xb[n][3]);
-      }
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (g < mt) v = *reinterpret_cast<const uint4*>(st + (x_at ^ (b << 6)));
+      // token g's columns j and j + 4 as pairs
+      const uint32_t xb[4] = {__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
+                              __byte_perm(v.y, v.w, 0x7632)};
+      mma_16816<F16>(r, ones, xb[0], xb[1]);
+      mma_16816<F16>(r, ones, xb[2], xb[3]);
       const uint8_t* wrow = st + w_at + ((b ^ w_swz) << 4);
 #pragma unroll
       for (int t = 0; t < kRt; ++t) {
@@ -139,29 +146,27 @@ __global__ void __launch_bounds__(w4a16::kWarps * 32, 1) w4a16_kernel(const W4A1
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t wa[4] = {p0[2 * h], p1[2 * h], p0[2 * h + 1], p1[2 * h + 1]};
-#pragma unroll
-          for (int n = 0; n < NT; ++n) mma_16816<F16>(p[t][n], wa, xb[n][2 * h], xb[n][2 * h + 1]);
+          mma_16816<F16>(p[t], wa, xb[2 * h], xb[2 * h + 1]);
         }
       }
       if ((b + 1) % (G / 32) == 0) {                          // the group's end
-        // scale and zero of row `lane`; past the last group there are none, and the tokens there are zeros
-        const int grp = ch * kGroups + b / (G / 32), odd = grp & a.N & 1;
-        uint32_t mine = 0;
-        if (b / (G / 32) == 0 || grp * G < a.K) {
-          const unsigned short* sz = reinterpret_cast<const unsigned short*>(st + kWBytes + 2 * (b / (G / 32)) * kSBytes);
-          mine = sz[(s_odd ^ odd) + lane] | static_cast<uint32_t>(sz[kSBytes / 2 + (z_odd ^ odd) + lane]) << 16;
+        // scales and zeros of rows lane, lane + 32, ...; past the last group there are none, and the tokens are zeros
+        const int i = b / (G / 32), odd = (ch * kGroups + i) & a.N & 1;
+        uint32_t mine[(kRows + 31) / 32] = {};
+        if (i == 0 || (ch * kGroups + i) * G < a.K) {
+          const unsigned short* sz = reinterpret_cast<const unsigned short*>(st + kWBytes + 2 * i * kSBytes) + lane;
+#pragma unroll
+          for (int q = 0; q < (kRows + 31) / 32; ++q)
+            mine[q] = sz[(s_odd ^ odd) + 32 * q] | static_cast<uint32_t>(sz[kSBytes / 2 + (z_odd ^ odd) + 32 * q]) << 16;
         }
 #pragma unroll
         for (int t = 0; t < kRt; ++t)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint32_t v = __shfl_sync(0xffffffffu, mine, 16 * t + 8 * h + g);
-            const float s = __uint_as_float(v << 16), z = fmaf(-widen_offset<F16>(), s, __uint_as_float(v & 0xffff0000u));
+            const uint32_t u = __shfl_sync(0xffffffffu, mine[t / 2], 16 * (t & 1) + 8 * h + g);
+            const float s = __uint_as_float(u << 16), z = fmaf(-widen_offset<F16>(), s, __uint_as_float(u & 0xffff0000u));
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int j = 0; j < 2; ++j)
-                acc[t][n][2 * h + j] = fmaf(s, p[t][n][2 * h + j], fmaf(z, r[n][j], acc[t][n][2 * h + j]));
+            for (int j = 0; j < 2; ++j) acc[t][2 * h + j] = fmaf(s, p[t][2 * h + j], fmaf(z, r[j], acc[t][2 * h + j]));
           }
       }
     }
@@ -175,17 +180,15 @@ __global__ void __launch_bounds__(w4a16::kWarps * 32, 1) w4a16_kernel(const W4A1
 #pragma unroll
   for (int t = 0; t < kRt; ++t)
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        red[(warp * 8 * NT + 8 * n + 2 * c + (j & 1)) * kRedStride + 16 * t + g + 8 * (j >> 1)] = acc[t][n][j];
+    for (int j = 0; j < 4; ++j)
+      red[(warp * 8 + 2 * c + (j & 1)) * kRedStride + 16 * t + g + 8 * (j >> 1)] = acc[t][j];
   __syncthreads();
   for (int i = threadIdx.x; i < mt * kRows; i += kWarps * 32) {
     const int m = i / kRows, r = i - m * kRows, n = n0 + r;
     if (n >= a.N) continue;
     float y = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) y += red[(w * 8 * NT + m) * kRedStride + r];
+    for (int w = 0; w < kWarps; ++w) y += red[(w * 8 + m) * kRedStride + r];
     const int64_t at = static_cast<int64_t>(m0 + m) * a.N + n;
     if constexpr (F16) {
       if (a.bias != nullptr) y += __half2float(static_cast<const __half*>(a.bias)[n]);
@@ -197,28 +200,30 @@ __global__ void __launch_bounds__(w4a16::kWarps * 32, 1) w4a16_kernel(const W4A1
   }
 }
 
-template <bool F16, int G, int NT>
+template <bool F16, int G, int RT, int S>
 cudaError_t run_w4a16(const W4A16Args& a, cudaStream_t st) {
-  using namespace w4a16;
-  const int tokens = a.M < 8 * NT ? a.M : 8 * NT;
-  const int ring = kWarps * kStages * (kWBytes + 2 * (kChunk / G) * kSBytes + tokens * 2 * kChunk), red = kWarps * 8 * NT * kRedStride * 4;
-  const int smem = ring > red ? ring : red;
-  constexpr int kMost = kWarps * kStages * (kWBytes + 2 * (kChunk / G) * kSBytes + 8 * NT * 2 * kChunk);
+  using P = w4a16::Plan<G, RT, S>;
   static unsigned long long devices = 0;
-  const cudaError_t e = allow_shared(w4a16_kernel<F16, G, NT>, kMost, devices);
+  const cudaError_t e = allow_shared(w4a16_kernel<F16, G, RT, S>, P::shared(8), devices);
   if (e != cudaSuccess) return e;
-  const dim3 grid((a.N + kRows - 1) / kRows, (a.M + tokens - 1) / tokens);
-  w4a16_kernel<F16, G, NT><<<grid, kWarps * 32, smem, st>>>(a, tokens);
+  const int tokens = a.M < 8 ? a.M : 8;
+  w4a16_kernel<F16, G, RT, S><<<dim3((a.N + P::kRows - 1) / P::kRows, (a.M + tokens - 1) / tokens), w4a16::kWarps * 32,
+                                P::shared(tokens), st>>>(a, tokens);
   return cudaGetLastError();
 }
 
-// Up to eight tokens one tile of this kernel holds them all; beyond, w4a16_tc.cu.
+template <bool F16, int G>
+cudaError_t pick_w4a16(const W4A16Args& a, cudaStream_t st) {
+  return run_w4a16<F16, G, 2, 3>(a, st);
+}
+
+// Up to eight tokens one tile of this kernel holds them all; beyond, w4a16_mid.cu.
 cudaError_t launch_w4a16(const W4A16Args& a, void* ws, cudaStream_t st) {
-  if (w4a16_uses_tc(a.M)) return launch_w4a16_tc(a, ws, st);
+  if (w4a16_shares_tokens(a.M)) return launch_w4a16_mid(a, ws, st);
   switch (a.group) {
-    case 32: return a.f16 ? run_w4a16<true, 32, 1>(a, st) : run_w4a16<false, 32, 1>(a, st);
-    case 64: return a.f16 ? run_w4a16<true, 64, 1>(a, st) : run_w4a16<false, 64, 1>(a, st);
-    default: return a.f16 ? run_w4a16<true, 128, 1>(a, st) : run_w4a16<false, 128, 1>(a, st);
+    case 32: return a.f16 ? pick_w4a16<true, 32>(a, st) : pick_w4a16<false, 32>(a, st);
+    case 64: return a.f16 ? pick_w4a16<true, 64>(a, st) : pick_w4a16<false, 64>(a, st);
+    default: return a.f16 ? pick_w4a16<true, 128>(a, st) : pick_w4a16<false, 128>(a, st);
   }
 }
 
