@@ -16,7 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 SRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libcq_b200.so")
-SOURCES = ["libcq.cu", "rotquant.cu", "gemm_sm100.cu", "gemm_pair.cu", "gemv.cu", "dit.cu", "w4a16.cu", "w4a16_mid.cu", "paged_attention.cu",
+SOURCES = ["libcq.cu", "rotquant.cu", "gemm_sm100.cu", "gemm_pair.cu", "gemv.cu", "dit.cu", "w4a16.cu", "w4a16_tokens.cu", "w4a16_mid.cu", "w4a16_tc.cu", "paged_attention.cu",
            "kvpages.cu", "selftest.cu", "capi.cu", "capi_decode.cu", "noalloc.cu", "kernels.cuh", "decode_common.cuh",
            "cq_common.cuh"]
 HEADER = os.path.join(ROOT, "include", "cq_b200.h")

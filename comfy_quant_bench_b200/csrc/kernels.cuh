@@ -140,9 +140,7 @@ struct W4A16Args {
   int M, N, K, group, f16;
 };
 int64_t w4a16_workspace(int M, int K, int G);
-bool w4a16_shares_tokens(int M);
 cudaError_t launch_w4a16(const W4A16Args& a, void* ws, cudaStream_t st);
-cudaError_t launch_w4a16_mid(const W4A16Args& a, void* ws, cudaStream_t st);
 
 // attention of one new token per sequence over a paged cache
 struct PagedAttnArgs {

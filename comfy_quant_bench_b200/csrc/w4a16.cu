@@ -217,9 +217,24 @@ cudaError_t pick_w4a16(const W4A16Args& a, cudaStream_t st) {
   return run_w4a16<F16, G, 2, 3>(a, st);
 }
 
-// Up to eight tokens one tile of this kernel holds them all; beyond, w4a16_mid.cu.
+template <bool F16, int G>
+cudaError_t pick_w4a16_shared(const W4A16Args& a, const W4Tokens& t, cudaStream_t st) {
+  if (w4a16_tensor_memory(a.M)) return run_w4a16_tc<F16, G, 64>(a, t, st);
+  return w4a16_tile(a.M) == 16 ? run_w4a16_mid<F16, G, 2>(a, t, st) : run_w4a16_mid<F16, G, 4>(a, t, st);
+}
+
+// Up to eight tokens this file's kernel; beyond, the forms that share the tokens between rows.
 cudaError_t launch_w4a16(const W4A16Args& a, void* ws, cudaStream_t st) {
-  if (w4a16_shares_tokens(a.M)) return launch_w4a16_mid(a, ws, st);
+  if (w4a16_shares_tokens(a.M)) {
+    W4Tokens t;
+    const cudaError_t e = launch_w4a16_tokens(a, ws, t, st);
+    if (e != cudaSuccess) return e;
+    switch (a.group) {
+      case 32: return a.f16 ? pick_w4a16_shared<true, 32>(a, t, st) : pick_w4a16_shared<false, 32>(a, t, st);
+      case 64: return a.f16 ? pick_w4a16_shared<true, 64>(a, t, st) : pick_w4a16_shared<false, 64>(a, t, st);
+      default: return a.f16 ? pick_w4a16_shared<true, 128>(a, t, st) : pick_w4a16_shared<false, 128>(a, t, st);
+    }
+  }
   switch (a.group) {
     case 32: return a.f16 ? pick_w4a16<true, 32>(a, st) : pick_w4a16<false, 32>(a, st);
     case 64: return a.f16 ? pick_w4a16<true, 64>(a, st) : pick_w4a16<false, 64>(a, st);

@@ -11,11 +11,8 @@
 // tensor or shared memory and each group's P read back: measured in that form (codes widened into tensor memory, roles
 // meeting at mbarriers) 64 tokens at 8192 x 28672 took 110 us, bound by that traffic and the hand-overs.
 //
-// Codes are widened in pairs (j, j + 4) of a word, so a small kernel first writes the tokens with each eight columns in
-// the order 0, 4, 1, 5, 2, 6, 3, 7 and sums the groups (R).  bf16 tokens become f16 there, each token divided by the
-// power of two that brings its largest element to [2^13, 2^14), which f16 holds exactly down to 2^-28 of that element
-// and to 2^-38 of it below; the sums are multiplied by it again at the end.  The product is launched as its programmatic
-// dependent: its weights are on their way while the tokens are written.
+// The tokens come from w4a16_tokens.cu, as f16 in the order the codes are widened in, with R.  The product is launched as
+// its programmatic dependent: its weights are on their way while the tokens are written.
 //
 // With few row tiles a cluster of CTAs splits K and adds its partial sums over distributed shared memory in rank order.
 #include "decode_common.cuh"
@@ -58,62 +55,6 @@ struct Args {
   int M, N, K, ksplit;
 };
 }  // namespace w4mid
-
-// One token per CTA: f16 columns in the order 0, 4, 1, 5, 2, 6, 3, 7 of each eight, their sums over the scale groups,
-// and the power of two a bf16 token was divided by.  Tokens past the last one get sums of zero.
-template <bool F16>
-__global__ void __launch_bounds__(256) w4a16_tokens_kernel(const void* x, int64_t ldx, int M, int K, int G, int ntok,
-                                                           int groups_padded, uint4* xp, float* r, float* factor) {
-  __shared__ float tops[8];
-  grid_dep_launch();
-  const int m = blockIdx.x, per = G / 8;                      // lanes of a group: 4, 8 or 16
-  const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + m * ldx);
-  float down = 1.0f;
-  if constexpr (!F16) {
-    float top = 0.0f;
-    if (m < M)
-      for (int c = threadIdx.x; c < K / 8; c += 256) {
-        const uint4 v = src[c];
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[j] << 16)), fabsf(__uint_as_float(w[j] & 0xffff0000u))));
-      }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = fmaxf(top, tops[i]);
-    // both powers are normal numbers; a token with an infinity keeps its values and overflows
-    const int ex = static_cast<int>(__float_as_uint(top) >> 23) - 127;
-    const int by = top > 0.0f && ex < 128 ? min(max(ex - 13, -100), 114) : 0;
-    down = __uint_as_float(static_cast<uint32_t>(127 - by) << 23);
-    if (m < M && threadIdx.x == 0) factor[m] = __uint_as_float(static_cast<uint32_t>(127 + by) << 23);
-  }
-  for (int c0 = 0; c0 < K / 8; c0 += 256) {
-    const int c = c0 + threadIdx.x;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (m < M && c < K / 8) v = src[c];
-    uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    float sum = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (!F16) {
-        const __half2 h = __floats2half2_rn(__uint_as_float(w[j] << 16) * down, __uint_as_float(w[j] & 0xffff0000u) * down);
-        w[j] = *reinterpret_cast<const uint32_t*>(&h);
-      }
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-      sum += f.x;
-      sum += f.y;
-    }
-    if (m < M && c < K / 8)
-      xp[static_cast<int64_t>(m) * (K / 8) + c] = make_uint4(__byte_perm(w[0], w[2], 0x5410), __byte_perm(w[0], w[2], 0x7632),
-                                                             __byte_perm(w[1], w[3], 0x5410), __byte_perm(w[1], w[3], 0x7632));
-    for (int o = per / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (c < K / 8 && c % per == 0) r[(static_cast<int64_t>(m / ntok) * groups_padded + c / per) * ntok + m % ntok] = sum;
-  }
-}
 
 template <bool F16, int G, int NT>
 __global__ void __launch_bounds__(w4mid::kThreads, (w4mid::Plan<G, NT>::kCtas)) w4a16_mid_kernel(const w4mid::Args a) {
@@ -283,41 +224,19 @@ __global__ void __launch_bounds__(w4mid::kThreads, (w4mid::Plan<G, NT>::kCtas)) 
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-namespace {
-int w4a16_tile(int M) { return M <= 16 ? 16 : M <= 32 ? 32 : 64; }
-int64_t w4a16_groups_padded(int K, int G) { return static_cast<int64_t>((K + 127) / 128) * (128 / G); }
-}  // namespace
-
-bool w4a16_shares_tokens(int M) { return M > 8; }
-
-int64_t w4a16_workspace(int M, int K, int G) {
-  if (!w4a16_shares_tokens(M)) return 0;
-  const int tile = w4a16_tile(M);
-  const int64_t tokens = (static_cast<int64_t>(M) * K * 2 + 255) / 256 * 256;
-  return tokens + static_cast<int64_t>((M + tile - 1) / tile) * tile * (w4a16_groups_padded(K, G) + 1) * 4;
-}
-
 template <bool F16, int G, int NT>
-cudaError_t run_w4a16_mid(const W4A16Args& a, void* ws, cudaStream_t st) {
+cudaError_t run_w4a16_mid(const W4A16Args& a, const W4Tokens& t, cudaStream_t st) {
   using P = w4mid::Plan<G, NT>;
   auto kern = w4a16_mid_kernel<F16, G, NT>;
   static unsigned long long devices = 0;
-  cudaError_t e = allow_shared(kern, P::kSmem, devices);
+  const cudaError_t e = allow_shared(kern, P::kSmem, devices);
   if (e != cudaSuccess) return e;
   const int tiles = (a.M + P::kTokens - 1) / P::kTokens, chunks = (a.K + w4mid::kChunk - 1) / w4mid::kChunk;
-  const int groups = static_cast<int>(w4a16_groups_padded(a.K, G));
-  uint16_t* xp = static_cast<uint16_t*>(ws);
-  float* r = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + (static_cast<int64_t>(a.M) * a.K * 2 + 255) / 256 * 256);
-  float* factor = r + static_cast<int64_t>(tiles) * P::kTokens * groups;
-  w4a16_tokens_kernel<F16><<<tiles * P::kTokens, 256, 0, st>>>(a.x, a.ldx, a.M, a.K, G, P::kTokens, groups,
-                                                              reinterpret_cast<uint4*>(xp), r, factor);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
   const int row_tiles = (a.N + w4mid::kRows - 1) / w4mid::kRows;
   // K split over a cluster while that leaves no resident CTA without work and each has four chunks
   int ksplit = 1;
   while (ksplit < 8 && row_tiles * tiles * ksplit * 2 <= P::kCtas * num_sms() && chunks / (2 * ksplit) >= 4) ksplit *= 2;
-  const w4mid::Args args{a.b, xp, a.s, a.z, factor, r, a.bias, a.out, a.M, a.N, a.K, ksplit};
+  const w4mid::Args args{a.b, t.x, a.s, a.z, t.factor, t.r, a.bias, a.out, a.M, a.N, a.K, ksplit};
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -333,23 +252,6 @@ cudaError_t run_w4a16_mid(const W4A16Args& a, void* ws, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, kern, args);
-}
-
-template <bool F16, int G>
-cudaError_t pick_w4a16_mid(const W4A16Args& a, void* ws, cudaStream_t st) {
-  switch (w4a16_tile(a.M)) {
-    case 16: return run_w4a16_mid<F16, G, 2>(a, ws, st);
-    case 32: return run_w4a16_mid<F16, G, 4>(a, ws, st);
-    default: return run_w4a16_mid<F16, G, 8>(a, ws, st);
-  }
-}
-
-cudaError_t launch_w4a16_mid(const W4A16Args& a, void* ws, cudaStream_t st) {
-  switch (a.group) {
-    case 32: return a.f16 ? pick_w4a16_mid<true, 32>(a, ws, st) : pick_w4a16_mid<false, 32>(a, ws, st);
-    case 64: return a.f16 ? pick_w4a16_mid<true, 64>(a, ws, st) : pick_w4a16_mid<false, 64>(a, ws, st);
-    default: return a.f16 ? pick_w4a16_mid<true, 128>(a, ws, st) : pick_w4a16_mid<false, 128>(a, ws, st);
-  }
 }
 
 }  // namespace cq

@@ -1,0 +1,486 @@
+// W4A16 linear for more than a few tokens: the product of w4a16.cu on tcgen05 tensor cores.
+//
+// A CTA owns 128 weight rows and up to 64 tokens.  Thread r of four widening warps is weight row r = TMEM lane r: it
+// takes its packed codes from shared memory, forms q - 8 as f16 in registers (nine instructions per eight codes) and
+// stores them straight into the A operand in tensor memory, so the widened weights never pass through shared
+// memory.  The tokens are the B operand, in K-major 128-byte-swizzled tiles.  Each scale group is one accumulation
+// P = sum x (q - 8) in TMEM; four adding warps per 32 tokens read it back and add s P + z R to their fp32 sums, with R = sum x per group and token.  A and P are double buffered, and the roles only meet at mbarriers: a
+// group's latency (copy, widening, product, read-back) is several times its work, so the roles run ahead of one
+// another instead of taking turns.
+//
+// Codes are widened in pairs (j, j + 4) of a word, so a small kernel first writes the tokens with each eight columns in
+// the order 0, 4, 1, 5, 2, 6, 3, 7 and sums the groups (R).  The product is launched as its programmatic dependent: its
+// weights are on their way while the tokens are written.
+//
+// With few row tiles a cluster of CTAs splits K and adds its partial sums over distributed shared memory in rank order.
+#include "decode_common.cuh"
+
+namespace cq {
+
+namespace w4tc {
+constexpr int kRows = 128;
+constexpr int kChunk = 128;                    // columns of a ring stage
+constexpr int kAheadWarps = 4;                 // widening warps, one per TMEM lane quadrant
+constexpr int kWBytes = kRows * kChunk / 2;
+constexpr int kSite = 120;                     // device status sites of the waits
+
+template <int G, int NTOK>
+struct Plan {
+  static constexpr int kXBytes = NTOK * kChunk * 2;
+  static constexpr int kScaleBytes = 272;                      // 128 scales of a group, and room for a shift
+  static constexpr int kStageBytes = (kWBytes + kXBytes + kChunk / G * kScaleBytes + 1023) / 1024 * 1024;
+  static constexpr int kStages = 100 * 1024 / kStageBytes < 8 ? 100 * 1024 / kStageBytes : 8;
+  static constexpr int kSmem = kStages * kStageBytes + 1024 + 256;      // alignment, barriers
+  static constexpr int kSums = NTOK < 32 ? NTOK : 32;          // tokens of an adding warp
+  static constexpr int kAddWarps = 4 * (NTOK / kSums);
+  static constexpr int kThreads = 32 * (kAheadWarps + kAddWarps + 2);   // and the copying and the multiplying warp
+  static_assert(kRows * NTOK * 4 <= kStages * kStageBytes, "partial sums fit the ring");
+};
+
+struct Args {
+  const __nv_bfloat16* s;
+  const __nv_bfloat16* z;
+  const float* factor;         // [M] what a bf16 token was divided by
+  const void* bias;
+  void* out;
+  int M, N, K, ksplit;
+};
+}  // namespace w4tc
+
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// 32 lanes x 16 columns; the registers hold them after the wait, which names them so that no read moves before it
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld_x16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               : : "memory");
+}
+// D(tmem) (+)= A(tmem, 16-bit pairs per column) * B(smem desc), fp32 accumulation
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// mbar_wait for roles that hand over every few hundred cycles: the plain hardware wait (the form with a time limit is
+// built from sleeps of about a microsecond), then, out of line, the one that reads the clock
+__device__ __noinline__ bool mbar_wait_long(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int where) {
+  return mbar_wait(bar, parity, abort_flag, where);
+}
+__device__ __forceinline__ bool mbar_wait_short(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int where) {
+  for (int i = 0; i < 1000; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    if (ok) return true;
+  }
+  return mbar_wait_long(bar, parity, abort_flag, where);
+}
+
+template <bool F16, int G, int NTOK>
+__global__ void __launch_bounds__(w4tc::Plan<G, NTOK>::kThreads, 2)
+    w4a16_tc_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
+                    const __grid_constant__ CUtensorMap tm_r, const w4tc::Args a) {
+  using namespace w4tc;
+  using P = Plan<G, NTOK>;
+  constexpr int kStages = P::kStages, kSteps = kChunk / G, kSums = P::kSums;
+  constexpr int kCopyWarp = kAheadWarps + P::kAddWarps, kMmaWarp = kCopyWarp + 1;
+  constexpr uint32_t kCols = 256;                             // TMEM: two P of NTOK columns, A's buffers in the rest
+  static_assert(2 * NTOK + 128 <= kCols, "two 128-column A operands");
+  extern __shared__ __align__(128) uint8_t smem_any[];
+  uint8_t* smem = smem_any + ((1024 - (smem_u32(smem_any) & 1023)) & 1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * P::kStageBytes);
+  uint64_t* empty = full + kStages;
+  uint64_t* a_full = empty + kStages;                         // [2] an operand's codes (or zeros) are in TMEM
+  uint64_t* p_full = a_full + 2;                              // [2] a product is done: P to be read, A free
+  uint64_t* p_empty = p_full + 2;                             // [2] P is read
+  uint64_t* z_done = p_empty + 2;                             // [2] A's buffer of the zeros' product is free
+  uint32_t* holder = reinterpret_cast<uint32_t*>(z_done + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(holder + 1);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = a.ksplit > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int n0 = blockIdx.x * kRows, m0 = blockIdx.y * NTOK;
+  const int chunks = (a.K + kChunk - 1) / kChunk;
+  const int c0 = rank * chunks / a.ksplit, c1 = (rank + 1) * chunks / a.ksplit;
+  const int steps = min(c1 * kSteps, a.K / G) - c0 * kSteps;  // groups of this CTA
+  // the zeros' term sum_g z R: products of 32 groups each, this rank's share of them; they come before the groups'
+  const int blocks = (a.K / G + 31) / 32, z0 = rank * blocks / a.ksplit, z1 = (rank + 1) * blocks / a.ksplit;
+  const int nz = z1 - z0;
+
+  if (tid == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 1 + 32);                            // the bulk copies, and each lane's scales
+      mbar_init(&empty[s], kAheadWarps + P::kAddWarps + 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&a_full[b], kAheadWarps);
+      mbar_init(&p_full[b], 1);
+      mbar_init(&p_empty[b], P::kAddWarps);
+      mbar_init(&z_done[b], 1);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(holder, kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t d_col = *holder, a_col = d_col + 2 * NTOK;
+  const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;    // the warp's quadrant of TMEM lanes
+  const int row = (warp & 3) * 32 + lane, n = n0 + row;       // this thread's weight row (widening and adding warps)
+  float2 acc[kSums / 2];
+#pragma unroll
+  for (int j = 0; j < kSums / 2; ++j) acc[j] = make_float2(0.0f, 0.0f);
+  const int first_sum = warp >= kAheadWarps && warp < kCopyWarp ? (warp - kAheadWarps) / 4 * kSums : 0;   // of the tile's tokens
+
+  if (warp == kCopyWarp) {
+    // ---- stages: nz of the groups' sums (as the tokens' operand), then a chunk's codes, tokens and scales each ----
+    const int loads = nz + c1 - c0;
+    auto early = [&](int i, int s) {                          // what no earlier kernel writes
+      uint8_t* st = smem + s * P::kStageBytes;
+      if (i < nz) {
+        if (lane == 0) mbar_arrive_expect_tx(&full[s], P::kXBytes);
+        mbar_arrive(&full[s]);
+        return;
+      }
+      const int ch = c0 + i - nz;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&full[s], kWBytes + P::kXBytes);
+        tma_load_2d(st + P::kXBytes, &tm_w, &full[s], ch * (kChunk / 2), n0);
+      }
+      // rows of N 16-bit values: any alignment
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) {
+        const int grp = ch * kSteps + k;
+        if (grp * G < a.K)
+          cp_async_halves(smem_u32(st + P::kXBytes + kWBytes + k * P::kScaleBytes),
+                          reinterpret_cast<const unsigned short*>(a.s) + static_cast<int64_t>(grp) * a.N + n0,
+                          min(kRows, a.N - n0), lane);
+      }
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[s])) : "memory");
+    };
+    auto tokens = [&](int i, int s) {
+      if (lane != 0) return;
+      uint8_t* st = smem + s * P::kStageBytes;
+      const CUtensorMap* map = i < nz ? &tm_r : &tm_x;
+      const int at = (i < nz ? z0 + i : c0 + i - nz) * kChunk * 2;
+      tma_load_2d(st, map, &full[s], at, m0);
+      tma_load_2d(st + P::kXBytes / 2, map, &full[s], at + 128, m0);
+    };
+    const int first = min(kStages, loads);
+    for (int i = 0; i < first; ++i) early(i, i);
+    grid_dep_wait();                                          // the tokens and their sums are written
+    for (int i = 0; i < first; ++i) tokens(i, i);
+    uint32_t issued = first, phase = 0;
+    int s = 0;
+    for (int i = first; i < loads; ++i) {
+      if (!mbar_wait_short(&empty[s], phase, abort_flag, kSite)) break;
+      early(i, s);
+      tokens(i, s);
+      ++issued;
+      if (++s == kStages) { s = 0; phase ^= 1u; }
+    }
+    cp_async_wait_all();
+    if (lane == 0) drain_ring(full, kStages, issued, 50000000ull);
+    __syncwarp();
+  } else if (warp == kMmaWarp) {
+    // ---- products: the zeros' first, then each group's P = codes x tokens ----
+    constexpr uint32_t shape = (1u << 4) | (static_cast<uint32_t>(NTOK >> 3) << 17) | (8u << 24);   // f32, M = 128
+    constexpr uint32_t idesc_z = shape | (1u << 7) | (1u << 10);                                    // bf16 x bf16
+    int stage = 0, issued = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    auto next_stage = [&]() {
+      if (++stage == kStages) { stage = 0; phase ^= 1u; }
+    };
+    for (int j = 0; j < nz; ++j) {
+      const int buf = j & 1;
+      ok = ok && mbar_wait_short(&full[stage], phase, abort_flag, kSite + 1) &&
+           mbar_wait_short(&a_full[buf], (j >> 1) & 1, abort_flag, kSite + 2);
+      if (!ok) break;
+      tc_fence_after();
+      const uint64_t x = smem_desc_k_sw128(smem_u32(smem + stage * P::kStageBytes));
+      if (lane == 0) {
+#pragma unroll
+        for (int k = 0; k < 6; ++k) {                         // three parts of 32 sums; the last 32 columns are empty
+          const int col = 16 * k;
+          mma_f16_ts(d_col, a_col + buf * 64 + 8 * k, x + ((col >> 6) * (P::kXBytes / 2) + (col & 63) * 2) / 16, idesc_z,
+                     j + k != 0);
+        }
+        tc_commit(&z_done[buf]);
+        tc_commit(&empty[stage]);
+        if (j + 1 == nz) tc_commit(&p_full[0]);
+      }
+      __syncwarp();
+      issued = 1;
+      next_stage();
+    }
+    if (nz == 0 && lane == 0) mbar_arrive(&p_full[0]);
+    // product i (0: the zeros', 1 ..: the groups') takes P buffer i & 1; a_full goes on counting from the zeros' blocks
+    for (int i = 1; i <= steps && ok; next_stage()) {
+      if (!(ok = mbar_wait_short(&full[stage], phase, abort_flag, kSite + 3))) break;
+      const uint64_t x = smem_desc_k_sw128(smem_u32(smem + stage * P::kStageBytes));
+#pragma unroll
+      for (int sub = 0; sub < kSteps; ++sub) {
+        if (i > steps) break;
+        const int buf = i & 1, use = nz + i - 1;
+        ok = mbar_wait_short(&p_empty[buf], ((i >> 1) & 1) ^ 1u, abort_flag, kSite + 4) &&
+             mbar_wait_short(&a_full[use & 1], (use >> 1) & 1, abort_flag, kSite + 5);
+        if (!ok) break;
+        tc_fence_after();
+        if (lane == 0) {
+#pragma unroll
+          for (int k = 0; k < G / 16; ++k) {
+            const int col = sub * G + 16 * k;                 // 64 columns per 128-byte-wide half
+            mma_f16_ts(d_col + buf * NTOK, a_col + (use & 1) * 64 + 8 * k,
+                       x + ((col >> 6) * (P::kXBytes / 2) + (col & 63) * 2) / 16, shape, k != 0);
+          }
+          tc_commit(&p_full[buf]);
+          if (sub == kSteps - 1) tc_commit(&empty[stage]);
+        }
+        __syncwarp();
+        issued = ++i;
+      }
+    }
+    // after a wait that ran out: the products in flight end before TMEM and the ring go away
+    if (!ok && lane == 0) {
+      for (int j = max(nz - 2, 0); j < nz && issued <= 1; ++j) mbar_wait_drain(&z_done[j & 1], (j >> 1) & 1, 50000000ull);
+      for (int i = max(issued - 2, 0); i < issued; ++i) mbar_wait_drain(&p_full[i & 1], (i >> 1) & 1, 50000000ull);
+    }
+    __syncwarp();
+  } else if (warp < kAheadWarps) {
+    // ---- operands: 32 groups' zeros, three times, then each group's codes widened ----
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    auto hand_over = [&](int buf, bool last) {
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&a_full[buf]);
+        if (last) mbar_arrive(&empty[stage]);
+      }
+    };
+    for (int j = 0; j < nz && ok; ++j) {
+      const int buf = j & 1;
+      uint32_t pairs[16];
+      const unsigned short* zp = reinterpret_cast<const unsigned short*>(a.z) + static_cast<int64_t>(z0 + j) * 32 * a.N + n;
+      const int left = n < a.N ? a.K / G - (z0 + j) * 32 : 0;
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+        const uint32_t lo = 2 * q < left ? __ldg(zp + static_cast<int64_t>(2 * q) * a.N) : 0;
+        const uint32_t hi = 2 * q + 1 < left ? __ldg(zp + static_cast<int64_t>(2 * q + 1) * a.N) : 0;
+        pairs[q] = lo | hi << 16;
+      }
+      ok = mbar_wait_short(&full[stage], phase, abort_flag, kSite + 6) &&
+           (j < 2 || mbar_wait_short(&z_done[buf], ((j - 2) >> 1) & 1, abort_flag, kSite + 7));
+      if (!ok) break;
+      __syncwarp();
+      tc_fence_after();
+#pragma unroll
+      for (int part = 0; part < 3; ++part) tmem_st_x16(a_col + buf * 64 + 16 * part + lane_base, pairs);
+      hand_over(buf, true);
+      if (++stage == kStages) { stage = 0; phase ^= 1u; }
+    }
+    const uint8_t* w = smem + P::kXBytes + row * 64;
+    const int sw = (row >> 1 & 3) << 4;
+    for (int i = 1; i <= steps && ok;) {
+      if (!(ok = mbar_wait_short(&full[stage], phase, abort_flag, kSite + 8))) break;
+#pragma unroll
+      for (int sub = 0; sub < kSteps; ++sub) {
+        if (i > steps) break;
+        const int buf = (nz + i - 1) & 1;
+        uint4 codes[G / 32];
+#pragma unroll
+        for (int b = 0; b < G / 32; ++b)                      // 32 columns: 16 bytes
+          codes[b] = *reinterpret_cast<const uint4*>(w + stage * P::kStageBytes + (((sub * (G / 32) + b) << 4) ^ sw));
+        // A's buffer is free when the product two before is done; the zeros' products took both
+        const int free_at = i <= 2 ? 0 : i - 2;
+        if ((i > 2 || nz > 0) && !(ok = mbar_wait_short(&p_full[free_at & 1], (free_at >> 1) & 1, abort_flag, kSite + 9))) break;
+        __syncwarp();
+        tc_fence_after();
+#pragma unroll
+        for (int b = 0; b < G / 32; ++b) {
+          const uint32_t v[4] = {codes[b].x, codes[b].y, codes[b].z, codes[b].w};
+          uint32_t pairs[16];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) widen8<true>(v[j], reinterpret_cast<uint32_t(&)[4]>(pairs[4 * j]));
+          tmem_st_x16(a_col + buf * 64 + 16 * b + lane_base, pairs);
+        }
+        hand_over(buf, sub == kSteps - 1);
+        ++i;
+      }
+      if (++stage == kStages) { stage = 0; phase ^= 1u; }
+    }
+  } else {
+    // ---- the zeros' product, and each group's scaled, added up ----
+    const int s_odd = half_shift(reinterpret_cast<const unsigned short*>(a.s) + n0);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int j = 0; j < nz && ok; ++j) {
+      ok = mbar_wait_short(&full[stage], phase, abort_flag, kSite + 10);
+      if (ok && lane == 0) mbar_arrive(&empty[stage]);
+      if (++stage == kStages) { stage = 0; phase ^= 1u; }
+    }
+    auto add = [&](int i, float scale, bool last) {
+      const int buf = i & 1;
+      if (!(ok = mbar_wait_short(&p_full[buf], (i >> 1) & 1, abort_flag, kSite + 11))) return;
+      __syncwarp();
+      tc_fence_after();
+      const float2 s2 = make_float2(scale, scale);
+#pragma unroll
+      for (int q = 0; q < kSums / 16; ++q) {
+        uint32_t v[16];
+        tmem_ld_x16(d_col + buf * NTOK + first_sum + 16 * q + lane_base, v);
+        tmem_wait_ld_x16(v);
+        if (q == kSums / 16 - 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&p_empty[buf]);
+            if (last) mbar_arrive(&empty[stage]);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          acc[8 * q + j] = fma2(s2, make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), acc[8 * q + j]);
+      }
+    };
+    if (nz > 0 && ok) add(0, 1.0f, false);
+    if (nz == 0 && lane == 0) mbar_arrive(&p_empty[0]);       // product 0 has nothing in it
+    for (int i = 1; i <= steps && ok;) {
+      if (!(ok = mbar_wait_short(&full[stage], phase, abort_flag, kSite + 12))) break;
+#pragma unroll
+      for (int sub = 0; sub < kSteps; ++sub) {
+        if (i > steps || !ok) break;
+        const int odd = (c0 * kSteps + i - 1) & a.N & 1;      // an odd N moves every other group's scales by a half
+        const float s = bf16_bits_to_f32(reinterpret_cast<const unsigned short*>(
+            smem + stage * P::kStageBytes + P::kXBytes + kWBytes + sub * P::kScaleBytes)[row + (s_odd ^ odd)]);
+        add(i, s, sub == kSteps - 1);
+        ++i;
+      }
+      if (++stage == kStages) { stage = 0; phase ^= 1u; }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(d_col, kCols);
+  }
+
+  auto store = [&](int m, int col, float y) {
+    const int64_t at = static_cast<int64_t>(m) * a.N + col;
+    if constexpr (F16) {
+      if (a.bias != nullptr) y += __half2float(static_cast<const __half*>(a.bias)[col]);
+      static_cast<__half*>(a.out)[at] = __float2half_rn(y);
+    } else {
+      y *= __ldg(a.factor + m);
+      if (a.bias != nullptr) y += __bfloat162float(static_cast<const __nv_bfloat16*>(a.bias)[col]);
+      static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(y);
+    }
+  };
+  const bool adds = warp >= kAheadWarps && warp < kCopyWarp;
+  const int mt = min(NTOK, a.M - m0);
+  if (a.ksplit == 1) {
+    if (adds && n < a.N) {
+#pragma unroll
+      for (int j = 0; j < kSums; ++j)
+        if (first_sum + j < mt) store(m0 + first_sum + j, n, j & 1 ? acc[j / 2].y : acc[j / 2].x);
+    }
+    return;
+  }
+  // ---- partial sums of the cluster: [token][row] in each CTA's ring, added in rank order ----
+  float* part = reinterpret_cast<float*>(smem);
+  if (adds) {
+#pragma unroll
+    for (int j = 0; j < kSums; ++j) part[(first_sum + j) * kRows + row] = j & 1 ? acc[j / 2].y : acc[j / 2].x;
+  }
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (adds && n < a.N) {
+    for (int m = rank + first_sum / kSums * a.ksplit; m < mt; m += a.ksplit * (P::kAddWarps / 4)) {
+      float y = 0.0f;
+      for (int q = 0; q < a.ksplit; ++q) {
+        float v;
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(smem_u32(part + m * kRows + row), q)));
+        y += v;
+      }
+      store(m0 + m, n, y);
+    }
+  }
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+namespace {
+bool w4a16_map(CUtensorMap* map, const void* base, int64_t rows, int64_t bytes, int box_bytes, int box_rows, CUtensorMapSwizzle sw) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(bytes), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(bytes)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_bytes), static_cast<cuuint32_t>(box_rows)}, estr[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
+         CUDA_SUCCESS;
+}
+}  // namespace
+
+template <bool F16, int G, int NTOK>
+cudaError_t run_w4a16_tc(const W4A16Args& a, const W4Tokens& t, cudaStream_t st) {
+  using P = w4tc::Plan<G, NTOK>;
+  auto kern = w4a16_tc_kernel<F16, G, NTOK>;
+  static unsigned long long devices = 0;
+  const cudaError_t e = allow_shared(kern, P::kSmem, devices);
+  if (e != cudaSuccess) return e;
+  const int tiles = (a.M + NTOK - 1) / NTOK, chunks = (a.K + w4tc::kChunk - 1) / w4tc::kChunk;
+  CUtensorMap tm_w, tm_x, tm_r;
+  if (!w4a16_map(&tm_w, a.b, a.N, a.K / 2, 64, w4tc::kRows, CU_TENSOR_MAP_SWIZZLE_64B) ||
+      !w4a16_map(&tm_x, t.x, a.M, static_cast<int64_t>(a.K) * 2, 128, NTOK, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !w4a16_map(&tm_r, t.parts, a.M, t.blocks * 256, 128, NTOK, CU_TENSOR_MAP_SWIZZLE_128B))
+    return cudaErrorInvalidValue;
+  const int row_tiles = (a.N + w4tc::kRows - 1) / w4tc::kRows;
+  // K split over a cluster while that leaves no resident CTA (two per SM) without work and each has four chunks
+  int ksplit = 1;
+  while (ksplit < 8 && row_tiles * tiles * ksplit * 2 <= 2 * num_sms() && chunks / (2 * ksplit) >= 4) ksplit *= 2;
+  const w4tc::Args args{a.s, a.z, t.factor, a.bias, a.out, a.M, a.N, a.K, ksplit};
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = static_cast<unsigned>(ksplit);
+  cfg.gridDim = dim3(row_tiles, tiles, ksplit);
+  cfg.blockDim = dim3(P::kThreads);
+  cfg.dynamicSmemBytes = P::kSmem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kern, tm_w, tm_x, tm_r, args);
+}
+
+}  // namespace cq
