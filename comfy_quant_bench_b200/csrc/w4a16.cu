@@ -220,7 +220,11 @@ cudaError_t pick_w4a16(const W4A16Args& a, cudaStream_t st) {
 template <bool F16, int G>
 cudaError_t pick_w4a16_shared(const W4A16Args& a, const W4Tokens& t, cudaStream_t st) {
   if (w4a16_tensor_memory(a.M)) return run_w4a16_tc<F16, G, 64>(a, t, st);
-  return w4a16_tile(a.M) == 16 ? run_w4a16_mid<F16, G, 2>(a, t, st) : run_w4a16_mid<F16, G, 4>(a, t, st);
+  switch (w4a16_tile(a.M)) {
+    case 16: return run_w4a16_mid<F16, G, 2>(a, t, st);
+    case 24: return run_w4a16_mid<F16, G, 3>(a, t, st);
+    default: return run_w4a16_mid<F16, G, 4>(a, t, st);
+  }
 }
 
 // Up to eight tokens this file's kernel; beyond, the forms that share the tokens between rows.

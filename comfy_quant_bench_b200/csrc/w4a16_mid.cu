@@ -1,15 +1,13 @@
 // W4A16 linear for more than eight tokens: the tiles of w4a16.cu, with the tokens shared by a CTA.
 //
-// A CTA owns 256 weight rows, 32 for each of its eight warps, and up to 64 tokens.  With more tokens the tokens are most
+// A CTA owns 256 weight rows, 32 for each of its eight warps, and up to 32 tokens.  With more tokens the tokens are most
 // of what a tile reads, so they are brought into shared memory once per CTA and chunk of 128 columns; weights, scales,
 // tokens and their sums arrive through one ring of asynchronous copies.  A warp forms q - 8 as f16 in registers (nine
 // instructions per eight codes), multiplies it with every eight tokens in mma.sync tiles, and after each scale group
 // adds s P + z R (P = sum x (q - 8), R = sum x) to its fp32 sums.
 //
-// Bound by the tiles' rate from about 32 tokens on (a tile of 16 x 8 x 16 takes eight cycles of an SM's quarter), by
-// reading the weights below.  tcgen05 would multiply eight times faster, but its weight operand has to be written to
-// tensor or shared memory and each group's P read back: measured in that form (codes widened into tensor memory, roles
-// meeting at mbarriers) 64 tokens at 8192 x 28672 took 110 us, bound by that traffic and the hand-overs.
+// Bound by the tiles' rate (a tile of 16 x 8 x 16 takes eight cycles of an SM's quarter): 18 tokens of a 5120 x 13824
+// weight need 16 us of them with four tiles of tokens, 12 us with three.  Measured: see launch_w4a16.
 //
 // The tokens come from w4a16_tokens.cu, as f16 in the order the codes are widened in, with R.  The product is launched as
 // its programmatic dependent: its weights are on their way while the tokens are written.
@@ -25,7 +23,7 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kRt = 2;                         // 16-row tiles of a warp
 constexpr int kRows = 16 * kRt * kWarps;
 constexpr int kChunk = 128;                    // columns of a ring stage
-constexpr int kStages = 4;
+constexpr int kStages = 3;
 constexpr int kWBytes = kRows * kChunk / 2;
 constexpr int kScaleBytes = 544;               // 256 scales (or zeros) of a group, and room for a shift
 
@@ -40,7 +38,6 @@ struct Plan {
   static constexpr int kPartStride = kRows + 4;               // floats between tokens of a partial tile
   static constexpr int kRing = kStages * kStageBytes, kPart = kTokens * kPartStride * 4;
   static constexpr int kSmem = kRing > kPart ? kRing : kPart;
-  static constexpr int kCtas = NT <= 2 ? 2 : 1;
 };
 
 struct Args {
@@ -57,7 +54,7 @@ struct Args {
 }  // namespace w4mid
 
 template <bool F16, int G, int NT>
-__global__ void __launch_bounds__(w4mid::kThreads, (w4mid::Plan<G, NT>::kCtas)) w4a16_mid_kernel(const w4mid::Args a) {
+__global__ void __launch_bounds__(w4mid::kThreads, 2) w4a16_mid_kernel(const w4mid::Args a) {
   using namespace w4mid;
   using P = Plan<G, NT>;
   constexpr int kGroups = P::kGroups;
@@ -233,9 +230,9 @@ cudaError_t run_w4a16_mid(const W4A16Args& a, const W4Tokens& t, cudaStream_t st
   if (e != cudaSuccess) return e;
   const int tiles = (a.M + P::kTokens - 1) / P::kTokens, chunks = (a.K + w4mid::kChunk - 1) / w4mid::kChunk;
   const int row_tiles = (a.N + w4mid::kRows - 1) / w4mid::kRows;
-  // K split over a cluster while that leaves no resident CTA without work and each has four chunks
+  // K split over a cluster while that leaves no resident CTA (two per SM) without work and each has two chunks
   int ksplit = 1;
-  while (ksplit < 8 && row_tiles * tiles * ksplit * 2 <= P::kCtas * num_sms() && chunks / (2 * ksplit) >= 4) ksplit *= 2;
+  while (ksplit < 8 && row_tiles * tiles * ksplit * 2 <= 2 * num_sms() && chunks / (2 * ksplit) >= 2) ksplit *= 2;
   const w4mid::Args args{a.b, t.x, a.s, a.z, t.factor, t.r, a.bias, a.out, a.M, a.N, a.K, ksplit};
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];

@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(256) w4a16_tokens_kernel(const void* x, int64_
 
 namespace {
 // tokens of a tile; from 33 on the tensor-memory form takes 64
-int w4a16_tile(int M) { return M <= 16 ? 16 : M <= 32 ? 32 : 64; }
+int w4a16_tile(int M) { return M <= 16 ? 16 : M <= 24 ? 24 : M <= 32 ? 32 : 64; }
 bool w4a16_tensor_memory(int M) { return M > 32; }
 int64_t w4a16_tokens_bytes(int M, int K) { return (static_cast<int64_t>(M) * K * 2 + 255) / 256 * 256; }
 int64_t w4a16_sums_bytes(int M, int K, int G) {
