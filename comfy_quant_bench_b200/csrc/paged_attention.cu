@@ -16,8 +16,9 @@
 // the warps' running maxima, sums and outputs are joined in shared memory; a row that several CTAs share is joined
 // by a second small kernel in the order of its parts.  Both orders are fixed, so equal calls give equal bits.
 //
-// Softmax statistics, scores and outputs are fp32.  The weights p enter the second product as two 16-bit parts,
-// p = hi + lo (relative error 2^-16), since one part alone would add as much error as rounding the output does.
+// Softmax statistics, scores and outputs are fp32.  The weights p enter the second product as two parts of the cache's
+// 16-bit type, p = hi + lo, since one part alone would add as much error as rounding the output does.  Where the type is
+// f16 (an 8-bit cache) and the output bf16, one part is enough: its error, 2^-12, is a sixteenth of the rounding's.
 // 8-bit caches are widened exactly to f16; a bf16 query is scaled by a power of two per head so that f16 holds it to
 // 2^-24 of its largest element.
 #include "decode_common.cuh"
@@ -61,9 +62,13 @@ __device__ __forceinline__ uint32_t movmatrix_t(uint32_t x) {   // transpose of 
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
   return d;
 }
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t pair) {   // exact; NaN stays NaN
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(pair), __NV_E4M3);
-  return static_cast<uint32_t>(h.x) | static_cast<uint32_t>(h.y) << 16;
+// four e4m3 values as two f16 pairs: exact; NaN stays NaN
+__device__ __forceinline__ void e4m3x4_to_f16(uint32_t x, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\t"
+      "mov.b32 {l, h}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi) : "r"(x));
 }
 // two fp32 values as 16-bit pairs: hi = the nearest, lo = the nearest of what is left
 template <bool F16>
@@ -132,6 +137,7 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
   using C = pattn::Cfg<D, FP8 ? 1 : 2, NT>;
   constexpr int ES = FP8 ? 1 : 2, kRow = C::kRow, kStages = C::kStages;
   constexpr bool kF16Math = F16 || FP8;
+  constexpr bool kSplit = !FP8 || F16;                  // the weights enter as two parts
   constexpr int kHeads = 8 * NT;                        // heads of a tile
   constexpr int kMt = D / 16;                           // 16-wide slices of the head dim
   extern __shared__ __align__(128) uint8_t smem[];
@@ -381,9 +387,9 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
           ldsm_x4(raw, kt + swz<kRow>(kr, 2 * kp + kc));
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const uint32_t r0 = raw[2 * half], r1 = raw[2 * half + 1];
-            const uint32_t ka[4] = {e4m3x2_to_f16x2(r0 & 0xffffu), e4m3x2_to_f16x2(r1 & 0xffffu),
-                                    e4m3x2_to_f16x2(r0 >> 16), e4m3x2_to_f16x2(r1 >> 16)};
+            uint32_t ka[4];
+            e4m3x4_to_f16(raw[2 * half], ka[0], ka[2]);
+            e4m3x4_to_f16(raw[2 * half + 1], ka[1], ka[3]);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               const uint2 q = qfrag[((2 * kp + half) * NT + n) * 32 + lane];
@@ -420,7 +426,7 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           ph[n][j] = movmatrix_t(ph[n][j]);
-          pl[n][j] = movmatrix_t(pl[n][j]);
+          if constexpr (kSplit) pl[n][j] = movmatrix_t(pl[n][j]);
         }
       }
       if (__any_sync(0xffffffffu, grew)) {
@@ -451,13 +457,13 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
           ldsm_x4_t(raw, vt + swz<kRow>(kr, 2 * ip + kc));
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const uint32_t r0 = __byte_perm(raw[2 * half], 0, 0x3120), r1 = __byte_perm(raw[2 * half + 1], 0, 0x3120);
-            const uint32_t va[4] = {e4m3x2_to_f16x2(r0 & 0xffffu), e4m3x2_to_f16x2(r0 >> 16),
-                                    e4m3x2_to_f16x2(r1 & 0xffffu), e4m3x2_to_f16x2(r1 >> 16)};
+            uint32_t va[4];
+            e4m3x4_to_f16(__byte_perm(raw[2 * half], 0, 0x3120), va[0], va[1]);
+            e4m3x4_to_f16(__byte_perm(raw[2 * half + 1], 0, 0x3120), va[2], va[3]);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               mma_16816<true>(o[2 * ip + half][n], va, ph[n][0], ph[n][1]);
-              mma_16816<true>(o[2 * ip + half][n], va, pl[n][0], pl[n][1]);
+              if constexpr (kSplit) mma_16816<true>(o[2 * ip + half][n], va, pl[n][0], pl[n][1]);
             }
           }
         }
