@@ -159,6 +159,23 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+_decode = None
+
+
+def decode():
+    """The host side of the decode-side operators (csrc/decode_bind.cpp).  Raises if it is absent, as ``load`` does."""
+    global _decode
+    if _decode is None:
+        import torch  # noqa: F401 - the module's symbols come from torch's libraries
+        load()
+        path = os.path.join(_HERE, "_decode.so")
+        if not os.path.exists(path):
+            raise ImportError(f"{path} is missing: build it with `python -m comfy_quant_bench_b200.build`")
+        from . import _decode as module
+        _decode = module
+    return _decode
+
+
 def status_string(status: int) -> str:
     return load().cq_status_string(status).decode()
 

@@ -17,7 +17,6 @@ on the CPU or on a non-sm_100 device are rejected: there is no eager fallback.
 from __future__ import annotations
 
 import ctypes
-import functools
 
 import torch
 
@@ -476,50 +475,6 @@ def w4a8_affine_linear(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tens
     return out if dt == torch.bfloat16 else out.to(dt)
 
 
-# Decode-side operators take a few microseconds, so their host side is plain attribute checks and one native call.
-
-# the current stream's handle; the first form makes no stream object
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
-    lambda idx: torch.cuda.current_stream(idx).cuda_stream)
-
-
-def _cuda_index(*ts: torch.Tensor | None) -> int:
-    """The CUDA device index that all the tensors are on."""
-    idx = None
-    for t in ts:
-        if t is None:
-            continue
-        i = t.get_device() if t.is_cuda else -1
-        if i != idx:
-            if i < 0:
-                raise ValueError("comfy_quant_bench_b200 ops run on CUDA tensors only (no CPU fallback)")
-            if idx is not None:
-                raise ValueError(f"tensors on different devices: cuda:{idx} and cuda:{i}")
-            idx = i
-    return idx
-
-
-@functools.lru_cache(maxsize=1024)
-def _w4a16_workspace(m: int, k: int, group: int) -> int:
-    return _lib.load().cq_w4a16_workspace_bytes(m, k, group)
-
-
-def _w4a16_refusal(x, qweight, scale, zeros, group_size) -> ValueError:
-    """Why ``w4a16_linear`` refuses these arguments."""
-    k, n = x.shape[-1], qweight.shape[0]
-    if x.dtype not in (torch.bfloat16, torch.float16):
-        return ValueError(f"x must be bf16 or f16, got {x.dtype}")
-    if k != qweight.shape[-1] * 2:
-        return ValueError(f"Input K={k} does not match qweight K={qweight.shape[-1] * 2}")
-    if group_size not in (32, 64, 128) or k % group_size:
-        return ValueError(f"group_size must be 32, 64 or 128 and divide K={k}, got {group_size}")
-    if qweight.dtype not in (torch.int8, torch.uint8) or qweight.dim() != 2:
-        return ValueError("qweight must be int8 or uint8 [N, K/2]")
-    if any(t.dtype != torch.bfloat16 or t.shape != (k // group_size, n) for t in (scale, zeros)):
-        return ValueError(f"scale and zeros must be bf16 [{k // group_size}, {n}]")
-    return ValueError("qweight, scale and zeros must be contiguous")
-
-
 def w4a16_linear(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor, zeros: torch.Tensor,
                  bias: torch.Tensor | None = None, *, group_size: int = 128,
                  out: torch.Tensor | None = None) -> torch.Tensor:
@@ -528,44 +483,7 @@ def w4a16_linear(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor, ze
     x [..., K] bf16 or f16 (its rows may be strided), qweight int8 or uint8 [N, K/2] (low nibble = even column),
     scale and zeros bf16 [K/group_size, N] (group_size 32, 64 or 128), bias [N].  Products and sums are fp32, rounded
     once to the type of x.  For the few tokens of a decode step; ``w4a8_affine_linear`` takes many tokens."""
-    shape, wshape = x.shape, qweight.shape
-    k, n, dt, wt = shape[-1], wshape[0], x.dtype, qweight.dtype
-    if not ((dt is torch.bfloat16 or dt is torch.float16) and (wt is torch.int8 or wt is torch.uint8)
-            and group_size in (32, 64, 128) and k % group_size == 0 and wshape == (n, k // 2)
-            and scale.dtype is torch.bfloat16 and zeros.dtype is torch.bfloat16
-            and scale.shape == (k // group_size, n) and zeros.shape == scale.shape
-            and qweight.is_contiguous() and scale.is_contiguous() and zeros.is_contiguous()):
-        raise _w4a16_refusal(x, qweight, scale, zeros, group_size)
-    idx = _cuda_index(x, qweight, scale, zeros, bias, out)
-    if idx != torch.cuda.current_device():
-        with torch.cuda.device(idx):
-            return w4a16_linear(x, qweight, scale, zeros, bias, group_size=group_size, out=out)
-    x2 = x if len(shape) == 2 else x.reshape(-1, k)
-    m, ldx, xp = x2.shape[0], k, x2.data_ptr()
-    if xp % 16 or not x2.is_contiguous():
-        ldx = x2.stride(0)
-        if xp % 16 or x2.stride(1) != 1 or ldx % 8 or ldx < k:
-            x2, ldx = x2.clone(memory_format=torch.contiguous_format), k
-            xp = x2.data_ptr()
-    bp = None
-    if bias is not None:
-        if bias.dtype is not dt or bias.shape != (n,) or not bias.is_contiguous():
-            if bias.numel() != n:
-                raise ValueError(f"bias must have {n} elements")
-            bias = bias.reshape(n).to(dt).contiguous()
-        bp = bias.data_ptr()
-    if out is None:
-        out = x.new_empty((m, n) if len(shape) == 2 else (*shape[:-1], n))
-    elif out.dtype is not dt or out.shape != (*shape[:-1], n) or not out.is_contiguous():
-        raise ValueError(f"out must be contiguous {dt} of shape {(*shape[:-1], n)}")
-    nbytes = _w4a16_workspace(m, k, group_size)
-    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes > 0 else None
-    status = _lib.load().cq_w4a16_linear(xp, ldx, 0 if dt is torch.bfloat16 else 1, m, k, n, qweight.data_ptr(),
-                                         scale.data_ptr(), zeros.data_ptr(), group_size, bp, out.data_ptr(), _ptr(ws),
-                                         nbytes, _raw_stream(idx))
-    if status:
-        _lib.check("cq_w4a16_linear", status)
-    return out
+    return _lib.decode().w4a16_linear(x, qweight, scale, zeros, bias, group_size, out)
 
 
 def w4a8_affine_linear_into(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor, zeros_prepared: torch.Tensor,

@@ -101,3 +101,23 @@ def test_operators_reject_cpu_tensors():
                 lambda: c.attend(0, new, rows=one)):
         with pytest.raises(ValueError, match="CUDA"):
             bad()
+
+
+def test_refusals_say_what_is_wrong():
+    from comfy_quant_bench_b200 import kvcache, ops
+    x, q = torch.zeros(2, 256, dtype=torch.bfloat16), torch.zeros(16, 128, dtype=torch.int8)
+    s, b = torch.zeros(4, 16, dtype=torch.bfloat16), torch.zeros(16, dtype=torch.bfloat16)
+    k, n = torch.zeros(6, 2, 16, 64, dtype=torch.bfloat16), torch.zeros(2, dtype=torch.int32)
+    t, query = torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, 4, 64, dtype=torch.bfloat16)
+    for says, call in (("bf16 or f16, got Float", lambda: ops.w4a16_linear(x.float(), q, s, s, b, group_size=64)),
+                       ("K=128 does not match qweight K=256", lambda: ops.w4a16_linear(x[:, :128], q, s, s, b, group_size=64)),
+                       ("divide K=256, got 16", lambda: ops.w4a16_linear(x, q, s, s, b, group_size=16)),
+                       (r"\[4, 16\]", lambda: ops.w4a16_linear(x, q, s.float(), s, b, group_size=64)),
+                       ("16 elements", lambda: ops.w4a16_linear(x, q, s, s, b[:5], group_size=64)),
+                       ("multiple of kv_heads", lambda: kvcache.paged_attention(query[:, :3], k, k, t, n)),
+                       ("64, 128 or 256", lambda: kvcache.paged_attention(query[..., :32], k, k, t, n)),
+                       ("one entry per table row", lambda: kvcache.paged_attention(query, k, k, t, n[:1])),
+                       ("2 queries for 1", lambda: kvcache.paged_attention(query, k, k, t[:1], n[:1])),
+                       ("do not fit", lambda: kvcache.append_kv(query, query, k, k, t, n, n))):
+        with pytest.raises(ValueError, match=says):
+            call()
