@@ -69,13 +69,20 @@ __device__ void free_bitmap(const int* refs, int num_pages, uint32_t* bits) {
   __syncthreads();
 }
 
+// Lanes that work on one table row: each row is a chain of dependent loads, so with short rows many of them at a time.
+// 128 rows of 56 pages: 23 us with a warp per row, 13 us with eight lanes.
+__device__ __forceinline__ int lanes_of_row(int width) { return width >= 512 ? 32 : 8; }
+
 __global__ void __launch_bounds__(pages::kThreads) pages_branch_kernel(const PagesArgs a) {
   extern __shared__ uint32_t dyn[];
   __shared__ int warp_sums[32];
   __shared__ int bad, over;
   uint32_t* seen = dyn;                                  // [table_rows] bits
   uint32_t* bits = dyn + (a.table_rows + 31) / 32;       // [num_pages] bits
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nwarps = blockDim.x >> 5;
+  const int tid = threadIdx.x;
+  const int per = lanes_of_row(a.table_width), sub = tid & (per - 1), group = tid / per, groups = blockDim.x / per;
+  const uint32_t mates = per == 32 ? 0xffffffffu : 0xffu << (tid & 24);   // the lanes of this thread's row
+  grid_dep_launch();                                     // the copies may be set up while this runs
   if (tid == 0) { bad = 0; over = 0; }
   __syncthreads();
 
@@ -84,23 +91,24 @@ __global__ void __launch_bounds__(pages::kThreads) pages_branch_kernel(const Pag
     mark_rows(a.free_rows, a.n_free, a.table_rows, seen, &bad);
     if (bad) site = pages::kSiteFree;
     else {
-      for (int i = warp; i < a.n_free; i += nwarps) {
+      for (int i = group; i < a.n_free; i += groups) {
         const int r = a.free_rows[i];
         int* row = a.table + r * a.table_stride;
         const int held = held_pages(a.lens[r], a.page_size, a.table_width);
-        __syncwarp();
-        for (int j = lane; j < held; j += 32) {
+        __syncwarp(mates);                                // every lane has read the row's length
+#pragma unroll 4
+        for (int j = sub; j < held; j += per) {
           const int p = row[j];
           if (p >= 0 && p < a.num_pages) atomicSub(&a.refs[p], 1);
           row[j] = -1;
         }
-        if (lane == 0) a.lens[r] = 0;
+        if (sub == 0) a.lens[r] = 0;
       }
     }
     __syncthreads();
   }
   if (site == 0 && a.n_fork > 0) {
-    mark_rows(a.dst, a.n_fork, a.table_rows, seen, &bad);
+    if (a.dst != a.free_rows || a.n_fork != a.n_free) mark_rows(a.dst, a.n_fork, a.table_rows, seen, &bad);
     for (int i = tid; i < a.n_fork; i += blockDim.x) {
       const int s = a.src[i], d = a.dst[i];
       if (s < 0 || s >= a.table_rows || (seen[s >> 5] >> (s & 31) & 1u)) bad = 1;    // a source is no destination
@@ -109,15 +117,16 @@ __global__ void __launch_bounds__(pages::kThreads) pages_branch_kernel(const Pag
     __syncthreads();
     if (bad) site = pages::kSiteFork;
     else {
-      for (int i = warp; i < a.n_fork; i += nwarps) {
+      for (int i = group; i < a.n_fork; i += groups) {
         const int s = a.src[i], d = a.dst[i];
         const int len = a.lens[s], held = held_pages(len, a.page_size, a.table_width);
-        for (int j = lane; j < held; j += 32) {
+#pragma unroll 4
+        for (int j = sub; j < held; j += per) {
           const int p = a.table[s * a.table_stride + j];
           a.table[d * a.table_stride + j] = p;
           if (p >= 0 && p < a.num_pages) atomicAdd(&a.refs[p], 1);
         }
-        if (lane == 0) a.lens[d] = len;
+        if (sub == 0) a.lens[d] = len;
       }
     }
     __syncthreads();
@@ -129,7 +138,7 @@ __global__ void __launch_bounds__(pages::kThreads) pages_branch_kernel(const Pag
   int code = site != 0 ? CQ_ERR_ARG : CQ_OK;
   if (site == 0) {
     site = pages::kSiteReserve;
-    mark_rows(a.res_rows, a.n_res, a.table_rows, seen, &bad);
+    if (a.res_rows != a.dst || a.n_res != a.n_fork) mark_rows(a.res_rows, a.n_res, a.table_rows, seen, &bad);
     if (bad) code = CQ_ERR_ARG;
   }
   int total = 0;
@@ -181,20 +190,19 @@ __global__ void __launch_bounds__(pages::kThreads) pages_branch_kernel(const Pag
     return;
   }
   const int* list = a.ws + 2 * a.n_res;
-  for (int i = warp; i < a.n_res; i += nwarps) {
+  for (int i = group; i < a.n_res; i += groups) {
     const int r = a.res_rows[i], need = a.ws[2 * i], first = a.ws[2 * i + 1], len = max(__ldcg(a.lens + r), 0);
     const bool cow = need >> 30 & 1;
     const int own = need & ~(1 << 30), at = (len + a.page_size - 1) / a.page_size - (cow ? 1 : 0);
     int* row = a.table + r * a.table_stride;
     const int old = cow ? __ldcg(row + at) : -1;
-    __syncwarp();
-    for (int j = lane; j < own; j += 32) {
+    __syncwarp(mates);                                // every lane has read the row's length
+    for (int j = sub; j < own; j += per) {
       const int p = list[first + j];
       row[at + j] = p;
       a.refs[p] = 1;
     }
-    __syncwarp();
-    if (lane == 0) {
+    if (sub == 0) {
       a.start[i] = len;
       a.copies[2 * i] = old;
       a.copies[2 * i + 1] = cow ? list[first] : -1;
@@ -222,6 +230,8 @@ cudaError_t launch_pages_branch(const PagesArgs& a, cudaStream_t st) {
 // pages_copy_kernel: page moves[i][0] -> page moves[i][1] in every layer of the key and the value cache; a negative
 // entry moves nothing.  No destination is a source, so the order does not matter.
 __global__ void __launch_bounds__(256) pages_copy_kernel(const PagesCopyArgs a) {
+  grid_dep_launch();
+  grid_dep_wait();                                        // the list is written
   const int2 mv = reinterpret_cast<const int2*>(a.moves)[blockIdx.x];
   if (mv.x < 0 || mv.x >= a.num_pages || mv.y < 0 || mv.y >= a.num_pages) return;
   const int64_t layer = blockIdx.y * a.layer_bytes;
@@ -231,18 +241,36 @@ __global__ void __launch_bounds__(256) pages_copy_kernel(const PagesCopyArgs a) 
   for (int64_t i = threadIdx.x; i < a.page_bytes / 16; i += 256) to[i] = __ldcs(from + i);
 }
 
+namespace {
+// a launch that may be set up before the kernel before it in the stream has ended (which the kernel itself waits for)
+template <typename... Params, typename... Args>
+cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, int threads, int smem, cudaStream_t st, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+}  // namespace
+
 cudaError_t launch_pages_copy(const PagesCopyArgs& a, cudaStream_t st) {
   if (a.n == 0) return cudaSuccess;
-  pages_copy_kernel<<<dim3(a.n, a.layers, 2), 256, 0, st>>>(a);
-  return cudaGetLastError();
+  return launch_early(pages_copy_kernel, dim3(a.n, a.layers, 2), 256, 0, st, a);
 }
 
 // pages_compact_kernel: with L live pages (held by some row), the live pages at L and above move, in order, to the
 // free pages below L, in order.  map[p]: the new index of page p.  refs_out may be refs.
-__global__ void __launch_bounds__(pages::kThreads) pages_compact_kernel(const CompactArgs a) {
+__global__ void __launch_bounds__(pages::kThreads) pages_compact_kernel(const CompactArgs a, const int remap) {
   extern __shared__ uint32_t bits[];
   __shared__ int warp_sums[32];
   const int tid = threadIdx.x;
+  grid_dep_launch();
   free_bitmap(a.refs, a.num_pages, bits);
   const int words = (a.num_pages + 31) / 32, each = (words + blockDim.x - 1) / blockDim.x;
   const int w0 = min(words, tid * each), w1 = min(words, (tid + 1) * each);
@@ -281,11 +309,20 @@ __global__ void __launch_bounds__(pages::kThreads) pages_compact_kernel(const Co
   }
   __syncthreads();
   for (int p = live + tid; p < a.num_pages; p += blockDim.x) a.refs_out[p] = 0;
+  if (remap) {
+    for (int i = tid; i < a.table_rows * a.table_width; i += blockDim.x) {
+      const int r = i / a.table_width, j = i - r * a.table_width;
+      const int p = a.table[r * a.table_stride + j];
+      a.table_out[r * a.out_stride + j] = p >= 0 && p < a.num_pages ? a.map[p] : p;
+    }
+  }
 }
 
 // table entries to the pages' new indexes; table_out may be table
 __global__ void __launch_bounds__(256) pages_remap_kernel(const CompactArgs a) {
   const int64_t n = static_cast<int64_t>(a.table_rows) * a.table_width;
+  grid_dep_launch();
+  grid_dep_wait();                                        // the map is written
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
     const int64_t r = i / a.table_width, j = i - r * a.table_width;
     const int p = a.table[r * a.table_stride + j];
@@ -300,50 +337,61 @@ cudaError_t launch_pages_compact(const CompactArgs& a, cudaStream_t st) {
     const cudaError_t e = allow_shared(pages_compact_kernel, pages::kMaxShared, devices);
     if (e != cudaSuccess) return e;
   }
-  pages_compact_kernel<<<1, pages::kThreads, smem, st>>>(a);
+  // a table of a few thousand entries is remapped by the planning CTA itself: one launch (3 us) less
   const int64_t n = static_cast<int64_t>(a.table_rows) * a.table_width;
-  if (n > 0) {
-    const int64_t ctas = (n + 255) / 256;
-    pages_remap_kernel<<<static_cast<unsigned>(ctas < 1184 ? ctas : 1184), 256, 0, st>>>(a);
-  }
-  return cudaGetLastError();
+  const bool small = n <= 8 * pages::kThreads;
+  pages_compact_kernel<<<1, pages::kThreads, smem, st>>>(a, small ? 1 : 0);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || small) return e;
+  const int64_t ctas = (n + 255) / 256;
+  return launch_early(pages_remap_kernel, dim3(static_cast<unsigned>(ctas < 1184 ? ctas : 1184)), 256, 0, st, a);
 }
 
 // kv_append_kernel: new keys and values [layers, T, Hkv, D] into their rows' pages.  A token whose row, position or
 // page is out of range is skipped (a refused reservation gives positions of -1).  An 8-bit cache holds x / scale,
 // rounded to the nearest even and kept inside the format's finite range (NaN stays NaN).
+// A thread moves eight elements (16 bytes in, 16 or 8 out): bound by launch and latency up to a few MB, by HBM beyond.
 __global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
+  grid_dep_launch();
   const int64_t t = blockIdx.x, layer = blockIdx.y;
+  const int per = a.Hkv * a.D / 8;                        // eights of a token's keys, and of its values
+  grid_dep_wait();                                        // positions, tables and copied pages are written
   const int row = a.rows[t];
   const int pos = a.positions[t];
   if (row < 0 || row >= a.table_rows || pos < 0 || pos / a.page_size >= a.table_width) return;
   const int page = a.table[row * a.table_stride + pos / a.page_size];
   if (page < 0 || page >= a.num_pages) return;
   const int64_t base = layer * a.layer_stride + page * a.page_stride + (pos % a.page_size) * a.tok_stride;
-  const bool value = blockIdx.z != 0;
-  const void* src = value ? a.v_new : a.k_new;
-  void* cache = value ? a.v : a.k;
-  const float* scales = value ? a.v_scale : a.k_scale;
-  const int64_t from = layer * (value ? a.vn_sl : a.kn_sl) + t * (value ? a.vn_st : a.kn_st);
-  const int64_t from_h = value ? a.vn_sh : a.kn_sh;
-  for (int i = threadIdx.x; i < a.Hkv * a.D; i += 256) {
-    const int h = i / a.D, d = i - h * a.D;
+  for (int i = threadIdx.x; i < 2 * per; i += blockDim.x) {
+    const bool value = i >= per;
+    const int e = 8 * (value ? i - per : i), h = e / a.D, d = e - h * a.D;
+    const int64_t from = layer * (value ? a.vn_sl : a.kn_sl) + t * (value ? a.vn_st : a.kn_st) + h * (value ? a.vn_sh : a.kn_sh) + d;
     const int64_t at = base + h * a.head_stride + d;
-    const uint16_t raw = static_cast<const uint16_t*>(src)[from + h * from_h + d];
+    const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(value ? a.v_new : a.k_new) + from);
+    void* cache = value ? a.v : a.k;
     if (a.cache_dtype != CQ_DT_FP8_E4M3) {
-      static_cast<uint16_t*>(cache)[at] = raw;
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(cache) + at) = raw;
       continue;
     }
-    const float x = a.dtype == CQ_DT_F16 ? __half2float(__ushort_as_half(raw)) : bf16_bits_to_f32(raw);
-    static_cast<__nv_fp8_storage_t*>(cache)[at] =
-        __nv_cvt_float_to_fp8(scales != nullptr ? __fdiv_rn(x, scales[h]) : x, __NV_SATFINITE, __NV_E4M3);
+    const float* scales = value ? a.v_scale : a.k_scale;
+    const float scale = scales != nullptr ? scales[h] : 1.0f;
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    uint32_t out[2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = a.dtype == CQ_DT_F16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[j]))
+                                            : make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+      const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(f.x, scale), __fdiv_rn(f.y, scale)), __NV_SATFINITE, __NV_E4M3);
+      out[j >> 1] = j & 1 ? out[j >> 1] | two << 16 : two;
+    }
+    *reinterpret_cast<uint2*>(static_cast<__nv_fp8_storage_t*>(cache) + at) = make_uint2(out[0], out[1]);
   }
 }
 
 cudaError_t launch_kv_append(const AppendArgs& a, cudaStream_t st) {
   if (a.T == 0 || a.layers == 0) return cudaSuccess;
-  kv_append_kernel<<<dim3(a.T, a.layers, 2), 256, 0, st>>>(a);
-  return cudaGetLastError();
+  const int threads = (2 * a.Hkv * a.D / 8 + 31) / 32 * 32;
+  return launch_early(kv_append_kernel, dim3(a.T, a.layers), threads < 256 ? threads : 256, 0, st, a);
 }
 
 }  // namespace cq

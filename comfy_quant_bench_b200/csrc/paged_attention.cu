@@ -17,8 +17,7 @@
 // by a second small kernel in the order of its parts.  Both orders are fixed, so equal calls give equal bits.
 //
 // Softmax statistics, scores and outputs are fp32.  The weights p enter the second product as two parts of the cache's
-// 16-bit type, p = hi + lo, since one part alone would add as much error as rounding the output does.  Where the type is
-// f16 (an 8-bit cache) and the output bf16, one part is enough: its error, 2^-12, is a sixteenth of the rounding's.
+// 16-bit type, p = hi + lo, since one part alone would add up to as much error as rounding the output does.
 // 8-bit caches are widened exactly to f16; a bf16 query is scaled by a power of two per head so that f16 holds it to
 // 2^-24 of its largest element.
 #include "decode_common.cuh"
@@ -137,7 +136,6 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
   using C = pattn::Cfg<D, FP8 ? 1 : 2, NT>;
   constexpr int ES = FP8 ? 1 : 2, kRow = C::kRow, kStages = C::kStages;
   constexpr bool kF16Math = F16 || FP8;
-  constexpr bool kSplit = !FP8 || F16;                  // the weights enter as two parts
   constexpr int kHeads = 8 * NT;                        // heads of a tile
   constexpr int kMt = D / 16;                           // 16-wide slices of the head dim
   extern __shared__ __align__(128) uint8_t smem[];
@@ -426,7 +424,7 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           ph[n][j] = movmatrix_t(ph[n][j]);
-          if constexpr (kSplit) pl[n][j] = movmatrix_t(pl[n][j]);
+          pl[n][j] = movmatrix_t(pl[n][j]);
         }
       }
       if (__any_sync(0xffffffffu, grew)) {
@@ -463,7 +461,7 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               mma_16816<true>(o[2 * ip + half][n], va, ph[n][0], ph[n][1]);
-              if constexpr (kSplit) mma_16816<true>(o[2 * ip + half][n], va, pl[n][0], pl[n][1]);
+              mma_16816<true>(o[2 * ip + half][n], va, pl[n][0], pl[n][1]);
             }
           }
         }
