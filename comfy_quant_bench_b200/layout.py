@@ -176,6 +176,21 @@ class B200AffineW4A8Layout(QuantizedLayout):
                                   zeros_prepared=cls.prepared_zeros(params))
 
 
+class B200AwqW4A16Layout(B200AffineW4A8Layout):
+    """awq_w4a16: the affine int4 weight with 16-bit activations (a language model's weights; groups of 32, 64 or 128).
+    The activations are not quantized, so an activation function before the linear is not folded in."""
+    QUANTIZES_INPUT = False
+
+    @classmethod
+    def linear(cls, x, qdata, params, bias=None, input_act=None):
+        from .ops import w4a16_linear
+        if input_act is not None:
+            raise ValueError("awq_w4a16 has no activation quantizer to fold input_act into")
+        if x.dtype not in (torch.bfloat16, torch.float16):
+            x = x.to(torch.bfloat16)
+        return w4a16_linear(x, qdata, params.scale, params.zeros, bias, group_size=params.group_size)
+
+
 class B200TensorWiseINT8Layout(QuantizedLayout):
     """int8_tensorwise: int8 weight [N, K] (optionally ConvRot) + f32 scale [N, 1]."""
 
@@ -275,6 +290,12 @@ def _affine_params(layer_name, module, weight, pop_scale, layer_conf):
             "convrot_groupsize": int(layer_conf.get("convrot_groupsize", params_conf.get("convrot_groupsize", 0)))}
 
 
+def _awq_params(layer_name, module, weight, pop_scale, layer_conf):
+    # the tensors of the affine layout, never rotated; without a group size in the metadata, groups of 64
+    params = _affine_params(layer_name, module, weight, pop_scale, layer_conf)
+    return {"scale": params["scale"], "zeros": params["zeros"], "group_size": F.format_from_config(layer_conf).group_size}
+
+
 def _int8_params(layer_name, module, weight, pop_scale, layer_conf):
     scale = pop_scale("weight_scale")
     if scale is None:
@@ -286,6 +307,7 @@ def _int8_params(layer_name, module, weight, pop_scale, layer_conf):
 LAYOUTS = {
     "B200ConvRotW4A4Layout": B200ConvRotW4A4Layout,
     "B200AffineW4A8Layout": B200AffineW4A8Layout,
+    "B200AwqW4A16Layout": B200AwqW4A16Layout,
     "B200TensorWiseINT8Layout": B200TensorWiseINT8Layout,
 }
 
@@ -296,6 +318,9 @@ ALGOS = {
     F.AffineW4A8.name: {"storage_t": torch.int8, "parameters": {"weight_scale", "weight_zeros"},
                         "comfy_tensor_layout": "B200AffineW4A8Layout", "quantize_input": True,
                         "params_from_state_dict": _affine_params},
+    F.AwqW4A16.name: {"storage_t": torch.int8, "parameters": {"weight_scale", "weight_zeros"},
+                      "comfy_tensor_layout": "B200AwqW4A16Layout", "quantize_input": False,
+                      "params_from_state_dict": _awq_params},
     F.Int8Tensorwise.name: {"storage_t": torch.int8, "parameters": {"weight_scale"},
                             "comfy_tensor_layout": "B200TensorWiseINT8Layout", "quantize_input": True,
                             "params_from_state_dict": _int8_params},
