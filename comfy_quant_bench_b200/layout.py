@@ -307,7 +307,6 @@ def _int8_params(layer_name, module, weight, pop_scale, layer_conf):
 LAYOUTS = {
     "B200ConvRotW4A4Layout": B200ConvRotW4A4Layout,
     "B200AffineW4A8Layout": B200AffineW4A8Layout,
-    "B200AwqW4A16Layout": B200AwqW4A16Layout,
     "B200TensorWiseINT8Layout": B200TensorWiseINT8Layout,
 }
 
@@ -318,28 +317,43 @@ ALGOS = {
     F.AffineW4A8.name: {"storage_t": torch.int8, "parameters": {"weight_scale", "weight_zeros"},
                         "comfy_tensor_layout": "B200AffineW4A8Layout", "quantize_input": True,
                         "params_from_state_dict": _affine_params},
-    F.AwqW4A16.name: {"storage_t": torch.int8, "parameters": {"weight_scale", "weight_zeros"},
-                      "comfy_tensor_layout": "B200AwqW4A16Layout", "quantize_input": False,
-                      "params_from_state_dict": _awq_params},
     F.Int8Tensorwise.name: {"storage_t": torch.int8, "parameters": {"weight_scale"},
                             "comfy_tensor_layout": "B200TensorWiseINT8Layout", "quantize_input": True,
                             "params_from_state_dict": _int8_params},
 }
 
 
+# Registered on request only: a ComfyUI with the awq_w4a16 patch has an entry of its own for the format.
+W4A16_LAYOUTS = {"B200AwqW4A16Layout": B200AwqW4A16Layout}
+W4A16_ALGOS = {
+    F.AwqW4A16.name: {"storage_t": torch.int8, "parameters": {"weight_scale", "weight_zeros"},
+                      "comfy_tensor_layout": "B200AwqW4A16Layout", "quantize_input": False,
+                      "params_from_state_dict": _awq_params},
+}
+
+
 def register(target=None) -> str:
     """Register the layouts and formats.  ``target``: a ``comfy.quant_ops``-like module; by default the live
     ComfyUI one if importable, else this module's registry.  Returns where they went."""
+    return _register(target, LAYOUTS, ALGOS)
+
+
+def register_w4a16(target=None) -> str:
+    """``register`` for awq_w4a16: checkpoints of that format run through ``ops.w4a16_linear``."""
+    return _register(target, W4A16_LAYOUTS, W4A16_ALGOS)
+
+
+def _register(target, layouts, algos) -> str:
     if target is None:
         try:
             import comfy.quant_ops as target  # type: ignore[no-redef]
         except Exception:  # noqa: BLE001 - no ComfyUI in this process
             target = None
-    for name, cls in LAYOUTS.items():
+    for name, cls in layouts.items():
         register_layout_class(name, cls)
         if target is not None:
             target.register_layout_class(name, cls)
-    for fmt, algo in ALGOS.items():
+    for fmt, algo in algos.items():
         QUANT_ALGOS[fmt] = dict(algo)
         if target is not None:
             target.QUANT_ALGOS[fmt] = dict(algo)

@@ -121,3 +121,21 @@ def test_refusals_say_what_is_wrong():
                        ("do not fit", lambda: kvcache.append_kv(query, query, k, k, t, n, n))):
         with pytest.raises(ValueError, match=says):
             call()
+
+
+def test_awq_layout_is_registered_on_request():
+    import types
+
+    from comfy_quant_bench_b200 import layout
+    fake = types.SimpleNamespace(QUANT_ALGOS={}, layouts={}, __name__="comfy.quant_ops")
+    fake.register_layout_class = lambda name, cls: fake.layouts.__setitem__(name, cls)
+    layout.register(target=fake)
+    assert "awq_w4a16" not in fake.QUANT_ALGOS
+    assert layout.register_w4a16(target=fake) == "comfy.quant_ops"
+    algo = fake.QUANT_ALGOS["awq_w4a16"]
+    assert algo["comfy_tensor_layout"] in fake.layouts and not algo["quantize_input"]
+    params = algo["params_from_state_dict"]("l", None, None, {"weight_scale": 1, "weight_zeros": 2}.get,
+                                            {"format": "awq_w4a16", "group_size": 32})
+    assert params == {"scale": 1, "zeros": 2, "group_size": 32}
+    with pytest.raises(ValueError):
+        algo["params_from_state_dict"]("l", None, None, lambda name: None, {"format": "awq_w4a16"})

@@ -147,7 +147,7 @@ def test_awq_layer_of_a_checkpoint_runs(tg):
     import json
 
     from comfy_quant_bench_b200 import comfy_ops, layout, ops
-    layout.register()
+    layout.register_w4a16()
     g = torch.Generator(device="cuda").manual_seed(2)
     w = torch.randn(96, 256, generator=g, device="cuda")
     q, s, z = ops.quantize_affine_w4_weight(w, 64)
