@@ -33,22 +33,22 @@ constexpr int kMinUnits = 4;
 // Rows of at most this many units are never split: one launch, no join.
 constexpr int kWholeUnits = 12;
 
-// shared memory: ring, query fragments, joined output, per-warp statistics
+// shared memory: ring (a consumed stage holds its warp's outputs while the warps are joined), query fragments, statistics
 template <int D, int ES, int NT>
 struct Cfg {
   static constexpr int kRow = D * ES;                          // bytes of one key
   static constexpr int kTileBytes = kTile * kRow;              // one operand's tile
   static constexpr int kStageBytes = 2 * kTileBytes;
   static constexpr int kQ = D / 16 * NT * 256;
-  static constexpr int kO = 8 * NT * D * 4;
   static constexpr int kMisc = 8 * NT * 4 * (2 * kWarps + 1) + 16;
-  static constexpr int kFixed = kQ + kO + kMisc;
+  static constexpr int kFixed = kQ + kMisc;
   static constexpr int kCtas = 3 * kWarps * kStageBytes + kFixed <= 112 * 1024 ? 2 : 1;
   static constexpr int kFit = ((kCtas == 2 ? 112 : 224) * 1024 - kFixed) / (kWarps * kStageBytes);
   static constexpr int kStages = kFit < 8 ? kFit : 8;
   static constexpr int kMaskBytes = kWarps * kStages * 4;
   static constexpr int kSmem = kWarps * kStages * kStageBytes + kFixed + kMaskBytes;
   static_assert(kStages >= 3, "ring of three stages");
+  static_assert(8 * D * 4 <= kStageBytes, "eight heads' outputs fit a stage");
 };
 
 struct Meta {          // one CTA's run, for the join: its first part's segment, first unit there, the segment's units
@@ -114,21 +114,30 @@ __device__ __forceinline__ RowView row_view(const PagedAttnArgs& a, int b) {
   return v;
 }
 
-// a place in the sequence of units: row b, head tile, unit of that segment
+// a place in the sequence of units: row b, key-value head, tile of its query heads, unit of that segment
 struct UnitIter {
-  int b, head, unit;
+  int b, hk, ht, unit;
   RowView v;
-  __device__ __forceinline__ void next(const PagedAttnArgs& a, int heads) {
+  __device__ __forceinline__ void next(const PagedAttnArgs& a, int head_tiles) {
     if (++unit < v.units) return;
     unit = 0;
-    if (++head < heads) return;
-    head = 0;
+    if (++ht < head_tiles) return;
+    ht = 0;
+    if (++hk < a.Hkv) return;
+    hk = 0;
     while (++b < a.B) {
       v = row_view(a, b);
       if (v.units > 0) break;
     }
   }
 };
+
+// 2^x to 2^-22 of it; below 2^-126 zero
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 template <bool F16, bool FP8, int D, int NT>
 __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2, NT>::kCtas)
@@ -141,8 +150,7 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* ring = smem;
   uint2* qfrag = reinterpret_cast<uint2*>(smem + pattn::kWarps * kStages * C::kStageBytes);
-  float* obuf = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(qfrag) + C::kQ);   // [D][kHeads]
-  float* sm_m = obuf + kHeads * D;                      // [kWarps][kHeads]
+  float* sm_m = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(qfrag) + C::kQ);   // [kWarps][kHeads]
   float* sm_l = sm_m + pattn::kWarps * kHeads;
   float* qmul = sm_l + pattn::kWarps * kHeads;          // [kHeads] score multiplier
   int* start = reinterpret_cast<int*>(qmul + kHeads);   // the run's first (b, head, unit)
@@ -167,7 +175,8 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
       s = upto;
     }
     it.b = b0;
-    it.head = h0;
+    it.hk = h0 / head_tiles;
+    it.ht = h0 - it.hk * head_tiles;
     it.unit = 0;
   } else {                                              // equal runs of units
     __shared__ int64_t wsum[pattn::kWarps];
@@ -209,7 +218,9 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
     }
     __syncthreads();
     it.b = count > 0 ? start[0] : 0;
-    it.head = count > 0 ? start[1] : 0;
+    const int head = count > 0 ? start[1] : 0;
+    it.hk = head / head_tiles;
+    it.ht = head - it.hk * head_tiles;
     it.unit = count > 0 ? start[2] : 0;
   }
   // rows that see nothing belong to no unit: their zeros
@@ -223,7 +234,7 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
   float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) + gridDim.x * sizeof(pattn::Meta));
   if (!whole && tid == 0) {
     pattn::Meta m{0, 0, 0, static_cast<int>(count)};
-    if (count > 0) m = {it.b * heads + it.head, it.unit, row_view(a, it.b).units, static_cast<int>(count)};
+    if (count > 0) m = {it.b * heads + it.hk * head_tiles + it.ht, it.unit, row_view(a, it.b).units, static_cast<int>(count)};
     static_cast<pattn::Meta*>(a.ws)[blockIdx.x] = m;
   }
   if (count == 0) return;
@@ -234,65 +245,66 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
   const uint32_t my_ring_u = smem_u32(my_ring);
   uint32_t* my_masks = masks + warp * kStages;
   const int page_shift = 31 - __clz(a.page_size), page_mask = a.page_size - 1;
-  // lane r < 16 looks after key r of the tile; its page index is loaded one step before the copies need it
+  // lane r < 16 looks after key r of the tile; its page index is loaded a step before the copies need it
+  struct Place {
+    int page;
+    int64_t inner;
+  };
   UnitIter ahead = it;
-  int page = -1;
-  int64_t inner = 0;
   auto look_up = [&]() {
     const int i = ahead.unit * pattn::kUnit + warp * pattn::kTile + (lane & 15);
-    page = -1;
+    Place p{-1, 0};
     if (i < ahead.v.vis) {
       const int j = i < ahead.v.nsink ? i : ahead.v.n - ahead.v.vis + i;
-      page = __ldg(a.table + ahead.v.row * a.table_stride + (j >> page_shift));
-      inner = (ahead.head / head_tiles) * a.head_stride + (j & page_mask) * a.tok_stride;
+      p.page = __ldg(a.table + ahead.v.row * a.table_stride + (j >> page_shift));
+      p.inner = ahead.hk * a.head_stride + (j & page_mask) * a.tok_stride;
+    }
+    ahead.next(a, head_tiles);
+    return p;
+  };
+  auto copy = [&](int stage, const Place& p) {
+    const bool ok = p.page >= 0 && p.page < a.num_pages;
+    const uint32_t mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+    if (lane == 0) my_masks[stage] = mask;
+    if (mask == 0) return;
+    const int64_t off = ok ? (p.page * a.page_stride + p.inner) * ES : 0;
+    constexpr int kChunks = kRow / 16;                  // 16-byte chunks of a row: 4 to 32
+    constexpr int kRows = 32 / kChunks;                 // rows of one copy instruction
+    const uint32_t dst = my_ring_u + stage * C::kStageBytes;
+    const int ch = lane % kChunks;
+#pragma unroll
+    for (int r0 = 0; r0 < pattn::kTile; r0 += kRows) {
+      const int r = r0 + lane / kChunks;
+      const int64_t o = __shfl_sync(0xffffffffu, off, r) + 16 * ch;
+      const bool valid = mask >> r & 1u;
+      const uint32_t to = dst + swz<kRow>(r, ch);
+      cp_async16(to, static_cast<const uint8_t*>(a.k) + o, valid);
+      cp_async16(to + C::kTileBytes, static_cast<const uint8_t*>(a.v) + o, valid);
     }
   };
-  int64_t looked = 0;                                   // units looked up
-  auto issue = [&](int stage) {                         // copies of the tile looked up last, and the next look-up
-    if (looked <= count) {
-      const bool ok = page >= 0 && page < a.num_pages;
-      const uint32_t mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
-      if (lane == 0) my_masks[stage] = mask;
-      if (mask != 0) {
-        const int64_t off = ok ? (page * a.page_stride + inner) * ES : 0;
-        const uint32_t dst = my_ring_u + stage * C::kStageBytes;
-        constexpr int kChunks = kRow / 16;              // 16-byte chunks of a row: 4 to 32
-        constexpr int kRows = 32 / kChunks;             // rows of one copy instruction
+  Place place[kStages], next_place{-1, 0};
 #pragma unroll
-        for (int r0 = 0; r0 < pattn::kTile; r0 += kRows) {
-          const int r = r0 + lane / kChunks, ch = lane % kChunks;
-          const int64_t o = __shfl_sync(0xffffffffu, off, r);
-          const bool valid = mask >> r & 1u;
-          const uint32_t to = dst + swz<kRow>(r, ch);
-          cp_async16(to, static_cast<const uint8_t*>(a.k) + o + 16 * ch, valid);
-          cp_async16(to + C::kTileBytes, static_cast<const uint8_t*>(a.v) + o + 16 * ch, valid);
-        }
-      }
-    }
+  for (int s = 0; s < kStages; ++s)                     // the first pages' indexes are loaded together
+    if (s < count) place[s] = look_up();
+#pragma unroll
+  for (int s = 0; s < kStages; ++s) {
+    if (s < count) copy(s, place[s]);
     cp_async_commit();
-    if (looked < count) {
-      ahead.next(a, heads);
-      look_up();
-    }
-    ++looked;
-  };
-  look_up();
-  ++looked;
-#pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) issue(s);
+  }
+  if (kStages < count) next_place = look_up();
 
   // ---- units --------------------------------------------------------------------------------
   const float log2e = 1.4426950408889634f;
   float o[kMt][NT][4], m[NT][2], l[NT][2], mul[NT][2];
-  int part = 0, part_begin = 0;
+  int part = 0, part_begin = 0, h0 = 0, nh = 0;
   bool fresh = true;
   int stage = 0;
   for (int64_t t = 0; t < count; ++t) {
-    const int hk = it.head / head_tiles, h0 = hk * group + (it.head - hk * head_tiles) * kHeads;
-    const int nh = min(kHeads, (hk + 1) * group - h0);
     if (fresh) {
       fresh = false;
       part_begin = it.unit;
+      h0 = it.hk * group + it.ht * kHeads;
+      nh = min(kHeads, (it.hk + 1) * group - h0);
       // the tile's query heads as the second operand's fragments, one warp per head
       for (int h = warp; h < kHeads; h += pattn::kWarps) {
         const uint16_t* src = static_cast<const uint16_t*>(a.q) + it.b * a.q_sb + (h0 + h) * a.q_sh;
@@ -341,7 +353,7 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
           if (e < D / 4) qfrag[((e >> 2) * NT + (h >> 3)) * 32 + (h & 7) * 4 + (e & 3)] = w[i];
         }
         if (lane == 0)
-          qmul[h] = a.scale * log2e * factor * (FP8 && a.k_scale != nullptr ? __ldg(a.k_scale + hk) : 1.0f);
+          qmul[h] = a.scale * log2e * factor * (FP8 && a.k_scale != nullptr ? __ldg(a.k_scale + it.hk) : 1.0f);
       }
       __syncthreads();
 #pragma unroll
@@ -356,7 +368,7 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
           for (int j = 0; j < 4; ++j) o[i][n][j] = 0.0f;
       }
     }
-    cp_async_wait<kStages - 2>();
+    cp_async_wait<kStages - 1>();
     __syncwarp();
     const uint32_t mask = my_masks[stage];
     if (mask != 0) {
@@ -412,11 +424,11 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
           const float mn = fmaxf(m[n][j], top), base = mn == -INFINITY ? 0.0f : mn;   // all may be -inf so far
-          f[n][j] = exp2f(m[n][j] - base);
+          f[n][j] = exp2_fast(m[n][j] - base);
           grew |= mn != m[n][j];
           m[n][j] = mn;
-          s[n][j] = exp2f(x0 - base);
-          s[n][2 + j] = exp2f(x1 - base);
+          s[n][j] = exp2_fast(x0 - base);
+          s[n][2 + j] = exp2_fast(x1 - base);
           l[n][j] = l[n][j] * f[n][j] + (s[n][j] + s[n][2 + j]);
         }
         split16<kF16Math>(s[n][0], s[n][1], ph[n][0], pl[n][0]);
@@ -468,92 +480,99 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
       }
     }
     __syncwarp();
-    issue(stage == 0 ? kStages - 1 : stage - 1);
-    stage = stage + 1 == kStages ? 0 : stage + 1;
-
     const bool seg_end = it.unit + 1 == it.v.units;
-    if (!seg_end && t + 1 < count) { ++it.unit; continue; }
-
-    // ---- the end of this CTA's part of the segment: join the warps ------------------------------
+    if (seg_end || t + 1 == count) {
+      // ---- the end of this CTA's part of the segment: join the warps, eight heads at a time ------
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < 2; ++j) {
 #pragma unroll
-        for (int x = 4; x < 32; x <<= 1) l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], x);
-        if (g == 0) {
-          sm_m[warp * kHeads + 8 * n + 2 * c + j] = m[n][j];
-          sm_l[warp * kHeads + 8 * n + 2 * c + j] = l[n][j];
+          for (int x = 4; x < 32; x <<= 1) l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], x);
+          if (g == 0) {
+            sm_m[warp * kHeads + 8 * n + 2 * c + j] = m[n][j];
+            sm_l[warp * kHeads + 8 * n + 2 * c + j] = l[n][j];
+          }
         }
-      }
-    __syncthreads();
+      __syncthreads();                                    // and every warp is done with its tile
+      const bool complete = seg_end && part_begin == 0;
+      const float vs = FP8 && a.v_scale != nullptr ? __ldg(a.v_scale + it.hk) : 1.0f;
+      const uint8_t* slot = ring + stage * C::kStageBytes;
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) {
+        float* mine = reinterpret_cast<float*>(my_ring + stage * C::kStageBytes);   // [D][8]
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int h = 8 * n + 2 * c + j;
-        float top = sm_m[h];
+        for (int j = 0; j < 2; ++j) {
+          const int h = 8 * n + 2 * c + j;
+          float top = sm_m[h];
 #pragma unroll
-        for (int w = 1; w < pattn::kWarps; ++w) top = fmaxf(top, sm_m[w * kHeads + h]);
-        const float f = m[n][j] == -INFINITY ? 0.0f : exp2f(m[n][j] - top);
+          for (int w = 1; w < pattn::kWarps; ++w) top = fmaxf(top, sm_m[w * kHeads + h]);
+          const float f = m[n][j] == -INFINITY ? 0.0f : exp2_fast(m[n][j] - top);
 #pragma unroll
-        for (int i = 0; i < kMt; ++i) {
-          o[i][n][j] *= f;
-          o[i][n][2 + j] *= f;
+          for (int i = 0; i < kMt; ++i) {
+            o[i][n][j] *= f;
+            o[i][n][2 + j] *= f;
+          }
         }
-      }
-    for (int w = 0; w < pattn::kWarps; ++w) {
-      if (w == warp) {
 #pragma unroll
         for (int i = 0; i < kMt; ++i)
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+          for (int r = 0; r < 2; ++r) {
+            const int d = FP8 ? 16 * i + 2 * g + r : 16 * i + g + 8 * r;
+            *reinterpret_cast<float2*>(mine + d * 8 + 2 * c) = make_float2(o[i][n][2 * r], o[i][n][2 * r + 1]);
+          }
+        __syncthreads();
+        const int h8 = tid & 7, h = 8 * n + h8;           // this thread's head
+        float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const int d = FP8 ? 16 * i + 2 * g + r : 16 * i + g + 8 * r;
-              float2* to = reinterpret_cast<float2*>(obuf + d * kHeads + 8 * n + 2 * c);
-              float2 v = make_float2(o[i][n][2 * r], o[i][n][2 * r + 1]);
-              if (w > 0) { const float2 u = *to; v.x += u.x; v.y += u.y; }
-              *to = v;
-            }
-      }
-      __syncthreads();
-    }
-    const bool complete = seg_end && part_begin == 0;
-    const float vs = FP8 && a.v_scale != nullptr ? __ldg(a.v_scale + hk) : 1.0f;
-    for (int i = tid; i < nh * (D / 2); i += blockDim.x) {
-      const int h = i / (D / 2), d = 2 * (i - h * (D / 2));
-      float top = -INFINITY, sum = 0.0f;
+        for (int w = 0; w < pattn::kWarps; ++w) top = fmaxf(top, sm_m[w * kHeads + h]);
 #pragma unroll
-      for (int w = 0; w < pattn::kWarps; ++w) top = fmaxf(top, sm_m[w * kHeads + h]);
-#pragma unroll
-      for (int w = 0; w < pattn::kWarps; ++w)
-        if (sm_m[w * kHeads + h] != -INFINITY) sum += sm_l[w * kHeads + h] * exp2f(sm_m[w * kHeads + h] - top);
-        else sum += sm_l[w * kHeads + h];                 // zero, or NaN where a score was NaN
-      float2 v = make_float2(obuf[d * kHeads + h], obuf[(d + 1) * kHeads + h]);
-      if (complete) {
-        const float inv = sum == 0.0f ? 0.0f : vs / sum;
-        const int64_t at = (static_cast<int64_t>(it.b) * a.Hq + h0 + h) * D + d;
-        if constexpr (F16)
-          *reinterpret_cast<__half2*>(static_cast<__half*>(a.out) + at) = __floats2half2_rn(v.x * inv, v.y * inv);
-        else
-          *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.out) + at) =
-              __floats2bfloat162_rn(v.x * inv, v.y * inv);
-        if (d == 0 && a.lse != nullptr)
-          a.lse[static_cast<int64_t>(it.b) * a.Hq + h0 + h] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) / log2e;
-      } else {
-        float* p = parts + (static_cast<int64_t>(blockIdx.x) * 2 + min(part, 1)) * kHeads * (D + 2);
-        *reinterpret_cast<float2*>(p + h * D + d) = v;
-        if (d == 0) {
-          p[kHeads * D + h] = top;
-          p[kHeads * D + kHeads + h] = sum;
+        for (int w = 0; w < pattn::kWarps; ++w) {
+          const float mw = sm_m[w * kHeads + h], lw = sm_l[w * kHeads + h];
+          sum += mw == -INFINITY ? lw : lw * exp2_fast(mw - top);   // without a maximum: zero, or NaN where a score was NaN
         }
+        if (h < nh) {
+          const float inv = sum == 0.0f ? 0.0f : vs / sum;
+          float* p = parts + (static_cast<int64_t>(blockIdx.x) * 2 + min(part, 1)) * kHeads * (D + 2);
+          const int64_t to = (static_cast<int64_t>(it.b) * a.Hq + h0 + h) * D;
+#pragma unroll
+          for (int d = 2 * (tid >> 3); d < D; d += 2 * (pattn::kWarps * 32 / 8)) {
+            float2 v = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < pattn::kWarps; ++w) {     // in the order of the warps
+              const float* from = reinterpret_cast<const float*>(slot + w * kStages * C::kStageBytes) + d * 8 + h8;
+              v.x += from[0];
+              v.y += from[8];
+            }
+            if (!complete) {
+              *reinterpret_cast<float2*>(p + h * D + d) = v;
+            } else if constexpr (F16) {
+              *reinterpret_cast<__half2*>(static_cast<__half*>(a.out) + to + d) = __floats2half2_rn(v.x * inv, v.y * inv);
+            } else {
+              *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.out) + to + d) =
+                  __floats2bfloat162_rn(v.x * inv, v.y * inv);
+            }
+          }
+          if (tid < 8 && !complete) {
+            p[kHeads * D + h] = top;
+            p[kHeads * D + kHeads + h] = sum;
+          }
+          if (tid < 8 && complete && a.lse != nullptr)
+            a.lse[static_cast<int64_t>(it.b) * a.Hq + h0 + h] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) / log2e;
+        }
+        __syncthreads();                                  // the slots and the statistics are read
       }
+      ++part;
+      fresh = true;
     }
-    __syncthreads();                                      // obuf and the statistics are read
-    ++part;
-    fresh = true;
-    it.next(a, heads);
+    // the consumed stage takes the tile kStages ahead
+    if (t + kStages < count) {
+      copy(stage, next_place);
+      if (t + kStages + 1 < count) next_place = look_up();
+    }
+    cp_async_commit();
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+    it.next(a, head_tiles);
   }
   cp_async_wait<0>();
 }
