@@ -30,8 +30,12 @@ constexpr int kTile = 16;                    // keys per warp and step
 constexpr int kUnit = kWarps * kTile;
 // A row is split no finer than this: a part costs its CTA a start and an end (about two units' time), and the join.
 constexpr int kMinUnits = 4;
-// Rows of at most this many units are never split: one launch, no join.
+// Rows of at most this many units are never split over runs: one launch, no join.
 constexpr int kWholeUnits = 12;
+// CTAs of a resident grid (two per SM), and the most units of a cluster's CTA: with few segments of up to so many units
+// a cluster each is quicker than runs over all SMs and their join (8 segments of 4000 keys: 14 and 10 us).
+constexpr int kMaxRuns = 2 * 148;
+constexpr int kClusterUnits = 16;
 
 // shared memory: ring (a consumed stage holds its warp's outputs while the warps are joined), query fragments, statistics
 template <int D, int ES, int NT>
@@ -50,6 +54,10 @@ struct Cfg {
   static_assert(kStages >= 3, "ring of three stages");
   static_assert(8 * D * 4 <= kStageBytes, "eight heads' outputs fit a stage");
 };
+
+// How the units are dealt out: equal runs of units, joined by a second kernel where a row is split; runs of whole
+// segments; or a cluster of CTAs per segment, which join over distributed shared memory.
+enum Mode { kRuns, kSegments, kClusters };
 
 struct Meta {          // one CTA's run, for the join: its first part's segment, first unit there, the segment's units
   int seg, unit0, units, count;
@@ -139,9 +147,10 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-template <bool F16, bool FP8, int D, int NT>
+// kCluster: the form for Mode kClusters, apart so that the others do not hold its registers
+template <bool F16, bool FP8, int D, int NT, bool kCluster>
 __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2, NT>::kCtas)
-    paged_attention_kernel(const PagedAttnArgs a, const int head_tiles, const int whole) {
+    paged_attention_kernel(const PagedAttnArgs a, const int head_tiles, const pattn::Mode mode, const int cluster) {
   using C = pattn::Cfg<D, FP8 ? 1 : 2, NT>;
   constexpr int ES = FP8 ? 1 : 2, kRow = C::kRow, kStages = C::kStages;
   constexpr bool kF16Math = F16 || FP8;
@@ -157,12 +166,20 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
   uint32_t* masks = reinterpret_cast<uint32_t*>(start + 4);   // [kWarps][kStages] valid keys of a tile
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
   const int group = a.Hq / a.Hkv, heads = a.Hkv * head_tiles;
-  if (!whole) grid_dep_launch();                        // the join may be set up while this grid runs
+  if (mode == pattn::kRuns) grid_dep_launch();                        // the join may be set up while this grid runs
 
   // ---- this CTA's run of units --------------------------------------------------------------
   int64_t count = 0;
   UnitIter it;
-  if (whole) {                                          // runs of whole segments
+  if constexpr (kCluster) {                             // this CTA's share of the cluster's segment
+    const int seg = blockIdx.x / cluster, rank = static_cast<int>(cluster_ctarank());
+    it.b = seg / heads;
+    const int head = seg - it.b * heads, units = row_view(a, it.b).units;
+    it.hk = head / head_tiles;
+    it.ht = head - it.hk * head_tiles;
+    it.unit = static_cast<int>(static_cast<int64_t>(rank) * units / cluster);
+    count = static_cast<int64_t>(rank + 1) * units / cluster - it.unit;
+  } else if (mode == pattn::kSegments) {                // runs of whole segments
     const int64_t segs = static_cast<int64_t>(a.B) * heads;
     const int64_t s0 = blockIdx.x * segs / gridDim.x, s1 = (blockIdx.x + 1) * segs / gridDim.x;
     int b0 = static_cast<int>(s0 / heads), h0 = static_cast<int>(s0 % heads);
@@ -232,13 +249,13 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
       for (int i = tid; i < a.Hq; i += blockDim.x) a.lse[static_cast<int64_t>(b) * a.Hq + i] = -INFINITY;
   }
   float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) + gridDim.x * sizeof(pattn::Meta));
-  if (!whole && tid == 0) {
+  if (mode == pattn::kRuns && tid == 0) {
     pattn::Meta m{0, 0, 0, static_cast<int>(count)};
     if (count > 0) m = {it.b * heads + it.hk * head_tiles + it.ht, it.unit, row_view(a, it.b).units, static_cast<int>(count)};
     static_cast<pattn::Meta*>(a.ws)[blockIdx.x] = m;
   }
-  if (count == 0) return;
   it.v = row_view(a, it.b);
+  if (count == 0 && (!kCluster || it.v.units == 0)) return;
 
   // ---- the warp's ring ----------------------------------------------------------------------
   uint8_t* my_ring = ring + warp * kStages * C::kStageBytes;
@@ -296,7 +313,17 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
   // ---- units --------------------------------------------------------------------------------
   const float log2e = 1.4426950408889634f;
   float o[kMt][NT][4], m[NT][2], l[NT][2], mul[NT][2];
-  int part = 0, part_begin = 0, h0 = 0, nh = 0;
+  int part = 0, part_begin = 0, h0 = it.hk * group + it.ht * kHeads, nh = min(kHeads, (it.hk + 1) * group - h0);
+  // a cluster's CTA: its part of the segment, as the join's parts are
+  float2 mine_o[NT][D / 32];
+  float mine_top[NT], mine_sum[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    mine_top[n] = -INFINITY;
+    mine_sum[n] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) mine_o[n][i] = make_float2(0.0f, 0.0f);
+  }
   bool fresh = true;
   int stage = 0;
   for (int64_t t = 0; t < count; ++t) {
@@ -495,7 +522,7 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
           }
         }
       __syncthreads();                                    // and every warp is done with its tile
-      const bool complete = seg_end && part_begin == 0;
+      const bool complete = seg_end && part_begin == 0 && !kCluster;
       const float vs = FP8 && a.v_scale != nullptr ? __ldg(a.v_scale + it.hk) : 1.0f;
       const uint8_t* slot = ring + stage * C::kStageBytes;
 #pragma unroll
@@ -535,8 +562,11 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
           const float inv = sum == 0.0f ? 0.0f : vs / sum;
           float* p = parts + (static_cast<int64_t>(blockIdx.x) * 2 + min(part, 1)) * kHeads * (D + 2);
           const int64_t to = (static_cast<int64_t>(it.b) * a.Hq + h0 + h) * D;
+          mine_top[n] = top;
+          mine_sum[n] = sum;
 #pragma unroll
-          for (int d = 2 * (tid >> 3); d < D; d += 2 * (pattn::kWarps * 32 / 8)) {
+          for (int i = 0; i < D / 32; ++i) {
+            const int d = 2 * (tid >> 3) + 32 * i;
             float2 v = make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int w = 0; w < pattn::kWarps; ++w) {     // in the order of the warps
@@ -544,16 +574,18 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
               v.x += from[0];
               v.y += from[8];
             }
-            if (!complete) {
+            if constexpr (kCluster) {
+              mine_o[n][i] = v;
+            } else if (!complete) {
               *reinterpret_cast<float2*>(p + h * D + d) = v;
-            } else if constexpr (F16) {
+            } else if (F16) {
               *reinterpret_cast<__half2*>(static_cast<__half*>(a.out) + to + d) = __floats2half2_rn(v.x * inv, v.y * inv);
             } else {
               *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.out) + to + d) =
                   __floats2bfloat162_rn(v.x * inv, v.y * inv);
             }
           }
-          if (tid < 8 && !complete) {
+          if (tid < 8 && !complete && !kCluster) {
             p[kHeads * D + h] = top;
             p[kHeads * D + kHeads + h] = sum;
           }
@@ -572,9 +604,56 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
     }
     cp_async_commit();
     stage = stage + 1 == kStages ? 0 : stage + 1;
-    it.next(a, head_tiles);
+    if (t + 1 < count) it.next(a, head_tiles);
   }
   cp_async_wait<0>();
+  if constexpr (kCluster) {
+    // ---- the cluster's join: every rank's part in its shared memory, the outputs dealt out over the ranks -------
+    __syncthreads();                                        // the ring is free
+    float* box = reinterpret_cast<float*>(ring);            // [kHeads][D] outputs, maxima, sums
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int h = 8 * n + (tid & 7);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) *reinterpret_cast<float2*>(box + h * D + 2 * (tid >> 3) + 32 * i) = mine_o[n][i];
+      if (tid < 8) {
+        box[kHeads * D + h] = mine_top[n];
+        box[kHeads * D + kHeads + h] = mine_sum[n];
+      }
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    const int rank = static_cast<int>(cluster_ctarank());
+    const float vs = FP8 && a.v_scale != nullptr ? __ldg(a.v_scale + it.hk) : 1.0f;
+    const uint32_t box_u = smem_u32(box);
+    auto remote = [&](int q, int i) {
+      float v;
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(box_u + 4 * i, q)));
+      return v;
+    };
+    for (int i = rank * blockDim.x + tid; i < nh * (D / 2); i += cluster * blockDim.x) {
+      const int h = i / (D / 2), d = 2 * (i - h * (D / 2));
+      float top = -INFINITY, sum = 0.0f;
+      for (int q = 0; q < cluster; ++q) top = fmaxf(top, remote(q, kHeads * D + h));
+      float2 v = make_float2(0.0f, 0.0f);
+      for (int q = 0; q < cluster; ++q) {                   // in the order of the ranks
+        const float m = remote(q, kHeads * D + h), s = remote(q, kHeads * D + kHeads + h);
+        const float f = m == -INFINITY ? 0.0f : exp2_fast(m - top);
+        sum += m == -INFINITY ? s : s * f;
+        v.x = fmaf(remote(q, h * D + d), f, v.x);
+        v.y = fmaf(remote(q, h * D + d + 1), f, v.y);
+      }
+      const float inv = sum == 0.0f ? 0.0f : vs / sum;
+      const int64_t to = (static_cast<int64_t>(it.b) * a.Hq + h0 + h) * D + d;
+      if constexpr (F16)
+        *reinterpret_cast<__half2*>(static_cast<__half*>(a.out) + to) = __floats2half2_rn(v.x * inv, v.y * inv);
+      else
+        *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.out) + to) = __floats2bfloat162_rn(v.x * inv, v.y * inv);
+      if (d == 0 && a.lse != nullptr)
+        a.lse[static_cast<int64_t>(it.b) * a.Hq + h0 + h] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) / log2e;
+    }
+    // a CTA's part stays until every rank has read it
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
 }
 
 // Joins the parts of a row that several CTAs shared, in their order.  CTA (r, h): the segment whose first boundary
@@ -636,51 +715,72 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(const PagedAt
 }
 
 namespace {
-constexpr int kMaxRuns = 2 * 148;
 }  // namespace
 
-// units of the row with the most visible keys
-static int64_t most_units(int64_t span, int64_t window, int64_t sinks) {
+namespace {
+struct Deal {
+  pattn::Mode mode;
+  int64_t units, segs;         // of the row with the most visible keys; segments
+  int cluster;
+};
+Deal deal_units(int64_t batch, int Hq, int Hkv, int64_t span, int64_t window, int64_t sinks) {
   if (window > 0 && window < span) span = sinks < span - window ? window + sinks : span;
-  return (span + pattn::kUnit - 1) / pattn::kUnit;
+  const int group = Hq / Hkv, tile = group <= 8 ? 8 : 16;
+  Deal d{pattn::kRuns, (span + pattn::kUnit - 1) / pattn::kUnit, batch * Hkv * ((group + tile - 1) / tile), 1};
+  while (d.cluster < 8 && d.cluster < d.units && d.segs * d.cluster * 2 <= pattn::kMaxRuns) d.cluster *= 2;
+  if (d.cluster > 1 && d.units <= static_cast<int64_t>(pattn::kClusterUnits) * d.cluster) d.mode = pattn::kClusters;
+  else if (d.units <= pattn::kWholeUnits) d.mode = pattn::kSegments;
+  return d;
 }
+}  // namespace
 
 int64_t paged_attention_workspace(int64_t batch, int Hq, int Hkv, int D, int64_t span, int64_t window, int64_t sinks) {
   const int heads = Hq / Hkv <= 8 ? 8 : 16;
-  return batch == 0 || most_units(span, window, sinks) <= pattn::kWholeUnits ? 0 : kMaxRuns * static_cast<int64_t>(sizeof(pattn::Meta) + 2 * heads * (D + 2) * sizeof(float));
+  return batch == 0 || deal_units(batch, Hq, Hkv, span, window, sinks).mode != pattn::kRuns
+             ? 0
+             : pattn::kMaxRuns * static_cast<int64_t>(sizeof(pattn::Meta) + 2 * heads * (D + 2) * sizeof(float));
 }
 
 template <bool F16, bool FP8, int D, int NT>
 cudaError_t run_paged_attention(const PagedAttnArgs& a, cudaStream_t st) {
   using C = pattn::Cfg<D, FP8 ? 1 : 2, NT>;
-  auto kern = paged_attention_kernel<F16, FP8, D, NT>;
-  static unsigned long long devices = 0;
-  cudaError_t e = allow_shared(kern, C::kSmem, devices);
-  if (e != cudaSuccess) return e;
   const int group = a.Hq / a.Hkv, tiles = (group + 8 * NT - 1) / (8 * NT);
-  const int64_t units = most_units(static_cast<int64_t>(a.table_width) * a.page_size, a.window, a.sinks);
-  const int64_t segs = static_cast<int64_t>(a.B) * a.Hkv * tiles;
-  int grid = num_sms() * C::kCtas;
-  if (grid > kMaxRuns) grid = kMaxRuns;
-  const bool whole = units <= pattn::kWholeUnits;
-  if (whole) {
-    if (segs < grid) grid = static_cast<int>(segs);
-  } else if (segs * ((units + pattn::kMinUnits - 1) / pattn::kMinUnits) < grid) {
-    grid = static_cast<int>(segs * ((units + pattn::kMinUnits - 1) / pattn::kMinUnits));
-  }
-  kern<<<grid, pattn::kWarps * 32, C::kSmem, st>>>(a, tiles, whole ? 1 : 0);
-  e = cudaGetLastError();
-  if (e != cudaSuccess || whole || grid == 1) return e;
+  const Deal deal = deal_units(a.B, a.Hq, a.Hkv, static_cast<int64_t>(a.table_width) * a.page_size, a.window, a.sinks);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(grid - 1, group < 8 * NT ? group : 8 * NT);
-  cfg.blockDim = dim3(128);
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<F16, D, NT>, a, grid, tiles);
+  if (deal.mode == pattn::kClusters) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(deal.cluster);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(deal.segs * deal.cluster));
+    cfg.blockDim = dim3(pattn::kWarps * 32);
+    cfg.dynamicSmemBytes = C::kSmem;
+    auto kern = paged_attention_kernel<F16, FP8, D, NT, true>;
+    static unsigned long long devices = 0;
+    const cudaError_t e = allow_shared(kern, C::kSmem, devices);
+    return e != cudaSuccess ? e : cudaLaunchKernelEx(&cfg, kern, a, tiles, deal.mode, deal.cluster);
+  }
+  auto kern = paged_attention_kernel<F16, FP8, D, NT, false>;
+  static unsigned long long devices = 0;
+  cudaError_t e = allow_shared(kern, C::kSmem, devices);
+  if (e != cudaSuccess) return e;
+  int64_t grid = static_cast<int64_t>(num_sms()) * C::kCtas;
+  if (grid > pattn::kMaxRuns) grid = pattn::kMaxRuns;
+  const int64_t most = deal.mode == pattn::kSegments ? deal.segs
+                                                     : deal.segs * ((deal.units + pattn::kMinUnits - 1) / pattn::kMinUnits);
+  if (most < grid) grid = most;
+  kern<<<static_cast<unsigned>(grid), pattn::kWarps * 32, C::kSmem, st>>>(a, tiles, deal.mode, 1);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || deal.mode != pattn::kRuns || grid == 1) return e;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(static_cast<unsigned>(grid - 1), group < 8 * NT ? group : 8 * NT);
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = 0;
+  return cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<F16, D, NT>, a, static_cast<int>(grid), tiles);
 }
 
 template <bool F16, bool FP8>
