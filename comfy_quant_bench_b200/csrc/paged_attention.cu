@@ -30,10 +30,15 @@ constexpr int kTile = 16;                    // keys per warp and step
 constexpr int kUnit = kWarps * kTile;
 // A row is split no finer than this: a part costs its CTA a start and an end (about two units' time), and the join.
 constexpr int kMinUnits = 4;
-// Rows of at most this many units are never split over runs: one launch, no join.
-constexpr int kWholeUnits = 12;
+// Segments of at most kWholeUnits go whole to CTAs, one launch and no join, where that keeps the SMs busy: all of them at
+// once, or in waves whose last one idles for less than kJoinUnits a CTA, about what runs pay for their parts and join.  Us
+// whole and as runs, 8 heads of D 128: 30 rows of 500 keys 14 and 19, of 1500 32 and 36; 64 rows of 500 27 and 31; but 40
+// rows (320 segments) of 500 26 and 24, of 1000 47 and 37.
+constexpr int kWholeUnits = 24;
+constexpr int kJoinUnits = 5;
 // CTAs of a resident grid (two per SM), and the most units of a cluster's CTA: with few segments of up to so many units
-// a cluster each is quicker than runs over all SMs and their join (8 segments of 4000 keys: 14 and 10 us).
+// a cluster each is quicker than runs over all SMs and their join (8 segments of 4000 keys: 12 and
+// 14 us).
 constexpr int kMaxRuns = 2 * 148;
 constexpr int kClusterUnits = 16;
 
@@ -729,7 +734,10 @@ Deal deal_units(int64_t batch, int Hq, int Hkv, int64_t span, int64_t window, in
   Deal d{pattn::kRuns, (span + pattn::kUnit - 1) / pattn::kUnit, batch * Hkv * ((group + tile - 1) / tile), 1};
   while (d.cluster < 8 && d.cluster < d.units && d.segs * d.cluster * 2 <= pattn::kMaxRuns) d.cluster *= 2;
   if (d.cluster > 1 && d.units <= static_cast<int64_t>(pattn::kClusterUnits) * d.cluster) d.mode = pattn::kClusters;
-  else if (d.units <= pattn::kWholeUnits) d.mode = pattn::kSegments;
+  else if (d.units <= pattn::kWholeUnits) {
+    const int64_t idle = (d.segs + pattn::kMaxRuns - 1) / pattn::kMaxRuns * pattn::kMaxRuns - d.segs;   // in the last wave
+    if (d.segs <= pattn::kMaxRuns || idle * d.units <= pattn::kJoinUnits * pattn::kMaxRuns) d.mode = pattn::kSegments;
+  }
   return d;
 }
 }  // namespace
