@@ -22,19 +22,20 @@ constexpr int kRows = 128;
 constexpr int kChunk = 128;                    // columns of a ring stage
 constexpr int kAheadWarps = 4;                 // widening warps, one per TMEM lane quadrant
 constexpr int kWBytes = kRows * kChunk / 2;
+constexpr int kAheadScales = 4;
 constexpr int kSite = 120;                     // device status sites of the waits
 
 template <int G, int NTOK>
 struct Plan {
   static constexpr int kXBytes = NTOK * kChunk * 2;
-  static constexpr int kScaleBytes = 272;                      // 128 scales of a group, and room for a shift
-  static constexpr int kStageBytes = (kWBytes + kXBytes + kChunk / G * kScaleBytes + 1023) / 1024 * 1024;
-  static constexpr int kStages = 100 * 1024 / kStageBytes < 8 ? 100 * 1024 / kStageBytes : 8;
-  static constexpr int kSmem = kStages * kStageBytes + 1024 + 256;      // alignment, barriers
+  static constexpr int kXStages = 3, kWStages = 7;
+  static constexpr int kRing = kXStages * kXBytes + kWStages * kWBytes;
+  static constexpr int kSmem = kRing + 1024 + 256;             // alignment, barriers
   static constexpr int kSums = NTOK < 32 ? NTOK : 32;          // tokens of an adding warp
   static constexpr int kAddWarps = 4 * (NTOK / kSums);
   static constexpr int kThreads = 32 * (kAheadWarps + kAddWarps + 2);   // and the copying and the multiplying warp
-  static_assert(kRows * NTOK * 4 <= kStages * kStageBytes, "partial sums fit the ring");
+  static_assert(kRows * NTOK * 4 <= kRing, "partial sums fit the rings");
+  static_assert(kWStages >= kXStages, "the copying warp's order");
 };
 
 struct Args {
@@ -78,6 +79,13 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uin
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
       ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
 }
+// one lane of a converged warp, in a form that lets the compiler keep a branch on it uniform (64 tokens at 8192 x
+// 28672: 66 us, and 78 with a branch on the lane's number)
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
 // mbar_wait for roles that hand over every few hundred cycles: the plain hardware wait (the form with a time limit is
 // built from sleeps of about a microsecond), then, out of line, the one that reads the clock
 __device__ __noinline__ bool mbar_wait_long(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int where) {
@@ -102,15 +110,18 @@ __global__ void __launch_bounds__(w4tc::Plan<G, NTOK>::kThreads, 2)
                     const __grid_constant__ CUtensorMap tm_r, const w4tc::Args a) {
   using namespace w4tc;
   using P = Plan<G, NTOK>;
-  constexpr int kStages = P::kStages, kSteps = kChunk / G, kSums = P::kSums;
+  constexpr int kXStages = P::kXStages, kWStages = P::kWStages, kSteps = kChunk / G, kSums = P::kSums;
   constexpr int kCopyWarp = kAheadWarps + P::kAddWarps, kMmaWarp = kCopyWarp + 1;
   constexpr uint32_t kCols = 256;                             // TMEM: two P of NTOK columns, A's buffers in the rest
   static_assert(2 * NTOK + 128 <= kCols, "two 128-column A operands");
   extern __shared__ __align__(128) uint8_t smem_any[];
   uint8_t* smem = smem_any + ((1024 - (smem_u32(smem_any) & 1023)) & 1023);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * P::kStageBytes);
-  uint64_t* empty = full + kStages;
-  uint64_t* a_full = empty + kStages;                         // [2] an operand's codes (or zeros) are in TMEM
+  uint8_t* codes_at = smem + kXStages * P::kXBytes;           // the ring of codes comes after the tokens'
+  uint64_t* x_full = reinterpret_cast<uint64_t*>(smem + P::kRing);
+  uint64_t* x_empty = x_full + kXStages;
+  uint64_t* w_full = x_empty + kXStages;
+  uint64_t* w_empty = w_full + kWStages;
+  uint64_t* a_full = w_empty + kWStages;                      // [2] an operand's codes (or zeros) are in TMEM
   uint64_t* p_full = a_full + 2;                              // [2] a product is done: P to be read, A free
   uint64_t* p_empty = p_full + 2;                             // [2] P is read
   uint64_t* z_done = p_empty + 2;                             // [2] A's buffer of the zeros' product is free
@@ -127,9 +138,13 @@ __global__ void __launch_bounds__(w4tc::Plan<G, NTOK>::kThreads, 2)
   const int nz = z1 - z0;
 
   if (tid == 0) {
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(&full[s], 1 + 32);                            // the bulk copies, and each lane's scales
-      mbar_init(&empty[s], kAheadWarps + P::kAddWarps + 1);
+    for (int s = 0; s < kXStages; ++s) {
+      mbar_init(&x_full[s], 1);
+      mbar_init(&x_empty[s], 1);
+    }
+    for (int s = 0; s < kWStages; ++s) {
+      mbar_init(&w_full[s], 1);
+      mbar_init(&w_empty[s], kAheadWarps);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&a_full[b], kAheadWarps);
@@ -156,73 +171,64 @@ __global__ void __launch_bounds__(w4tc::Plan<G, NTOK>::kThreads, 2)
   const int first_sum = warp >= kAheadWarps && warp < kCopyWarp ? (warp - kAheadWarps) / 4 * kSums : 0;   // of the tile's tokens
 
   if (warp == kCopyWarp) {
-    // ---- stages: nz of the groups' sums (as the tokens' operand), then a chunk's codes, tokens and scales each ----
-    const int loads = nz + c1 - c0;
-    auto early = [&](int i, int s) {                          // what no earlier kernel writes
-      uint8_t* st = smem + s * P::kStageBytes;
-      if (i < nz) {
-        if (lane == 0) mbar_arrive_expect_tx(&full[s], P::kXBytes);
-        mbar_arrive(&full[s]);
-        return;
-      }
-      const int ch = c0 + i - nz;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&full[s], kWBytes + P::kXBytes);
-        tma_load_2d(st + P::kXBytes, &tm_w, &full[s], ch * (kChunk / 2), n0);
-      }
-      // rows of N 16-bit values: any alignment
-#pragma unroll
-      for (int k = 0; k < kSteps; ++k) {
-        const int grp = ch * kSteps + k;
-        if (grp * G < a.K)
-          cp_async_halves(smem_u32(st + P::kXBytes + kWBytes + k * P::kScaleBytes),
-                          reinterpret_cast<const unsigned short*>(a.s) + static_cast<int64_t>(grp) * a.N + n0,
-                          min(kRows, a.N - n0), lane);
-      }
-      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[s])) : "memory");
+    // ---- a ring of codes, freed when they are widened, and one of tokens (the zeros' nz blocks of sums first), freed by
+    // the products ----
+    const int wloads = c1 - c0, xloads = nz + wloads;
+    int wi = 0, ws = 0, xi = 0, xs = 0;
+    auto codes = [&]() {
+      mbar_arrive_expect_tx(&w_full[ws], kWBytes);
+      tma_load_2d(codes_at + ws * kWBytes, &tm_w, &w_full[ws], (c0 + wi) * (kChunk / 2), n0);
+      ++wi;
+      if (++ws == kWStages) ws = 0;
     };
-    auto tokens = [&](int i, int s) {
-      if (lane != 0) return;
-      uint8_t* st = smem + s * P::kStageBytes;
-      const CUtensorMap* map = i < nz ? &tm_r : &tm_x;
-      const int at = (i < nz ? z0 + i : c0 + i - nz) * kChunk * 2;
-      tma_load_2d(st, map, &full[s], at, m0);
-      tma_load_2d(st + P::kXBytes / 2, map, &full[s], at + 128, m0);
+    auto tokens = [&]() {
+      uint8_t* st = smem + xs * P::kXBytes;
+      const CUtensorMap* map = xi < nz ? &tm_r : &tm_x;
+      const int at = (xi < nz ? z0 + xi : c0 + xi - nz) * kChunk * 2;
+      mbar_arrive_expect_tx(&x_full[xs], P::kXBytes);
+      tma_load_2d(st, map, &x_full[xs], at, m0);
+      tma_load_2d(st + P::kXBytes / 2, map, &x_full[xs], at + 128, m0);
+      ++xi;
+      if (++xs == kXStages) xs = 0;
     };
-    const int first = min(kStages, loads);
-    for (int i = 0; i < first; ++i) early(i, i);
-    grid_dep_wait();                                          // the tokens and their sums are written
-    for (int i = 0; i < first; ++i) tokens(i, i);
-    uint32_t issued = first, phase = 0;
-    int s = 0;
-    for (int i = first; i < loads; ++i) {
-      if (!mbar_wait_short(&empty[s], phase, abort_flag, kSite)) break;
-      early(i, s);
-      tokens(i, s);
-      ++issued;
-      if (++s == kStages) { s = 0; phase ^= 1u; }
+    if (lane == 0) {
+      while (wi < min(kWStages, wloads)) codes();             // no earlier kernel writes them
+      grid_dep_wait();                                        // the tokens and their sums are written
+      while (xi < min(kXStages, xloads)) tokens();
+      // one after the other: a block's codes are widened before its product is done
+      while (wi < wloads || xi < xloads) {
+        if (wi < wloads && xi - kXStages - nz >= wi - kWStages) {
+          if (!mbar_wait_short(&w_empty[ws], ((wi / kWStages) & 1) ^ 1u, abort_flag, kSite)) break;
+          codes();
+        }
+        if (xi < xloads) {
+          if (!mbar_wait_short(&x_empty[xs], ((xi / kXStages) & 1) ^ 1u, abort_flag, kSite + 1)) break;
+          tokens();
+        }
+      }
+      drain_ring(w_full, kWStages, wi, 50000000ull);
+      drain_ring(x_full, kXStages, xi, 50000000ull);
     }
-    cp_async_wait_all();
-    if (lane == 0) drain_ring(full, kStages, issued, 50000000ull);
     __syncwarp();
   } else if (warp == kMmaWarp) {
-    // ---- products: the zeros' first, then each group's P = codes x tokens ----
-    constexpr uint32_t shape = (1u << 4) | (static_cast<uint32_t>(NTOK >> 3) << 17) | (8u << 24);   // f32, M = 128
-    constexpr uint32_t idesc_z = shape | (1u << 7) | (1u << 10);                                    // bf16 x bf16
-    int stage = 0, issued = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    auto next_stage = [&]() {
-      if (++stage == kStages) { stage = 0; phase ^= 1u; }
-    };
-    for (int j = 0; j < nz; ++j) {
-      const int buf = j & 1;
-      ok = ok && mbar_wait_short(&full[stage], phase, abort_flag, kSite + 1) &&
-           mbar_wait_short(&a_full[buf], (j >> 1) & 1, abort_flag, kSite + 2);
-      if (!ok) break;
-      tc_fence_after();
-      const uint64_t x = smem_desc_k_sw128(smem_u32(smem + stage * P::kStageBytes));
-      if (lane == 0) {
+    // ---- products: the zeros' first, then each group's P = codes x tokens.  One thread, which neither waits for the
+    // warp's other lanes nor makes them poll: it paces the CTA ----
+    if (elect_one()) {
+      constexpr uint32_t shape = (1u << 4) | (static_cast<uint32_t>(NTOK >> 3) << 17) | (8u << 24);   // f32, M = 128
+      constexpr uint32_t idesc_z = shape | (1u << 7) | (1u << 10);                                    // bf16 x bf16
+      int stage = 0, issued = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      auto next_stage = [&]() {
+        if (++stage == kXStages) { stage = 0; phase ^= 1u; }
+      };
+      for (int j = 0; j < nz; ++j) {
+        const int buf = j & 1;
+        ok = ok && mbar_wait_short(&x_full[stage], phase, abort_flag, kSite + 2) &&
+             mbar_wait_short(&a_full[buf], (j >> 1) & 1, abort_flag, kSite + 3);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t x = smem_desc_k_sw128(smem_u32(smem + stage * P::kXBytes));
 #pragma unroll
         for (int k = 0; k < 6; ++k) {                         // three parts of 32 sums; the last 32 columns are empty
           const int col = 16 * k;
@@ -230,27 +236,24 @@ __global__ void __launch_bounds__(w4tc::Plan<G, NTOK>::kThreads, 2)
                      j + k != 0);
         }
         tc_commit(&z_done[buf]);
-        tc_commit(&empty[stage]);
+        tc_commit(&x_empty[stage]);
         if (j + 1 == nz) tc_commit(&p_full[0]);
+        issued = 1;
+        next_stage();
       }
-      __syncwarp();
-      issued = 1;
-      next_stage();
-    }
-    if (nz == 0 && lane == 0) mbar_arrive(&p_full[0]);
-    // product i (0: the zeros', 1 ..: the groups') takes P buffer i & 1; a_full goes on counting from the zeros' blocks
-    for (int i = 1; i <= steps && ok; next_stage()) {
-      if (!(ok = mbar_wait_short(&full[stage], phase, abort_flag, kSite + 3))) break;
-      const uint64_t x = smem_desc_k_sw128(smem_u32(smem + stage * P::kStageBytes));
+      if (nz == 0) mbar_arrive(&p_full[0]);
+      // product i (0: the zeros', 1 ..: the groups') takes P buffer i & 1; a_full goes on counting from the zeros' blocks
+      for (int i = 1; i <= steps && ok; next_stage()) {
+        if (!(ok = mbar_wait_short(&x_full[stage], phase, abort_flag, kSite + 4))) break;
+        const uint64_t x = smem_desc_k_sw128(smem_u32(smem + stage * P::kXBytes));
 #pragma unroll
-      for (int sub = 0; sub < kSteps; ++sub) {
-        if (i > steps) break;
-        const int buf = i & 1, use = nz + i - 1;
-        ok = mbar_wait_short(&p_empty[buf], ((i >> 1) & 1) ^ 1u, abort_flag, kSite + 4) &&
-             mbar_wait_short(&a_full[use & 1], (use >> 1) & 1, abort_flag, kSite + 5);
-        if (!ok) break;
-        tc_fence_after();
-        if (lane == 0) {
+        for (int sub = 0; sub < kSteps; ++sub) {
+          if (i > steps) break;
+          const int buf = i & 1, use = nz + i - 1;
+          ok = mbar_wait_short(&p_empty[buf], ((i >> 1) & 1) ^ 1u, abort_flag, kSite + 5) &&
+               mbar_wait_short(&a_full[use & 1], (use >> 1) & 1, abort_flag, kSite + 6);
+          if (!ok) break;
+          tc_fence_after();
 #pragma unroll
           for (int k = 0; k < G / 16; ++k) {
             const int col = sub * G + 16 * k;                 // 64 columns per 128-byte-wide half
@@ -258,16 +261,15 @@ __global__ void __launch_bounds__(w4tc::Plan<G, NTOK>::kThreads, 2)
                        x + ((col >> 6) * (P::kXBytes / 2) + (col & 63) * 2) / 16, shape, k != 0);
           }
           tc_commit(&p_full[buf]);
-          if (sub == kSteps - 1) tc_commit(&empty[stage]);
+          if (sub == kSteps - 1) tc_commit(&x_empty[stage]);
+          issued = ++i;
         }
-        __syncwarp();
-        issued = ++i;
       }
-    }
-    // after a wait that ran out: the products in flight end before TMEM and the ring go away
-    if (!ok && lane == 0) {
-      for (int j = max(nz - 2, 0); j < nz && issued <= 1; ++j) mbar_wait_drain(&z_done[j & 1], (j >> 1) & 1, 50000000ull);
-      for (int i = max(issued - 2, 0); i < issued; ++i) mbar_wait_drain(&p_full[i & 1], (i >> 1) & 1, 50000000ull);
+      // after a wait that ran out: the products in flight end before TMEM and the ring go away
+      if (!ok) {
+        for (int j = max(nz - 2, 0); j < nz && issued <= 1; ++j) mbar_wait_drain(&z_done[j & 1], (j >> 1) & 1, 50000000ull);
+        for (int i = max(issued - 2, 0); i < issued; ++i) mbar_wait_drain(&p_full[i & 1], (i >> 1) & 1, 50000000ull);
+      }
     }
     __syncwarp();
   } else if (warp < kAheadWarps) {
@@ -275,14 +277,11 @@ __global__ void __launch_bounds__(w4tc::Plan<G, NTOK>::kThreads, 2)
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    auto hand_over = [&](int buf, bool last) {
+    auto hand_over = [&](int buf) {
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&a_full[buf]);
-        if (last) mbar_arrive(&empty[stage]);
-      }
+      if (lane == 0) mbar_arrive(&a_full[buf]);
     };
     for (int j = 0; j < nz && ok; ++j) {
       const int buf = j & 1;
@@ -295,20 +294,17 @@ __global__ void __launch_bounds__(w4tc::Plan<G, NTOK>::kThreads, 2)
         const uint32_t hi = 2 * q + 1 < left ? __ldg(zp + static_cast<int64_t>(2 * q + 1) * a.N) : 0;
         pairs[q] = lo | hi << 16;
       }
-      ok = mbar_wait_short(&full[stage], phase, abort_flag, kSite + 6) &&
-           (j < 2 || mbar_wait_short(&z_done[buf], ((j - 2) >> 1) & 1, abort_flag, kSite + 7));
-      if (!ok) break;
+      if (j >= 2 && !(ok = mbar_wait_short(&z_done[buf], ((j - 2) >> 1) & 1, abort_flag, kSite + 7))) break;
       __syncwarp();
       tc_fence_after();
 #pragma unroll
       for (int part = 0; part < 3; ++part) tmem_st_x16(a_col + buf * 64 + 16 * part + lane_base, pairs);
-      hand_over(buf, true);
-      if (++stage == kStages) { stage = 0; phase ^= 1u; }
+      hand_over(buf);
     }
-    const uint8_t* w = smem + P::kXBytes + row * 64;
+    const uint8_t* w = codes_at + row * 64;
     const int sw = (row >> 1 & 3) << 4;
     for (int i = 1; i <= steps && ok;) {
-      if (!(ok = mbar_wait_short(&full[stage], phase, abort_flag, kSite + 8))) break;
+      if (!(ok = mbar_wait_short(&w_full[stage], phase, abort_flag, kSite + 8))) break;
 #pragma unroll
       for (int sub = 0; sub < kSteps; ++sub) {
         if (i > steps) break;
@@ -316,39 +312,45 @@ __global__ void __launch_bounds__(w4tc::Plan<G, NTOK>::kThreads, 2)
         uint4 codes[G / 32];
 #pragma unroll
         for (int b = 0; b < G / 32; ++b)                      // 32 columns: 16 bytes
-          codes[b] = *reinterpret_cast<const uint4*>(w + stage * P::kStageBytes + (((sub * (G / 32) + b) << 4) ^ sw));
+          codes[b] = *reinterpret_cast<const uint4*>(w + stage * kWBytes + (((sub * (G / 32) + b) << 4) ^ sw));
+        auto widen = [&](int b, uint32_t (&pairs)[16]) {
+          const uint32_t v[4] = {codes[b].x, codes[b].y, codes[b].z, codes[b].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) widen8<true>(v[j], reinterpret_cast<uint32_t(&)[4]>(pairs[4 * j]));
+        };
+        uint32_t first[16];
+        widen(0, first);
+        if (sub == kSteps - 1) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&w_empty[stage]);
+        }
         // A's buffer is free when the product two before is done; the zeros' products took both
         const int free_at = i <= 2 ? 0 : i - 2;
         if ((i > 2 || nz > 0) && !(ok = mbar_wait_short(&p_full[free_at & 1], (free_at >> 1) & 1, abort_flag, kSite + 9))) break;
         __syncwarp();
         tc_fence_after();
+        tmem_st_x16(a_col + buf * 64 + lane_base, first);
 #pragma unroll
-        for (int b = 0; b < G / 32; ++b) {
-          const uint32_t v[4] = {codes[b].x, codes[b].y, codes[b].z, codes[b].w};
+        for (int b = 1; b < G / 32; ++b) {
           uint32_t pairs[16];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) widen8<true>(v[j], reinterpret_cast<uint32_t(&)[4]>(pairs[4 * j]));
+          widen(b, pairs);
           tmem_st_x16(a_col + buf * 64 + 16 * b + lane_base, pairs);
         }
-        hand_over(buf, sub == kSteps - 1);
+        hand_over(buf);
         ++i;
       }
-      if (++stage == kStages) { stage = 0; phase ^= 1u; }
+      if (++stage == kWStages) { stage = 0; phase ^= 1u; }
     }
   } else {
-    // ---- the zeros' product, and each group's scaled, added up ----
-    const int s_odd = half_shift(reinterpret_cast<const unsigned short*>(a.s) + n0);
-    int stage = 0;
-    uint32_t phase = 0;
+    // ---- the zeros' product, and each group's scaled, added up; scales are loaded kAheadScales groups ahead ----
+    const unsigned short* sp = reinterpret_cast<const unsigned short*>(a.s) + static_cast<int64_t>(c0) * kSteps * a.N + min(n, a.N - 1);
+    uint32_t scales[kAheadScales];
+#pragma unroll
+    for (int u = 0; u < kAheadScales; ++u) scales[u] = u < steps ? __ldg(sp + static_cast<int64_t>(u) * a.N) : 0;
     bool ok = true;
-    for (int j = 0; j < nz && ok; ++j) {
-      ok = mbar_wait_short(&full[stage], phase, abort_flag, kSite + 10);
-      if (ok && lane == 0) mbar_arrive(&empty[stage]);
-      if (++stage == kStages) { stage = 0; phase ^= 1u; }
-    }
-    auto add = [&](int i, float scale, bool last) {
+    auto add = [&](int i, float scale) {
       const int buf = i & 1;
-      if (!(ok = mbar_wait_short(&p_full[buf], (i >> 1) & 1, abort_flag, kSite + 11))) return;
+      if (!(ok = mbar_wait_short(&p_full[buf], (i >> 1) & 1, abort_flag, kSite + 10))) return;
       __syncwarp();
       tc_fence_after();
       const float2 s2 = make_float2(scale, scale);
@@ -360,30 +362,22 @@ __global__ void __launch_bounds__(w4tc::Plan<G, NTOK>::kThreads, 2)
         if (q == kSums / 16 - 1) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&p_empty[buf]);
-            if (last) mbar_arrive(&empty[stage]);
-          }
+          if (lane == 0) mbar_arrive(&p_empty[buf]);
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           acc[8 * q + j] = fma2(s2, make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), acc[8 * q + j]);
       }
     };
-    if (nz > 0 && ok) add(0, 1.0f, false);
-    if (nz == 0 && lane == 0) mbar_arrive(&p_empty[0]);       // product 0 has nothing in it
-    for (int i = 1; i <= steps && ok;) {
-      if (!(ok = mbar_wait_short(&full[stage], phase, abort_flag, kSite + 12))) break;
+    if (nz > 0) add(0, 1.0f);
+    else if (lane == 0) mbar_arrive(&p_empty[0]);             // product 0 has nothing in it
+    for (int i = 0; i < steps && ok; i += kAheadScales) {
 #pragma unroll
-      for (int sub = 0; sub < kSteps; ++sub) {
-        if (i > steps || !ok) break;
-        const int odd = (c0 * kSteps + i - 1) & a.N & 1;      // an odd N moves every other group's scales by a half
-        const float s = bf16_bits_to_f32(reinterpret_cast<const unsigned short*>(
-            smem + stage * P::kStageBytes + P::kXBytes + kWBytes + sub * P::kScaleBytes)[row + (s_odd ^ odd)]);
-        add(i, s, sub == kSteps - 1);
-        ++i;
+      for (int u = 0; u < kAheadScales; ++u) {
+        if (i + u >= steps || !ok) break;
+        add(i + u + 1, bf16_bits_to_f32(static_cast<unsigned short>(scales[u])));
+        if (i + u + kAheadScales < steps) scales[u] = __ldg(sp + static_cast<int64_t>(i + u + kAheadScales) * a.N);
       }
-      if (++stage == kStages) { stage = 0; phase ^= 1u; }
     }
   }
   tc_fence_before();
