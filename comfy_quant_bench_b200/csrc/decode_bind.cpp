@@ -2,7 +2,7 @@
 // (include/cq_b200.h) on the tensors' device and its current stream.
 //
 // These operators take a few microseconds on the GPU, less than their checks and a ctypes call with thirty arguments
-// take in Python (11 us for the W4A16 linear, 15 us for the attention; here 6 and 7 us), so a decode step would wait for
+// take in Python (11 us for the W4A16 linear, 15 us for the attention; here 5.8 and 5.7 us), so a decode step would wait for
 // its host.  The Python functions of ops.py and kvcache.py document them and pass their arguments on.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>

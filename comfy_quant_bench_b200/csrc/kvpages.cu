@@ -70,7 +70,7 @@ __device__ void free_bitmap(const int* refs, int num_pages, uint32_t* bits) {
 }
 
 // Lanes that work on one table row: each row is a chain of dependent loads, so with short rows many of them at a time.
-// 128 rows of 56 pages: 23 us with a warp per row, 13 us with eight lanes.
+// 128 rows of 56 pages, the whole branching kernel: 23 us with a warp per row, 15 us with eight lanes.
 __device__ __forceinline__ int lanes_of_row(int width) { return width >= 512 ? 32 : 8; }
 
 __global__ void __launch_bounds__(pages::kThreads) pages_branch_kernel(const PagesArgs a) {
@@ -228,7 +228,8 @@ cudaError_t launch_pages_branch(const PagesArgs& a, cudaStream_t st) {
 }
 
 // pages_copy_kernel: page moves[i][0] -> page moves[i][1] in every layer of the key and the value cache; a negative
-// entry moves nothing.  No destination is a source, so the order does not matter.
+// entry moves nothing.  No destination is a source, so the order does not matter.  A CTA per page, layer and cache: bound by
+// HBM (moving 0.69 GB takes 224 us, 6.2 TB/s counting both ways, and few pages the launch).
 __global__ void __launch_bounds__(256) pages_copy_kernel(const PagesCopyArgs a) {
   grid_dep_launch();
   grid_dep_wait();                                        // the list is written
@@ -350,7 +351,8 @@ cudaError_t launch_pages_compact(const CompactArgs& a, cudaStream_t st) {
 // kv_append_kernel: new keys and values [layers, T, Hkv, D] into their rows' pages.  A token whose row, position or
 // page is out of range is skipped (a refused reservation gives positions of -1).  An 8-bit cache holds x / scale,
 // rounded to the nearest even and kept inside the format's finite range (NaN stays NaN).
-// A thread moves eight elements (16 bytes in, 16 or 8 out): bound by launch and latency up to a few MB, by HBM beyond.
+// A thread moves eight elements (16 bytes in, 16 or 8 out): bound by launch and latency (128 tokens in 32 layers, 8 heads
+// of 128: 11.5 us; element by element it took 28).
 __global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
   grid_dep_launch();
   const int64_t t = blockIdx.x, layer = blockIdx.y;

@@ -7,7 +7,8 @@
 // adds s P + z R (P = sum x (q - 8), R = sum x) to its fp32 sums.
 //
 // Bound by the tiles' rate (a tile of 16 x 8 x 16 takes eight cycles of an SM's quarter): 18 tokens of a 5120 x 13824
-// weight need 16 us of them with four tiles of tokens, 12 us with three.  Measured: see launch_w4a16.
+// weight need 16 us of them with four tiles of tokens, 12 us with three.  Measured (device time, the tokens' kernel
+// included): 27 us with groups of 64, 31 us with groups of 32, whose ends, s P + z R, come twice as often.
 //
 // The tokens come from w4a16_tokens.cu, as f16 in the order the codes are widened in, with R.  The product is launched as
 // its programmatic dependent: its weights are on their way while the tokens are written.
