@@ -107,6 +107,17 @@ def test_linear_ordinary_sizes(ops, m, k, n):
     _linear_holds(ops, *_linear_problem(m, k, n, 128, torch.bfloat16), 128)
 
 
+@pytest.mark.parametrize("m,k,n,group", [(33, 4160, 19001, 32), (64, 2112, 19100, 64), (70, 1152, 18950, 128), (40, 9600, 300, 32)])
+def test_linear_many_tokens_deep_and_wide(ops, m, k, n, group):
+    """More blocks of zeros and chunks than the rings hold, whole K and split, last chunks that are not full."""
+    x, q, s, z, b = _linear_problem(m, k, n, group, torch.float16 if m == 64 else torch.bfloat16)
+    y = ops.w4a16_linear(x, q, s, z, b, group_size=group)
+    _linear_holds(ops, x, q, s, z, b, group, y)
+    for _ in range(3):
+        assert torch.equal(ops.w4a16_linear(x, q, s, z, b, group_size=group), y)
+    assert _status()[0] == 0
+
+
 def test_linear_strided_rows_leading_dims_and_out(ops):
     x, q, s, z, b = _linear_problem(6, 512, 96, 64, torch.float16)
     wide = torch.zeros(6, 1200, dtype=torch.float16, device="cuda")
@@ -302,6 +313,18 @@ def test_attention_long_and_split(kv, b, n, hk):
     a = _attention_holds(kv, q, k, v, table, ln)
     for _ in range(3):                                    # the join's order is fixed
         assert torch.equal(kv.paged_attention(q, k, v, table, ln), a)
+
+
+@pytest.mark.parametrize("b,n,hk,d", [(40, 700, 8, 64), (40, 1300, 8, 64), (30, 1000, 8, 128), (38, 200, 8, 64), (5, 900, 8, 128),
+                                      (10, 1500, 8, 64), (20, 900, 16, 64), (1, 600, 2, 256), (33, 1536, 9, 64), (1, 8300, 1, 64)])
+def test_attention_ways_to_deal_the_work(kv, b, n, hk, d):
+    """Runs, whole segments and clusters, at and past the sizes where one takes over from another; ragged and empty rows."""
+    host = random.Random(b * n)
+    lens = [n if i == 0 else host.choice([0, 1, n, n - 1, host.randint(0, n)]) for i in range(b)]
+    k, v, table, ln = _cache(lens, hk, 16, d, torch.bfloat16, seed=n)
+    q = _query(b, 2 * hk, d, torch.bfloat16, b)
+    a = _attention_holds(kv, q, k, v, table, ln)
+    assert torch.equal(kv.paged_attention(q, k, v, table, ln), a)
 
 
 def test_attention_many_ragged_rows(kv):
