@@ -150,9 +150,18 @@ const float* head_scale(const Opt& s, int64_t heads, at::ScalarType cache, const
   return s->data_ptr<float>();
 }
 
-int64_t row_stride(const Tensor& table) { return std::max(table.stride(0), table.size(1)); }
+// Rows that share memory (one row expanded to several, an overlapping view): the kernels take tables whose rows lie at
+// least their width apart.
+bool rows_overlap(const Tensor& table) { return table.size(0) > 1 && table.stride(0) < table.size(1); }
+// a table that is only read: such a view is taken as its copy
+Tensor read_table(const Tensor& table) { return rows_overlap(table) ? table.contiguous() : table; }
+// one that is written has to have rows of its own
+void written_table(const Tensor& table, const char* name) {
+  if (rows_overlap(table)) refuse(name, " is written, but its rows share memory: strides ", table.strides(), " for shape ", table.sizes());
+}
+int64_t row_stride(const Tensor& table) { return table.size(0) > 1 ? table.stride(0) : table.size(1); }
 
-py::object paged_attention(const Tensor& q_arg, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table,
+py::object paged_attention(const Tensor& q_arg, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table_arg,
                            const Tensor& lens, const Opt& rows, std::optional<double> scale, int64_t window, int64_t sinks,
                            const Opt& k_scale, const Opt& v_scale, const Opt& out_arg, bool return_lse) {
   const at::ScalarType dt = q_arg.scalar_type(), ct = k_cache.scalar_type();
@@ -165,9 +174,9 @@ py::object paged_attention(const Tensor& q_arg, const Tensor& k_cache, const Ten
   if (hk < 1 || hq < 1 || hq % hk != 0) refuse("q_heads (", hq, ") must be a multiple of kv_heads (", hk, ")");
   if (ct != dt && ct != at::kFloat8_e4m3fn) refuse("the caches must hold ", dt, " or float8_e4m3fn, got ", ct);
   if (window < 0 || sinks < 0) refuse("window and sinks must not be negative");
-  i32(table, 2, "block_table");
+  i32(table_arg, 2, "block_table");
   i32(lens, 1, "seq_lens");
-  const int64_t table_rows = table.size(0), width = table.size(1);
+  const int64_t table_rows = table_arg.size(0), width = table_arg.size(1);
   if (lens.size(0) != table_rows) refuse("seq_lens must have one entry per table row (", table_rows, ")");
   if (rows) {
     i32(*rows, 1, "rows");
@@ -175,11 +184,12 @@ py::object paged_attention(const Tensor& q_arg, const Tensor& k_cache, const Ten
   } else if (b > table_rows) {
     refuse(b, " queries for ", table_rows, " table rows");
   }
-  const int index = device_of(q_arg, k_cache, v_cache, table, lens, rows, k_scale, v_scale, out_arg);
+  const int index = device_of(q_arg, k_cache, v_cache, table_arg, lens, rows, k_scale, v_scale, out_arg);
   const float* ks = head_scale(k_scale, hk, ct, "k_scale");
   const float* vs = head_scale(v_scale, hk, ct, "v_scale");
   const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(index));
 
+  const Tensor table = read_table(table_arg);
   Tensor q = q_arg;
   if (!aligned16(q) || q.stride(2) != 1 || q.stride(0) % 8 != 0 || q.stride(1) % 8 != 0)
     q = q.clone(at::MemoryFormat::Contiguous);
@@ -213,7 +223,7 @@ Tensor aligned_rows(const Tensor& x) {
   return ok ? x : x.clone(at::MemoryFormat::Contiguous);
 }
 
-void append_kv(const Tensor& k_arg, const Tensor& v_arg, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table,
+void append_kv(const Tensor& k_arg, const Tensor& v_arg, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table_arg,
                const Tensor& rows, const Tensor& positions, const Opt& k_scale, const Opt& v_scale) {
   const at::ScalarType dt = k_arg.scalar_type(), ct = k_cache.scalar_type();
   const int64_t dim = k_arg.dim();
@@ -224,14 +234,15 @@ void append_kv(const Tensor& k_arg, const Tensor& v_arg, const Tensor& k_cache, 
   if ((dim == 4 && k_cache.size(0) != layers) || k_cache.size(-3) != hk || k_cache.size(-1) != d)
     refuse("caches ", k_cache.sizes(), " do not fit k ", k_arg.sizes());
   if (ct != dt && ct != at::kFloat8_e4m3fn) refuse("the caches must hold ", dt, " or float8_e4m3fn, got ", ct);
-  i32(table, 2, "block_table");
+  i32(table_arg, 2, "block_table");
   i32(rows, 1, "rows");
   i32(positions, 1, "positions");
   if (rows.size(0) != t || positions.size(0) != t) refuse("rows and positions must have one entry per token (", t, ")");
-  const int index = device_of(k_arg, v_arg, k_cache, v_cache, table, rows, positions, k_scale, v_scale);
+  const int index = device_of(k_arg, v_arg, k_cache, v_cache, table_arg, rows, positions, k_scale, v_scale);
   const float* ks = head_scale(k_scale, hk, ct, "k_scale");
   const float* vs = head_scale(v_scale, hk, ct, "v_scale");
   const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(index));
+  const Tensor table = read_table(table_arg);
   const Tensor k = aligned_rows(k_arg), v = aligned_rows(v_arg);
   check_status("cq_kv_append",
                cq_kv_append(k.data_ptr(), dim == 4 ? k.stride(0) : 0, k.stride(-3), k.stride(-2), v.data_ptr(),
@@ -261,6 +272,7 @@ py::object pages_update(const Tensor& table, const Tensor& lens, const Tensor& r
                         const Opt& src, const Opt& dst, const Opt& reserve, const Opt& counts, int64_t count,
                         const Opt& k_cache, const Opt& v_cache) {
   i32(table, 2, "block_table");
+  written_table(table, "block_table");
   i32(lens, 1, "seq_lens");
   i32(refs, 1, "ref_counts");
   if (lens.size(0) != table.size(0)) refuse("seq_lens must have one entry per table row (", table.size(0), ")");
@@ -299,22 +311,24 @@ py::object pages_update(const Tensor& table, const Tensor& lens, const Tensor& r
   return py::make_tuple(*start, *copies);
 }
 
-py::tuple compact_pages(const Tensor& table, const Tensor& refs, const Tensor& k_cache, const Tensor& v_cache,
+py::tuple compact_pages(const Tensor& table_arg, const Tensor& refs, const Tensor& k_cache, const Tensor& v_cache,
                         const Opt& out_table_arg, const Opt& out_refs_arg) {
-  i32(table, 2, "block_table");
+  i32(table_arg, 2, "block_table");
   i32(refs, 1, "ref_counts");
-  const int index = device_of(table, refs, k_cache, v_cache, out_table_arg, out_refs_arg);
-  const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(index));
-  const int64_t pages = refs.size(0);
-  const PageLayout layout = page_layout(k_cache, v_cache, pages);
   if (out_table_arg) {
     i32(*out_table_arg, 2, "out_table");
-    if (out_table_arg->sizes() != table.sizes()) refuse("out_table must have the shape of block_table");
+    written_table(*out_table_arg, "out_table");
+    if (out_table_arg->sizes() != table_arg.sizes()) refuse("out_table must have the shape of block_table");
   }
   if (out_refs_arg) {
     i32(*out_refs_arg, 1, "out_refs");
-    if (out_refs_arg->size(0) != pages) refuse("out_refs must have the shape of ref_counts");
+    if (out_refs_arg->size(0) != refs.size(0)) refuse("out_refs must have the shape of ref_counts");
   }
+  const int index = device_of(table_arg, refs, k_cache, v_cache, out_table_arg, out_refs_arg);
+  const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(index));
+  const int64_t pages = refs.size(0);
+  const PageLayout layout = page_layout(k_cache, v_cache, pages);
+  const Tensor table = read_table(table_arg);
   const Tensor out_table = out_table_arg ? *out_table_arg : at::empty(table.sizes(), refs.options());
   const Tensor out_refs = out_refs_arg ? *out_refs_arg : at::empty({pages}, refs.options());
   const Tensor moves = at::empty({pages / 2, 2}, refs.options());

@@ -139,3 +139,23 @@ def test_awq_layout_is_registered_on_request():
     assert params == {"scale": 1, "zeros": 2, "group_size": 32}
     with pytest.raises(ValueError):
         algo["params_from_state_dict"]("l", None, None, lambda name: None, {"format": "awq_w4a16"})
+
+
+def test_written_tables_have_rows_of_their_own():
+    """A view whose rows share memory cannot be written row by row: refused before anything else."""
+    from comfy_quant_bench_b200 import kvcache
+    k, refs = torch.zeros(1, 6, 1, 16, 64, dtype=torch.bfloat16), torch.zeros(6, dtype=torch.int32)
+    lens, rows = torch.zeros(3, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    plain = torch.zeros(3, 4, dtype=torch.int32)
+    for view in (plain[:1].expand(3, 4), torch.zeros(8, dtype=torch.int32).as_strided((3, 4), (2, 1))):
+        for name, call in (("block_table", lambda: kvcache.free_rows(view, lens, refs, rows, 16)),
+                           ("block_table", lambda: kvcache.fork_rows(view, lens, refs, rows, rows + 1, 16)),
+                           ("block_table", lambda: kvcache.reserve_tokens(view, lens, refs, rows, 1, k, k)),
+                           ("block_table", lambda: kvcache.branch_rows(view, lens, refs, rows, rows + 1, 1, k, k)),
+                           ("out_table", lambda: kvcache.compact_pages(plain, refs, k, k, out_table=view)),
+                           ("out_table", lambda: kvcache.compact_pages(view, refs, k, k, out_table=view))):
+            with pytest.raises(ValueError, match=f"{name} is written, but its rows share memory"):
+                call()
+    for fine in (plain[:1], torch.zeros(3, 9, dtype=torch.int32)[:, 2:6]):       # one row of any stride, rows further apart
+        with pytest.raises(ValueError, match="CUDA"):
+            kvcache.free_rows(fine, lens[:len(fine)], refs, rows, 16)

@@ -793,3 +793,46 @@ def test_branch_equals_its_three_calls(kv):
     for x, y in zip((a.block_table, a.seq_lens, a.ref_counts, a.k, a.v), (b.block_table, b.seq_lens, b.ref_counts, b.k, b.v)):
         assert torch.equal(x, y)
     assert _status() == (0, 0)
+
+
+# ----------------------------------------------------------------------------------------------------------
+# tables whose rows share memory
+# ----------------------------------------------------------------------------------------------------------
+
+def _shared_views():
+    """(view, the same table with rows of its own): one row for four queries, and rows that overlap by a page."""
+    row = torch.tensor([[4, 1, 3]], dtype=torch.int32, device="cuda")
+    run = torch.tensor([0, 5, 2, 6, 1, 3], dtype=torch.int32, device="cuda").as_strided((4, 3), (1, 1))
+    return [(v, v.clone(memory_format=torch.contiguous_format)) for v in (row.expand(4, 3), run)]
+
+
+@pytest.mark.parametrize("cache_type", [torch.bfloat16, FP8])
+def test_attention_over_a_table_whose_rows_share_memory(kv, cache_type):
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k, v = ((20 * torch.randn(7, 2, 16, 64, generator=g, device="cuda")).to(cache_type) for _ in range(2))
+    n = torch.tensor([48, 1, 0, 33], dtype=torch.int32, device="cuda")
+    q = _query(4, 6, 64, torch.bfloat16, 2, 0.1)
+    for view, own in _shared_views():
+        want = _attention_holds(kv, q, k, v, own, n)
+        assert torch.equal(_attention_holds(kv, q, k, v, view, n), want)
+        rows = _rows(3, 3, 0, 1)
+        assert torch.equal(_attention_holds(kv, q, k, v, view, n, rows=rows), kv.paged_attention(q, k, v, own, n, rows=rows))
+
+
+def test_append_and_compact_read_a_table_whose_rows_share_memory(kv):
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x, y = (torch.randn(4, 2, 64, generator=g, device="cuda").bfloat16() for _ in range(2))
+    rows, pos = _rows(0, 1, 2, 3), _rows(0, 17, 3, 47)
+    for view, own in _shared_views():
+        made = []
+        for table in (own, view):
+            k, v = (torch.zeros(1, 7, 2, 16, 64, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+            kv.append_kv(x, y, k[0], v[0], table, rows, pos)
+            for t in range(4):
+                p, s = int(own[t, int(pos[t]) // 16]), int(pos[t]) % 16
+                assert torch.equal(k[0, p, :, s], x[t]) and torch.equal(v[0, p, :, s], y[t])
+            refs = torch.bincount(own.flatten(), minlength=7).int()
+            made.append((k, v, *kv.compact_pages(table, refs, k, v)))
+        for a, b in zip(*made):
+            assert torch.equal(a, b)
+    assert _status() == (0, 0)
