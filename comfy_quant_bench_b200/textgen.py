@@ -87,7 +87,8 @@ class TextModel:
         self.cache = kvcache.PagedKVCache(cfg.layers, cfg.pages, cfg.kv_heads, cfg.head_dim, cfg.rows, cfg.max_tokens,
                                           cfg.page_size, cfg.cache_dtype, device, scale, scale)
         inv = cfg.rope_base ** (-torch.arange(0, cfg.head_dim, 2, device=device, dtype=torch.float32) / cfg.head_dim)
-        angle = torch.outer(torch.arange(cfg.max_tokens, device=device, dtype=torch.float32), inv)
+        room = self.cache.block_table.shape[1] * cfg.page_size               # max_tokens up to whole pages: any position
+        angle = torch.outer(torch.arange(room, device=device, dtype=torch.float32), inv)
         self.rope = torch.stack([angle.cos(), angle.sin()], dim=-1)          # [tokens, D/2, 2]
 
     def _heads(self, x: torch.Tensor, weight: torch.Tensor, rope: torch.Tensor) -> torch.Tensor:
@@ -114,6 +115,8 @@ class TextModel:
     def prompt(self, tokens: torch.Tensor, row: int) -> torch.Tensor:
         """A prompt [tokens] into the empty cache row; logits [tokens, vocab]."""
         n = len(tokens)
+        if n > self.cfg.max_tokens:
+            raise ValueError(f"a prompt of {n} tokens for rows of max_tokens = {self.cfg.max_tokens}")
         where = torch.tensor([row], dtype=torch.int32, device=self.device)
         self.cache.reserve(where, n)
         positions = torch.arange(n, dtype=torch.int32, device=self.device)

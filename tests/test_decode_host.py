@@ -159,3 +159,15 @@ def test_written_tables_have_rows_of_their_own():
     for fine in (plain[:1], torch.zeros(3, 9, dtype=torch.int32)[:, 2:6]):       # one row of any stride, rows further apart
         with pytest.raises(ValueError, match="CUDA"):
             kvcache.free_rows(fine, lens[:len(fine)], refs, rows, 16)
+
+
+def test_textgen_has_a_rotary_entry_for_every_position(monkeypatch):
+    """A row's last page may reach past max_tokens, and a prompt may not: an index past the table would fault the device."""
+    from comfy_quant_bench_b200 import textgen
+    monkeypatch.setattr(textgen.ops, "quantize_affine_w4_weight", lambda w, group: (w, w, w))
+    m = textgen.TextModel(textgen.TextConfig(vocab=8, hidden=64, layers=1, heads=1, kv_heads=1, head_dim=64, ffn=64, group_size=64,
+                                             max_tokens=150, rows=2, pages=4, page_size=16), device="cpu")
+    positions = m.cache.block_table.shape[1] * m.cache.page_size           # what a row can reserve
+    assert positions == 160 and m.rope.shape == (positions, 32, 2)
+    with pytest.raises(ValueError, match="prompt of 151 tokens for rows of max_tokens = 150"):
+        m.prompt(torch.zeros(151, dtype=torch.long), 0)

@@ -165,3 +165,18 @@ def test_awq_layer_of_a_checkpoint_runs(tg):
     assert out.shape == (3, 96)
     with pytest.raises(ValueError, match="input_act"):
         lin.weight.linear(x, bias, input_act="swiglu")
+
+
+def test_rows_fill_their_last_page(tg):
+    """Steps at and past max_tokens, up to the end of the row's last page; the next one is refused."""
+    m = tg.TextModel(_config(tg, max_tokens=40, pages=8))
+    tokens = torch.arange(48, device="cuda")
+    want = _reference(m, tokens)
+    m.prompt(tokens[:38], 1)
+    row = torch.ones(1, dtype=torch.int32, device="cuda")
+    for i in range(38, 48):
+        assert _rel(m.step(tokens[i:i + 1], row)[0], want[i]) <= 1.5 * BOUND
+    m.cache.check()
+    m.step(tokens[:1], row)
+    with pytest.raises(RuntimeError, match="reserve"):
+        m.cache.check()
