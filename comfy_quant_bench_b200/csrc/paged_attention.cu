@@ -19,7 +19,9 @@
 // so equal calls give equal bits.
 //
 // Softmax statistics, scores and outputs are fp32.  The weights p enter the second product as two parts of the cache's
-// 16-bit type, p = hi + lo, since one part alone would add up to as much error as rounding the output does.
+// 16-bit type, p = hi + lo, since one part alone would add up to as much error as rounding the output does.  f16 parts
+// hold 2^15 p, and the sum is taken over the same: without it a weight of 2^-25 of the largest, which a long tail behind
+// one strong key has many of, would count in the sum alone.  So they are held to 2^-40 of the largest.
 // 8-bit caches are widened exactly to f16; a bf16 query is scaled by a power of two per head so that f16 holds it to
 // 2^-24 of its largest element.
 //
@@ -153,6 +155,14 @@ struct UnitIter {
   }
 };
 
+// what the weights' exponents are raised by: f16 parts reach up to 2^15, bf16 parts have fp32's range
+template <bool F16Math>
+__device__ __forceinline__ constexpr float weight_lift() { return F16Math ? 15.0f : 0.0f; }
+// log of the softmax's sum, from the largest score (a power of 2) and the sum of the raised weights
+__device__ __forceinline__ float log_sum(float top, float sum, float lift) {
+  return sum == 0.0f ? -INFINITY : (top + (log2f(sum) - lift)) / 1.4426950408889634f;
+}
+
 // 2^x to 2^-22 of it; below 2^-126 zero
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -167,6 +177,7 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
   using C = pattn::Cfg<D, FP8 ? 1 : 2, NT>;
   constexpr int ES = FP8 ? 1 : 2, kRow = C::kRow, kStages = C::kStages;
   constexpr bool kF16Math = F16 || FP8;
+  constexpr float kLift = weight_lift<kF16Math>();
   constexpr int kHeads = 8 * NT;                        // heads of a tile
   constexpr int kMt = D / 16;                           // 16-wide slices of the head dim
   extern __shared__ __align__(128) uint8_t smem[];
@@ -467,8 +478,8 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
           f[n][j] = exp2_fast(m[n][j] - base);
           grew |= mn != m[n][j];
           m[n][j] = mn;
-          s[n][j] = exp2_fast(x0 - base);
-          s[n][2 + j] = exp2_fast(x1 - base);
+          s[n][j] = exp2_fast((x0 - base) + kLift);        // two steps: the first one is never above 0
+          s[n][2 + j] = exp2_fast((x1 - base) + kLift);
           l[n][j] = l[n][j] * f[n][j] + (s[n][j] + s[n][2 + j]);
         }
         split16<kF16Math>(s[n][0], s[n][1], ph[n][0], pl[n][0]);
@@ -603,7 +614,7 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
             p[kHeads * D + kHeads + h] = sum;
           }
           if (tid < 8 && complete && a.lse != nullptr)
-            a.lse[static_cast<int64_t>(it.b) * a.Hq + h0 + h] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) / log2e;
+            a.lse[static_cast<int64_t>(it.b) * a.Hq + h0 + h] = log_sum(top, sum, kLift);
         }
         __syncthreads();                                  // the slots and the statistics are read
       }
@@ -662,7 +673,7 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
       else
         *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.out) + to) = __floats2bfloat162_rn(v.x * inv, v.y * inv);
       if (d == 0 && a.lse != nullptr)
-        a.lse[static_cast<int64_t>(it.b) * a.Hq + h0 + h] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) / log2e;
+        a.lse[static_cast<int64_t>(it.b) * a.Hq + h0 + h] = log_sum(top, sum, kLift);
     }
     // a CTA's part stays until every rank has read it
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -715,7 +726,8 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(const PagedAt
 #pragma unroll
   for (int j = 0; j < kPer; ++j) sum_o[warp][lane + 32 * j] = o[j];
   __syncthreads();
-  const float vs = a.cache_dtype == CQ_DT_FP8_E4M3 && a.v_scale != nullptr ? __ldg(a.v_scale + hk) : 1.0f;
+  const bool fp8 = a.cache_dtype == CQ_DT_FP8_E4M3;
+  const float vs = fp8 && a.v_scale != nullptr ? __ldg(a.v_scale + hk) : 1.0f;
   const float inv = l == 0.0f ? 0.0f : vs / l;
   const int64_t to = (static_cast<int64_t>(b) * a.Hq + h0 + h) * D;
   for (int d = threadIdx.x; d < D; d += 128) {
@@ -724,7 +736,7 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(const PagedAt
     else static_cast<__nv_bfloat16*>(a.out)[to + d] = __float2bfloat16_rn(y);
   }
   if (threadIdx.x == 0 && a.lse != nullptr)
-    a.lse[static_cast<int64_t>(b) * a.Hq + h0 + h] = l == 0.0f ? -INFINITY : (top + log2f(l)) / 1.4426950408889634f;
+    a.lse[static_cast<int64_t>(b) * a.Hq + h0 + h] = log_sum(top, l, fp8 ? weight_lift<true>() : weight_lift<F16>());
 }
 
 namespace {

@@ -836,3 +836,28 @@ def test_append_and_compact_read_a_table_whose_rows_share_memory(kv):
         for a, b in zip(*made):
             assert torch.equal(a, b)
     assert _status() == (0, 0)
+
+
+# ----------------------------------------------------------------------------------------------------------
+# weights far below the largest
+# ----------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("b,n", [(1, 600), (30, 600), (2, 9000)])
+@pytest.mark.parametrize("dtype,cache_type", [(torch.float16, torch.float16), (torch.float16, FP8), (torch.bfloat16, FP8),
+                                              (torch.bfloat16, torch.bfloat16)])
+def test_attention_long_tail_behind_one_strong_key(kv, dtype, cache_type, b, n):
+    """One key with a value of zero takes nearly all the weight, the others e^-16 to e^-18 of it (2^-23 to 2^-26), and the
+    output is made of them alone.  f16 parts of a weight are held to 2^-40 of the largest, 2^-14 of such a weight: within
+    the module's bound, whose A is the tail's.  Clusters, whole segments and runs with their join."""
+    k, v, table, lens = _cache([n] * b, 8, 16, 64, torch.float32, seed=n + b, poison=False)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    k[..., 0] = -16 - 2 * torch.rand(k.shape[:-1], generator=g, device="cuda")
+    v *= 20
+    first = table[:, 0].long()
+    k[first, :, 0, 0], v[first, :, 0] = 0.0, 0.0
+    q = torch.zeros(b, 16, 64, device="cuda")
+    q[..., 0] = 1.0
+    kw = {}
+    if cache_type == FP8:
+        kw = {"k_scale": torch.ones(8, device="cuda"), "v_scale": torch.full((8,), 50.0, device="cuda")}
+    _attention_holds(kv, q.to(dtype), k.to(cache_type), v.to(cache_type), table, lens, scale=1.0, **kw)
