@@ -7,7 +7,9 @@
 // pages_branch_kernel: free a list of rows, fork rows (destination rows take the source rows' pages and one more
 // reference to each), then make room for new tokens: a row whose last page is partly filled and held by another row
 // too gets its own copy of it (copy on write), and pages are taken for what does not fit.  One CTA: each phase is
-// short, needs the one before it, and a list of rows is checked whole before any of it is applied.
+// short and needs the one before it.  All lists of rows are checked before any phase begins, so a wrong list changes
+// nothing; whether the free pages suffice is known when the rows are freed and forked, and then only the reservation is
+// refused.
 #include "decode_common.cuh"
 
 namespace cq {
@@ -40,16 +42,18 @@ __device__ __forceinline__ int block_scan(int v, int* warp_sums, int* total) {
   return v + (warp > 0 ? before : 0);
 }
 
-// marks `rows` in the bitmap `seen`; *bad is set where one is out of range or already marked
-__device__ void mark_rows(const int* rows, int n, int table_rows, uint32_t* seen, int* bad) {
+// marks `rows` in the bitmap `seen`; whether each is in range and listed once (the same answer to all threads)
+__device__ bool mark_rows(const int* rows, int n, int table_rows, uint32_t* seen) {
   for (int i = threadIdx.x; i < (table_rows + 31) / 32; i += blockDim.x) seen[i] = 0;
   __syncthreads();
+  int bad = 0;
   for (int i = threadIdx.x; i < n; i += blockDim.x) {
     const int r = rows[i];
-    if (r < 0 || r >= table_rows || (atomicOr(&seen[r >> 5], 1u << (r & 31)) >> (r & 31) & 1u)) *bad = 1;
+    if (r < 0 || r >= table_rows || (atomicOr(&seen[r >> 5], 1u << (r & 31)) >> (r & 31) & 1u)) bad = 1;
   }
-  __syncthreads();
+  return !__syncthreads_or(bad);
 }
+__device__ __forceinline__ bool marked(const uint32_t* seen, int r) { return seen[r >> 5] >> (r & 31) & 1u; }
 
 __device__ __forceinline__ int held_pages(int len, int page_size, int width) {
   if (len <= 0) return 0;
@@ -76,58 +80,66 @@ __device__ __forceinline__ int lanes_of_row(int width) { return width >= 512 ? 3
 __global__ void __launch_bounds__(pages::kThreads) pages_branch_kernel(const PagesArgs a) {
   extern __shared__ uint32_t dyn[];
   __shared__ int warp_sums[32];
-  __shared__ int bad, over;
+  __shared__ int over;
   uint32_t* seen = dyn;                                  // [table_rows] bits
   uint32_t* bits = dyn + (a.table_rows + 31) / 32;       // [num_pages] bits
   const int tid = threadIdx.x;
   const int per = lanes_of_row(a.table_width), sub = tid & (per - 1), group = tid / per, groups = blockDim.x / per;
   const uint32_t mates = per == 32 ? 0xffffffffu : 0xffu << (tid & 24);   // the lanes of this thread's row
   grid_dep_launch();                                     // the copies may be set up while this runs
-  if (tid == 0) { bad = 0; over = 0; }
-  __syncthreads();
+  if (tid == 0) over = 0;
 
+  // the lists: each names rows of the table once, a fork's source is no destination, and a destination is empty or freed
+  // here; `site` has the same value in all threads
   int site = 0;
-  if (a.n_free > 0) {
-    mark_rows(a.free_rows, a.n_free, a.table_rows, seen, &bad);
-    if (bad) site = pages::kSiteFree;
+  if (a.n_free > 0 && !mark_rows(a.free_rows, a.n_free, a.table_rows, seen)) site = pages::kSiteFree;
+  if (site == 0 && a.n_fork > 0) {
+    int bad = 0;
+    for (int i = tid; i < a.n_fork; i += blockDim.x) {
+      const int d = a.dst[i];
+      if (d < 0 || d >= a.table_rows || !((a.n_free > 0 && marked(seen, d)) || a.lens[d] == 0)) bad = 1;
+    }
+    if (__syncthreads_or(bad) || ((a.dst != a.free_rows || a.n_fork != a.n_free) && !mark_rows(a.dst, a.n_fork, a.table_rows, seen)))
+      site = pages::kSiteFork;
     else {
-      for (int i = group; i < a.n_free; i += groups) {
-        const int r = a.free_rows[i];
-        int* row = a.table + r * a.table_stride;
-        const int held = held_pages(a.lens[r], a.page_size, a.table_width);
-        __syncwarp(mates);                                // every lane has read the row's length
-#pragma unroll 4
-        for (int j = sub; j < held; j += per) {
-          const int p = row[j];
-          if (p >= 0 && p < a.num_pages) atomicSub(&a.refs[p], 1);
-          row[j] = -1;
-        }
-        if (sub == 0) a.lens[r] = 0;
+      for (int i = tid; i < a.n_fork; i += blockDim.x) {
+        const int s = a.src[i];
+        if (s < 0 || s >= a.table_rows || marked(seen, s)) bad = 1;
       }
+      if (__syncthreads_or(bad)) site = pages::kSiteFork;
+    }
+  }
+  if (site == 0 && a.n_res > 0 && (a.res_rows != a.dst || a.n_res != a.n_fork) &&
+      !mark_rows(a.res_rows, a.n_res, a.table_rows, seen))
+    site = pages::kSiteReserve;
+
+  if (site == 0 && a.n_free > 0) {
+    for (int i = group; i < a.n_free; i += groups) {
+      const int r = a.free_rows[i];
+      int* row = a.table + r * a.table_stride;
+      const int held = held_pages(a.lens[r], a.page_size, a.table_width);
+      __syncwarp(mates);                                  // every lane has read the row's length
+#pragma unroll 4
+      for (int j = sub; j < held; j += per) {
+        const int p = row[j];
+        if (p >= 0 && p < a.num_pages) atomicSub(&a.refs[p], 1);
+        row[j] = -1;
+      }
+      if (sub == 0) a.lens[r] = 0;
     }
     __syncthreads();
   }
   if (site == 0 && a.n_fork > 0) {
-    if (a.dst != a.free_rows || a.n_fork != a.n_free) mark_rows(a.dst, a.n_fork, a.table_rows, seen, &bad);
-    for (int i = tid; i < a.n_fork; i += blockDim.x) {
+    for (int i = group; i < a.n_fork; i += groups) {
       const int s = a.src[i], d = a.dst[i];
-      if (s < 0 || s >= a.table_rows || (seen[s >> 5] >> (s & 31) & 1u)) bad = 1;    // a source is no destination
-      if (d >= 0 && d < a.table_rows && a.lens[d] != 0) bad = 1;                     // a destination is empty
-    }
-    __syncthreads();
-    if (bad) site = pages::kSiteFork;
-    else {
-      for (int i = group; i < a.n_fork; i += groups) {
-        const int s = a.src[i], d = a.dst[i];
-        const int len = a.lens[s], held = held_pages(len, a.page_size, a.table_width);
+      const int len = a.lens[s], held = held_pages(len, a.page_size, a.table_width);
 #pragma unroll 4
-        for (int j = sub; j < held; j += per) {
-          const int p = a.table[s * a.table_stride + j];
-          a.table[d * a.table_stride + j] = p;
-          if (p >= 0 && p < a.num_pages) atomicAdd(&a.refs[p], 1);
-        }
-        if (sub == 0) a.lens[d] = len;
+      for (int j = sub; j < held; j += per) {
+        const int p = a.table[s * a.table_stride + j];
+        a.table[d * a.table_stride + j] = p;
+        if (p >= 0 && p < a.num_pages) atomicAdd(&a.refs[p], 1);
       }
+      if (sub == 0) a.lens[d] = len;
     }
     __syncthreads();
   }
@@ -135,12 +147,9 @@ __global__ void __launch_bounds__(pages::kThreads) pages_branch_kernel(const Pag
     if (site != 0 && tid == 0) record_status(CQ_ERR_ARG, site);
     return;
   }
-  int code = site != 0 ? CQ_ERR_ARG : CQ_OK;
-  if (site == 0) {
-    site = pages::kSiteReserve;
-    if (a.res_rows != a.dst || a.n_res != a.n_fork) mark_rows(a.res_rows, a.n_res, a.table_rows, seen, &bad);
-    if (bad) code = CQ_ERR_ARG;
-  }
+  int code = CQ_OK;
+  if (site != 0) code = CQ_ERR_ARG;
+  else site = pages::kSiteReserve;
   int total = 0;
   if (code == CQ_OK) {
     // pages that each row needs, and where its share of the free pages begins

@@ -6,8 +6,9 @@ that hold each page stay on the device, so a decode step never waits for the hos
 graph.  Pages are taken lowest index first; every result is a function of the state alone.
 
 The functions work on plain tensors; ``PagedKVCache`` keeps them together.  As with the other operators there is no
-CPU path: CPU tensors are rejected.  A call that the device has to refuse (too few free pages, a row named twice)
-leaves the state as it was and is recorded in the device status word: ``check()``.
+CPU path: CPU tensors are rejected.  What the device has to refuse is recorded in its status word (``check()``): a
+call with a wrong list of rows (out of range, named twice) changes nothing; a reservation without room (too few free
+pages, too narrow a table) reserves nothing - ``branch_rows`` has freed and forked its rows by then.
 """
 from __future__ import annotations
 
@@ -69,7 +70,10 @@ def reserve_tokens(block_table, seq_lens, ref_counts, rows, count, k_cache, v_ca
 
 def branch_rows(block_table, seq_lens, ref_counts, src, dst, count, k_cache, v_cache):
     """One resampling step: the rows ``dst`` are freed, become copies of ``src`` and get room for ``count`` new tokens
-    - ``free_rows(dst)``, ``fork_rows(src, dst)`` and ``reserve_tokens(dst, count)`` in one call."""
+    - ``free_rows(dst)``, ``fork_rows(src, dst)`` and ``reserve_tokens(dst, count)`` in one call.  A wrong list (a source
+    among the destinations, a row out of range or named twice) changes nothing.  With too few free pages the
+    reservation alone is refused: what ``dst`` held is gone, the rows are copies of ``src`` without the new room, and
+    ``reserve_tokens(dst, count)`` gives it to them once other rows are freed."""
     counts, count = (count, 0) if isinstance(count, torch.Tensor) else (None, count)
     return _lib.decode().pages_update(block_table, seq_lens, ref_counts, k_cache.shape[3], dst, src, dst, dst, counts, count,
                                       k_cache, v_cache)

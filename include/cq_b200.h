@@ -538,10 +538,12 @@ CQ_API int cq_kv_append(const void* k_new, int64_t k_layer_stride, int64_t k_tok
  *            destination page, else -1, -1), copied in every layer of k_cache and v_cache (layers of layer_bytes, a
  *            page contiguous in page_bytes; layers == 0: not copied).  Free pages are taken lowest index first, for
  *            the rows in order; a page given up in this phase is free only after it.  start[i]: tokens before.
- * A phase that cannot be done whole is refused: it and the phases after it change nothing, start and copies are -1,
- * and the device status word (cq_take_device_status) gets CQ_ERR_ARG (rows out of range, repeated, a destination
- * that is not empty) or CQ_ERR_CAPACITY (too few free pages or too narrow a table) with site 101 (free), 102 (fork)
- * or 103 (reserve).  workspace: cq_pages_workspace_bytes(num_pages, n_reserve).
+ * All lists are checked before the first phase: where one is wrong (rows out of range, repeated, a source that is a
+ * destination, a destination that is neither empty nor freed by this call) nothing changes, and the device status word
+ * (cq_take_device_status) gets CQ_ERR_ARG with site 101 (free), 102 (fork) or 103 (reserve).  A reservation without
+ * room (too few free pages or too narrow a table) is refused whole, CQ_ERR_CAPACITY with site 103; the rows are freed
+ * and forked by then.  start and copies are -1 after a refusal.  workspace: cq_pages_workspace_bytes(num_pages,
+ * n_reserve).
  */
 CQ_API int64_t cq_pages_workspace_bytes(int64_t num_pages, int64_t reserved_rows);
 CQ_API int cq_pages_update(int32_t* block_table, int64_t table_rows, int64_t table_width, int64_t table_stride,

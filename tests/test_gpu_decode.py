@@ -861,3 +861,77 @@ def test_attention_long_tail_behind_one_strong_key(kv, dtype, cache_type, b, n):
     if cache_type == FP8:
         kw = {"k_scale": torch.ones(8, device="cuda"), "v_scale": torch.full((8,), 50.0, device="cuda")}
     _attention_holds(kv, q.to(dtype), k.to(cache_type), v.to(cache_type), table, lens, scale=1.0, **kw)
+
+
+# ----------------------------------------------------------------------------------------------------------
+# refused branches
+# ----------------------------------------------------------------------------------------------------------
+
+def _state(c):
+    return [t.clone() for t in (c.block_table, c.seq_lens, c.ref_counts, c.k.view(torch.int16), c.v.view(torch.int16))]
+
+
+def _three_rows(kv, pages=8):
+    """Rows 0, 1 and 2 of 20, 33 and 5 tokens, 2 + 3 + 1 of the pages, and rows 3 and 4 without any."""
+    c = kv.PagedKVCache(2, pages, 1, 64, 5, 64, page_size=16, dtype=torch.bfloat16)
+    c.reserve(_rows(0, 1, 2), _rows(20, 33, 5))
+    c.k.normal_(), c.v.normal_()
+    assert _status() == (0, 0)
+    return c
+
+
+@pytest.mark.parametrize("src,dst", [((0,), (0,)), ((0, 1), (1, 2)), ((5,), (1,)), ((-1,), (1,)), ((0, 7), (1, 2)),
+                                     ((2 ** 31 - 1,), (2,))])
+def test_branch_with_a_wrong_source_changes_nothing(kv, src, dst):
+    c = _three_rows(kv)
+    before = _state(c)
+    assert c.branch(_rows(*src), _rows(*dst), 1).tolist() == [-1] * len(src)
+    assert _status() == (1, 102)
+    assert all(torch.equal(a, b) for a, b in zip(before, _state(c)))
+
+
+@pytest.mark.parametrize("free,src,dst,reserve,site", [((1, 1), (0,), (3,), (3,), 101), ((1, 9), (0,), (3,), (3,), 101),
+                                                       ((1,), (0,), (2,), (2,), 102),      # neither empty nor freed
+                                                       ((1,), (0, 2), (3, 3), (3,), 102), ((1,), (0,), (-2,), (3,), 102),
+                                                       ((1,), (0,), (3,), (0, 0), 103), ((1,), (0,), (3,), (5,), 103),
+                                                       ((1,), (0,), (3,), (-1,), 103)])
+def test_a_wrong_list_stops_the_phases_before_it_too(kv, free, src, dst, reserve, site):
+    from comfy_quant_bench_b200 import _lib
+    c = _three_rows(kv)
+    before = _state(c)
+    start, copies = _lib.decode().pages_update(c.block_table, c.seq_lens, c.ref_counts, 16, _rows(*free), _rows(*src), _rows(*dst),
+                                               _rows(*reserve), None, 1, c.k, c.v)
+    assert _status() == (1, site) and bool((start == -1).all()) and bool((copies == -1).all())
+    assert all(torch.equal(a, b) for a, b in zip(before, _state(c)))
+
+
+def test_phases_on_lists_of_their_own(kv):
+    """A destination may be empty or freed by the same call, a freed row may be a (then empty) source, and the rows that grow
+    may be others."""
+    from comfy_quant_bench_b200 import _lib
+    c = _three_rows(kv)
+    m = Model(2, 8, 1, 64, 5, 4, 16)
+    m.reserve([0, 1, 2], [20, 33, 5])
+    m.agrees(c)
+    free, src, dst, reserve = [1, 2], [0, 2, 0], [3, 4, 1], [0, 4]
+    m.free(free), m.fork(src, dst)
+    want = m.reserve(reserve, [3, 3])
+    start, copies = _lib.decode().pages_update(c.block_table, c.seq_lens, c.ref_counts, 16, _rows(*free), _rows(*src), _rows(*dst),
+                                               _rows(*reserve), None, 3, c.k, c.v)
+    assert _status() == (0, 0) and (start.tolist(), copies.tolist()) == want
+    m.agrees(c)
+
+
+def test_branch_without_room_is_completed_by_a_reservation(kv):
+    """The reservation alone is refused: the rows are copies of their sources, and get their room once there is some."""
+    c = _three_rows(kv, pages=6)
+    c.branch(_rows(1, 1), _rows(3, 4), 1)                      # two copies of the last page of 33 tokens, no page free
+    assert _status() == (7, 103)
+    assert c.seq_lens.tolist() == [20, 33, 5, 33, 33]
+    assert torch.equal(c.block_table[3], c.block_table[1]) and torch.equal(c.block_table[4], c.block_table[1])
+    c.free(_rows(0))
+    last = int(c.block_table[1, 2])
+    assert c.reserve(_rows(3, 4), 1).tolist() == [33, 33] and _status() == (0, 0)
+    for r in (3, 4):
+        own = int(c.block_table[r, 2])
+        assert own != last and torch.equal(c.k[:, own], c.k[:, last]) and torch.equal(c.v[:, own], c.v[:, last])
