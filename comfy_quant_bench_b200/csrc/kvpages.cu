@@ -17,6 +17,7 @@ namespace cq {
 namespace pages {
 constexpr int kThreads = 1024;
 constexpr int kMaxShared = 200 * 1024;   // bytes of the row and page bitmaps
+constexpr int kPlainShared = 47 * 1024;  // what a launch may ask for as it is: 48 KB less the kernels' static arrays
 constexpr int kSiteFree = 101, kSiteFork = 102, kSiteReserve = 103;   // device status sites
 }  // namespace pages
 
@@ -227,7 +228,7 @@ int64_t pages_branch_shared(int table_rows, int num_pages) {
 
 cudaError_t launch_pages_branch(const PagesArgs& a, cudaStream_t st) {
   const int64_t smem = pages_branch_shared(a.table_rows, a.num_pages);
-  if (smem > 48 * 1024) {
+  if (smem > pages::kPlainShared) {
     static unsigned long long devices = 0;
     const cudaError_t e = allow_shared(pages_branch_kernel, pages::kMaxShared, devices);
     if (e != cudaSuccess) return e;
@@ -342,7 +343,7 @@ __global__ void __launch_bounds__(256) pages_remap_kernel(const CompactArgs a) {
 
 cudaError_t launch_pages_compact(const CompactArgs& a, cudaStream_t st) {
   const int smem = (a.num_pages + 31) / 32 * 4;
-  if (smem > 48 * 1024) {
+  if (smem > pages::kPlainShared) {
     static unsigned long long devices = 0;
     const cudaError_t e = allow_shared(pages_compact_kernel, pages::kMaxShared, devices);
     if (e != cudaSuccess) return e;

@@ -935,3 +935,14 @@ def test_branch_without_room_is_completed_by_a_reservation(kv):
     for r in (3, 4):
         own = int(c.block_table[r, 2])
         assert own != last and torch.equal(c.k[:, own], c.k[:, last]) and torch.equal(c.v[:, own], c.v[:, last])
+
+
+@pytest.mark.parametrize("pages", [392960, 393216])
+def test_pages_pools_at_the_default_limit_of_shared_memory(kv, pages):
+    """Bitmaps of 48 KB or just below, which fit the limit of a plain launch only without the kernels' static arrays."""
+    c = kv.PagedKVCache(1, pages, 1, 8, 2, 8 * 40, page_size=8, dtype=torch.bfloat16)
+    assert c.reserve(_rows(0, 1), _rows(300, 9)).tolist() == [0, 0]
+    c.free(_rows(0))
+    c.compact()
+    assert _status() == (0, 0)
+    assert c.block_table[1, :2].tolist() == [0, 1] and c.ref_counts[:3].tolist() == [1, 1, 0] and int(c.ref_counts.sum()) == 2
