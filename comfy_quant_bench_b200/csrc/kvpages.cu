@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(pages::kThreads) pages_branch_kernel(const Pag
 }
 
 int64_t pages_branch_shared(int table_rows, int num_pages) {
-  return 4 * (static_cast<int64_t>((table_rows + 31) / 32) + (num_pages + 31) / 32);
+  return 4 * ((static_cast<int64_t>(table_rows) + 31) / 32 + (static_cast<int64_t>(num_pages) + 31) / 32);
 }
 
 cudaError_t launch_pages_branch(const PagesArgs& a, cudaStream_t st) {

@@ -171,3 +171,12 @@ def test_textgen_has_a_rotary_entry_for_every_position(monkeypatch):
     assert positions == 160 and m.rope.shape == (positions, 32, 2)
     with pytest.raises(ValueError, match="prompt of 151 tokens for rows of max_tokens = 150"):
         m.prompt(torch.zeros(151, dtype=torch.long), 0)
+
+
+@pytest.mark.parametrize("pages", [(1 << 31) - 1, (1 << 31) - 31, 1 << 30])
+def test_pools_near_the_integer_limit_are_refused_as_too_large(lib, pages):
+    from comfy_quant_bench_b200 import _lib as L
+    assert lib.cq_pages_update(VP, 4, 8, 8, VP, VP, pages, 16, VP, 1, None, None, 0, None, 0, None, 0, None, None, None, None, 0,
+                               0, 0, None, 0, None) == L.CQ_ERR_CAPACITY
+    assert lib.cq_pages_compact(VP, 4, 8, 8, VP, 8, VP, VP, pages, VP, None, None, 0, 0, 0, VP, 1 << 40, None) == \
+        L.CQ_ERR_CAPACITY
