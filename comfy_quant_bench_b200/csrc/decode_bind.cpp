@@ -276,6 +276,10 @@ py::object pages_update(const Tensor& table, const Tensor& lens, const Tensor& r
   i32(lens, 1, "seq_lens");
   i32(refs, 1, "ref_counts");
   if (lens.size(0) != table.size(0)) refuse("seq_lens must have one entry per table row (", table.size(0), ")");
+  if (!free_rows && !src && !dst && !reserve) refuse("rows must be an int32 tensor");
+  if (src.has_value() != dst.has_value()) refuse("src and dst must both be int32 tensors");
+  if (counts && !reserve) refuse("rows must be an int32 tensor, one entry per count");
+  if (reserve && (!k_cache || !v_cache)) refuse("the caches are needed to reserve");
   if (free_rows) i32(*free_rows, 1, "rows");
   if (src) i32(*src, 1, "src");
   if (dst) i32(*dst, 1, "dst");

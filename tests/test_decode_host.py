@@ -180,3 +180,20 @@ def test_pools_near_the_integer_limit_are_refused_as_too_large(lib, pages):
                                0, 0, None, 0, None) == L.CQ_ERR_CAPACITY
     assert lib.cq_pages_compact(VP, 4, 8, 8, VP, 8, VP, VP, pages, VP, None, None, 0, 0, 0, VP, 1 << 40, None) == \
         L.CQ_ERR_CAPACITY
+
+
+def test_a_list_left_out_is_refused():
+    """None in place of a list of rows; the page calls take their lists as optional ones."""
+    from comfy_quant_bench_b200 import kvcache
+    table, lens, refs = (torch.zeros(s, dtype=torch.int32) for s in ((3, 4), 3, 6))
+    k, one = torch.zeros(1, 6, 1, 16, 64, dtype=torch.bfloat16), torch.zeros(1, dtype=torch.int32)
+    for call in (lambda: kvcache.free_rows(table, lens, refs, None, 16), lambda: kvcache.fork_rows(table, lens, refs, one, None, 16),
+                 lambda: kvcache.fork_rows(table, lens, refs, None, one, 16),
+                 lambda: kvcache.fork_rows(table, lens, refs, None, None, 16),
+                 lambda: kvcache.reserve_tokens(table, lens, refs, None, 1, k, k),
+                 lambda: kvcache.reserve_tokens(table, lens, refs, None, one, k, k),
+                 lambda: kvcache.reserve_tokens(table, lens, refs, one, 1, k, None),
+                 lambda: kvcache.branch_rows(table, lens, refs, None, one, 1, k, k),
+                 lambda: kvcache.branch_rows(table, lens, refs, one, None, one, k, k)):
+        with pytest.raises(ValueError, match="int32 tensor|caches are needed"):
+            call()
