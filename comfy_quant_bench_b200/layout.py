@@ -178,7 +178,8 @@ class B200AffineW4A8Layout(QuantizedLayout):
 
 class B200AwqW4A16Layout(B200AffineW4A8Layout):
     """awq_w4a16: the affine int4 weight with 16-bit activations (a language model's weights; groups of 32, 64 or 128).
-    The activations are not quantized, so an activation function before the linear is not folded in."""
+    The activations are not quantized, so an activation function before the linear is not folded in.  Activations of
+    another type than bf16 or f16 are rounded to bf16; the result has the caller's type."""
     QUANTIZES_INPUT = False
 
     @classmethod
@@ -186,9 +187,11 @@ class B200AwqW4A16Layout(B200AffineW4A8Layout):
         from .ops import w4a16_linear
         if input_act is not None:
             raise ValueError("awq_w4a16 has no activation quantizer to fold input_act into")
-        if x.dtype not in (torch.bfloat16, torch.float16):
+        dt = x.dtype
+        if dt not in (torch.bfloat16, torch.float16):
             x = x.to(torch.bfloat16)
-        return w4a16_linear(x, qdata, params.scale, params.zeros, bias, group_size=params.group_size)
+        y = w4a16_linear(x, qdata, params.scale, params.zeros, bias, group_size=params.group_size)
+        return y if y.dtype == dt else y.to(dt)
 
 
 class B200TensorWiseINT8Layout(QuantizedLayout):

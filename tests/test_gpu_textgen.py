@@ -180,3 +180,26 @@ def test_rows_fill_their_last_page(tg):
     m.step(tokens[:1], row)
     with pytest.raises(RuntimeError, match="reserve"):
         m.cache.check()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.float16, torch.bfloat16])
+def test_awq_layer_returns_the_type_it_is_given(tg, dtype):
+    """With and without a weight patch.  Other types are rounded to bf16 on the way in; the patched path takes the weight
+    rounded to bf16."""
+    from comfy_quant_bench_b200 import comfy_ops, layout, ops
+    layout.register_w4a16()
+    g = torch.Generator(device="cuda").manual_seed(6)
+    q, s, z = ops.quantize_affine_w4_weight(torch.randn(96, 256, generator=g, device="cuda"), 64)
+    bias = torch.randn(96, generator=g, device="cuda").bfloat16()
+    params = layout.get_layout_class("B200AwqW4A16Layout").Params(scale=s, zeros=z, orig_dtype=torch.bfloat16, orig_shape=(96, 256),
+                                                                  group_size=64)
+    lin = comfy_ops.Linear.from_quantized(layout.QuantizedWeight(q, "B200AwqW4A16Layout", params), bias)
+    for tokens in (1, 3, 40):
+        x = torch.randn(tokens, 256, generator=g, device="cuda").to(dtype)
+        y = lin(x)
+        held = x if dtype in (torch.bfloat16, torch.float16) else x.bfloat16()
+        assert y.dtype == dtype and torch.equal(y, ops.w4a16_linear(held, q, s, z, bias, group_size=64).to(dtype))
+        lin.weight_function = [lambda w: w]
+        patched = lin(x)
+        lin.weight_function = []
+        assert patched.dtype == dtype and _rel(y, patched.float()) <= 2.0 ** -7
