@@ -44,9 +44,10 @@ __global__ void __launch_bounds__(256) w4a16_tokens_kernel(const void* x, int64_
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = fmaxf(top, tops[i]);
-    // both powers are normal numbers; a token with an infinity keeps its values and overflows
+    // from 2^-126 on both powers are normal numbers, and the smallest bf16 becomes 2^-7; a token with an infinity keeps its
+    // values and overflows
     const int ex = static_cast<int>(__float_as_uint(top) >> 23) - 127;
-    const int by = top > 0.0f && ex < 128 ? min(max(ex - 13, -100), 114) : 0;
+    const int by = top > 0.0f && ex < 128 ? max(ex - 13, -126) : 0;
     down = __uint_as_float(static_cast<uint32_t>(127 - by) << 23);
     if (m < M && threadIdx.x == 0) factor[m] = __uint_as_float(static_cast<uint32_t>(127 + by) << 23);
   }

@@ -946,3 +946,19 @@ def test_pages_pools_at_the_default_limit_of_shared_memory(kv, pages):
     c.compact()
     assert _status() == (0, 0)
     assert c.block_table[1, :2].tolist() == [0, 1] and c.ref_counts[:3].tolist() == [1, 1, 0] and int(c.ref_counts.sum()) == 2
+
+
+# ----------------------------------------------------------------------------------------------------------
+# sizes near the ends of bf16's range
+# ----------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("power", [-130, -122, -118, -110, -95, 90, 110])
+@pytest.mark.parametrize("m", [1, 8, 9, 32, 33, 64])
+def test_linear_tokens_of_any_size(ops, m, power):
+    """Tokens of about 2^power, one of ordinary size among them, in each of the three kernels: bf16 tokens beyond eight are
+    multiplied as f16 with a power of two per token, which has to bring every bf16 value into f16's range."""
+    x, q, s, z, _ = _linear_problem(m, 1024, 200, 64, torch.bfloat16, seed=power)
+    size = torch.full((m, 1), 2.0 ** power, device="cuda")
+    size[m // 2] = 1.0 if m > 1 else size[0]
+    x = (x.float() * size).bfloat16()
+    _linear_holds(ops, x, q, s, z, None, 64)
