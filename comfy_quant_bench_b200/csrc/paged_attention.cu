@@ -382,9 +382,9 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
         if constexpr (FP8 && !F16) {
 #pragma unroll
           for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-          // 2^e with top in [2^e', 2^(e'+1)) taken to [2^13, 2^14); both powers are normal numbers
+          // top in [2^e, 2^(e + 1)) is taken to [2^13, 2^14); from 2^-126 on both powers are normal numbers
           const int ex = static_cast<int>(__float_as_uint(top) >> 23) - 127;
-          const int by = top > 0.0f && ex < 128 ? min(max(ex - 13, -100), 100) : 0;
+          const int by = top > 0.0f && ex < 128 ? max(ex - 13, -126) : 0;
           factor = __uint_as_float(static_cast<uint32_t>(127 + by) << 23);
           const float down = __uint_as_float(static_cast<uint32_t>(127 - by) << 23);
 #pragma unroll

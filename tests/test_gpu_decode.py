@@ -962,3 +962,14 @@ def test_linear_tokens_of_any_size(ops, m, power):
     size[m // 2] = 1.0 if m > 1 else size[0]
     x = (x.float() * size).bfloat16()
     _linear_holds(ops, x, q, s, z, None, 64)
+
+
+@pytest.mark.parametrize("power", [-120, -110, -90, 0, 90, 110, 120])
+@pytest.mark.parametrize("cache_type", [torch.bfloat16, FP8])
+def test_attention_queries_of_any_size(kv, cache_type, power):
+    """Queries of about 2^power and a scale that brings the scores back: a bf16 query of an 8-bit cache is multiplied as f16
+    with a power of two per head."""
+    k, v, table, n = _cache([300, 37], 2, 16, 64, cache_type, seed=3)
+    kw = {} if cache_type != FP8 else {"k_scale": torch.tensor([0.05, 0.02], device="cuda"), "v_scale": torch.ones(2, device="cuda")}
+    q = (_query(2, 8, 64, torch.bfloat16, 1).float() * 2.0 ** power).bfloat16()
+    _attention_holds(kv, q, k, v, table, n, scale=2.0 ** (-power - 3), **kw)
