@@ -399,7 +399,7 @@ __global__ void __launch_bounds__(w4tc::Plan<G, NTOK>::kThreads, 2)
       if (a.bias != nullptr) y += __half2float(static_cast<const __half*>(a.bias)[col]);
       static_cast<__half*>(a.out)[at] = __float2half_rn(y);
     } else {
-      y *= __ldg(a.factor + m);
+      y *= __ldcg(a.factor + m);                              // written while this grid was already there: no read-only load
       if (a.bias != nullptr) y += __bfloat162float(static_cast<const __nv_bfloat16*>(a.bias)[col]);
       static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(y);
     }

@@ -973,3 +973,18 @@ def test_attention_queries_of_any_size(kv, cache_type, power):
     kw = {} if cache_type != FP8 else {"k_scale": torch.tensor([0.05, 0.02], device="cuda"), "v_scale": torch.ones(2, device="cuda")}
     q = (_query(2, 8, 64, torch.bfloat16, 1).float() * 2.0 ** power).bfloat16()
     _attention_holds(kv, q, k, v, table, n, scale=2.0 ** (-power - 3), **kw)
+
+
+@pytest.mark.parametrize("m", [12, 40])
+def test_linear_calls_that_follow_each_other_use_their_own_tokens_sizes(ops, m):
+    """The product's grid is already there when the kernel before it writes what each token was divided by; with a
+    workspace that is taken again, the value before is another call's."""
+    x, q, s, z, b = _linear_problem(m, 512, 384, 64, torch.bfloat16)
+    sizes = [1.0, 2.0 ** 30, 2.0 ** -30, 2.0 ** 7]
+    wants = [ops.w4a16_linear((x.float() * p).bfloat16(), q, s, z, group_size=64) for p in sizes]
+    torch.cuda.synchronize()
+    many = [(i, ops.w4a16_linear((x.float() * sizes[i]).bfloat16(), q, s, z, group_size=64)) for i in [0, 1, 2, 3] * 25]
+    for i, y in many:
+        assert torch.equal(y, wants[i])
+    for p, y in zip(sizes, wants):
+        assert torch.equal((y.double() / p).bfloat16(), wants[0])
