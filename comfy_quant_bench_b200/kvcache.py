@@ -88,9 +88,11 @@ def compact_pages(block_table, ref_counts, k_cache, v_cache, *, out_table: torch
     return _lib.decode().compact_pages(block_table, ref_counts, k_cache, v_cache, out_table, out_refs)
 
 
-def check() -> None:
-    """Raise if the device refused a call since the last check (synchronizes the current stream)."""
-    status, site = _lib.take_device_status(torch.cuda.current_stream().cuda_stream)
+def check(device=None) -> None:
+    """Raise if the device (default: the current one) refused a call since the last check.  Synchronizes its current
+    stream."""
+    with torch.cuda.device(device):                      # each device has a status word of its own
+        status, site = _lib.take_device_status(torch.cuda.current_stream().cuda_stream)
     if status:
         raise _lib.CQError(f"cache {_SITES.get(site, f'site {site}')}", status, _lib.status_string(status))
 
@@ -143,4 +145,4 @@ class PagedKVCache:
                                k_scale=self.k_scale, v_scale=self.v_scale, **kw)
 
     def check(self) -> None:
-        check()
+        check(self.k.device)

@@ -197,3 +197,31 @@ def test_a_list_left_out_is_refused():
                  lambda: kvcache.branch_rows(table, lens, refs, one, None, one, k, k)):
         with pytest.raises(ValueError, match="int32 tensor|caches are needed"):
             call()
+
+
+def test_a_cache_asks_its_own_device_for_refusals(monkeypatch):
+    """A cache on another device than the current one: the status word and the stream are that device's."""
+    import contextlib
+    import types
+
+    from comfy_quant_bench_b200 import kvcache
+    current, asked = ["cuda:0"], []
+
+    @contextlib.contextmanager
+    def device(d):
+        before, current[0] = current[0], current[0] if d is None else str(d)
+        yield
+        current[0] = before
+
+    def take(stream):
+        asked.append((current[0], stream))
+        return (7, 103) if current[0] == "cuda:1" else (0, 0)
+    monkeypatch.setattr(kvcache.torch.cuda, "device", device)
+    monkeypatch.setattr(kvcache.torch.cuda, "current_stream", lambda: types.SimpleNamespace(cuda_stream="of " + current[0]))
+    monkeypatch.setattr(kvcache._lib, "take_device_status", take)
+    c = kvcache.PagedKVCache(1, 4, 1, 64, 2, 32, device="cpu")
+    c.k = types.SimpleNamespace(device=torch.device("cuda:1"))
+    with pytest.raises(RuntimeError, match="reserve"):
+        c.check()
+    kvcache.check()
+    assert asked == [("cuda:1", "of cuda:1"), ("cuda:0", "of cuda:0")] and current == ["cuda:0"]
