@@ -30,7 +30,12 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     caches [num_pages, kv_heads, page_size, D] of q's type or float8_e4m3fn (with ``k_scale`` / ``v_scale`` f32
     [kv_heads]); q_heads a multiple of kv_heads, D 64, 128 or 256.  ``window`` > 0: only the last ``window`` tokens
     and the first ``sinks`` ones are visible.  A row that sees nothing gives zeros (lse -inf).  ``scale`` defaults to
-    D ** -0.5.  Returns out [B, q_heads, D], with ``return_lse`` also f32 [B, q_heads]."""
+    D ** -0.5.  Returns out [B, q_heads, D], with ``return_lse`` also f32 [B, q_heads].
+
+    Scores, exponentials and sums are fp32.  A softmax weight enters the product with the values as two 16-bit parts: to
+    2^-16 of itself with a bf16 cache, to 2^-22 of itself and 2^-40 of the largest with the others.  An infinite value in
+    sight makes its element of the output not finite, but NaN also where the definition gives an infinity.  A table
+    whose rows share memory (one row expanded to several queries) is copied first."""
     return _lib.decode().paged_attention(q, k_cache, v_cache, block_table, seq_lens, rows, scale, window, sinks, k_scale,
                                          v_scale, out, return_lse)
 

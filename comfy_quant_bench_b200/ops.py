@@ -481,8 +481,13 @@ def w4a16_linear(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor, ze
     """Linear of 16-bit activations with awq-layout weights: W = (q - 8) * scale + zeros, y = x W^T + bias.
 
     x [..., K] bf16 or f16 (its rows may be strided), qweight int8 or uint8 [N, K/2] (low nibble = even column),
-    scale and zeros bf16 [K/group_size, N] (group_size 32, 64 or 128), bias [N].  Products and sums are fp32, rounded
-    once to the type of x.  For the few tokens of a decode step; ``w4a8_affine_linear`` takes many tokens."""
+    scale and zeros bf16 [K/group_size, N] (group_size 32, 64 or 128), bias [N] (rounded to the type of x if it has
+    another one).  Products and sums are fp32, rounded once to the type of x.  For the few tokens of a decode step;
+    ``w4a8_affine_linear`` takes many tokens.
+
+    More than eight bf16 tokens are multiplied as f16 after a power of two per token: less exact below 2^-28 of the
+    token's largest element, zero below 2^-38.  The scale's and the zero's terms of a group are added apart, so a token
+    with an infinity or a NaN gets outputs that are not finite, but NaN also where the definition gives an infinity."""
     return _lib.decode().w4a16_linear(x, qweight, scale, zeros, bias, group_size, out)
 
 

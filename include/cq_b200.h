@@ -475,7 +475,9 @@ typedef enum {
  *   workspace  cq_w4a16_workspace_bytes (0 for M <= 8), 256-byte aligned, of this call alone
  * group 32, 64 or 128, K a multiple of it and at most 32768; any N; M up to 1048576.  Built for the few tokens of a
  * decode step (it reads the weights once per 64 tokens); cq_linear_w4a8_affine is the linear for many tokens.  A
- * token with an infinite or NaN activation gets outputs that are not finite.
+ * token with an infinite or NaN activation gets outputs that are not finite (NaN, too, where the sum as written is an
+ * infinity).  For M > 8 bf16 tokens are multiplied as f16 after a power of two per token: less exact below 2^-28 of the
+ * token's largest element, zero below 2^-38.
  */
 CQ_API int64_t cq_w4a16_workspace_bytes(int64_t M, int64_t K, int group);
 CQ_API int cq_w4a16_linear(const void* x, int64_t ldx, int dtype, int64_t M, int64_t K, int64_t N,
@@ -492,7 +494,9 @@ CQ_API int cq_w4a16_linear(const void* x, int64_t ldx, int dtype, int64_t M, int
  * cq_paged_attention: out[b, h] = sum_j p_j v_j / sum_j p_j with p_j = exp(scale q[b, h] . k_j - max) over the visible
  * tokens j of table row rows[b] (NULL: row b): j < seq_lens[row] and, with window > 0, j >= seq_lens[row] - window or
  * j < sinks.  Query head h reads key-value head h / (q_heads / kv_heads).  A row that sees nothing (no tokens, no
- * page, a row out of range) gives zeros.
+ * page, a row out of range) gives zeros.  Scores, exponentials (2^-20) and sums are fp32; a weight enters the product with
+ * v as two 16-bit parts, to 2^-16 of itself (bf16 caches) or, others, to 2^-22 of itself and 2^-40 of the largest.  An
+ * infinite v_j makes its element not finite (NaN, too, where the sum as written is an infinity).
  *   q    [batch, q_heads, head_dim] of `dtype` (bf16 or f16) with strides in elements; out the same, contiguous
  *   lse  f32 [batch, q_heads] or NULL: log sum_j exp(scale q . k_j) (-inf for a row that sees nothing)
  *   cache_dtype  dtype, or CQ_DT_FP8_E4M3 with k_scale / v_scale f32 [kv_heads] (NULL: 1)

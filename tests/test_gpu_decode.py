@@ -988,3 +988,44 @@ def test_linear_calls_that_follow_each_other_use_their_own_tokens_sizes(ops, m):
         assert torch.equal(y, wants[i])
     for p, y in zip(sizes, wants):
         assert torch.equal((y.double() / p).bfloat16(), wants[0])
+
+
+# ----------------------------------------------------------------------------------------------------------
+# infinities
+# ----------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("m", [3, 8, 9, 32, 33, 70])
+def test_linear_infinite_tokens_are_not_finite_and_stay_in_their_rows(ops, m, group, dtype):
+    """In each of the three kernels: rows with an infinity or a NaN have no finite output, the others do not change."""
+    x, q, s, z, b = _linear_problem(m, 384, 140, group, dtype)
+    clean = ops.w4a16_linear(x, q, s, z, b, group_size=group)
+    hit = torch.zeros(m, dtype=torch.bool, device="cuda")
+    hit[[0, m - 1]] = True
+    for one, two in ((float("inf"), -float("inf")), (float("nan"), float("inf"))):
+        x[0, 383], x[m - 1, 7] = one, two
+        y = ops.w4a16_linear(x, q, s, z, b, group_size=group)
+        assert not bool(torch.isfinite(y[hit]).any()) and torch.equal(y[~hit], clean[~hit])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [40, 700, 20000])
+def test_attention_infinite_keys_and_values_in_sight(kv, dtype, n):
+    """An infinite value leaves its element of the output not finite and the others as they were; a key whose score is
+    -infinity weighs nothing."""
+    k, v, table, lens = _cache([n, n], 1, 16, 64, dtype, seed=8)
+    q = _query(2, 2, 64, dtype, 1)
+    clean = kv.paged_attention(q, k, v, table, lens)
+    held = v.clone()
+    at = int(table[0, 1]), 0, 3
+    for value in (float("inf"), -float("inf")):
+        v[at + (9,)] = value
+        out = kv.paged_attention(q, k, v, table, lens)
+        bad = ~torch.isfinite(out)
+        assert bool(bad[0, :, 9].all()) and int(bad.sum()) == 2 and torch.equal(out[~bad], clean[~bad])
+    v.copy_(held)
+    q[..., 5] = q[..., 5].abs() + 0.5
+    k[at + (5,)] = -float("inf")
+    got = _attention_holds(kv, q, k, v, table, lens)
+    assert bool(torch.isfinite(got).all())
