@@ -197,6 +197,7 @@ __global__ void __launch_bounds__(w4mid::kThreads, 2) w4a16_mid_kernel(const w4m
     __syncthreads();
   if (tid < rows) {
     for (int m = rank; m < mt; m += a.ksplit) {
+      const float factor = F16 ? 1.0f : a.factor[m0 + m];     // written while this grid may be there already: a plain load
       float y = part[m * P::kPartStride + tid];
       if (a.ksplit > 1) {
         y = 0.0f;
@@ -212,7 +213,7 @@ __global__ void __launch_bounds__(w4mid::kThreads, 2) w4a16_mid_kernel(const w4m
         if (a.bias != nullptr) y += __half2float(static_cast<const __half*>(a.bias)[n0 + tid]);
         static_cast<__half*>(a.out)[at] = __float2half_rn(y);
       } else {
-        y *= __ldcg(a.factor + m0 + m);                       // written while this grid was already there: no read-only load
+        y *= factor;
         if (a.bias != nullptr) y += __bfloat162float(static_cast<const __nv_bfloat16*>(a.bias)[n0 + tid]);
         static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(y);
       }
