@@ -9,7 +9,6 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool o
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
@@ -76,8 +75,9 @@ __device__ __forceinline__ uint32_t and_or(uint32_t v, uint32_t mask, uint32_t b
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(v), "r"(mask), "r"(bits));
   return d;
 }
-// The eight 4-bit codes of a word as 16-bit floats; pair j holds nibbles j and j + 4.  Logic operations run at half the
-// rate of the floating-point pipe, so f16 takes five of them and four fused multiply-adds:
+// The eight 4-bit codes of a word as 16-bit floats; pair j holds nibbles j and j + 4.  The published way to widen integer
+// codes: masked into the mantissa of a power of two, whose value is then taken off.  Logic operations run at half the
+// rate of the floating-point pipe, so f16 takes five of them and four additions or fused multiply-adds:
 //   f16:  q - 8, exact, from 1024 + q (the code in mantissa bits 0..3) and 1024 + 16 q (bits 4..7)
 //   bf16: 16 + q, exact, the code in mantissa bits 3..6 of 2^4; its seven bits have no room for the other form
 template <bool F16>

@@ -740,9 +740,6 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(const PagedAt
 }
 
 namespace {
-}  // namespace
-
-namespace {
 struct Deal {
   pattn::Mode mode;
   int64_t units, segs;         // of the row with the most visible keys; segments

@@ -23,30 +23,30 @@ namespace cq {
 namespace w4a16 {
 constexpr int kWarps = 8;
 constexpr int kChunk = 128;                // columns of a ring stage
+constexpr int kStages = 3;                 // of a warp's ring
+constexpr int kRt = 2;                     // tiles of 16 weight rows of a CTA
+constexpr int kRows = 16 * kRt;
+constexpr int kWBytes = kRows * kChunk / 2;
+constexpr int kSBytes = 128;               // scales (or zeros) of a group's rows, and room for a shift
+constexpr int kRedStride = kRows + 4;      // floats between tokens of a partial tile: no bank conflicts
 
-// a CTA of RT tiles of 16 weight rows, eight tokens and a ring of S chunks per warp
-template <int G, int RT, int S>
+template <int G>
 struct Plan {
-  static constexpr int kRows = 16 * RT;
-  static constexpr int kWBytes = kRows * kChunk / 2;
   static constexpr int kGroups = kChunk / G;             // scale groups of a chunk
-  static constexpr int kSBytes = RT <= 2 ? 128 : 256;    // scales (or zeros) of a group's rows, and room for a shift
   static constexpr int kXAt = kWBytes + 2 * kGroups * kSBytes;
-  static constexpr int kRedStride = kRows + 4;           // floats between tokens of a partial tile: no bank conflicts
   static constexpr int stage(int tokens) { return kXAt + tokens * 2 * kChunk; }
   static constexpr int shared(int tokens) {
-    const int ring = kWarps * S * stage(tokens), red = kWarps * 8 * kRedStride * 4;
+    const int ring = kWarps * kStages * stage(tokens), red = kWarps * 8 * kRedStride * 4;
     return ring > red ? ring : red;
   }
 };
 }  // namespace w4a16
 
-template <bool F16, int G, int RT, int S>
+template <bool F16, int G>
 __global__ void __launch_bounds__(w4a16::kWarps * 32, 1) w4a16_kernel(const W4A16Args a, const int tokens) {
   using namespace w4a16;
-  using P = Plan<G, RT, S>;
-  constexpr int kRt = RT, kRows = P::kRows, kStages = S, kWBytes = P::kWBytes, kGroups = P::kGroups, kSBytes = P::kSBytes;
-  constexpr int kXAt = P::kXAt, kRedStride = P::kRedStride;
+  using P = Plan<G>;
+  constexpr int kGroups = P::kGroups, kXAt = P::kXAt;
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int n0 = blockIdx.x * kRows, m0 = blockIdx.y * tokens;
@@ -154,20 +154,18 @@ __global__ void __launch_bounds__(w4a16::kWarps * 32, 1) w4a16_kernel(const W4A1
         }
       }
       if ((b + 1) % (G / 32) == 0) {                          // the group's end
-        // scales and zeros of rows lane, lane + 32, ...; past the last group there are none, and the tokens are zeros
+        // the scale and zero of row `lane`; past the last group there are none, and the tokens are zeros
         const int i = b / (G / 32), odd = (ch * kGroups + i) & a.N & 1;
-        uint32_t mine[(kRows + 31) / 32] = {};
+        uint32_t mine = 0;
         if (i == 0 || (ch * kGroups + i) * G < a.K) {
           const unsigned short* sz = reinterpret_cast<const unsigned short*>(st + kWBytes + 2 * i * kSBytes) + lane;
-#pragma unroll
-          for (int q = 0; q < (kRows + 31) / 32; ++q)
-            mine[q] = sz[(s_odd ^ odd) + 32 * q] | static_cast<uint32_t>(sz[kSBytes / 2 + (z_odd ^ odd) + 32 * q]) << 16;
+          mine = sz[s_odd ^ odd] | static_cast<uint32_t>(sz[kSBytes / 2 + (z_odd ^ odd)]) << 16;
         }
 #pragma unroll
         for (int t = 0; t < kRt; ++t)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint32_t u = __shfl_sync(0xffffffffu, mine[t / 2], 16 * (t & 1) + 8 * h + g);
+            const uint32_t u = __shfl_sync(0xffffffffu, mine, 16 * t + 8 * h + g);
             const float s = __uint_as_float(u << 16), z = fmaf(-widen_offset<F16>(), s, __uint_as_float(u & 0xffff0000u));
 #pragma unroll
             for (int j = 0; j < 2; ++j) acc[t][2 * h + j] = fmaf(s, p[t][2 * h + j], fmaf(z, r[j], acc[t][2 * h + j]));
@@ -204,26 +202,21 @@ __global__ void __launch_bounds__(w4a16::kWarps * 32, 1) w4a16_kernel(const W4A1
   }
 }
 
-template <bool F16, int G, int RT, int S>
+template <bool F16, int G>
 cudaError_t run_w4a16(const W4A16Args& a, cudaStream_t st) {
-  using P = w4a16::Plan<G, RT, S>;
+  using P = w4a16::Plan<G>;
   static unsigned long long devices = 0;
-  const cudaError_t e = allow_shared(w4a16_kernel<F16, G, RT, S>, P::shared(8), devices);
+  const cudaError_t e = allow_shared(w4a16_kernel<F16, G>, P::shared(8), devices);
   if (e != cudaSuccess) return e;
   const int tokens = a.M < 8 ? a.M : 8;
-  w4a16_kernel<F16, G, RT, S><<<dim3((a.N + P::kRows - 1) / P::kRows, (a.M + tokens - 1) / tokens), w4a16::kWarps * 32,
-                                P::shared(tokens), st>>>(a, tokens);
+  w4a16_kernel<F16, G><<<dim3((a.N + w4a16::kRows - 1) / w4a16::kRows, (a.M + tokens - 1) / tokens), w4a16::kWarps * 32,
+                         P::shared(tokens), st>>>(a, tokens);
   return cudaGetLastError();
 }
 
 template <bool F16, int G>
-cudaError_t pick_w4a16(const W4A16Args& a, cudaStream_t st) {
-  return run_w4a16<F16, G, 2, 3>(a, st);
-}
-
-template <bool F16, int G>
 cudaError_t pick_w4a16_shared(const W4A16Args& a, const W4Tokens& t, cudaStream_t st) {
-  if (w4a16_tensor_memory(a.M)) return run_w4a16_tc<F16, G, 64>(a, t, st);
+  if (w4a16_tensor_memory(a.M)) return run_w4a16_tc<F16, G>(a, t, st);
   switch (w4a16_tile(a.M)) {
     case 16: return run_w4a16_mid<F16, G, 2>(a, t, st);
     case 24: return run_w4a16_mid<F16, G, 3>(a, t, st);
@@ -248,9 +241,9 @@ cudaError_t launch_w4a16(const W4A16Args& a, void* ws, cudaStream_t st) {
     }
   }
   switch (a.group) {
-    case 32: return a.f16 ? pick_w4a16<true, 32>(a, st) : pick_w4a16<false, 32>(a, st);
-    case 64: return a.f16 ? pick_w4a16<true, 64>(a, st) : pick_w4a16<false, 64>(a, st);
-    default: return a.f16 ? pick_w4a16<true, 128>(a, st) : pick_w4a16<false, 128>(a, st);
+    case 32: return a.f16 ? run_w4a16<true, 32>(a, st) : run_w4a16<false, 32>(a, st);
+    case 64: return a.f16 ? run_w4a16<true, 64>(a, st) : run_w4a16<false, 64>(a, st);
+    default: return a.f16 ? run_w4a16<true, 128>(a, st) : run_w4a16<false, 128>(a, st);
   }
 }
 

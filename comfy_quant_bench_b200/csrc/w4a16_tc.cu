@@ -26,23 +26,20 @@ namespace cq {
 namespace w4tc {
 constexpr int kRows = 128;
 constexpr int kChunk = 128;                    // columns of a ring stage
+constexpr int kTokens = 64;                    // of a CTA
 constexpr int kAheadWarps = 4;                 // widening warps, one per TMEM lane quadrant
 constexpr int kWBytes = kRows * kChunk / 2;
 constexpr int kAheadScales = 4;
 constexpr int kSite = 120;                     // device status sites of the waits
-
-template <int G, int NTOK>
-struct Plan {
-  static constexpr int kXBytes = NTOK * kChunk * 2;
-  static constexpr int kXStages = 3, kWStages = 7;
-  static constexpr int kRing = kXStages * kXBytes + kWStages * kWBytes;
-  static constexpr int kSmem = kRing + 1024 + 256;             // alignment, barriers
-  static constexpr int kSums = NTOK < 32 ? NTOK : 32;          // tokens of an adding warp
-  static constexpr int kAddWarps = 4 * (NTOK / kSums);
-  static constexpr int kThreads = 32 * (kAheadWarps + kAddWarps + 2);   // and the copying and the multiplying warp
-  static_assert(kRows * NTOK * 4 <= kRing, "partial sums fit the rings");
-  static_assert(kWStages >= kXStages, "the copying warp's order");
-};
+constexpr int kTokenBytes = kTokens * kChunk * 2;
+constexpr int kXStages = 3, kWStages = 7;
+constexpr int kRing = kXStages * kTokenBytes + kWStages * kWBytes;
+constexpr int kSmem = kRing + 1024 + 256;      // alignment, barriers
+constexpr int kSums = 32;                      // tokens of an adding warp
+constexpr int kAddWarps = 4 * (kTokens / kSums);
+constexpr int kThreads = 32 * (kAheadWarps + kAddWarps + 2);   // and the copying and the multiplying warp
+static_assert(kRows * kTokens * 4 <= kRing, "partial sums fit the rings");
+static_assert(kWStages >= kXStages, "the copying warp's order");
 
 struct Args {
   const __nv_bfloat16* s;
@@ -110,20 +107,19 @@ __device__ __forceinline__ bool mbar_wait_short(uint64_t* bar, uint32_t parity, 
   return mbar_wait_long(bar, parity, abort_flag, where);
 }
 
-template <bool F16, int G, int NTOK>
-__global__ void __launch_bounds__(w4tc::Plan<G, NTOK>::kThreads, 2)
+template <bool F16, int G>
+__global__ void __launch_bounds__(w4tc::kThreads, 2)
     w4a16_tc_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
                     const __grid_constant__ CUtensorMap tm_r, const w4tc::Args a) {
   using namespace w4tc;
-  using P = Plan<G, NTOK>;
-  constexpr int kXStages = P::kXStages, kWStages = P::kWStages, kSteps = kChunk / G, kSums = P::kSums;
-  constexpr int kCopyWarp = kAheadWarps + P::kAddWarps, kMmaWarp = kCopyWarp + 1;
-  constexpr uint32_t kCols = 256;                             // TMEM: two P of NTOK columns, A's buffers in the rest
-  static_assert(2 * NTOK + 128 <= kCols, "two 128-column A operands");
+  constexpr int kSteps = kChunk / G;                          // scale groups of a chunk
+  constexpr int kCopyWarp = kAheadWarps + kAddWarps, kMmaWarp = kCopyWarp + 1;
+  constexpr uint32_t kCols = 256;                             // TMEM: two P of kTokens columns, A's buffers in the rest
+  static_assert(2 * kTokens + 128 <= kCols, "two 128-column A operands");
   extern __shared__ __align__(128) uint8_t smem_any[];
   uint8_t* smem = smem_any + ((1024 - (smem_u32(smem_any) & 1023)) & 1023);
-  uint8_t* codes_at = smem + kXStages * P::kXBytes;           // the ring of codes comes after the tokens'
-  uint64_t* x_full = reinterpret_cast<uint64_t*>(smem + P::kRing);
+  uint8_t* codes_at = smem + kXStages * kTokenBytes;              // the ring of codes comes after the tokens'
+  uint64_t* x_full = reinterpret_cast<uint64_t*>(smem + kRing);
   uint64_t* x_empty = x_full + kXStages;
   uint64_t* w_full = x_empty + kXStages;
   uint64_t* w_empty = w_full + kWStages;
@@ -135,7 +131,7 @@ __global__ void __launch_bounds__(w4tc::Plan<G, NTOK>::kThreads, 2)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(holder + 1);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = a.ksplit > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-  const int n0 = blockIdx.x * kRows, m0 = blockIdx.y * NTOK;
+  const int n0 = blockIdx.x * kRows, m0 = blockIdx.y * kTokens;
   const int chunks = (a.K + kChunk - 1) / kChunk;
   const int c0 = rank * chunks / a.ksplit, c1 = (rank + 1) * chunks / a.ksplit;
   const int steps = min(c1 * kSteps, a.K / G) - c0 * kSteps;  // groups of this CTA
@@ -155,7 +151,7 @@ __global__ void __launch_bounds__(w4tc::Plan<G, NTOK>::kThreads, 2)
     for (int b = 0; b < 2; ++b) {
       mbar_init(&a_full[b], kAheadWarps);
       mbar_init(&p_full[b], 1);
-      mbar_init(&p_empty[b], P::kAddWarps);
+      mbar_init(&p_empty[b], kAddWarps);
       mbar_init(&z_done[b], 1);
     }
     *abort_flag = 0;
@@ -168,7 +164,7 @@ __global__ void __launch_bounds__(w4tc::Plan<G, NTOK>::kThreads, 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t d_col = *holder, a_col = d_col + 2 * NTOK;
+  const uint32_t d_col = *holder, a_col = d_col + 2 * kTokens;
   const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;    // the warp's quadrant of TMEM lanes
   const int row = (warp & 3) * 32 + lane, n = n0 + row;       // this thread's weight row (widening and adding warps)
   float2 acc[kSums / 2];
@@ -188,12 +184,12 @@ __global__ void __launch_bounds__(w4tc::Plan<G, NTOK>::kThreads, 2)
       if (++ws == kWStages) ws = 0;
     };
     auto tokens = [&]() {
-      uint8_t* st = smem + xs * P::kXBytes;
+      uint8_t* st = smem + xs * kTokenBytes;
       const CUtensorMap* map = xi < nz ? &tm_r : &tm_x;
       const int at = (xi < nz ? z0 + xi : c0 + xi - nz) * kChunk * 2;
-      mbar_arrive_expect_tx(&x_full[xs], P::kXBytes);
+      mbar_arrive_expect_tx(&x_full[xs], kTokenBytes);
       tma_load_2d(st, map, &x_full[xs], at, m0);
-      tma_load_2d(st + P::kXBytes / 2, map, &x_full[xs], at + 128, m0);
+      tma_load_2d(st + kTokenBytes / 2, map, &x_full[xs], at + 128, m0);
       ++xi;
       if (++xs == kXStages) xs = 0;
     };
@@ -220,7 +216,7 @@ __global__ void __launch_bounds__(w4tc::Plan<G, NTOK>::kThreads, 2)
     // ---- products: the zeros' first, then each group's P = codes x tokens.  One thread, which neither waits for the
     // warp's other lanes nor makes them poll: it paces the CTA ----
     if (elect_one()) {
-      constexpr uint32_t shape = (1u << 4) | (static_cast<uint32_t>(NTOK >> 3) << 17) | (8u << 24);   // f32, M = 128
+      constexpr uint32_t shape = (1u << 4) | (static_cast<uint32_t>(kTokens >> 3) << 17) | (8u << 24);   // f32, M = 128
       constexpr uint32_t idesc_z = shape | (1u << 7) | (1u << 10);                                    // bf16 x bf16
       int stage = 0, issued = 0;
       uint32_t phase = 0;
@@ -234,11 +230,11 @@ __global__ void __launch_bounds__(w4tc::Plan<G, NTOK>::kThreads, 2)
              mbar_wait_short(&a_full[buf], (j >> 1) & 1, abort_flag, kSite + 3);
         if (!ok) break;
         tc_fence_after();
-        const uint64_t x = smem_desc_k_sw128(smem_u32(smem + stage * P::kXBytes));
+        const uint64_t x = smem_desc_k_sw128(smem_u32(smem + stage * kTokenBytes));
 #pragma unroll
         for (int k = 0; k < 6; ++k) {                         // three parts of 32 sums; the last 32 columns are empty
           const int col = 16 * k;
-          mma_f16_ts(d_col, a_col + buf * 64 + 8 * k, x + ((col >> 6) * (P::kXBytes / 2) + (col & 63) * 2) / 16, idesc_z,
+          mma_f16_ts(d_col, a_col + buf * 64 + 8 * k, x + ((col >> 6) * (kTokenBytes / 2) + (col & 63) * 2) / 16, idesc_z,
                      j + k != 0);
         }
         tc_commit(&z_done[buf]);
@@ -251,7 +247,7 @@ __global__ void __launch_bounds__(w4tc::Plan<G, NTOK>::kThreads, 2)
       // product i (0: the zeros', 1 ..: the groups') takes P buffer i & 1; a_full goes on counting from the zeros' blocks
       for (int i = 1; i <= steps && ok; next_stage()) {
         if (!(ok = mbar_wait_short(&x_full[stage], phase, abort_flag, kSite + 4))) break;
-        const uint64_t x = smem_desc_k_sw128(smem_u32(smem + stage * P::kXBytes));
+        const uint64_t x = smem_desc_k_sw128(smem_u32(smem + stage * kTokenBytes));
 #pragma unroll
         for (int sub = 0; sub < kSteps; ++sub) {
           if (i > steps) break;
@@ -263,8 +259,8 @@ __global__ void __launch_bounds__(w4tc::Plan<G, NTOK>::kThreads, 2)
 #pragma unroll
           for (int k = 0; k < G / 16; ++k) {
             const int col = sub * G + 16 * k;                 // 64 columns per 128-byte-wide half
-            mma_f16_ts(d_col + buf * NTOK, a_col + (use & 1) * 64 + 8 * k,
-                       x + ((col >> 6) * (P::kXBytes / 2) + (col & 63) * 2) / 16, shape, k != 0);
+            mma_f16_ts(d_col + buf * kTokens, a_col + (use & 1) * 64 + 8 * k,
+                       x + ((col >> 6) * (kTokenBytes / 2) + (col & 63) * 2) / 16, shape, k != 0);
           }
           tc_commit(&p_full[buf]);
           if (sub == kSteps - 1) tc_commit(&x_empty[stage]);
@@ -363,7 +359,7 @@ __global__ void __launch_bounds__(w4tc::Plan<G, NTOK>::kThreads, 2)
 #pragma unroll
       for (int q = 0; q < kSums / 16; ++q) {
         uint32_t v[16];
-        tmem_ld_x16(d_col + buf * NTOK + first_sum + 16 * q + lane_base, v);
+        tmem_ld_x16(d_col + buf * kTokens + first_sum + 16 * q + lane_base, v);
         tmem_wait_ld_x16(v);
         if (q == kSums / 16 - 1) {
           tc_fence_before();
@@ -409,7 +405,7 @@ __global__ void __launch_bounds__(w4tc::Plan<G, NTOK>::kThreads, 2)
     }
   };
   const bool adds = warp >= kAheadWarps && warp < kCopyWarp;
-  const int mt = min(NTOK, a.M - m0);
+  const int mt = min(kTokens, a.M - m0);
   if (a.ksplit == 1) {
     if (adds && n < a.N) {
 #pragma unroll
@@ -426,7 +422,7 @@ __global__ void __launch_bounds__(w4tc::Plan<G, NTOK>::kThreads, 2)
   }
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (adds && n < a.N) {
-    for (int m = rank + first_sum / kSums * a.ksplit; m < mt; m += a.ksplit * (P::kAddWarps / 4)) {
+    for (int m = rank + first_sum / kSums * a.ksplit; m < mt; m += a.ksplit * (kAddWarps / 4)) {
       const float factor = factor_of(m0 + m);
       float y = 0.0f;
       for (int q = 0; q < a.ksplit; ++q) {
@@ -453,18 +449,17 @@ bool w4a16_map(CUtensorMap* map, const void* base, int64_t rows, int64_t bytes, 
 }
 }  // namespace
 
-template <bool F16, int G, int NTOK>
+template <bool F16, int G>
 cudaError_t run_w4a16_tc(const W4A16Args& a, const W4Tokens& t, cudaStream_t st) {
-  using P = w4tc::Plan<G, NTOK>;
-  auto kern = w4a16_tc_kernel<F16, G, NTOK>;
+  auto kern = w4a16_tc_kernel<F16, G>;
   static unsigned long long devices = 0;
-  const cudaError_t e = allow_shared(kern, P::kSmem, devices);
+  const cudaError_t e = allow_shared(kern, w4tc::kSmem, devices);
   if (e != cudaSuccess) return e;
-  const int tiles = (a.M + NTOK - 1) / NTOK, chunks = (a.K + w4tc::kChunk - 1) / w4tc::kChunk;
+  const int tiles = (a.M + w4tc::kTokens - 1) / w4tc::kTokens, chunks = (a.K + w4tc::kChunk - 1) / w4tc::kChunk;
   CUtensorMap tm_w, tm_x, tm_r;
   if (!w4a16_map(&tm_w, a.b, a.N, a.K / 2, 64, w4tc::kRows, CU_TENSOR_MAP_SWIZZLE_64B) ||
-      !w4a16_map(&tm_x, t.x, a.M, static_cast<int64_t>(a.K) * 2, 128, NTOK, CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !w4a16_map(&tm_r, t.parts, a.M, t.blocks * 256, 128, NTOK, CU_TENSOR_MAP_SWIZZLE_128B))
+      !w4a16_map(&tm_x, t.x, a.M, static_cast<int64_t>(a.K) * 2, 128, w4tc::kTokens, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !w4a16_map(&tm_r, t.parts, a.M, t.blocks * 256, 128, w4tc::kTokens, CU_TENSOR_MAP_SWIZZLE_128B))
     return cudaErrorInvalidValue;
   const int row_tiles = (a.N + w4tc::kRows - 1) / w4tc::kRows;
   // K split over a cluster while that leaves no resident CTA (two per SM) without work and each has four chunks
@@ -480,8 +475,8 @@ cudaError_t run_w4a16_tc(const W4A16Args& a, const W4Tokens& t, cudaStream_t st)
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = static_cast<unsigned>(ksplit);
   cfg.gridDim = dim3(row_tiles, tiles, ksplit);
-  cfg.blockDim = dim3(P::kThreads);
-  cfg.dynamicSmemBytes = P::kSmem;
+  cfg.blockDim = dim3(w4tc::kThreads);
+  cfg.dynamicSmemBytes = w4tc::kSmem;
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
