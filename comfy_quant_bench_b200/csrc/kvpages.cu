@@ -95,18 +95,17 @@ __global__ void __launch_bounds__(pages::kThreads) pages_branch_kernel(const Pag
   int site = 0;
   if (a.n_free > 0 && !mark_rows(a.free_rows, a.n_free, a.table_rows, seen)) site = pages::kSiteFree;
   if (site == 0 && a.n_fork > 0) {
+    const bool same = a.dst == a.free_rows && a.n_fork == a.n_free;      // `seen` has the destinations already
     int bad = 0;
     for (int i = tid; i < a.n_fork; i += blockDim.x) {
-      const int d = a.dst[i];
+      const int s = a.src[i], d = a.dst[i];
       if (d < 0 || d >= a.table_rows || !((a.n_free > 0 && marked(seen, d)) || a.lens[d] == 0)) bad = 1;
+      if (s < 0 || s >= a.table_rows || (same && marked(seen, s))) bad = 1;
     }
-    if (__syncthreads_or(bad) || ((a.dst != a.free_rows || a.n_fork != a.n_free) && !mark_rows(a.dst, a.n_fork, a.table_rows, seen)))
-      site = pages::kSiteFork;
-    else {
-      for (int i = tid; i < a.n_fork; i += blockDim.x) {
-        const int s = a.src[i];
-        if (s < 0 || s >= a.table_rows || marked(seen, s)) bad = 1;
-      }
+    if (__syncthreads_or(bad) || (!same && !mark_rows(a.dst, a.n_fork, a.table_rows, seen))) site = pages::kSiteFork;
+    else if (!same) {
+      for (int i = tid; i < a.n_fork; i += blockDim.x)
+        if (marked(seen, a.src[i])) bad = 1;
       if (__syncthreads_or(bad)) site = pages::kSiteFork;
     }
   }

@@ -478,8 +478,9 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
           f[n][j] = exp2_fast(m[n][j] - base);
           grew |= mn != m[n][j];
           m[n][j] = mn;
-          s[n][j] = exp2_fast((x0 - base) + kLift);        // two steps: the first one is never above 0
-          s[n][2 + j] = exp2_fast((x1 - base) + kLift);
+          const float y0 = x0 - base, y1 = x1 - base;      // never above 0: a lift of the base could round past it
+          s[n][j] = exp2_fast(kF16Math ? y0 + kLift : y0);
+          s[n][2 + j] = exp2_fast(kF16Math ? y1 + kLift : y1);
           l[n][j] = l[n][j] * f[n][j] + (s[n][j] + s[n][2 + j]);
         }
         split16<kF16Math>(s[n][0], s[n][1], ph[n][0], pl[n][0]);
