@@ -1029,3 +1029,42 @@ def test_attention_infinite_keys_and_values_in_sight(kv, dtype, n):
     k[at + (5,)] = -float("inf")
     got = _attention_holds(kv, q, k, v, table, lens)
     assert bool(torch.isfinite(got).all())
+
+
+# ----------------------------------------------------------------------------------------------------------
+# calls that overlap
+# ----------------------------------------------------------------------------------------------------------
+
+def test_calls_on_two_streams_do_not_share_anything(ops, kv):
+    """The three linears (workspaces for two of them), split and short attention and a cache's bookkeeping, on two streams at
+    a time, against the same calls one after the other."""
+    linears = [_linear_problem(m, 2048, 640, 64, dt, seed=i) for i, (m, dt) in
+               enumerate([(4, torch.bfloat16), (20, torch.bfloat16), (64, torch.float16), (40, torch.bfloat16)])]
+    k, v, table, n = _cache([5000, 300, 0, 9000], 2, 16, 128, torch.bfloat16, seed=1)
+    short = _cache([40, 9], 2, 16, 128, torch.bfloat16, seed=2)
+    q = _query(4, 8, 128, torch.bfloat16, 1)
+
+    def work(c):
+        out = [ops.w4a16_linear(*p, group_size=64) for p in linears]
+        out.append(kv.paged_attention(q, k, v, table, n))
+        out.append(kv.paged_attention(q[:2], *short))
+        out.append(c.reserve(_rows(0, 1), _rows(20, 33)))
+        out.append(c.branch(_rows(0, 1), _rows(2, 3), 1))
+        c.free(_rows(0))
+        c.compact()
+        return out + [c.block_table.clone(), c.seq_lens.clone(), c.ref_counts.clone()]
+
+    def cache():
+        return kv.PagedKVCache(2, 30, 1, 64, 5, 64, page_size=16, dtype=torch.bfloat16)
+    want = work(cache())
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    caches = [cache() for _ in range(40)]
+    torch.cuda.synchronize()
+    got = []
+    for i, c in enumerate(caches):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(work(c))
+    torch.cuda.synchronize()
+    for each in got:
+        assert all(torch.equal(a, b) for a, b in zip(each, want))
+    assert _status() == (0, 0)
