@@ -46,9 +46,9 @@ constexpr int kMinUnits = 4;
 // rows (320 segments) of 500 26 and 24, of 1000 47 and 37.
 constexpr int kWholeUnits = 24;
 constexpr int kJoinUnits = 5;
-// CTAs of a resident grid (two per SM), and the most units of a cluster's CTA: with few segments of up to so many units
-// a cluster each is quicker than runs over all SMs and their join (8 segments of 4000 keys: 12 and
-// 14 us).
+// CTAs of a resident grid (two per SM; at D 256 with 16-bit caches one fits, and the rules above and below, measured at D
+// 64 and 128, count two all the same), and the most units of a cluster's CTA: with few segments of up to so many units a
+// cluster each is quicker than runs over all SMs and their join (8 segments of 4000 keys: 12 and 14 us).
 constexpr int kMaxRuns = 2 * 148;
 constexpr int kClusterUnits = 16;
 
@@ -741,6 +741,8 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(const PagedAt
 }
 
 namespace {
+// By what the table's width allows, not by the lengths on the device, so that a captured launch stays right as rows grow: a
+// short row in a wide table is dealt out as runs (333 keys: 8.8 us, and 6.1 as a cluster).
 struct Deal {
   pattn::Mode mode;
   int64_t units, segs;         // of the row with the most visible keys; segments

@@ -7,15 +7,19 @@
 // widen a weight to fp32 and multiply it for even one token.  So the products run as mma.sync tiles of 16 weight rows
 // x 16 columns x 8 tokens whose weight operand is formed in registers, about two instructions per pair of weights, as
 // q - 8 (f16) or 16 + q (bf16), both exact.  With P the group's sum of x times those and R = sum x (from the same tile
-// shape against ones), the group adds s P + z R (f16) or s P + (z - 24 s) R (bf16) in fp32.
+// shape against ones), the group adds s P + z R (f16) or s P + (z - 24 s) R (bf16) in fp32; for bf16 the rounding is thus that
+// of sum |x| (16 + q), some five times that of sum |x| |q - 8|.
 //
 // A CTA owns 32 weight rows and its eight warps split K in chunks of 128 columns; each warp keeps a ring of
 // asynchronous copies of its weights and tokens in flight and nothing is exchanged before the end, when the partial
 // sums are added in the order of the warps (equal calls give equal bits).
 //
-// Measured on a B200 (device time): one token at 4096 x 16384, groups of 128: 13.1 us, 2.7 TB/s; one and eight tokens at
-// 8192 x 28672: 38 and 44 us, 3.2 and 2.8 TB/s, bound by forming the operands (instruction issue), not by HBM; one token at
-// 1024 x 1001: 2.5 us, launch and latency.
+// Measured on a B200 (device time): one token at 4096 x 16384, groups of 128: 13.0 us, 2.7 TB/s; one and eight tokens at
+// 8192 x 28672: 38 and 44 us, 3.2 and 2.8 TB/s; one token at 1024 x 1001: 2.5 us, launch and latency.  No unit is full: at
+// the first size an SM with work issues in 54 % of its cycles, its integer pipe (forming the operands) is at 40 % and HBM at
+// 42 %.  What is lost is rounds of CTAs - 512 for 296 places are two rounds for 1.73, 896 at the second size four for 3.03 -
+// and a CTA's start and end, with four chunks a warp at K = 4096 through a ring of three.  At eight tokens and the second
+// size 65 % and 54 %.
 #include "decode_common.cuh"
 
 namespace cq {
