@@ -15,9 +15,9 @@
 // launched as its programmatic dependent: its weights are on their way while the tokens are written.
 //
 // Measured on a B200 (device time, the tokens' kernel included): 64 tokens at 8192 x 28672, groups of 128: 66 us, 450
-// TFLOP/s; at 5120 x 13824, groups of 64: 41 us (f16) and 42 us (bf16).  Bound by the hand-overs from one role to the next at each group: an SM
-// with two CTAs issues in two thirds of its slots, the polling of waiting warps among them, has its integer pipe half and
-// its tensor pipe a third full, and its warps stall at the mbarriers more than anywhere else.
+// TFLOP/s; at 5120 x 13824, groups of 64: 41 us (f16) and 42 us (bf16).  Bound by the hand-overs from one role to the next
+// at each group: an SM with two CTAs issues in two thirds of its slots, the polling of waiting warps among them, has its
+// integer pipe half and its tensor pipe a third full, and its warps stall at the mbarriers more than anywhere else.
 //
 // With few row tiles a cluster of CTAs splits K and adds its partial sums over distributed shared memory in rank order.
 #include "decode_common.cuh"
