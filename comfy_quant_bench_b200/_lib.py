@@ -44,6 +44,10 @@ CQ_DT_BF16 = 0
 CQ_DT_F16 = 1
 CQ_DT_FP8_E4M3 = 2
 
+CQ_NORM_SAME = 0
+CQ_NORM_INT8 = 1
+CQ_NORM_FP8 = 2
+
 CQ_OUT_PLAIN = 0
 CQ_OUT_GELU_TANH = 1
 CQ_OUT_GATED_RESIDUAL = 2
@@ -120,6 +124,7 @@ SIGNATURES = {
                                _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp]),
     "cq_pages_compact": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _vp,
                                 _i64, _vp]),
+    "cq_add_rmsnorm": (_int, [_vp, _i64, _vp, _i64, _vp, _int, _i64, _i64, _f32, _int, _i64, _vp, _i64, _vp, _vp, _vp]),
     "cq_linear_convrot_w4a4_swiglu": (_int, [_vp, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
 }
 

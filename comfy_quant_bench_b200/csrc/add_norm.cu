@@ -1,0 +1,269 @@
+// Root-mean-square norm with the residual's addition, and an output in 8 bits with scales.
+//
+//   h = x + r, rounded to the 16-bit type (the residual stream, written back);  y = h w / sqrt(mean(h^2) + eps)
+//
+// and y rounded once to the type, or in 8 bits: with p = h w and P the largest |p| of the row (or of a group of 32, 64 or
+// 128 columns), code = round(top p / P), scale = P / (top sqrt(mean(h^2) + eps)), top = 127 (int8) or 448 (e4m3).  The
+// root cancels in the code, and p is exact in fp32 (16-bit factors), so an int8 code is a function of exact values: next
+// to a border between two codes it is decided in 64 bits.
+//
+// Bound by reading x, r and writing h, y once: a row stays in registers between its sums and its outputs.  One reduction
+// serves both the sum of squares and the maximum.
+#include "decode_common.cuh"
+
+namespace cq {
+
+template <bool F16>
+__device__ __forceinline__ float2 widen16(uint32_t w) {
+  if constexpr (F16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t narrow16(float a, float b) {
+  if constexpr (F16) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    return bf16x2_bits(a, b);
+  }
+}
+
+// Codes of p against the largest P: `by` is top / P, or 0 where P is 0.
+struct Coder {
+  float most, by;
+  bool tiny;                                   // top / P would overflow: the quotient first
+};
+template <int OUT>
+__device__ __forceinline__ Coder coder(float most) {
+  constexpr float top = OUT == kNormInt8 ? 127.0f : 448.0f;
+  Coder c{most, 0.0f, most < 1e-30f};
+  if (most > 0.0f) c.by = c.tiny ? top : __fdiv_rn(top, most);
+  return c;
+}
+template <int OUT>
+__device__ __forceinline__ float scaled(float p, const Coder& c) {
+  return c.tiny ? (c.most > 0.0f ? __fdiv_rn(p, c.most) * c.by : 0.0f) : p * c.by;
+}
+__device__ __forceinline__ uint32_t int8_code(float p, const Coder& c) {
+  const float t = scaled<kNormInt8>(p, c), k = rintf(t);
+  int code = static_cast<int>(k);
+  // t is off by 2^-22 of at most 127: only within 2^-14 of a border can the nearest code be another one
+  if (fabsf(fabsf(t - k) - 0.5f) < 6.2e-5f) code = static_cast<int>(rint(static_cast<double>(p) * 127.0 / static_cast<double>(c.most)));
+  return static_cast<uint32_t>(code) & 0xffu;
+}
+__device__ __forceinline__ uint32_t e4m3_pair(float a, float b) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+
+// The sum and the maximum over a row's threads: a warp, or a block of whole warps.
+template <bool WARP>
+__device__ __forceinline__ void row_reduce(float& sum, float& most, float* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  }
+  if constexpr (!WARP) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    if (lane == 0) {
+      red[warp] = sum;
+      red[32 + warp] = most;
+    }
+    __syncthreads();
+    sum = lane < warps ? red[lane] : 0.0f;
+    most = lane < warps ? red[32 + lane] : 0.0f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    }
+  }
+}
+
+// Widths that are a multiple of eight: a thread holds CHUNKS eights of its row, TEAM = 32 threads (WARP) or the block.
+template <bool F16, int OUT, bool GROUPS, int CHUNKS, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : CHUNKS < 4 ? 512 : 1024) add_norm_kernel(const AddNormArgs a) {
+  __shared__ float red[64];
+  const int team = WARP ? 32 : blockDim.x, tid = WARP ? threadIdx.x & 31 : threadIdx.x;
+  const int64_t row = WARP ? blockIdx.x * static_cast<int64_t>(blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+  grid_dep_launch();
+  grid_dep_wait();
+  if (WARP && row >= a.rows) return;
+  const uint16_t* x = static_cast<const uint16_t*>(a.x) + row * a.ldx;
+  const uint16_t* r = static_cast<const uint16_t*>(a.residual) + row * a.ldr;
+  const uint4* w = static_cast<const uint4*>(a.weight);
+  const int eights = a.width >> 3;
+  uint4 h[CHUNKS];
+  float sum = 0.0f, most = 0.0f;
+#pragma unroll
+  for (int i = 0; i < CHUNKS; ++i) {
+    const int c = tid + i * team;
+    h[i] = c < eights ? *reinterpret_cast<const uint4*>(x + 8 * c) : make_uint4(0, 0, 0, 0);
+  }
+  if (a.residual != nullptr) {
+    uint4 add[CHUNKS];
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+      const int c = tid + i * team;
+      add[i] = c < eights ? *reinterpret_cast<const uint4*>(r + 8 * c) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+      uint32_t* u = &h[i].x;
+      const uint32_t* v = &add[i].x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = widen16<F16>(u[j]), g = widen16<F16>(v[j]);
+        u[j] = narrow16<F16>(f.x + g.x, f.y + g.y);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < CHUNKS; ++i) {
+    const int c = tid + i * team;
+    constexpr bool kMost = OUT != kNormSame && !GROUPS;
+    const uint4 wc = kMost && c < eights ? __ldg(w + c) : make_uint4(0, 0, 0, 0);
+    const uint32_t *u = &h[i].x, *v = &wc.x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = widen16<F16>(u[j]), g = widen16<F16>(v[j]);
+      sum = fmaf(f.x, f.x, sum);
+      sum = fmaf(f.y, f.y, sum);
+      if (kMost) most = fmaxf(most, fmaxf(fabsf(f.x * g.x), fabsf(f.y * g.y)));
+    }
+    if (c < eights && a.h_out != nullptr) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.h_out) + row * a.ldh + 8 * c) = h[i];
+  }
+  row_reduce<WARP>(sum, most, red);
+  const float inv = rsqrtf(sum / static_cast<float>(a.width) + a.eps);
+  constexpr float kTop = OUT == kNormInt8 ? 127.0f : 448.0f;
+  if (OUT != kNormSame && !GROUPS && tid == 0) a.scale[row] = most * inv / kTop;
+#pragma unroll
+  for (int i = 0; i < CHUNKS; ++i) {
+    const int c = tid + i * team;
+    const uint4 wc = c < eights ? __ldg(w + c) : make_uint4(0, 0, 0, 0);
+    const uint32_t *u = &h[i].x, *v = &wc.x;
+    float p[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = widen16<F16>(u[j]), g = widen16<F16>(v[j]);
+      p[2 * j] = f.x * g.x;
+      p[2 * j + 1] = f.y * g.y;
+    }
+    if constexpr (OUT == kNormSame) {
+      if (c >= eights) continue;
+      uint4 y;
+      uint32_t* o = &y.x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = narrow16<F16>(p[2 * j] * inv, p[2 * j + 1] * inv);
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row * a.width + 8 * c) = y;
+    } else {
+      float top = most;
+      if constexpr (GROUPS) {
+        top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(p[j]));
+        for (int o = 1; o < a.group >> 3; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (c < eights && (8 * c & (a.group - 1)) == 0) a.scale[8 * c / a.group * a.rows + row] = top * inv / kTop;
+      }
+      if (c >= eights) continue;
+      const Coder by = coder<OUT>(top);
+      uint2 q;
+      if constexpr (OUT == kNormInt8) {
+        uint32_t b[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) b[j] = int8_code(p[j], by);
+        q.x = b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24;
+        q.y = b[4] | b[5] << 8 | b[6] << 16 | b[7] << 24;
+      } else {
+        float t[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[j] = scaled<OUT>(p[j], by);
+        q.x = e4m3_pair(t[0], t[1]) | e4m3_pair(t[2], t[3]) << 16;
+        q.y = e4m3_pair(t[4], t[5]) | e4m3_pair(t[6], t[7]) << 16;
+      }
+      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.out) + row * a.width + 8 * c) = q;
+    }
+  }
+}
+
+// Other widths: element by element, a row a block; the row's sum h goes through shared memory.
+template <bool F16, int OUT>
+__global__ void __launch_bounds__(256) add_norm_odd_kernel(const AddNormArgs a) {
+  extern __shared__ uint16_t row_h[];
+  __shared__ float red[64];
+  const int64_t row = blockIdx.x;
+  grid_dep_launch();
+  grid_dep_wait();
+  const uint16_t* x = static_cast<const uint16_t*>(a.x) + row * a.ldx;
+  const uint16_t* r = static_cast<const uint16_t*>(a.residual) + row * a.ldr;
+  const uint16_t* w = static_cast<const uint16_t*>(a.weight);
+  float sum = 0.0f, most = 0.0f;
+  for (int c = threadIdx.x; c < a.width; c += blockDim.x) {
+    uint32_t h = x[c];
+    if (a.residual != nullptr) h = narrow16<F16>(widen16<F16>(h).x + widen16<F16>(r[c]).x, 0.0f) & 0xffffu;
+    row_h[c] = static_cast<uint16_t>(h);
+    if (a.h_out != nullptr) static_cast<uint16_t*>(a.h_out)[row * a.ldh + c] = static_cast<uint16_t>(h);
+    const float f = widen16<F16>(h).x;
+    sum = fmaf(f, f, sum);
+    most = fmaxf(most, fabsf(f * widen16<F16>(w[c]).x));
+  }
+  row_reduce<false>(sum, most, red);
+  const float inv = rsqrtf(sum / static_cast<float>(a.width) + a.eps);
+  const Coder by = coder<OUT>(most);
+  if (OUT != kNormSame && threadIdx.x == 0) a.scale[row] = most * inv / (OUT == kNormInt8 ? 127.0f : 448.0f);
+  for (int c = threadIdx.x; c < a.width; c += blockDim.x) {
+    const float p = widen16<F16>(row_h[c]).x * widen16<F16>(w[c]).x;
+    const int64_t to = row * a.width + c;
+    if constexpr (OUT == kNormSame) static_cast<uint16_t*>(a.out)[to] = static_cast<uint16_t>(narrow16<F16>(p * inv, 0.0f));
+    else if constexpr (OUT == kNormInt8) static_cast<uint8_t*>(a.out)[to] = static_cast<uint8_t>(int8_code(p, by));
+    else static_cast<uint8_t*>(a.out)[to] = static_cast<uint8_t>(e4m3_pair(scaled<OUT>(p, by), 0.0f));
+  }
+}
+
+namespace {
+template <bool F16, int OUT, bool GROUPS>
+cudaError_t run_add_norm(const AddNormArgs& a, cudaStream_t st) {
+  const int eights = a.width / 8;
+  if (eights <= 32 * 4) {
+    const int warps = 8;
+    const dim3 grid(static_cast<unsigned>((a.rows + warps - 1) / warps));
+    if (eights <= 32) return launch_early(add_norm_kernel<F16, OUT, GROUPS, 1, true>, grid, 32 * warps, 0, st, a);
+    if (eights <= 64) return launch_early(add_norm_kernel<F16, OUT, GROUPS, 2, true>, grid, 32 * warps, 0, st, a);
+    return launch_early(add_norm_kernel<F16, OUT, GROUPS, 4, true>, grid, 32 * warps, 0, st, a);
+  }
+  const dim3 grid(static_cast<unsigned>(a.rows));
+  auto threads = [&](int chunks) { return ((eights + chunks - 1) / chunks + 31) / 32 * 32; };
+  if (threads(1) <= 512) return launch_early(add_norm_kernel<F16, OUT, GROUPS, 1, false>, grid, threads(1), 0, st, a);
+  if (threads(2) <= 512) return launch_early(add_norm_kernel<F16, OUT, GROUPS, 2, false>, grid, threads(2), 0, st, a);
+  return launch_early(add_norm_kernel<F16, OUT, GROUPS, 4, false>, grid, threads(4), 0, st, a);
+}
+template <bool F16>
+cudaError_t pick_add_norm(const AddNormArgs& a, cudaStream_t st) {
+  if (a.width % 8 != 0) {
+    const dim3 grid(static_cast<unsigned>(a.rows));
+    const int threads = a.width <= 256 ? (a.width + 31) / 32 * 32 : 256, bytes = 2 * a.width;
+    static unsigned long long devices[3] = {0, 0, 0};
+    auto launch = [&](auto kernel, unsigned long long& d) {
+      const cudaError_t e = allow_shared(kernel, 2 * kNormMaxWidth, d);
+      return e != cudaSuccess ? e : launch_early(kernel, grid, threads, bytes, st, a);
+    };
+    switch (a.out_kind) {
+      case kNormSame: return launch(add_norm_odd_kernel<F16, kNormSame>, devices[0]);
+      case kNormInt8: return launch(add_norm_odd_kernel<F16, kNormInt8>, devices[1]);
+      default: return launch(add_norm_odd_kernel<F16, kNormFp8>, devices[2]);
+    }
+  }
+  switch (a.out_kind) {
+    case kNormSame: return run_add_norm<F16, kNormSame, false>(a, st);
+    case kNormInt8: return a.group ? run_add_norm<F16, kNormInt8, true>(a, st) : run_add_norm<F16, kNormInt8, false>(a, st);
+    default: return a.group ? run_add_norm<F16, kNormFp8, true>(a, st) : run_add_norm<F16, kNormFp8, false>(a, st);
+  }
+}
+}  // namespace
+
+cudaError_t launch_add_norm(const AddNormArgs& a, cudaStream_t st) {
+  if (a.rows == 0 || a.width == 0) return cudaSuccess;
+  return a.dtype == CQ_DT_F16 ? pick_add_norm<true>(a, st) : pick_add_norm<false>(a, st);
+}
+
+}  // namespace cq

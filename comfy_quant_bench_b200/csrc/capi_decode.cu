@@ -1,5 +1,5 @@
-// extern "C" entry points of the decode-side operators (declared in include/cq_b200.h): the W4A16 linear and the
-// paged key-value cache.  Argument checks on the host, then kernel launches on the caller's stream.
+// extern "C" entry points of the decode-side operators (declared in include/cq_b200.h): the W4A16 linear, the paged
+// key-value cache, the residual norm, rotated appends, attention behind a shared prefix and sampling.  Argument checks on the host, then kernel launches on the caller's stream.
 #include <cstdint>
 
 #include "kernels.cuh"
@@ -204,6 +204,28 @@ int cq_kv_append(const void* k_new, int64_t k_layer_stride, int64_t k_token_stri
                          static_cast<int>(num_pages), static_cast<int>(page_size), static_cast<int>(table_rows),
                          static_cast<int>(table_width), dtype, cache_dtype};
   return cuda_status(cq::launch_kv_append(a, static_cast<cudaStream_t>(stream)));
+}
+
+int cq_add_rmsnorm(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int dtype,
+                   int64_t rows, int64_t width, float eps, int out_kind, int64_t group, void* h_out, int64_t ldh, void* out,
+                   float* scale, void* stream) {
+  if (!valid16(dtype) || out_kind < CQ_NORM_SAME || out_kind > CQ_NORM_FP8) return CQ_ERR_ARG;
+  if (group != 0 && (out_kind == CQ_NORM_SAME || (group != 32 && group != 64 && group != 128))) return CQ_ERR_ARG;
+  if (!fits_int(rows) || width < 1 || width > cq::kNormMaxWidth || (group != 0 && width % group != 0) || ldx < width ||
+      (residual != nullptr && ldr < width) || (h_out != nullptr && ldh < width))
+    return CQ_ERR_SHAPE;
+  if (rows == 0) return CQ_OK;
+  if (x == nullptr || weight == nullptr || out == nullptr || (out_kind != CQ_NORM_SAME && scale == nullptr)) return CQ_ERR_ARG;
+  const bool wide = width % 8 == 0;
+  const uintptr_t by = wide ? 16 : 2;
+  if (!aligned(x, by) || !aligned(residual, by) || !aligned(weight, by) || !aligned(h_out, by) ||
+      !aligned(out, out_kind == CQ_NORM_SAME ? by : wide ? 8 : 1) || !aligned(scale, 4) ||
+      (wide && (ldx % 8 != 0 || (residual != nullptr && ldr % 8 != 0) || (h_out != nullptr && ldh % 8 != 0))))
+    return CQ_ERR_ALIGN;
+  if (int dv = check_device()) return dv;
+  const cq::AddNormArgs a{x, residual, weight, h_out, out, scale, rows, ldx, ldr, ldh, static_cast<int>(width),
+                          static_cast<int>(group), out_kind, dtype, eps};
+  return cuda_status(cq::launch_add_norm(a, static_cast<cudaStream_t>(stream)));
 }
 
 }  // extern "C"

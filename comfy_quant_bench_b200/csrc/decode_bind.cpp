@@ -20,7 +20,7 @@ using Opt = std::optional<Tensor>;
 
 namespace {
 
-std::string text(const char* s) { return s; }
+std::string text(const std::string& s) { return s; }
 std::string text(int64_t v) { return std::to_string(v); }
 std::string text(at::ScalarType t) { return c10::toString(t); }
 std::string text(at::IntArrayRef v) {
@@ -123,6 +123,67 @@ Tensor w4a16_linear(const Tensor& x, const Tensor& qweight, const Tensor& scale,
                                zeros.data_ptr(), static_cast<int>(group), ptr(bias), out.data_ptr(), ptr(ws), bytes,
                                stream_of(index)));
   return out;
+}
+
+// -------------------------------------------------------------------------------------------------------------
+// root-mean-square norm with the residual's addition
+// -------------------------------------------------------------------------------------------------------------
+
+// x as rows [M, C] whose last dimension is contiguous, 16-byte aligned where the width allows; a copy where it has to be
+Tensor norm_rows(const Tensor& x, int64_t c) {
+  Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, c});
+  const int64_t ld = x2.size(0) > 1 ? x2.stride(0) : c;
+  if ((c > 1 && x2.stride(1) != 1) || ld < c || (c % 8 == 0 && (!aligned16(x2) || ld % 8 != 0)))
+    x2 = x2.clone(at::MemoryFormat::Contiguous);
+  return x2;
+}
+
+py::tuple add_rmsnorm(const Tensor& x, Tensor weight, const Opt& residual, double eps, const std::optional<std::string>& quant,
+                      int64_t group, const Opt& out_residual) {
+  const at::ScalarType dt = x.scalar_type();
+  if (!half_type(dt)) refuse("x must be bf16 or f16, got ", dt);
+  if (x.dim() < 1 || x.size(-1) < 1 || x.size(-1) > 32768) refuse("x must have a last dimension of 1 to 32768");
+  const int64_t c = x.size(-1);
+  if (weight.numel() != c) refuse("weight must have ", c, " elements");
+  if (residual && (residual->scalar_type() != dt || residual->sizes() != x.sizes()))
+    refuse("residual must be ", dt, " of shape ", x.sizes());
+  int kind = CQ_NORM_SAME;
+  if (quant) {
+    if (*quant == "int8") kind = CQ_NORM_INT8;
+    else if (*quant == "fp8") kind = CQ_NORM_FP8;
+    else refuse("quant must be None, 'int8' or 'fp8', got '", *quant, "'");
+  }
+  if (group != 0 && (kind == CQ_NORM_SAME || (group != 32 && group != 64 && group != 128) || c % group != 0))
+    refuse("group_size must be 0, or 32, 64 or 128 and divide ", c, " with an 8-bit output, got ", group);
+  if (out_residual) {
+    if (!residual) refuse("out_residual goes with a residual");
+    if (out_residual->scalar_type() != dt || out_residual->sizes() != x.sizes() || !out_residual->is_contiguous())
+      refuse("out_residual must be contiguous ", dt, " of shape ", x.sizes());
+    if (c % 8 == 0 && !aligned16(*out_residual)) refuse("out_residual must be 16-byte aligned");
+  }
+  const int index = device_of(x, weight, residual, out_residual);
+  const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(index));
+  const Tensor x2 = norm_rows(x, c);
+  const int64_t m = x2.size(0);
+  Opt r2, h;
+  if (residual) {
+    r2 = norm_rows(*residual, c);
+    h = out_residual ? *out_residual : at::empty(x.sizes(), x.options());
+  }
+  if (weight.scalar_type() != dt || weight.dim() != 1 || !weight.is_contiguous() || !aligned16(weight))
+    weight = weight.reshape({c}).to(dt).clone(at::MemoryFormat::Contiguous);
+  const at::ScalarType ot = kind == CQ_NORM_INT8 ? at::kChar : kind == CQ_NORM_FP8 ? at::kFloat8_e4m3fn : dt;
+  const Tensor out = at::empty(x.sizes(), x.options().dtype(ot));
+  Opt scale;
+  if (quant) scale = group ? at::empty({c / group, m}, x.options().dtype(at::kFloat)) : at::empty({m}, x.options().dtype(at::kFloat));
+  auto ld = [&](const Opt& t) { return t && t->dim() == 2 && m > 1 ? t->stride(0) : c; };
+  check_status("cq_add_rmsnorm",
+               cq_add_rmsnorm(x2.data_ptr(), ld(x2), ptr(r2), ld(r2), weight.data_ptr(), dtype_code(dt), m, c,
+                              static_cast<float>(eps), kind, group, ptr(h), c, out.data_ptr(), ptr<float>(scale),
+                              stream_of(index)));
+  const Tensor kept = residual ? *h : x;
+  if (quant) return py::make_tuple(out, *scale, kept);
+  return py::make_tuple(out, kept);
 }
 
 // -------------------------------------------------------------------------------------------------------------
@@ -350,6 +411,7 @@ py::tuple compact_pages(const Tensor& table_arg, const Tensor& refs, const Tenso
 
 PYBIND11_MODULE(_decode, m) {
   m.def("w4a16_linear", &w4a16_linear);
+  m.def("add_rmsnorm", &add_rmsnorm);
   m.def("paged_attention", &paged_attention);
   m.def("append_kv", &append_kv);
   m.def("pages_update", &pages_update);

@@ -59,6 +59,22 @@ inline cudaError_t allow_shared(Kernel kernel, int bytes, unsigned long long& de
   return e;
 }
 
+// a launch that may be set up before the kernel before it in the stream has ended (which the kernel itself waits for)
+template <typename... Params, typename... Args>
+inline cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, int threads, int smem, cudaStream_t st, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // (a.x, a.y) * (b.x, b.y) + (c.x, c.y) in one instruction, each rounded once
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;

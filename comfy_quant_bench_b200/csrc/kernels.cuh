@@ -128,6 +128,22 @@ bool gemv_affine_fits(int M, int a_kperm);
 cudaError_t launch_gemv_affine(const int8_t* a, const float* sa, const void* b, const void* s, const void* zt,
                                const void* bias, void* out, int M, int N, int K, cudaStream_t st, bool pdl = false);
 
+// root-mean-square norm with the residual's addition; the output in the type, or 8 bits with scales
+enum NormOut { kNormSame = CQ_NORM_SAME, kNormInt8 = CQ_NORM_INT8, kNormFp8 = CQ_NORM_FP8 };
+constexpr int kNormMaxWidth = 32768;
+struct AddNormArgs {
+  const void* x;              // [rows, width] bf16 or f16, rows ldx elements apart
+  const void* residual;       // the same, ldr; or null
+  const void* weight;         // [width]
+  void* h_out;                // x + residual, ldh; may be x or residual; or null
+  void* out;                  // [rows, width] of the type, int8 or e4m3
+  float* scale;               // [rows] or [width / group, rows] (8-bit outputs)
+  int64_t rows, ldx, ldr, ldh;
+  int width, group, out_kind, dtype;
+  float eps;
+};
+cudaError_t launch_add_norm(const AddNormArgs& a, cudaStream_t st);
+
 // W4A16 linear: 16-bit activations, packed uint4 weights, a scale and a zero per group (awq_w4a16)
 struct W4A16Args {
   const void* x;              // [M, K] bf16 or f16, rows ldx elements apart

@@ -251,24 +251,6 @@ __global__ void __launch_bounds__(256) pages_copy_kernel(const PagesCopyArgs a) 
   for (int64_t i = threadIdx.x; i < a.page_bytes / 16; i += 256) to[i] = __ldcs(from + i);
 }
 
-namespace {
-// a launch that may be set up before the kernel before it in the stream has ended (which the kernel itself waits for)
-template <typename... Params, typename... Args>
-cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, int threads, int smem, cudaStream_t st, const Args&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-}  // namespace
-
 cudaError_t launch_pages_copy(const PagesCopyArgs& a, cudaStream_t st) {
   if (a.n == 0) return cudaSuccess;
   return launch_early(pages_copy_kernel, dim3(a.n, a.layers, 2), 256, 0, st, a);

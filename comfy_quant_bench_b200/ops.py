@@ -777,6 +777,21 @@ def rmsnorm_rope_rows(x: torch.Tensor, weight: torch.Tensor, rope: torch.Tensor 
     return out.reshape(x.shape)
 
 
+def add_rmsnorm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, *, eps: float = 1e-6,
+                quant: str | None = None, group_size: int = 0, out_residual: torch.Tensor | None = None):
+    """The residual's addition and the root-mean-square norm after it: h = x + residual, rounded to x's type (bf16 or
+    f16), and y = h * weight / sqrt(mean(h^2) + eps) over the last dimension (1 to 32768), in fp32, rounded once.
+
+    Returns (y, h).  With ``quant`` "int8" or "fp8" (e4m3), (codes, scale, h): y ~ codes * scale with f32 scales [rows]
+    (rows: the leading dimensions flattened), or [C / group_size, rows] for groups of 32, 64 or 128 columns; they feed
+    the int8 GEMMs (``gemm_rowcol``) without another pass.  A code is round(127 p / P) (448 for fp8), p = h * weight, P
+    its largest magnitude in the row or group; int8 codes are the nearest-even ones of the exact quotient.
+
+    ``out_residual`` (contiguous; may be x or residual itself) takes h; without a residual h is x.  A row with a NaN
+    gives NaN, as scale too; a row of zeros zero codes and scales.  The weight is taken in x's type."""
+    return _lib.decode().add_rmsnorm(x, weight, residual, eps, quant, group_size, out_residual)
+
+
 def _out_ptrs(outs, rows: int, ldo: int):
     ptrs = []
     for o in outs:

@@ -569,6 +569,24 @@ CQ_API int cq_pages_compact(const int32_t* block_table, int64_t table_rows, int6
                             int64_t layer_bytes, int64_t page_bytes, void* workspace, int64_t workspace_bytes,
                             void* stream);
 
+/*
+ * cq_add_rmsnorm: h = x + residual, rounded to `dtype` (residual NULL: h = x), y = h * weight / sqrt(mean(h^2) + eps) in
+ * fp32, over rows of `width`.
+ *   x, residual, h_out  [rows, width] of `dtype` (bf16 or f16), rows ldx, ldr, ldh elements apart; h_out may be NULL, x or
+ *            residual (with the same row stride), and overlaps them in no other way
+ *   weight   [width] of `dtype`
+ *   out_kind CQ_NORM_SAME: out [rows, width] of `dtype`, y rounded once.  CQ_NORM_INT8 / CQ_NORM_FP8: out int8 / e4m3
+ *            codes round(top p / P) with p = h * weight, P its largest magnitude in the row (group == 0) or in each group of
+ *            32, 64 or 128 columns, top 127 / 448; scale f32 [rows] or [width / group, rows] = P / (top sqrt(mean(h^2) +
+ *            eps)).  int8 codes round to nearest even of the exact quotient.  Zero rows have zero codes and scales.
+ * width 1 to 32768.  Widths that are a multiple of 8 need 16-byte aligned bases and row strides that are multiples of 8.
+ * A row with a NaN gives NaN (scales NaN); one with an infinity what the formula gives (its scale NaN).
+ */
+enum cq_norm_out { CQ_NORM_SAME = 0, CQ_NORM_INT8 = 1, CQ_NORM_FP8 = 2 };
+CQ_API int cq_add_rmsnorm(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int dtype,
+                          int64_t rows, int64_t width, float eps, int out_kind, int64_t group, void* h_out, int64_t ldh,
+                          void* out, float* scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
