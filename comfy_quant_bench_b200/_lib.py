@@ -119,6 +119,9 @@ SIGNATURES = {
                                   _i64, _vp]),
     "cq_kv_append": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _int, _i64, _i64, _i64, _i64, _vp, _vp, _int,
                             _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "cq_kv_append_rotated": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _int, _i64, _i64, _i64, _i64, _vp,
+                                    _i64, _i64, _int, _vp, _vp, _f32, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _i64,
+                                    _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
     "cq_pages_workspace_bytes": (_i64, [_i64, _i64]),
     "cq_pages_update": (_int, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp,
                                _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp]),

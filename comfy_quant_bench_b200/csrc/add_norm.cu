@@ -13,21 +13,6 @@
 
 namespace cq {
 
-template <bool F16>
-__device__ __forceinline__ float2 widen16(uint32_t w) {
-  if constexpr (F16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
-  else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-}
-template <bool F16>
-__device__ __forceinline__ uint32_t narrow16(float a, float b) {
-  if constexpr (F16) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  } else {
-    return bf16x2_bits(a, b);
-  }
-}
-
 // Codes of p against the largest P: `by` is top / P, or 0 where P is 0.
 struct Coder {
   float most, by;

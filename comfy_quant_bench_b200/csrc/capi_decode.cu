@@ -1,6 +1,7 @@
 // extern "C" entry points of the decode-side operators (declared in include/cq_b200.h): the W4A16 linear, the paged
 // key-value cache, the residual norm, rotated appends, attention behind a shared prefix and sampling.  Argument checks on the host, then kernel launches on the caller's stream.
 #include <cstdint>
+#include <initializer_list>
 
 #include "kernels.cuh"
 
@@ -226,6 +227,43 @@ int cq_add_rmsnorm(const void* x, int64_t ldx, const void* residual, int64_t ldr
   const cq::AddNormArgs a{x, residual, weight, h_out, out, scale, rows, ldx, ldr, ldh, static_cast<int>(width),
                           static_cast<int>(group), out_kind, dtype, eps};
   return cuda_status(cq::launch_add_norm(a, static_cast<cudaStream_t>(stream)));
+}
+
+int cq_kv_append_rotated(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_new,
+                         int64_t k_token_stride, int64_t k_head_stride, const void* v_new, int64_t v_token_stride,
+                         int64_t v_head_stride, int dtype, int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                         const float* rope, int64_t rope_rows, int64_t rot_dim, int interleaved, const void* q_norm,
+                         const void* k_norm, float eps, void* q_out, void* k_out, void* k_cache, void* v_cache, int cache_dtype,
+                         int64_t num_pages, int64_t page_size, int64_t page_stride, int64_t head_stride, int64_t token_stride,
+                         const int32_t* block_table, int64_t table_rows, int64_t table_width, int64_t table_stride,
+                         const int32_t* rows, const int32_t* positions, const float* k_scale, const float* v_scale,
+                         void* stream) {
+  if (!valid16(dtype) || (cache_dtype != dtype && cache_dtype != CQ_DT_FP8_E4M3)) return CQ_ERR_ARG;
+  if (int rc = check_tables(table_rows, table_width, table_stride, num_pages, page_size)) return rc;
+  if (!fits_int(tokens) || q_heads < 1 || q_heads > 4096 || kv_heads < 1 || kv_heads > 4096 || head_dim < 16 || head_dim > 256 ||
+      head_dim % 8 != 0 || rot_dim < 16 || rot_dim % 16 != 0 || rot_dim > head_dim || rope_rows < 1 || !fits_int(rope_rows))
+    return CQ_ERR_SHAPE;
+  if (tokens == 0) return CQ_OK;
+  if (q == nullptr || k_new == nullptr || v_new == nullptr || rope == nullptr || q_out == nullptr || k_cache == nullptr ||
+      v_cache == nullptr || rows == nullptr || positions == nullptr || (block_table == nullptr && table_width > 0))
+    return CQ_ERR_ARG;
+  for (const void* p : {q, k_new, v_new, static_cast<const void*>(rope), q_norm, k_norm, static_cast<const void*>(q_out),
+                        static_cast<const void*>(k_out), static_cast<const void*>(k_cache), static_cast<const void*>(v_cache)})
+    if (!aligned(p, 16)) return CQ_ERR_ALIGN;
+  for (const int64_t s : {q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride,
+                          page_stride, head_stride, token_stride})
+    if (s % 8 != 0) return CQ_ERR_ALIGN;
+  if (!aligned(block_table, 4) || !aligned(rows, 4) || !aligned(positions, 4) || !aligned(k_scale, 4) || !aligned(v_scale, 4))
+    return CQ_ERR_ALIGN;
+  if (int dv = check_device()) return dv;
+  const cq::RotateArgs a{q, k_new, v_new, q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride,
+                         v_head_stride, rope, q_norm, k_norm, q_out, k_out, k_cache, v_cache, page_stride, head_stride,
+                         token_stride, block_table, table_stride, rows, positions, k_scale, v_scale, static_cast<int>(tokens),
+                         static_cast<int>(q_heads), static_cast<int>(kv_heads), static_cast<int>(head_dim),
+                         static_cast<int>(rot_dim), interleaved != 0, static_cast<int>(rope_rows), static_cast<int>(num_pages),
+                         static_cast<int>(page_size), static_cast<int>(table_rows), static_cast<int>(table_width), dtype,
+                         cache_dtype, eps, 0};
+  return cuda_status(cq::launch_rotate_append(a, static_cast<cudaStream_t>(stream)));
 }
 
 }  // extern "C"

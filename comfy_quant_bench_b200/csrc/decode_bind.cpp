@@ -315,6 +315,65 @@ void append_kv(const Tensor& k_arg, const Tensor& v_arg, const Tensor& k_cache, 
                             ks, vs, stream_of(index)));
 }
 
+void head_norm(const Opt& w, int64_t d, const char* name) {
+  if (w && w->numel() != d) refuse(name, " must have ", d, " elements");
+}
+// a norm weight as the kernel reads it: of the type, contiguous and aligned
+Opt norm_weight(const Opt& w, at::ScalarType dt) {
+  if (!w || (w->scalar_type() == dt && w->dim() == 1 && w->is_contiguous() && aligned16(*w))) return w;
+  return w->reshape({w->numel()}).to(dt).clone(at::MemoryFormat::Contiguous);
+}
+
+py::object append_rotated(const Tensor& q_arg, const Tensor& k_arg, const Tensor& v_arg, const Tensor& k_cache,
+                          const Tensor& v_cache, const Tensor& table_arg, const Tensor& rows, const Tensor& positions,
+                          const Tensor& rope_arg, bool interleaved, const Opt& q_norm_arg, const Opt& k_norm_arg, double eps,
+                          const Opt& k_scale, const Opt& v_scale, bool return_k) {
+  const at::ScalarType dt = q_arg.scalar_type(), ct = k_cache.scalar_type();
+  if (q_arg.dim() != 3 || !half_type(dt)) refuse("q must be bf16 or f16 [T, q_heads, D]");
+  if (k_arg.dim() != 3 || k_arg.sizes() != v_arg.sizes() || k_arg.scalar_type() != dt || v_arg.scalar_type() != dt)
+    refuse("k and v must be ", dt, " of one shape, [T, kv_heads, D]");
+  cache_pair(k_cache, v_cache, 4);
+  const int64_t t = q_arg.size(0), hq = q_arg.size(1), d = q_arg.size(2), hk = k_arg.size(1);
+  if (k_arg.size(0) != t || k_arg.size(2) != d) refuse("k ", k_arg.sizes(), " does not fit q ", q_arg.sizes());
+  if (k_cache.size(1) != hk || k_cache.size(3) != d) refuse("caches ", k_cache.sizes(), " do not fit k ", k_arg.sizes());
+  if (hq < 1 || hk < 1 || d < 16 || d > 256 || d % 8 != 0) refuse("head_dim must be a multiple of 8 from 16 to 256, got ", d);
+  if (ct != dt && ct != at::kFloat8_e4m3fn) refuse("the caches must hold ", dt, " or float8_e4m3fn, got ", ct);
+  i32(table_arg, 2, "block_table");
+  i32(rows, 1, "rows");
+  i32(positions, 1, "positions");
+  if (rows.size(0) != t || positions.size(0) != t) refuse("rows and positions must have one entry per token (", t, ")");
+  if (rope_arg.scalar_type() != at::kFloat || rope_arg.dim() != 3 || rope_arg.size(2) != 2 || rope_arg.size(0) < 1 ||
+      !rope_arg.is_contiguous())
+    refuse("rope must be contiguous f32 [positions, rot_dim / 2, 2]");
+  const int64_t rot = 2 * rope_arg.size(1);
+  if (rot < 16 || rot % 16 != 0 || rot > d) refuse("rope must turn a multiple of 16 columns, at most D=", d, ", got ", rot);
+  head_norm(q_norm_arg, d, "q_norm");
+  head_norm(k_norm_arg, d, "k_norm");
+  const int index = device_of(q_arg, k_arg, v_arg, k_cache, v_cache, table_arg, rows, positions, rope_arg, q_norm_arg,
+                              k_norm_arg, k_scale, v_scale);
+  const float* ks = head_scale(k_scale, hk, ct, "k_scale");
+  const float* vs = head_scale(v_scale, hk, ct, "v_scale");
+  const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(index));
+  const Tensor table = read_table(table_arg);
+  const Tensor rope = aligned16(rope_arg) ? rope_arg : rope_arg.clone();
+  const Tensor q = aligned_rows(q_arg), k = aligned_rows(k_arg), v = aligned_rows(v_arg);
+  const Opt q_norm = norm_weight(q_norm_arg, dt), k_norm = norm_weight(k_norm_arg, dt);
+  const Tensor q_out = at::empty({t, hq, d}, q.options());
+  Opt k_out;
+  if (return_k) k_out = at::empty({t, hk, d}, q.options());
+  check_status("cq_kv_append_rotated",
+               cq_kv_append_rotated(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+                                    v.stride(0), v.stride(1), dtype_code(dt), t, hq, hk, d, rope.data_ptr<float>(), rope.size(0),
+                                    rot, interleaved, ptr(q_norm), ptr(k_norm), static_cast<float>(eps), q_out.data_ptr(),
+                                    ptr(k_out), k_cache.data_ptr(), v_cache.data_ptr(), dtype_code(ct), k_cache.size(0),
+                                    k_cache.size(2), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
+                                    static_cast<const int32_t*>(table.data_ptr()), table.size(0), table.size(1),
+                                    row_stride(table), static_cast<const int32_t*>(rows.data_ptr()),
+                                    static_cast<const int32_t*>(positions.data_ptr()), ks, vs, stream_of(index)));
+  if (return_k) return py::make_tuple(q_out, *k_out);
+  return py::cast(q_out);
+}
+
 // caches [layers, num_pages, kv_heads, page_size, D] whose pages are one block each
 struct PageLayout {
   int64_t layers = 0, layer_bytes = 0, page_bytes = 0;
@@ -414,6 +473,7 @@ PYBIND11_MODULE(_decode, m) {
   m.def("add_rmsnorm", &add_rmsnorm);
   m.def("paged_attention", &paged_attention);
   m.def("append_kv", &append_kv);
+  m.def("append_rotated", &append_rotated);
   m.def("pages_update", &pages_update);
   m.def("compact_pages", &compact_pages);
 }

@@ -238,4 +238,30 @@ struct AppendArgs {
 };
 cudaError_t launch_kv_append(const AppendArgs& a, cudaStream_t st);
 
+// the same with rotary positions (and an RMS norm of each head) on the way, and the rotated queries
+struct RotateArgs {
+  const void* q;              // [T, Hq, D], token and head strides in elements
+  const void* k_new;          // [T, Hkv, D]
+  const void* v_new;
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;
+  const float* rope;          // [rope_rows, R / 2, 2] (cos, sin) of every position
+  const void* q_norm;         // [D] of the type, or null: no norm
+  const void* k_norm;
+  void* q_out;                // [T, Hq, D]
+  void* k_out;                // [T, Hkv, D] or null
+  void* k;                    // caches, strides in elements
+  void* v;
+  int64_t page_stride, head_stride, tok_stride;
+  const int* table;
+  int64_t table_stride;
+  const int* rows;            // [T]
+  const int* positions;       // [T]
+  const float* k_scale;       // [Hkv] or null: 1 (8-bit caches)
+  const float* v_scale;
+  int T, Hq, Hkv, D, R, interleaved, rope_rows, num_pages, page_size, table_rows, table_width, dtype, cache_dtype;
+  float eps;
+  int lane_bits;              // log2 of the threads of a head: set by the launch
+};
+cudaError_t launch_rotate_append(const RotateArgs& a, cudaStream_t st);
+
 }  // namespace cq

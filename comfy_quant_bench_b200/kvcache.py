@@ -12,12 +12,14 @@ pages, too narrow a table) reserves nothing - ``branch_rows`` has freed and fork
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _lib
 
 _DTYPES = (torch.bfloat16, torch.float16, torch.float8_e4m3fn)
-_SITES = {101: "free", 102: "fork", 103: "reserve"}
+_SITES = {101: "free", 102: "fork", 103: "reserve", 104: "append_rotated (a position beyond the table of angles)"}
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -49,6 +51,60 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     reservation, a missing page) is skipped.  A float8_e4m3fn cache receives x / scale of the head, rounded to
     nearest and kept inside the format's finite range."""
     _lib.decode().append_kv(k, v, k_cache, v_cache, block_table, rows, positions, k_scale, v_scale)
+
+
+def rope_table(positions: int, rot_dim: int, *, base: float = 10000.0, scaling: str | None = None, factor: float = 1.0,
+               original: int = 0, fast: float = 32.0, slow: float = 1.0, device="cuda") -> torch.Tensor:
+    """Angles of rotary positions: f32 [positions, rot_dim / 2, 2] = (cos, sin) of p * base ** (-2i / rot_dim), computed in
+    64 bits.  ``scaling`` stretches a model's context by ``factor``:
+
+    * "linear": every angle is divided by the factor;
+    * "base": the base grows to base * factor ** (rot_dim / (rot_dim - 2)), so that the slowest pair is divided by the
+      factor and the fastest stays;
+    * "parts": with ``original`` the context that the model was trained on, pairs that turn more than ``fast`` times in it
+      stay, those that turn less than ``slow`` times are divided by the factor, a linear blend between; cos and sin are
+      multiplied by 0.1 ln(factor) + 1."""
+    if rot_dim < 2 or rot_dim % 2:
+        raise ValueError(f"rot_dim must be even, got {rot_dim}")
+    if scaling not in (None, "linear", "base", "parts"):
+        raise ValueError(f"scaling must be None, 'linear', 'base' or 'parts', got {scaling!r}")
+    if scaling is not None and factor < 1:
+        raise ValueError(f"factor must be at least 1, got {factor}")
+    if scaling == "parts" and (original < 1 or not fast > slow):
+        raise ValueError("scaling 'parts' needs original > 0 and fast > slow")
+    if scaling == "base" and rot_dim > 2:
+        base = base * factor ** (rot_dim / (rot_dim - 2))
+    inv = base ** (-torch.arange(0, rot_dim, 2, device=device, dtype=torch.float64) / rot_dim)
+    size = 1.0
+    if scaling == "linear":
+        inv = inv / factor
+    elif scaling == "parts":
+        turns = original * inv / (2 * math.pi)
+        kept = ((turns - slow) / (fast - slow)).clamp(0, 1)
+        inv = inv * kept + inv / factor * (1 - kept)
+        size = 0.1 * math.log(factor) + 1
+    angle = torch.outer(torch.arange(positions, device=device, dtype=torch.float64), inv)
+    return (size * torch.stack([angle.cos(), angle.sin()], dim=-1)).float()
+
+
+def append_rotated(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   block_table: torch.Tensor, rows: torch.Tensor, positions: torch.Tensor, rope: torch.Tensor, *,
+                   interleaved: bool = False, q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None,
+                   eps: float = 1e-6, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                   return_k: bool = False):
+    """``append_kv`` of one layer with the rotary positions on the way: q [T, q_heads, D], k, v [T, kv_heads, D] (bf16 or
+    f16, strided views of one qkv tensor allowed) are token t of position ``positions[t]`` in table row ``rows[t]``.
+
+    Each head of q and k is normed if ``q_norm`` / ``k_norm`` [D] are given (x / sqrt(mean(x^2) + eps) * weight), then
+    turned by its position's angles, rope f32 [positions, rot_dim / 2, 2] (``rope_table``): the pairs (i, i + rot_dim / 2)
+    of a head's first rot_dim columns, or (2i, 2i + 1) with ``interleaved``.  fp32, one rounding.  k and v go into the
+    caches; returns q [T, q_heads, D], with ``return_k`` also the turned k [T, kv_heads, D].
+
+    A token without a place (see ``append_kv``) is turned as position max(position, 0) and not cached.  A position beyond
+    the table of angles is not cached, its turned columns are NaN, and ``check`` raises.  D a multiple of 8 from 16 to 256,
+    rot_dim a multiple of 16 up to D."""
+    return _lib.decode().append_rotated(q, k, v, k_cache, v_cache, block_table, rows, positions, rope, interleaved, q_norm,
+                                        k_norm, eps, k_scale, v_scale, return_k)
 
 
 def free_rows(block_table, seq_lens, ref_counts, rows, page_size: int) -> None:
@@ -144,6 +200,12 @@ class PagedKVCache:
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, rows: torch.Tensor, positions: torch.Tensor) -> None:
         append_kv(k, v, self.k[layer], self.v[layer], self.block_table, rows, positions, k_scale=self.k_scale,
                   v_scale=self.v_scale)
+
+    def append_rotated(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rows: torch.Tensor,
+                       positions: torch.Tensor, rope: torch.Tensor, **kw):
+        """q turned by its positions (with ``return_k`` also k); k and v are cached."""
+        return append_rotated(q, k, v, self.k[layer], self.v[layer], self.block_table, rows, positions, rope,
+                              k_scale=self.k_scale, v_scale=self.v_scale, **kw)
 
     def attend(self, layer: int, q: torch.Tensor, rows: torch.Tensor | None = None, **kw) -> torch.Tensor:
         return paged_attention(q, self.k[layer], self.v[layer], self.block_table, self.seq_lens, rows=rows,

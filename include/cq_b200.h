@@ -532,6 +532,27 @@ CQ_API int cq_kv_append(const void* k_new, int64_t k_layer_stride, int64_t k_tok
                         const int32_t* positions, const float* k_scale, const float* v_scale, void* stream);
 
 /*
+ * cq_kv_append_rotated: one layer's new queries, keys and values [tokens, heads, head_dim] (`dtype`, strides in elements).
+ * Queries and keys get an RMS norm over each head (q_norm, k_norm [head_dim] of `dtype`, NULL: none; eps), then the first
+ * rot_dim columns of each head are turned by the angles of the token's position: pairs (2i, 2i + 1) with `interleaved`, else
+ * (i, i + rot_dim / 2); rope f32 [rope_rows, rot_dim / 2, 2] = (cos, sin) of positions 0 to rope_rows - 1.  fp32, one rounding.
+ * q_out [tokens, q_heads, head_dim] (and k_out [tokens, kv_heads, head_dim], may be NULL), contiguous, not overlapping the
+ * inputs; keys and values go into the cache as cq_kv_append writes them, under its conditions.  A token without a place is
+ * turned as position max(position, 0).  A position >= rope_rows is not cached, its turned columns are NaN, and the device
+ * status word gets CQ_ERR_SHAPE with site 104.
+ * head_dim a multiple of 8 from 16 to 256, rot_dim a multiple of 16 up to it; 16-byte aligned bases, strides multiples of 8.
+ */
+CQ_API int cq_kv_append_rotated(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_new,
+                                int64_t k_token_stride, int64_t k_head_stride, const void* v_new, int64_t v_token_stride,
+                                int64_t v_head_stride, int dtype, int64_t tokens, int64_t q_heads, int64_t kv_heads,
+                                int64_t head_dim, const float* rope, int64_t rope_rows, int64_t rot_dim, int interleaved,
+                                const void* q_norm, const void* k_norm, float eps, void* q_out, void* k_out, void* k_cache,
+                                void* v_cache, int cache_dtype, int64_t num_pages, int64_t page_size, int64_t page_stride,
+                                int64_t head_stride, int64_t token_stride, const int32_t* block_table, int64_t table_rows,
+                                int64_t table_width, int64_t table_stride, const int32_t* rows, const int32_t* positions,
+                                const float* k_scale, const float* v_scale, void* stream);
+
+/*
  * cq_pages_update: the bookkeeping of a paged cache on the device, in up to three phases, each on a list of distinct
  * table rows (int32, device memory):
  *   free     free_rows [n_free] give up their pages and become empty;

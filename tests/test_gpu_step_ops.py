@@ -169,3 +169,145 @@ def test_norm_codes_feed_the_int8_gemm(ops):
     y = ops.gemm_rowcol(q, s, qw, sw.view(-1), b_int8=True)
     want = (q.double() @ qw.double().t()) * s.double().unsqueeze(1) * sw.double().view(1, -1)
     assert float((y.double() - want).abs().max()) <= 2.0 ** -7 * float(want.abs().max())
+
+
+# ----------------------------------------------------------------------------------------------------------
+# rotary positions and append
+# ----------------------------------------------------------------------------------------------------------
+
+def _turn(x, cos, sin, rot, interleaved):
+    """x [T, H, D] in 64 bits, turned, and the sum of the magnitudes that each result comes from."""
+    x, mag = x.clone(), x.abs()
+    i, j = (slice(0, rot, 2), slice(1, rot, 2)) if interleaved else (slice(0, rot // 2), slice(rot // 2, rot))
+    a, b = x[..., i].clone(), x[..., j].clone()
+    x[..., i], x[..., j] = a * cos - b * sin, a * sin + b * cos
+    mag[..., i] = mag[..., j] = a.abs() + b.abs()
+    return x, mag
+
+
+def _rotate_problem(t, hq, hk, d, rot, dtype, cache, seed=0, page=16, normed=True, far=40):
+    g = _gen(seed + 3 * t + d)
+    heads = hq + 2 * hk
+    qkv = (2 * torch.randn(t, heads, d, generator=g, device="cuda")).to(dtype)
+    pages = t + 5
+    k, v = (torch.randn(pages, hk, page, d, generator=g, device="cuda").to(cache) for _ in range(2))
+    host = torch.Generator().manual_seed(seed)
+    pos = torch.randint(0, far, (t,), generator=host)
+    table = torch.full((t + 1, -(-far // page)), -1, dtype=torch.int32)
+    order = torch.randperm(pages, generator=host)
+    rows = torch.randperm(t + 1, generator=host)[:t]
+    for n in range(t):
+        table[rows[n], pos[n] // page] = order[n]
+    w = [(1 + 0.3 * torch.randn(d, generator=g, device="cuda")).to(dtype) if normed else None for _ in range(2)]
+    scales = [0.02 + 0.02 * torch.rand(hk, generator=g, device="cuda") if cache == FP8 else None for _ in range(2)]
+    return qkv, k, v, table.cuda(), rows.int().cuda(), pos.int().cuda(), w, scales
+
+
+def _rotate_holds(kv, problem, hq, hk, rot, interleaved, rope):
+    qkv, k, v, table, rows, pos, w, scales = problem
+    d, page, dtype, cache = qkv.shape[2], k.shape[2], qkv.dtype, k.dtype
+    k0, v0 = k.clone(), v.clone()
+    q_new, k_new, v_new = qkv.split((hq, hk, hk), dim=1)
+    got, got_k = kv.append_rotated(q_new, k_new, v_new, k, v, table, rows, pos, rope, interleaved=interleaved, q_norm=w[0],
+                                   k_norm=w[1], k_scale=scales[0], v_scale=scales[1], return_k=True)
+    at = pos.long().clamp(min=0)
+    cos, sin = rope.double()[at].unsqueeze(1).unbind(-1)
+    slack = (d / 32 + 28) * 2.0 ** -24
+    want = []
+    for x, weight in ((q_new, w[0]), (k_new, w[1])):
+        x = x.double()
+        if weight is not None:
+            x = x / torch.sqrt(x.square().mean(-1, keepdim=True) + 1e-6) * weight.double()
+        want.append(_turn(x, cos, sin, rot, interleaved))
+    for g, (y, mag) in zip((got, got_k), want):
+        assert g.dtype == dtype and g.shape == y.shape and g.is_contiguous()
+        assert float(((g.double() - y).abs() - U[dtype] * y.abs() - slack * mag).max()) <= 2.0 ** -25
+    placed = [n for n in range(len(pos)) if pos[n] >= 0 and pos[n] // page < table.shape[1] and 0 <= rows[n] < len(table) and
+              0 <= table[rows[n], pos[n] // page] < len(k)]
+    for c, c0, new, scale in ((k, k0, want[1], scales[0]), (v, v0, (v_new.double(), None), scales[1])):
+        c, c0 = c.float(), c0.float()
+        for n in placed:
+            p, slot = int(table[rows[n], pos[n] // page]), int(pos[n]) % page
+            y = new[0][n] if scale is None else (new[0][n] / scale.double().view(-1, 1)).clamp(-448, 448)
+            m = y.abs() if new[1] is None else new[1][n] if scale is None else new[1][n] / scale.double().view(-1, 1)
+            u = U[dtype] if scale is None else 2.0 ** -4
+            tiny = 2.0 ** -25 if scale is None else 2.0 ** -10         # half the spacing of subnormal values
+            assert float(((c[p, :, slot].double() - y).abs() - u * y.abs() - (slack + 2.0 ** -23) * m).max()) <= tiny
+            c0[p, :, slot] = c[p, :, slot]
+        assert torch.equal(c, c0)                                      # and nothing else was written
+
+
+@pytest.mark.parametrize("cache", ["own", "fp8"])
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("t,hq,hk,d,rot", [(1, 1, 1, 16, 16), (1, 16, 2, 128, 128), (3, 7, 1, 64, 32), (40, 32, 8, 128, 64),
+                                           (5, 6, 3, 80, 80), (300, 3, 1, 96, 48), (2, 20, 4, 256, 256), (9, 64, 8, 256, 64),
+                                           (4, 5, 5, 24, 16), (310, 12, 4, 128, 128)])
+def test_rotated_append(kv, t, hq, hk, d, rot, interleaved, dtype, cache):
+    rope = kv.rope_table(64, rot)
+    for normed in (False, True):
+        problem = _rotate_problem(t, hq, hk, d, rot, dtype, FP8 if cache == "fp8" else dtype, normed=normed)
+        _rotate_holds(kv, problem, hq, hk, rot, interleaved, rope)
+
+
+def test_rotated_append_far_positions_scaled(kv):
+    rope = kv.rope_table(130000, 128, base=500000.0, scaling="parts", factor=8.0, original=8192)
+    problem = list(_rotate_problem(6, 4, 2, 128, 128, torch.bfloat16, torch.bfloat16, far=129999))
+    _rotate_holds(kv, problem, 4, 2, 128, False, rope)
+
+
+def test_rotated_append_tokens_without_a_place(kv):
+    from comfy_quant_bench_b200 import _lib
+    rope = kv.rope_table(64, 64)
+    problem = _rotate_problem(8, 4, 2, 64, 64, torch.float16, torch.float16)
+    qkv, k, v, table, rows, pos, w, scales = problem
+    pos[0], pos[1], pos[2] = -1, 63, -7                                # refused, beyond the table, refused
+    rows[3], rows[4] = -1, len(table)
+    table[rows[5].long(), pos[5].long() // 16] = -1
+    table[rows[6].long(), pos[6].long() // 16] = len(k)
+    _rotate_holds(kv, problem, 4, 2, 64, False, rope)
+    kv.check()
+    pos[0] = 64                                                        # no angle
+    before = k.clone()
+    q, k_new, v_new = qkv.split((4, 2, 2), dim=1)
+    got = kv.append_rotated(q[:1], k_new[:1], v_new[:1], k, v, table, rows[:1], pos[:1], rope[:, :16].contiguous())
+    assert bool(got[..., :32].isnan().all()) and torch.equal(got[..., 32:], q[:1, :, 32:]) and torch.equal(k, before)
+    with pytest.raises(_lib.CQError, match="append_rotated"):
+        kv.check()
+    none = kv.append_rotated(q[:0], k_new[:0], v_new[:0], k, v, table, rows[:0], pos[:0], rope)
+    assert none.shape == (0, 4, 64)
+
+
+def test_rotated_append_strides_special_values_and_streams(kv):
+    rope = kv.rope_table(64, 64)
+    problem = _rotate_problem(12, 4, 2, 64, 64, torch.bfloat16, torch.bfloat16, normed=False)
+    qkv, k, v, table, rows, pos, w, scales = problem
+    q, k_new, v_new = qkv.split((4, 2, 2), dim=1)
+    want = kv.append_rotated(q, k_new, v_new, k, v, table, rows, pos, rope)
+    kc, vc = k.clone(), v.clone()
+    k.zero_(), v.zero_()
+    odd = torch.zeros(12, 4, 65, device="cuda", dtype=torch.bfloat16)[..., 1:].copy_(q)    # not aligned: copied
+    expanded = table.t().contiguous().t()                                                  # a table of other strides
+    with pytest.raises(ValueError, match="contiguous"):
+        kv.append_rotated(odd, k_new, v_new, k, v, expanded, rows, pos, rope)
+    got = kv.append_rotated(odd, k_new.contiguous(), v_new.transpose(0, 1).contiguous().transpose(0, 1), k, v, table, rows, pos, rope)
+    assert torch.equal(got, want)
+    touched = kc != 0
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = kv.append_rotated(q, k_new, v_new, k, v, table, rows, pos, rope)
+    side.synchronize()
+    assert torch.equal(again, want)
+    for n in range(12):
+        p, slot = int(table[rows[n], pos[n] // 16]), int(pos[n]) % 16
+        assert torch.equal(k[p, :, slot], kc[p, :, slot]) and torch.equal(v[p, :, slot], vc[p, :, slot])
+    assert int((k != 0).any(-1).sum()) <= 12 * 2 and touched.any()
+    # values that are not finite stay in their pair
+    bad = q.clone()
+    bad[0, 0, 3] = float("inf")
+    bad[1, 1, 40] = float("nan")
+    got = kv.append_rotated(bad, k_new, v_new, k, v, table, rows, pos, rope)
+    off = got != want
+    assert {tuple(i) for i in off.nonzero().tolist()} <= {(0, 0, 3), (0, 0, 35), (1, 1, 8), (1, 1, 40)}
+    assert bool(got[1, 1, 40].isnan()) and not bool(got[0, 0, 3].isfinite())
