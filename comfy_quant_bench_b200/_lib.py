@@ -43,6 +43,7 @@ CQ_GEMM_PAIR = 2
 CQ_DT_BF16 = 0
 CQ_DT_F16 = 1
 CQ_DT_FP8_E4M3 = 2
+CQ_DT_F32 = 3
 
 CQ_NORM_SAME = 0
 CQ_NORM_INT8 = 1
@@ -128,6 +129,7 @@ SIGNATURES = {
     "cq_pages_compact": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _vp,
                                 _i64, _vp]),
     "cq_add_rmsnorm": (_int, [_vp, _i64, _vp, _i64, _vp, _int, _i64, _i64, _f32, _int, _i64, _vp, _i64, _vp, _vp, _vp]),
+    "cq_sample": (_int, [_vp, _i64, _int, _i64, _i64, _vp, _vp, _f32, _vp, _i64, _vp, _f32, _vp, _f32, _vp, _vp, _vp]),
     "cq_linear_convrot_w4a4_swiglu": (_int, [_vp, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
 }
 

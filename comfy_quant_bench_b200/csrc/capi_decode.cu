@@ -266,4 +266,22 @@ int cq_kv_append_rotated(const void* q, int64_t q_token_stride, int64_t q_head_s
   return cuda_status(cq::launch_rotate_append(a, static_cast<cudaStream_t>(stream)));
 }
 
+int cq_sample(const void* logits, int64_t ld, int dtype, int64_t rows, int64_t vocab, const float* uniform,
+              const float* temperatures, float temperature, const int32_t* top_ks, int64_t top_k, const float* top_ps,
+              float top_p, const float* min_ps, float min_p, int64_t* tokens, float* logprobs, void* stream) {
+  if (!valid16(dtype) && dtype != CQ_DT_F32) return CQ_ERR_ARG;
+  if (rows < 0 || rows > (1 << 27) || vocab < 1 || vocab > cq::kMaxVocab || ld < vocab || top_k < 0) return CQ_ERR_SHAPE;
+  if (rows == 0) return CQ_OK;
+  if (logits == nullptr || uniform == nullptr || tokens == nullptr) return CQ_ERR_ARG;
+  if (!aligned(logits, dtype == CQ_DT_F32 ? 4 : 2) || !aligned(uniform, 4) || !aligned(temperatures, 4) || !aligned(top_ks, 4) ||
+      !aligned(top_ps, 4) || !aligned(min_ps, 4) || !aligned(tokens, 8) || !aligned(logprobs, 4))
+    return CQ_ERR_ALIGN;
+  if (int dv = check_device()) return dv;
+  static_assert(sizeof(long long) == sizeof(int64_t), "tokens are 64 bits");
+  const cq::SampleArgs a{logits, ld, rows, static_cast<int>(vocab), dtype, uniform, temperatures, top_ks, top_ps, min_ps,
+                         temperature, static_cast<int>(top_k < vocab ? top_k : 0), top_p, min_p,
+                         reinterpret_cast<long long*>(tokens), logprobs};
+  return cuda_status(cq::launch_sample(a, static_cast<cudaStream_t>(stream)));
+}
+
 }  // extern "C"

@@ -11,6 +11,7 @@
 
 #include <optional>
 #include <string>
+#include <variant>
 
 #include "../../include/cq_b200.h"
 
@@ -184,6 +185,56 @@ py::tuple add_rmsnorm(const Tensor& x, Tensor weight, const Opt& residual, doubl
   const Tensor kept = residual ? *h : x;
   if (quant) return py::make_tuple(out, *scale, kept);
   return py::make_tuple(out, kept);
+}
+
+// -------------------------------------------------------------------------------------------------------------
+// sampling
+// -------------------------------------------------------------------------------------------------------------
+
+using Each = std::variant<Tensor, double>;     // one number, or one for each row
+
+// an [n] array of a row parameter, or none and its number
+Opt row_param(const Each& p, int64_t n, at::ScalarType type, const char* name, double least, double most, double& one) {
+  if (const Tensor* t = std::get_if<Tensor>(&p)) {
+    if (t->scalar_type() != type || t->dim() != 1 || t->size(0) != n) refuse(name, " must be a number or ", type, " [", n, "]");
+    return *t;
+  }
+  one = std::get<double>(p);
+  if (!(one >= least && one <= most)) refuse(name, " is out of range: ", std::to_string(one));
+  return std::nullopt;
+}
+
+py::object sample_tokens(const Tensor& logits_arg, const Tensor& uniform_arg, const Each& temperature, const Each& top_k,
+                         const Each& top_p, const Each& min_p, bool return_logprob) {
+  const at::ScalarType dt = logits_arg.scalar_type();
+  if (logits_arg.dim() != 2 || (!half_type(dt) && dt != at::kFloat)) refuse("logits must be bf16, f16 or f32 [rows, vocab]");
+  const int64_t rows = logits_arg.size(0), vocab = logits_arg.size(1);
+  if (vocab < 1 || vocab > 327680) refuse("vocab must be 1 to 327680, got ", vocab);
+  if (uniform_arg.scalar_type() != at::kFloat || uniform_arg.dim() != 1 || uniform_arg.size(0) != rows)
+    refuse("uniform must be f32 [", rows, "]");
+  double t = 0, k = 0, p = 0, m = 0;
+  Opt ts = row_param(temperature, rows, at::kFloat, "temperature", 0, 1e30, t);
+  Opt ks = row_param(top_k, rows, at::kInt, "top_k", 0, 2147483647.0, k);
+  Opt ps = row_param(top_p, rows, at::kFloat, "top_p", 0, 1, p);
+  Opt ms = row_param(min_p, rows, at::kFloat, "min_p", 0, 1, m);
+  const int index = device_of(logits_arg, uniform_arg, ts, ks, ps, ms);
+  const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(index));
+  Tensor logits = logits_arg;
+  if ((vocab > 1 && logits.stride(1) != 1) || (rows > 1 && logits.stride(0) < vocab)) logits = logits.clone(at::MemoryFormat::Contiguous);
+  const Tensor uniform = uniform_arg.contiguous();
+  for (Opt* o : {&ts, &ks, &ps, &ms})
+    if (*o) *o = (*o)->contiguous();
+  const Tensor tokens = at::empty({rows}, logits.options().dtype(at::kLong));
+  Opt logprob;
+  if (return_logprob) logprob = at::empty({rows}, logits.options().dtype(at::kFloat));
+  check_status("cq_sample",
+               cq_sample(logits.data_ptr(), rows > 1 ? logits.stride(0) : vocab, dt == at::kFloat ? CQ_DT_F32 : dtype_code(dt),
+                         rows, vocab, uniform.data_ptr<float>(), ptr<const float>(ts), static_cast<float>(t),
+                         ptr<const int32_t>(ks), static_cast<int64_t>(k), ptr<const float>(ps), static_cast<float>(p),
+                         ptr<const float>(ms), static_cast<float>(m), tokens.data_ptr<int64_t>(), ptr<float>(logprob),
+                         stream_of(index)));
+  if (return_logprob) return py::make_tuple(tokens, *logprob);
+  return py::cast(tokens);
 }
 
 // -------------------------------------------------------------------------------------------------------------
@@ -471,6 +522,7 @@ py::tuple compact_pages(const Tensor& table_arg, const Tensor& refs, const Tenso
 PYBIND11_MODULE(_decode, m) {
   m.def("w4a16_linear", &w4a16_linear);
   m.def("add_rmsnorm", &add_rmsnorm);
+  m.def("sample_tokens", &sample_tokens);
   m.def("paged_attention", &paged_attention);
   m.def("append_kv", &append_kv);
   m.def("append_rotated", &append_rotated);

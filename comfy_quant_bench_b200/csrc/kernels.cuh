@@ -264,4 +264,23 @@ struct RotateArgs {
 };
 cudaError_t launch_rotate_append(const RotateArgs& a, cudaStream_t st);
 
+// the next token of each row of logits
+constexpr int kMaxVocab = 327680;             // a row's eighth in f32 fits a CTA's shared memory; sums of 2^44 fit 64 bits
+struct SampleArgs {
+  const void* logits;         // [rows, vocab], rows ld elements apart
+  int64_t ld, rows;
+  int vocab, dtype;
+  const float* uniform;       // [rows]
+  const float* temperatures;  // [rows] or null: temperature; the others alike
+  const int* top_ks;
+  const float* top_ps;
+  const float* min_ps;
+  float temperature;
+  int top_k;
+  float top_p, min_p;
+  long long* tokens;          // [rows]
+  float* logprobs;            // [rows] or null
+};
+cudaError_t launch_sample(const SampleArgs& a, cudaStream_t st);
+
 }  // namespace cq

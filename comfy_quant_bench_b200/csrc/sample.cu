@@ -1,0 +1,590 @@
+// The next token of each row from its logits and one given uniform number: temperature, top-k, top-p, min-p.
+//
+//   weight_i = exp((l_i - max) / T); the first k tokens in the order (logit descending, index ascending); of those the
+//   shortest head whose sum reaches p times theirs; of those the ones with weight >= min_p; then the first token, in the
+//   order of the indexes, whose running sum exceeds u times the sum.
+//
+// The choice has to be the one of exact arithmetic, so weights are integers, round(2^44 weight): sums are exact, in any
+// order, and equal calls give equal bits.  2^x comes in 64 bits from a table of 2^(j/64) and a polynomial of degree four in
+// the rest, |rest| <= 1/128 (Taylor, 4e-14).  A token whose weight rounds to 0 can neither be chosen nor count.
+//
+// A cluster of CTAs takes a row and keeps it in shared memory: one read of the logits.  A cut (of top-k, of top-p) is an
+// element's composite, its logit's order in the high half and its index, reversed, in the low: what lies at or above it
+// stays.  To find one, tokens are counted into bins by max - logit, the sums of all bins above the border's are exact, and
+// the border's few tokens are ranked one against another; a bin with more of them (equal logits) is halved instead.
+#include "decode_common.cuh"
+
+namespace cq {
+
+namespace samp {
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kBins = 2048;
+constexpr int kList = 1024;                    // tokens of a border bin that are ranked; more are halved
+constexpr int kMaxCluster = 8;
+constexpr int kFixed = 44;                     // fractional bits of a weight
+constexpr float kReach = 31.2f;                // weights below e^-31.2 < 2^-45 round to 0
+using u64 = unsigned long long;
+
+struct Shared {
+  union {
+    u64 wsum[kBins];                           // weights of a bin near top-p's border
+    struct {
+      u64 list[kList], weight[kList];          // a border bin's tokens
+    };
+  };
+  u64 warp_sums[2][kWarps];
+  u64 slots[2][kMaxCluster][2];                // what the cluster's CTAs tell one another
+  u64 best[kWarps];
+  double power[64];                            // 2^(j / 64)
+  uint32_t hist[kBins];                        // this CTA's
+  uint32_t total[kBins];                       // the row's
+  uint32_t warp_counts[kWarps];
+  float extremes[2][kMaxCluster];
+  int list_n;
+  int found[4];
+  u64 found_sum;
+};
+}  // namespace samp
+
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void st_cluster_u64(uint32_t addr, unsigned long long v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
+__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ unsigned long long ld_cluster_u64(uint32_t addr) {
+  unsigned long long v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// A logit's place among all: larger for larger logits; -0 and 0 alike
+__device__ __forceinline__ uint32_t logit_order(float l) {
+  const uint32_t b = __float_as_uint(l + 0.0f);
+  return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
+}
+
+template <int TYPE>                            // CQ_DT_BF16, CQ_DT_F16, CQ_DT_F32
+struct Sampler {
+  using u64 = samp::u64;
+  static constexpr int kSize = TYPE == CQ_DT_F32 ? 4 : 2;
+  samp::Shared& s;
+  const uint8_t* data;                         // this CTA's elements
+  int rank, ranks, tid, lane, warp;
+  int first, span;                             // this warp's elements: [first, first + span)
+  int index0;                                  // row index of element 0; may be negative (before the row's first)
+  int vocab, count;                            // count: elements held
+  float top, range, inv_width;
+  double by;                                   // log2(e) / T
+  int parity;
+
+  __device__ __forceinline__ float logit(int e) const {
+    float l;
+    if constexpr (TYPE == CQ_DT_F32) l = reinterpret_cast<const float*>(data)[e];
+    else l = widen16<TYPE == CQ_DT_F16>(reinterpret_cast<const uint16_t*>(data)[e]).x;
+    return l;
+  }
+  // the bin of a logit, -1 where its weight is 0 (or it is NaN)
+  __device__ __forceinline__ int bin(float l) const {
+    const float d = l == top ? 0.0f : top - l;
+    if (!(d <= range)) return -1;
+    return min(max(static_cast<int>(d * inv_width), 0), samp::kBins - 1);
+  }
+  __device__ __forceinline__ double exponent(float l) const {
+    return l == top ? 0.0 : (static_cast<double>(l) - static_cast<double>(top)) * by;
+  }
+  __device__ __forceinline__ u64 weight_of(double y) const {          // round(2^44 2^y), y <= 0
+    if (!(y > -46.0)) return 0;
+    const double magic = 6755399441055744.0;                          // 1.5 * 2^52: the sum's low bits are the integer
+    const double t = fma(y, 64.0, magic);
+    const int k = static_cast<int>(__double2loint(t));
+    const double f = fma(t - magic, -1.0 / 64.0, y);
+    constexpr double l2 = 0.693147180559945309417;
+    double p = fma(f, l2 * l2 * l2 * l2 / 24.0, l2 * l2 * l2 / 6.0);
+    p = fma(f, p, l2 * l2 / 2.0);
+    p = fma(f, p, l2);
+    p = fma(f, p, 1.0) * s.power[k & 63];
+    const double w = __hiloint2double(__double2hiint(p) + ((samp::kFixed + (k >> 6)) << 20), __double2loint(p));
+    return static_cast<u64>(__double_as_longlong(w + 4503599627370496.0)) & ((1ull << 52) - 1);   // 2^52: the sum rounds
+  }
+  __device__ __forceinline__ u64 composite(float l, int e) const {
+    return static_cast<u64>(logit_order(l)) << 32 | (0xffffffffu - static_cast<uint32_t>(index0 + e));
+  }
+  __device__ __forceinline__ uint32_t there(const void* mine, int r) const { return mapa_shared(smem_u32(mine), r); }
+
+  // the sum over the CTA's threads, in every thread
+  __device__ __forceinline__ u64 block_sum(u64 v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    if (lane == 0) s.warp_sums[0][warp] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int w = 0; w < samp::kWarps; ++w) v += s.warp_sums[0][w];
+    return v;
+  }
+  // two values of each CTA, in every CTA, by rank, in s.slots[parity] after the call (until the call after the next)
+  __device__ __forceinline__ const u64 (*exchange(u64 a, u64 b))[2] {
+    parity ^= 1;
+    if (tid < ranks) {
+      const uint32_t to = there(&s.slots[parity][rank][0], tid);
+      st_cluster_u64(to, a);
+      st_cluster_u64(to + 8, b);
+    }
+    cluster_sync_all();
+    return s.slots[parity];
+  }
+  __device__ __forceinline__ u64 cluster_sum(u64 v) {
+    const u64(*all)[2] = exchange(block_sum(v), 0);
+    u64 sum = 0;
+    for (int r = 0; r < ranks; ++r) sum += all[r][0];
+    return sum;
+  }
+
+  // The elements of bin `b` that lie at or above `from`: the composite of the last one that has to stay, so that what is
+  // above the bin (`above`) and what stays of it reach `target`.  WEIGHTS: measured by weights, else counted.
+  template <bool WEIGHTS>
+  __device__ u64 cut_in_bin(int b, u64 from, u64 above, u64 target, u64 n) {
+    if (n <= samp::kList) {
+      if (tid == 0) s.list_n = 0;
+      cluster_sync_all();                                              // lists are empty, and what they held is read
+      for (int e = first + lane; e < first + span; e += 32) {
+        const float l = logit(e);
+        if (bin(l) != b) continue;
+        const u64 c = composite(l, e);
+        if (c < from) continue;
+        const uint32_t at = there(&s.list_n, 0);
+        int place;
+        asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(place) : "r"(at) : "memory");
+        const u64 w = WEIGHTS ? weight_of(exponent(l)) : 1;
+        for (int r = 0; r < ranks; ++r) {
+          st_cluster_u64(there(&s.list[place], r), c);
+          st_cluster_u64(there(&s.weight[place], r), w);
+        }
+      }
+      cluster_sync_all();
+      const int held = static_cast<int>(ld_cluster_u32(there(&s.list_n, 0)));
+      u64 best = 0;
+      for (int i = tid; i < held; i += samp::kThreads) {
+        const u64 c = s.list[i];
+        u64 sum = above;
+        for (int j = 0; j < held; ++j) sum += s.list[j] >= c ? s.weight[j] : 0;
+        if (sum >= target && c > best) best = c;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const u64 other = __shfl_xor_sync(0xffffffffu, best, o);
+        best = other > best ? other : best;
+      }
+      if (lane == 0) s.best[warp] = best;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < samp::kWarps; ++w) best = s.best[w] > best ? s.best[w] : best;
+      __syncthreads();
+      return best;
+    }
+    // halving: the largest c whose elements at or above it reach the target
+    u64 lo = from, hi = ~0ull;
+    while (lo < hi) {
+      const u64 mid = lo + (hi - lo) / 2 + 1;
+      u64 sum = 0;
+      for (int e = first + lane; e < first + span; e += 32) {
+        const float l = logit(e);
+        if (bin(l) == b && composite(l, e) >= mid) sum += WEIGHTS ? weight_of(exponent(l)) : 1;
+      }
+      if (above + cluster_sum(sum) >= target) lo = mid;
+      else hi = mid - 1;
+    }
+    return lo;
+  }
+};
+
+template <int TYPE>
+__global__ void __launch_bounds__(samp::kThreads, 2) sample_kernel(const SampleArgs a, const int ranks) {
+  using S = Sampler<TYPE>;
+  using u64 = samp::u64;
+  constexpr int kSize = S::kSize, kPer = 16 / kSize;                   // elements of a 16-byte word
+  extern __shared__ __align__(16) uint8_t smem[];
+  samp::Shared& sh = *reinterpret_cast<samp::Shared*>(smem);
+  uint8_t* data = smem + (sizeof(samp::Shared) + 15) / 16 * 16;
+  const int tid = threadIdx.x, rank = ranks > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int64_t row = blockIdx.x / ranks;
+  grid_dep_launch();
+  if (tid < 64) sh.power[tid] = exp2(tid / 64.0);
+  for (int i = tid; i < samp::kBins; i += samp::kThreads) sh.hist[i] = 0;
+  grid_dep_wait();
+
+  // ---- this CTA's share of the row's 16-byte words; elements outside the row become -inf ----
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(a.logits) + row * a.ld * kSize, end = begin + static_cast<int64_t>(a.vocab) * kSize;
+  const uintptr_t word0 = begin >> 4;
+  const int words = static_cast<int>((end + 15 >> 4) - word0), each = (words + ranks - 1) / ranks;
+  const int w0 = min(words, rank * each), w1 = min(words, w0 + each);
+  float most = -INFINITY, least = INFINITY;
+  for (int w = w0 + tid; w < w1; w += samp::kThreads) {
+    const uintptr_t at = word0 + w << 4;
+    uint4 v;
+    uint32_t* u = &v.x;
+    if (at >= begin && at + 16 <= end) {
+      v = *reinterpret_cast<const uint4*>(at);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uintptr_t p = at + 4 * j;
+        if constexpr (kSize == 4) {
+          u[j] = p >= begin && p + 4 <= end ? *reinterpret_cast<const uint32_t*>(p) : 0xff800000u;
+        } else {
+          const uint32_t none = TYPE == CQ_DT_F16 ? 0xfc00u : 0xff80u;
+          const uint32_t lo = p >= begin && p + 2 <= end ? *reinterpret_cast<const uint16_t*>(p) : none;
+          const uint32_t hi = p + 2 >= begin && p + 4 <= end ? *reinterpret_cast<const uint16_t*>(p + 2) : none;
+          u[j] = lo | hi << 16;
+        }
+      }
+    }
+    *reinterpret_cast<uint4*>(data + (w - w0) * 16) = v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (kSize == 4) {
+        const float l = __uint_as_float(u[j]);
+        most = fmaxf(most, l);                                         // NaN is passed over
+        if (l > -INFINITY) least = fminf(least, l);
+      } else {
+        const float2 l = widen16<TYPE == CQ_DT_F16>(u[j]);
+        most = fmaxf(most, fmaxf(l.x, l.y));
+        if (l.x > -INFINITY) least = fminf(least, l.x);
+        if (l.y > -INFINITY) least = fminf(least, l.y);
+      }
+    }
+  }
+  S s{sh, data, rank, ranks, tid, tid & 31, tid >> 5};
+  s.count = (w1 - w0) * kPer;
+  s.vocab = a.vocab;
+  s.index0 = static_cast<int>((static_cast<int64_t>(word0 + w0 << 4) - static_cast<int64_t>(begin)) / kSize);
+  s.parity = 0;
+  const int per_warp = ((s.count + samp::kWarps - 1) / samp::kWarps + 31) & ~31;
+  s.first = min(s.count, s.warp * per_warp);
+  s.span = min(s.count - s.first, per_warp);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
+  }
+  float* box = reinterpret_cast<float*>(sh.warp_sums);                 // [2][kWarps]
+  if (s.lane == 0) {
+    box[s.warp] = most;
+    box[samp::kWarps + s.warp] = least;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < samp::kWarps; ++w) {
+    most = fmaxf(most, box[w]);
+    least = fminf(least, box[samp::kWarps + w]);
+  }
+  __syncthreads();
+  {
+    const u64(*all)[2] = s.exchange(__float_as_uint(most), __float_as_uint(least));
+    for (int r = 0; r < ranks; ++r) {
+      most = fmaxf(most, __uint_as_float(static_cast<uint32_t>(all[r][0])));
+      least = fminf(least, __uint_as_float(static_cast<uint32_t>(all[r][1])));
+    }
+  }
+  const float temperature = a.temperatures != nullptr ? a.temperatures[row] : a.temperature;
+  const int top_k = a.top_ks != nullptr ? a.top_ks[row] : a.top_k;
+  const float top_p = a.top_ps != nullptr ? a.top_ps[row] : a.top_p;
+  const float min_p = a.min_ps != nullptr ? a.min_ps[row] : a.min_p;
+  s.top = most;
+  if (most == -INFINITY) {                                             // nothing to choose from
+    if (rank == 0 && tid == 0) {
+      a.tokens[row] = -1;
+      if (a.logprobs != nullptr) a.logprobs[row] = -INFINITY;
+    }
+    return;
+  }
+  if (!(temperature > 0.0f)) {                                         // the likeliest, lowest index first
+    int at = 0x7fffffff;
+    for (int e = s.first + s.lane; e < s.first + s.span; e += 32)
+      if (s.logit(e) == most) at = min(at, s.index0 + e);
+    at = __reduce_min_sync(0xffffffffu, at);
+    if (s.lane == 0) sh.warp_counts[s.warp] = at;
+    __syncthreads();
+    for (int w = 0; w < samp::kWarps; ++w) at = min(at, static_cast<int>(sh.warp_counts[w]));
+    const u64(*all)[2] = s.exchange(at, 0);
+    for (int r = 0; r < ranks; ++r) at = min(at, static_cast<int>(all[r][0]));
+    if (rank == 0 && tid == 0) {
+      a.tokens[row] = at;
+      if (a.logprobs != nullptr) a.logprobs[row] = 0.0f;
+    }
+    return;
+  }
+  s.by = 1.4426950408889634074 / static_cast<double>(temperature);
+  s.range = fminf(fminf(samp::kReach * temperature, most - least), 3e38f);
+  s.inv_width = s.range > 0.0f ? samp::kBins / s.range : 0.0f;
+  const bool cut_k = top_k > 0 && top_k < a.vocab, cut_p = top_p < 1.0f;
+
+  u64 cut = 0;                                                         // what lies at or above it stays
+  if (cut_k || cut_p) {
+    // ---- tokens by bins, over the whole row in every CTA ----
+    for (int e = s.first + s.lane; e < s.first + s.span; e += 32) {
+      const int b = s.bin(s.logit(e));
+      if (b >= 0) atomicAdd(&sh.hist[b], 1u);
+    }
+    cluster_sync_all();
+    const int per = samp::kBins / ranks;
+    for (int i = rank * per + tid; i < (rank + 1) * per; i += samp::kThreads) {
+      uint32_t sum = 0;
+      for (int r = 0; r < ranks; ++r) sum += ld_cluster_u32(s.there(&sh.hist[i], r));
+      for (int r = 0; r < ranks; ++r) st_cluster_u32(s.there(&sh.total[i], r), sum);
+    }
+    cluster_sync_all();
+  }
+  constexpr int kEach = samp::kBins / samp::kThreads;                  // bins of a thread in a scan
+  if (cut_k) {
+    // ---- the bin in which the k-th token lies ----
+    uint32_t mine = 0;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) mine += sh.total[tid * kEach + j];
+    uint32_t before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t u = __shfl_up_sync(0xffffffffu, before, o);
+      if (s.lane >= o) before += u;
+    }
+    if (s.lane == 31) sh.warp_counts[s.warp] = before;
+    if (tid == 0) sh.found[0] = -1;
+    __syncthreads();
+    before -= mine;
+    for (int w = 0; w < s.warp; ++w) before += sh.warp_counts[w];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const uint32_t n = sh.total[tid * kEach + j];
+      if (before < static_cast<uint32_t>(top_k) && before + n >= static_cast<uint32_t>(top_k)) {
+        sh.found[0] = tid * kEach + j;
+        sh.found[1] = static_cast<int>(before);
+      }
+      before += n;
+    }
+    __syncthreads();
+    const int b = sh.found[0];
+    if (b >= 0) {
+      const int above = sh.found[1];
+      cut = s.template cut_in_bin<false>(b, 0, above, top_k, sh.total[b]);
+    }
+  }
+  if (cut_p) {
+    // ---- bounds of the sums from the counts: a token of bin b weighs 2^-(b + 1) width .. 2^-b width; the border lies in a
+    // bin that the bounds allow; sums of the bins before are exact, and those of the allowed bins each ----
+    // top-k's cut ends the bins; its own one is counted whole in the upper bounds and not at all in the lower
+    const double step = s.inv_width > 0.0f ? s.by / static_cast<double>(s.inv_width) : 0.0;
+    const float ratio = static_cast<float>(exp2(step * 1.001));        // of a bin's bounds (1.001: fp32 bins)
+    const float stepf = static_cast<float>(step);
+    const int last = cut != 0 ? sh.found[0] : samp::kBins - 1;         // no token below this bin
+    float mine = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int b = tid * kEach + j;
+      mine += b <= last ? sh.total[b] * exp2f(-stepf * b) : 0.0f;      // upper bound
+    }
+    float before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const float u = __shfl_up_sync(0xffffffffu, before, o);
+      if (s.lane >= o) before += u;
+    }
+    float* fbox = reinterpret_cast<float*>(sh.warp_counts);
+    __syncthreads();
+    if (s.lane == 31) fbox[s.warp] = before;
+    if (tid == 0) {
+      sh.found[2] = samp::kBins;
+      sh.found[3] = -1;
+    }
+    __syncthreads();
+    before -= mine;
+    float whole = 0.0f;
+    for (int w = 0; w < samp::kWarps; ++w) {
+      if (w < s.warp) before += fbox[w];
+      whole += fbox[w];
+    }
+    // exact sum before a bin in [before / ratio, before], the row's in [whole / ratio - its border bin's, whole]
+    const float border = cut != 0 ? sh.total[last] * exp2f(-stepf * last) : 0.0f;
+    const float p = fmaxf(top_p, 0.0f), slack = 1.0f + 1e-3f;
+    const float least_target = p * fmaxf(whole - border, 0.0f) / (ratio * slack), most_target = p * whole * slack;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int b = tid * kEach + j;
+      const float up = b <= last ? sh.total[b] * exp2f(-stepf * b) : 0.0f;
+      // bin b can hold the border unless all of it is surely kept, or all of it surely dropped
+      if (up > 0.0f && (before + up) * slack >= least_target && before / (ratio * slack) <= most_target) {
+        atomicMin(&sh.found[2], b);
+        atomicMax(&sh.found[3], b);
+      }
+      before += up;
+    }
+    for (int i = tid; i < samp::kBins; i += samp::kThreads) sh.wsum[i] = 0;
+    __syncthreads();
+    const int lo = sh.found[2], hi = sh.found[3];
+    u64 above = 0, sum = 0;
+    for (int e = s.first + s.lane; e < s.first + s.span; e += 32) {
+      const float l = s.logit(e);
+      const int b = s.bin(l);
+      if (b < 0 || s.composite(l, e) < cut) continue;
+      const u64 w = s.weight_of(s.exponent(l));
+      sum += w;
+      if (b < lo) above += w;
+      else if (b <= hi) atomicAdd(&sh.wsum[b], w);
+    }
+    const u64 my_sum = s.block_sum(sum), my_above = s.block_sum(above);
+    const u64(*all)[2] = s.exchange(my_sum, my_above);
+    u64 total = 0;
+    above = 0;
+    for (int r = 0; r < ranks; ++r) {
+      total += all[r][0];
+      above += all[r][1];
+    }
+    // the allowed bins' sums over the cluster: every CTA adds them all up (they are few)
+    if (tid == 0) sh.found_sum = ~0ull;
+    const double wanted = ceil(static_cast<double>(p) * static_cast<double>(total));
+    u64 target = wanted >= 9.2e18 ? total : static_cast<u64>(wanted);
+    target = target < 1 ? 1 : target > total ? total : target;
+    __syncthreads();
+    // thread i takes the allowed bins in runs, so that a scan gives the sums before each
+    const int bins = hi - lo + 1, run = (bins + samp::kThreads - 1) / samp::kThreads;
+    u64 part = 0;
+    for (int j = 0; j < run; ++j) {
+      const int b = lo + tid * run + j;
+      if (b <= hi) {
+        u64 w = 0;
+        for (int r = 0; r < ranks; ++r) w += ld_cluster_u64(s.there(&sh.wsum[b], r));
+        part += w;
+      }
+    }
+    u64 incl = part;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 u = __shfl_up_sync(0xffffffffu, incl, o);
+      if (s.lane >= o) incl += u;
+    }
+    if (s.lane == 31) sh.warp_sums[1][s.warp] = incl;
+    __syncthreads();
+    u64 run_sum = above + incl - part;
+    for (int w = 0; w < s.warp; ++w) run_sum += sh.warp_sums[1][w];
+    for (int j = 0; j < run; ++j) {
+      const int b = lo + tid * run + j;
+      if (b <= hi) {
+        u64 w = 0;
+        for (int r = 0; r < ranks; ++r) w += ld_cluster_u64(s.there(&sh.wsum[b], r));
+        if (run_sum < target && run_sum + w >= target) {
+          sh.found[2] = b;
+          sh.found_sum = run_sum;
+        }
+        run_sum += w;
+      }
+    }
+    __syncthreads();
+    const int b = sh.found[2];
+    const u64 sum_above = sh.found_sum;
+    cluster_sync_all();                                                // everyone has read the sums
+    if (sum_above != ~0ull) cut = s.template cut_in_bin<true>(b, cut, sum_above, target, sh.total[b]);
+  }
+
+  // ---- what stays: sums by warps, then the token ----
+  const double floor_y = min_p > 0.0f ? log2(static_cast<double>(fminf(min_p, 1.0f))) : -100.0;
+  auto kept = [&](int e, double& y) {
+    const float l = s.logit(e);
+    if (s.bin(l) < 0 || s.composite(l, e) < cut) return static_cast<u64>(0);
+    y = s.exponent(l);
+    return y >= floor_y ? s.weight_of(y) : 0;
+  };
+  u64 sum = 0;
+  double y = 0.0;
+  for (int e = s.first + s.lane; e < s.first + s.span; e += 32) sum += kept(e, y);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  __syncthreads();
+  if (s.lane == 0) sh.warp_sums[0][s.warp] = sum;
+  __syncthreads();
+  u64 mine = 0, before = 0;
+  for (int w = 0; w < samp::kWarps; ++w) {
+    if (w < s.warp) before += sh.warp_sums[0][w];
+    mine += sh.warp_sums[0][w];
+  }
+  const u64(*all)[2] = s.exchange(mine, 0);
+  u64 total = 0;
+  for (int r = 0; r < ranks; ++r) {
+    if (r < rank) before += all[r][0];
+    total += all[r][0];
+  }
+  const double u = static_cast<double>(a.uniform[row]);
+  const double at = u > 0.0 ? u * static_cast<double>(total) : 0.0;    // NaN: the first
+  u64 goal = at >= 9.2e18 ? total - 1 : static_cast<u64>(at);
+  goal = goal > total - 1 ? total - 1 : goal;
+  if (goal < before || goal >= before + sum) return;                   // another warp's
+  for (int e0 = s.first; e0 < s.first + s.span; e0 += 32) {
+    const int e = e0 + s.lane;
+    const u64 w = e < s.first + s.span ? kept(e, y) : 0;
+    u64 incl = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (s.lane >= o) incl += v;
+    }
+    const uint32_t over = __ballot_sync(0xffffffffu, before + incl > goal);
+    if (over != 0) {
+      if (s.lane == __ffs(over) - 1) {
+        a.tokens[row] = s.index0 + e;
+        if (a.logprobs != nullptr)
+          a.logprobs[row] = static_cast<float>(y * 0.693147180559945309417 - log(static_cast<double>(total) * 5.6843418860808015e-14));   // 2^-44
+      }
+      return;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+}
+
+namespace {
+template <int TYPE>
+cudaError_t run_sample(const SampleArgs& a, cudaStream_t st) {
+  constexpr int kSize = TYPE == CQ_DT_F32 ? 4 : 2;
+  // a CTA for each 2048 tokens, up to a cluster of eight
+  int ranks = 1;
+  while (ranks < samp::kMaxCluster && ranks * 2048 < a.vocab) ranks *= 2;
+  const int words = (a.vocab * kSize + 15) / 16 + 1;
+  const int bytes = static_cast<int>((sizeof(samp::Shared) + 15) / 16 * 16) + (words + ranks - 1) / ranks * 16;
+  static unsigned long long devices = 0;
+  auto kern = sample_kernel<TYPE>;
+  const cudaError_t e = allow_shared(kern, 227 * 1024, devices);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(ranks);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(static_cast<unsigned>(a.rows * ranks));
+  cfg.blockDim = dim3(samp::kThreads);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kern, a, ranks);
+}
+}  // namespace
+
+cudaError_t launch_sample(const SampleArgs& a, cudaStream_t st) {
+  if (a.rows == 0) return cudaSuccess;
+  switch (a.dtype) {
+    case CQ_DT_BF16: return run_sample<CQ_DT_BF16>(a, st);
+    case CQ_DT_F16: return run_sample<CQ_DT_F16>(a, st);
+    default: return run_sample<CQ_DT_F32>(a, st);
+  }
+}
+
+}  // namespace cq

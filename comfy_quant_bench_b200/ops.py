@@ -792,6 +792,22 @@ def add_rmsnorm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | 
     return _lib.decode().add_rmsnorm(x, weight, residual, eps, quant, group_size, out_residual)
 
 
+def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                  return_logprob: bool = False):
+    """The next token of each row of logits [rows, vocab] (bf16, f16 or f32; vocab up to 327680) from one given number per
+    row, ``uniform`` f32 [rows] in [0, 1): int64 [rows].
+
+    With weights exp((l - max) / temperature): the first ``top_k`` tokens, by logit and then by index, stay (0: all); of
+    those the shortest head whose sum reaches ``top_p`` times theirs; of those the ones with a weight of at least ``min_p``
+    (of the largest).  The token is the first, by index, whose running sum exceeds uniform times the sum of what stays.
+    Each of the four is a number, or a tensor [rows] (f32; top_k int32).  Temperature 0: the likeliest, lowest index first.
+
+    Weights are held to 2^-45 of the largest and added without rounding, so equal calls give equal tokens.  NaN logits
+    count as -inf; tokens at +inf share the row among them.  A row without a logit above -inf gives -1.  With
+    ``return_logprob`` also f32 [rows]: the log of the token's share among those that stay."""
+    return _lib.decode().sample_tokens(logits, uniform, temperature, top_k, top_p, min_p, return_logprob)
+
+
 def _out_ptrs(outs, rows: int, ldo: int):
     ptrs = []
     for o in outs:

@@ -463,7 +463,8 @@ CQ_API int cq_qkv_rmsnorm_rope_layout(const void* y, int64_t S, int H, int D, co
 typedef enum {
   CQ_DT_BF16 = 0,
   CQ_DT_F16 = 1,
-  CQ_DT_FP8_E4M3 = 2  /* caches only: a value is its 8-bit code times the scale of its key-value head */
+  CQ_DT_FP8_E4M3 = 2, /* caches only: a value is its 8-bit code times the scale of its key-value head */
+  CQ_DT_F32 = 3       /* logits only */
 } cq_dtype;
 
 /*
@@ -607,6 +608,22 @@ enum cq_norm_out { CQ_NORM_SAME = 0, CQ_NORM_INT8 = 1, CQ_NORM_FP8 = 2 };
 CQ_API int cq_add_rmsnorm(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int dtype,
                           int64_t rows, int64_t width, float eps, int out_kind, int64_t group, void* h_out, int64_t ldh,
                           void* out, float* scale, void* stream);
+
+/*
+ * cq_sample: the next token of each row of logits [rows, vocab] (bf16, f16 or f32, rows ld elements apart) from one given
+ * number u = uniform[row]: with weights exp((l_i - max) / T), the first top_k tokens in the order (logit descending, index
+ * ascending) stay (0: all), of those the shortest head whose sum reaches top_p times theirs (1: all; the first always), of
+ * those the ones with weight >= min_p; the token is the first, by index, whose running sum exceeds u times the sum (u at or
+ * past 1: the last that stays; NaN: the first).  T not above 0: the likeliest token, lowest index first.  Weights are held
+ * to 2^-45 of the largest, sums of them exact.  NaN logits count as -inf; where one logit or more is +inf, those share the
+ * row.  tokens int64 [rows]: -1 where no logit is above -inf; logprobs f32 [rows] or NULL: the log of the token's share
+ * among those that stay (-inf with -1).
+ * Each of temperature, top_k, top_p, min_p is one number, or an array [rows] (f32; top_k int32) where that is not NULL.
+ * vocab 1 to 327680.
+ */
+CQ_API int cq_sample(const void* logits, int64_t ld, int dtype, int64_t rows, int64_t vocab, const float* uniform,
+                     const float* temperatures, float temperature, const int32_t* top_ks, int64_t top_k, const float* top_ps,
+                     float top_p, const float* min_ps, float min_p, int64_t* tokens, float* logprobs, void* stream);
 
 #ifdef __cplusplus
 }

@@ -311,3 +311,161 @@ def test_rotated_append_strides_special_values_and_streams(kv):
     off = got != want
     assert {tuple(i) for i in off.nonzero().tolist()} <= {(0, 0, 3), (0, 0, 35), (1, 1, 8), (1, 1, 40)}
     assert bool(got[1, 1, 40].isnan()) and not bool(got[0, 0, 3].isfinite())
+
+
+# ----------------------------------------------------------------------------------------------------------
+# sampling: tokens are compared exactly.  Weights are rounded at 2^-45 of the largest, so the shares of a test's choice are
+# off by n 2^-45 at most; numbers that near to a border (or shares that near to top-p's or min-p's) are not drawn but
+# built to be exact.  log of a share: 2^-24 relative, and n 2^-44 of the share.
+# ----------------------------------------------------------------------------------------------------------
+
+def _chosen(x, u, t, k, p, m):
+    """One row in 64 bits: (token, logprob)."""
+    x = x.double()
+    x = torch.where(x.isnan(), float("-inf"), x)
+    top = x.max()
+    if top == float("-inf"):
+        return -1, float("-inf")
+    if not t > 0:
+        return int((x == top).nonzero()[0]), 0.0
+    z = torch.where(x == top, 0.0, (x - top) / t)
+    order = torch.sort(x, descending=True, stable=True).indices
+    w = z.exp()[order]
+    w = w[: k if k else len(w)]
+    if p < 1:
+        before = w.cumsum(0) - w
+        w = w[: max(1, int((before < p * w.sum()).sum()))]
+    w = w[w >= m]
+    ids, place = torch.sort(order[: len(w)])
+    sums = w[place].cumsum(0)
+    live = (w[place] > 0).nonzero()
+    at = min(int((sums <= u * sums[-1]).sum()), int(live[-1]))
+    return int(ids[at]), float(z[ids[at]] - sums[-1].log())
+
+
+def _sample_holds(ops, x, u, t=1.0, k=0, p=1.0, m=0.0):
+    tokens, logs = ops.sample_tokens(x, u, temperature=t, top_k=k, top_p=p, min_p=m, return_logprob=True)
+    assert tokens.dtype == torch.int64 and logs.dtype == torch.float32
+    row = lambda v, r, f: float(v[r]) if isinstance(v, torch.Tensor) else float(torch.tensor(v, dtype=torch.float32)) if f else v  # noqa: E731
+    for r in range(len(x)):
+        want, log = _chosen(x[r], float(u[r]), row(t, r, True), int(row(k, r, False)), row(p, r, True), row(m, r, True))
+        assert int(tokens[r]) == want, (r, int(tokens[r]), want)
+        if want < 0 or math.isinf(log):
+            assert float(logs[r]) == log
+        else:
+            assert abs(float(logs[r]) - log) <= 2.0 ** -23 * abs(log) + x.shape[1] * 2.0 ** -44 / math.exp(log)
+    return tokens
+
+
+def _logits(rows, vocab, dtype, seed=0, scale=2.5):
+    g = _gen(seed + vocab)
+    x = scale * torch.randn(rows, vocab, generator=g, device="cuda")
+    x[:, ::5] = float("-inf")
+    x[:, 0] = 0.5
+    return x.to(dtype), torch.rand(rows, generator=g, device="cuda")
+
+
+@pytest.mark.parametrize("dtype", [*BOTH, torch.float32])
+@pytest.mark.parametrize("vocab", [1, 2, 7, 33, 500, 2047, 2049, 4100, 32000, 50257, 131073])
+@pytest.mark.parametrize("k,p,m", [(0, 1.0, 0.0), (0, 0.9, 0.0), (40, 1.0, 0.0), (50, 0.8, 0.05), (0, 0.3, 0.2), (1, 0.5, 0.0),
+                                   (0, 0.999, 0.0), (3000, 0.97, 0.0), (0, 1.0, 0.1), (0, 0.0, 0.0), (7, 1.0, 1.0)])
+def test_sample(ops, vocab, dtype, k, p, m):
+    x, u = _logits(6, vocab, dtype, seed=k)
+    _sample_holds(ops, x, u, 0.8, k, p, m)
+
+
+@pytest.mark.parametrize("scale,t", [(0.01, 1.0), (30.0, 1.0), (1.0, 0.01), (1.0, 50.0), (1.0, 1e6), (1e4, 1e4)])
+def test_sample_flat_and_peaked(ops, scale, t):
+    for vocab in (300, 40000):
+        x, u = _logits(8, vocab, torch.float32, scale=scale)
+        for k, p in ((0, 1.0), (0, 0.9), (100, 0.7), (0, 0.5)):
+            _sample_holds(ops, x, u, t, k, p, 0.0)
+
+
+@pytest.mark.parametrize("vocab", [64, 5000, 100001])
+def test_sample_equal_logits(ops, vocab):
+    """More equal logits than a border is ranked for: lowest indexes first; every border exact."""
+    x = torch.full((5, vocab), -3.0, device="cuda")
+    u = torch.tensor([0.0, 0.25, 0.5, 0.75, 1 - 2.0 ** -24], device="cuda")
+    for k, p in ((0, 1.0), (0, 0.5), (vocab // 2, 1.0), (vocab // 4, 0.5), (17, 1.0), (0, 0.25)):
+        for t in (1.0, 0.3):
+            _sample_holds(ops, x, u, t, k, p, 0.0)
+    x[:, ::2] = -3.0 - 1.0 / 128                                       # two values in one bin
+    x[:, 7] = 30.0
+    _sample_holds(ops, x, u, 40.0, vocab // 2 + 3, 1.0, 0.0)
+    x = torch.where(torch.arange(vocab, device="cuda") % 2 == 0, 0.0, -0.0).expand(5, -1).contiguous()
+    _sample_holds(ops, x, u, 1.0, 5, 1.0, 0.0)
+
+
+def test_sample_rows_of_their_own_parameters(ops):
+    n = 300
+    x, u = _logits(n, 3001, torch.bfloat16)
+    g = _gen(3)
+    t = 0.3 + torch.rand(n, generator=g, device="cuda")
+    t[::10] = 0.0
+    k = torch.randint(0, 400, (n,), generator=g, device="cuda", dtype=torch.int32)
+    k[::7] = 0
+    p = torch.rand(n, generator=g, device="cuda")
+    p[::5] = 1.0
+    m = 0.3 * torch.rand(n, generator=g, device="cuda")
+    m[::3] = 0.0
+    tokens = _sample_holds(ops, x, u, t, k, p, m)
+    for _ in range(3):
+        assert torch.equal(ops.sample_tokens(x, u, temperature=t, top_k=k, top_p=p, min_p=m), tokens)
+
+
+def test_sample_special_logits(ops):
+    inf, nan, low = float("inf"), float("nan"), torch.finfo(torch.float32).min
+    x = torch.full((8, 4000), -inf, device="cuda")
+    x[1, 3999] = -7.0                                                  # one token
+    x[2, 100:200] = nan
+    x[2, 150] = 1.0
+    x[3, ::3], x[3, 4] = 0.0, inf                                      # one at infinity takes the row
+    x[4, 9], x[4, 3000] = inf, inf
+    x[5] = low                                                         # masked by the type's lowest value
+    x[5, 77], x[5, 78] = 2.0, 1.0
+    x[6] = nan
+    x[7] = low                                                         # nothing but masked: all alike
+    u = torch.full((8,), 0.6, device="cuda")
+    for k, p, m in ((0, 1.0, 0.0), (2, 0.9, 0.0), (0, 0.5, 0.0), (500, 1.0, 0.5)):
+        for t in (1.0, 0.0, 3.0):
+            tokens = _sample_holds(ops, x, u, t, k, p, m)
+            assert tokens[0] == -1 and tokens[6] == -1 and tokens[1] == 3999
+    for dtype in BOTH:
+        y = torch.full((3, 600), torch.finfo(dtype).min, dtype=dtype, device="cuda")
+        y[1, 5], y[2, 6], y[2, 7] = 3.0, torch.finfo(dtype).max, torch.finfo(dtype).max
+        for k, p in ((0, 1.0), (3, 0.9), (0, 0.7)):
+            _sample_holds(ops, y, u[:3], 0.7, k, p, 0.0)
+
+
+def test_sample_numbers_at_the_ends(ops):
+    x = torch.tensor([[-1.0, 2.0, 2.0, -60.0]], device="cuda").expand(6, -1).contiguous()
+    u = torch.tensor([0.0, -1.0, float("nan"), 1.0, 7.0, float("inf")], device="cuda")
+    assert ops.sample_tokens(x, u, top_k=2).tolist() == [1, 1, 1, 2, 2, 2]
+    assert ops.sample_tokens(x, u).tolist() == [0, 0, 0, 2, 2, 2]      # a weight of e^-62 cannot be chosen
+
+
+def test_sample_strides_streams_and_graphs(ops):
+    x, u = _logits(9, 7000, torch.float16)
+    want = _sample_holds(ops, x, u, 1.0, 0, 0.9, 0.0)
+    wide = torch.full((9, 7100), 60000.0, device="cuda", dtype=torch.float16)
+    for off in (0, 1, 3, 8, 99):                                       # rows at every alignment; neighbours are not read
+        wide.fill_(60000.0)
+        wide[:, off:off + 7000] = x
+        assert torch.equal(ops.sample_tokens(wide[:, off:off + 7000], u, top_p=0.9), want)
+    assert torch.equal(ops.sample_tokens(x.t().contiguous().t(), u, top_p=0.9), want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = ops.sample_tokens(x, u, top_p=0.9)
+    side.synchronize()
+    assert torch.equal(got, want)
+    assert ops.sample_tokens(x[:0], u[:0]).shape == (0,)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held, logs = ops.sample_tokens(x, u, top_p=0.9, return_logprob=True)
+    u.copy_(1 - u)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(held, ops.sample_tokens(x, u, top_p=0.9))
+    assert bool((logs <= 0).all())
