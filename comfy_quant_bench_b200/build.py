@@ -17,7 +17,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 SRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libcq_b200.so")
-SOURCES = ["libcq.cu", "rotquant.cu", "gemm_sm100.cu", "gemm_pair.cu", "gemv.cu", "dit.cu", "w4a16.cu", "w4a16_tokens.cu", "w4a16_mid.cu", "w4a16_tc.cu", "paged_attention.cu",
+SOURCES = ["libcq.cu", "rotquant.cu", "gemm_sm100.cu", "gemm_pair.cu", "gemv.cu", "dit.cu", "w4a16.cu", "w4a16_tokens.cu", "w4a16_mid.cu", "w4a16_tc.cu", "paged_attention.cu", "prefix_attention.cu",
            "kvpages.cu", "add_norm.cu", "rotate_append.cu", "sample.cu",
            "selftest.cu", "capi.cu", "capi_decode.cu", "noalloc.cu", "kernels.cuh", "decode_common.cuh",
            "cq_common.cuh"]

@@ -103,6 +103,48 @@ int cq_paged_attention(const void* q, int64_t q_batch_stride, int64_t q_head_str
   return cuda_status(cq::launch_paged_attention(a, static_cast<cudaStream_t>(stream)));
 }
 
+int64_t cq_prefix_attention_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t span) {
+  if (!fits_int(batch) || q_heads < 1 || kv_heads < 1 || q_heads > 4096 || q_heads % kv_heads != 0 || !valid_head_dim(head_dim) ||
+      !fits_int(span))
+    return -1;
+  return cq::prefix_attention_workspace(batch, static_cast<int>(q_heads), static_cast<int>(kv_heads), static_cast<int>(head_dim),
+                                        span);
+}
+
+int cq_prefix_attention(const void* q, int64_t q_batch_stride, int64_t q_head_stride, int dtype, int64_t batch,
+                        int64_t q_heads, int64_t kv_heads, int64_t head_dim, const void* k_cache, const void* v_cache,
+                        int cache_dtype, int64_t num_pages, int64_t page_size, int64_t page_stride, int64_t head_stride,
+                        int64_t token_stride, const int32_t* block_table, int64_t table_rows, int64_t table_width,
+                        int64_t table_stride, const int32_t* rows, const int32_t* seq_lens, const int32_t* prefix,
+                        int64_t prefix_len, float scale, const float* k_scale, const float* v_scale, void* out, float* lse,
+                        void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!valid16(dtype) || (cache_dtype != dtype && cache_dtype != CQ_DT_FP8_E4M3)) return CQ_ERR_ARG;
+  if (int rc = check_tables(table_rows, table_width, table_stride, num_pages, page_size)) return rc;
+  if (!fits_int(batch) || batch > 65535 || q_heads < 1 || kv_heads < 1 || q_heads > 4096 || q_heads % kv_heads != 0 ||
+      !valid_head_dim(head_dim) || kv_heads > 65535 || !fits_int(prefix_len))
+    return CQ_ERR_SHAPE;
+  if (batch == 0) return CQ_OK;
+  if (workspace_bytes < cq_prefix_attention_workspace_bytes(batch, q_heads, kv_heads, head_dim, table_width * page_size))
+    return CQ_ERR_SHAPE;
+  if (q == nullptr || k_cache == nullptr || v_cache == nullptr || seq_lens == nullptr || out == nullptr ||
+      (block_table == nullptr && table_width > 0) || workspace == nullptr)
+    return CQ_ERR_ARG;
+  const int vec = cache_dtype == CQ_DT_FP8_E4M3 ? 16 : 8;      // elements of a 16-byte access
+  if (!aligned(q, 16) || q_batch_stride % 8 != 0 || q_head_stride % 8 != 0 || !aligned(k_cache, 16) ||
+      !aligned(v_cache, 16) || page_stride % vec != 0 || head_stride % vec != 0 || token_stride % vec != 0 ||
+      !aligned(block_table, 4) || !aligned(rows, 4) || !aligned(seq_lens, 4) || !aligned(prefix, 4) || !aligned(k_scale, 4) ||
+      !aligned(v_scale, 4) || !aligned(out, 16) || !aligned(lse, 4) || !aligned(workspace, 256))
+    return CQ_ERR_ALIGN;
+  if (int dv = check_device()) return dv;
+  const cq::PagedAttnArgs a{q, q_batch_stride, q_head_stride, k_cache, v_cache, page_stride, head_stride,
+                            token_stride, block_table, table_stride, rows, seq_lens, k_scale, v_scale, out, lse,
+                            workspace, static_cast<int>(batch), static_cast<int>(q_heads),
+                            static_cast<int>(kv_heads), static_cast<int>(head_dim), static_cast<int>(num_pages),
+                            static_cast<int>(page_size), static_cast<int>(table_rows), static_cast<int>(table_width),
+                            dtype, cache_dtype, 0, 0, scale, prefix, static_cast<int>(prefix_len), nullptr};
+  return cuda_status(cq::launch_prefix_attention(a, static_cast<cudaStream_t>(stream)));
+}
+
 int64_t cq_pages_workspace_bytes(int64_t num_pages, int64_t reserved_rows) {
   if (!fits_int(num_pages) || !fits_int(reserved_rows)) return -1;
   return 4 * (2 * reserved_rows + num_pages);

@@ -273,9 +273,11 @@ void written_table(const Tensor& table, const char* name) {
 }
 int64_t row_stride(const Tensor& table) { return table.size(0) > 1 ? table.stride(0) : table.size(1); }
 
-py::object paged_attention(const Tensor& q_arg, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table_arg,
-                           const Tensor& lens, const Opt& rows, std::optional<double> scale, int64_t window, int64_t sinks,
-                           const Opt& k_scale, const Opt& v_scale, const Opt& out_arg, bool return_lse) {
+using Prefix = std::variant<Tensor, int64_t>;   // tokens that all rows share
+
+py::object attention(const Tensor& q_arg, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table_arg,
+                     const Tensor& lens, const Prefix* shared, const Opt& rows, std::optional<double> scale, int64_t window,
+                     int64_t sinks, const Opt& k_scale, const Opt& v_scale, const Opt& out_arg, bool return_lse) {
   const at::ScalarType dt = q_arg.scalar_type(), ct = k_cache.scalar_type();
   if (q_arg.dim() != 3 || !half_type(dt)) refuse("q must be bf16 or f16 [B, q_heads, D]");
   const int64_t b = q_arg.size(0), hq = q_arg.size(1), d = q_arg.size(2);
@@ -296,7 +298,18 @@ py::object paged_attention(const Tensor& q_arg, const Tensor& k_cache, const Ten
   } else if (b > table_rows) {
     refuse(b, " queries for ", table_rows, " table rows");
   }
-  const int index = device_of(q_arg, k_cache, v_cache, table_arg, lens, rows, k_scale, v_scale, out_arg);
+  Opt prefix;
+  int64_t prefix_len = 0;
+  if (shared) {
+    if (const Tensor* t = std::get_if<Tensor>(shared)) {
+      if (t->scalar_type() != at::kInt || t->numel() != 1) refuse("prefix must be an int or an int32 tensor of one element");
+      prefix = *t;
+    } else {
+      prefix_len = std::get<int64_t>(*shared);
+      if (prefix_len < 0 || prefix_len > 2147483647) refuse("prefix must not be negative, got ", prefix_len);
+    }
+  }
+  const int index = device_of(q_arg, k_cache, v_cache, table_arg, lens, rows, k_scale, v_scale, out_arg, prefix);
   const float* ks = head_scale(k_scale, hk, ct, "k_scale");
   const float* vs = head_scale(v_scale, hk, ct, "v_scale");
   const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(index));
@@ -315,6 +328,20 @@ py::object paged_attention(const Tensor& q_arg, const Tensor& k_cache, const Ten
   }
   Opt lse, ws;
   if (return_lse) lse = at::empty({b, hq}, q.options().dtype(at::kFloat));
+  const float factor = static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(d)));
+  if (shared) {
+    const int64_t bytes = cq_prefix_attention_workspace_bytes(b, hq, hk, d, width * page);
+    ws = bytes_like(q, bytes);
+    check_status("cq_prefix_attention",
+                 cq_prefix_attention(q.data_ptr(), q.stride(0), q.stride(1), dtype_code(dt), b, hq, hk, d, k_cache.data_ptr(),
+                                     v_cache.data_ptr(), dtype_code(ct), pages, page, k_cache.stride(0), k_cache.stride(1),
+                                     k_cache.stride(2), static_cast<const int32_t*>(table.data_ptr()), table_rows, width,
+                                     row_stride(table), ptr<const int32_t>(rows), static_cast<const int32_t*>(lens.data_ptr()),
+                                     ptr<const int32_t>(prefix), prefix_len, factor, ks, vs, out.data_ptr(), ptr<float>(lse),
+                                     ptr(ws), bytes, stream_of(index)));
+    if (return_lse) return py::make_tuple(out, *lse);
+    return py::cast(out);
+  }
   const int64_t bytes = cq_paged_attention_workspace_bytes(b, hq, hk, d, width * page, window, sinks);
   if (bytes > 0) ws = bytes_like(q, bytes);
   check_status("cq_paged_attention",
@@ -322,10 +349,20 @@ py::object paged_attention(const Tensor& q_arg, const Tensor& k_cache, const Ten
                                   v_cache.data_ptr(), dtype_code(ct), pages, page, k_cache.stride(0), k_cache.stride(1),
                                   k_cache.stride(2), static_cast<const int32_t*>(table.data_ptr()), table_rows, width,
                                   row_stride(table), ptr<const int32_t>(rows), static_cast<const int32_t*>(lens.data_ptr()),
-                                  static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(d))), window, sinks,
-                                  ks, vs, out.data_ptr(), ptr<float>(lse), ptr(ws), bytes, stream_of(index)));
+                                  factor, window, sinks, ks, vs, out.data_ptr(), ptr<float>(lse), ptr(ws), bytes, stream_of(index)));
   if (return_lse) return py::make_tuple(out, *lse);
   return py::cast(out);
+}
+
+py::object paged_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table, const Tensor& lens,
+                           const Opt& rows, std::optional<double> scale, int64_t window, int64_t sinks, const Opt& k_scale,
+                           const Opt& v_scale, const Opt& out, bool return_lse) {
+  return attention(q, k_cache, v_cache, table, lens, nullptr, rows, scale, window, sinks, k_scale, v_scale, out, return_lse);
+}
+py::object prefix_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table,
+                            const Tensor& lens, const Prefix& prefix, const Opt& rows, std::optional<double> scale,
+                            const Opt& k_scale, const Opt& v_scale, const Opt& out, bool return_lse) {
+  return attention(q, k_cache, v_cache, table, lens, &prefix, rows, scale, 0, 0, k_scale, v_scale, out, return_lse);
 }
 
 // x, or a contiguous copy where its rows are not 16-byte aligned
@@ -524,6 +561,7 @@ PYBIND11_MODULE(_decode, m) {
   m.def("add_rmsnorm", &add_rmsnorm);
   m.def("sample_tokens", &sample_tokens);
   m.def("paged_attention", &paged_attention);
+  m.def("prefix_attention", &prefix_attention);
   m.def("append_kv", &append_kv);
   m.def("append_rotated", &append_rotated);
   m.def("pages_update", &pages_update);

@@ -176,7 +176,22 @@ struct PagedAttnArgs {
   void* ws;
   int B, Hq, Hkv, D, num_pages, page_size, table_rows, table_width, dtype, cache_dtype, window, sinks;
   float scale;
+  // attention behind a shared prefix: rows that hold its `prefix_len` (or *prefix) tokens see only what comes after them, and
+  // the outputs go to out32 in fp32 (out32 null: neither)
+  const int* prefix;
+  int prefix_len;
+  float* out32;               // [B, Hq, D]
 };
+// the call's own arguments (own.out32, own.lse and own.ws point into its workspace), and how it is dealt out
+struct PrefixArgs {
+  PagedAttnArgs own;
+  int members, teams;         // CTAs that share a run of keys, and runs
+  float* parts;               // [teams + Hkv, members * row tiles of a CTA] sums of a run
+  float* lse_out;             // [B, Hq] or null
+};
+// span: keys a table row can hold
+int64_t prefix_attention_workspace(int64_t batch, int Hq, int Hkv, int D, int64_t span);
+cudaError_t launch_prefix_attention(const PagedAttnArgs& a, cudaStream_t st);
 // span: keys a table row can hold; 0 bytes where no row is split
 int64_t paged_attention_workspace(int64_t batch, int Hq, int Hkv, int D, int64_t span, int64_t window, int64_t sinks);
 cudaError_t launch_paged_attention(const PagedAttnArgs& a, cudaStream_t st);

@@ -121,6 +121,7 @@ __device__ __forceinline__ int swz(int r, int c) {
 struct RowView {
   int row, n, vis, nsink, units;
 };
+__device__ __forceinline__ int prefix_of(const PagedAttnArgs& a) { return a.prefix != nullptr ? __ldg(a.prefix) : a.prefix_len; }
 __device__ __forceinline__ RowView row_view(const PagedAttnArgs& a, int b) {
   RowView v;
   v.row = a.rows != nullptr ? __ldg(a.rows + b) : b;
@@ -132,6 +133,10 @@ __device__ __forceinline__ RowView row_view(const PagedAttnArgs& a, int b) {
   if (a.window > 0 && n > a.window) {
     v.nsink = min(a.sinks, n - a.window);
     v.vis = a.window + v.nsink;
+  }
+  if (a.out32 != nullptr) {                             // behind a shared prefix, where the row holds it
+    const int prefix = max(0, min(prefix_of(a), a.table_width * a.page_size));
+    if (n >= prefix) v.vis = n - prefix;
   }
   v.units = (v.vis + pattn::kUnit - 1) / pattn::kUnit;
   return v;
@@ -154,6 +159,14 @@ struct UnitIter {
     }
   }
 };
+
+// two neighbouring outputs: element `to` and the next
+template <bool F16>
+__device__ __forceinline__ void store_out(const PagedAttnArgs& a, int64_t to, float x, float y) {
+  if (a.out32 != nullptr) *reinterpret_cast<float2*>(a.out32 + to) = make_float2(x, y);
+  else if constexpr (F16) *reinterpret_cast<__half2*>(static_cast<__half*>(a.out) + to) = __floats2half2_rn(x, y);
+  else *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.out) + to) = __floats2bfloat162_rn(x, y);
+}
 
 // what the weights' exponents are raised by: f16 parts reach up to 2^15, bf16 parts have fp32's range
 template <bool F16Math>
@@ -267,10 +280,11 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
   // rows that see nothing belong to no unit: their zeros
   for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
     if (row_view(a, b).units > 0) continue;
-    uint32_t* o = static_cast<uint32_t*>(a.out) + static_cast<int64_t>(b) * a.Hq * (D / 2);
-    for (int i = tid; i < a.Hq * (D / 2); i += blockDim.x) o[i] = 0;
     if (a.lse != nullptr)
       for (int i = tid; i < a.Hq; i += blockDim.x) a.lse[static_cast<int64_t>(b) * a.Hq + i] = -INFINITY;
+    if (a.out32 != nullptr) continue;                   // its log says that it has none
+    uint32_t* o = static_cast<uint32_t*>(a.out) + static_cast<int64_t>(b) * a.Hq * (D / 2);
+    for (int i = tid; i < a.Hq * (D / 2); i += blockDim.x) o[i] = 0;
   }
   float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) + gridDim.x * sizeof(pattn::Meta));
   if (mode == pattn::kRuns && tid == 0) {
@@ -603,11 +617,8 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
               mine_o[n][i] = v;
             } else if (!complete) {
               *reinterpret_cast<float2*>(p + h * D + d) = v;
-            } else if (F16) {
-              *reinterpret_cast<__half2*>(static_cast<__half*>(a.out) + to + d) = __floats2half2_rn(v.x * inv, v.y * inv);
             } else {
-              *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.out) + to + d) =
-                  __floats2bfloat162_rn(v.x * inv, v.y * inv);
+              store_out<F16>(a, to + d, v.x * inv, v.y * inv);
             }
           }
           if (tid < 8 && !complete && !kCluster) {
@@ -669,10 +680,7 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
       }
       const float inv = sum == 0.0f ? 0.0f : vs / sum;
       const int64_t to = (static_cast<int64_t>(it.b) * a.Hq + h0 + h) * D + d;
-      if constexpr (F16)
-        *reinterpret_cast<__half2*>(static_cast<__half*>(a.out) + to) = __floats2half2_rn(v.x * inv, v.y * inv);
-      else
-        *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.out) + to) = __floats2bfloat162_rn(v.x * inv, v.y * inv);
+      store_out<F16>(a, to, v.x * inv, v.y * inv);
       if (d == 0 && a.lse != nullptr)
         a.lse[static_cast<int64_t>(it.b) * a.Hq + h0 + h] = log_sum(top, sum, kLift);
     }
@@ -733,7 +741,8 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(const PagedAt
   const int64_t to = (static_cast<int64_t>(b) * a.Hq + h0 + h) * D;
   for (int d = threadIdx.x; d < D; d += 128) {
     const float y = ((sum_o[0][d] + sum_o[1][d]) + (sum_o[2][d] + sum_o[3][d])) * inv;
-    if constexpr (F16) static_cast<__half*>(a.out)[to + d] = __float2half_rn(y);
+    if (a.out32 != nullptr) a.out32[to + d] = y;
+    else if constexpr (F16) static_cast<__half*>(a.out)[to + d] = __float2half_rn(y);
     else static_cast<__nv_bfloat16*>(a.out)[to + d] = __float2bfloat16_rn(y);
   }
   if (threadIdx.x == 0 && a.lse != nullptr)

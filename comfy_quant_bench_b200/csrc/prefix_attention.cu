@@ -1,0 +1,637 @@
+// Attention of one new token per sequence where all sequences begin with the same tokens: the shared prefix is read once
+// for the whole batch.
+//
+//   o[b, h] = (sum over the prefix + sum over the row's own tokens) of p_j v_j / the same sums of p_j
+//
+// The prefix: the batch's B (q_heads / kv_heads) query rows of a key-value head are the rows of a matrix product with its
+// keys, so unlike decode's eight heads per key they fill tcgen05 tiles: S = Q K^T and O += P V on tiles of 128 rows and 128
+// keys (64 at D 256), S, P and O in tensor memory.  A CTA holds two row tiles (one at D 256) against the same keys; where
+// there is one row tile only, its two tile slots take every other key tile.  Four warps a slot turn S into P in place; one
+// thread issues the products; four warps gather keys and values from their pages (8-bit caches are widened on the way,
+// which is exact).  A row's maximum is only raised when a score exceeds it by 2^8, since raising it rewrites O.
+//
+// Work: teams of CTAs, a CTA for each pair of row tiles, take equal runs of key tiles, through as many key-value heads as
+// that covers; the team's CTAs read the same keys at the same time, from L2.  Every run leaves its sums (fp32) in the
+// workspace, the row's own tokens go through the kernel of paged_attention.cu, and a last kernel joins them in a fixed order.
+//
+// Weights enter P V in 16 bits: one part of the type (an error like that of rounding the output), or two parts, which adds
+// half to the product's work, where the batch has no more rows than one CTA takes and HBM is the limit.
+#include "decode_common.cuh"
+
+namespace cq {
+
+namespace pfx {
+constexpr int kSite = 130;                     // device status sites of the waits
+constexpr int kRows = 128;
+template <int D>
+struct Cfg {
+  static constexpr int kSlots = D == 256 ? 1 : 2;            // row tiles of a CTA
+  static constexpr int kBufs = D == 256 ? 2 : 1;             // score buffers of a slot
+  static constexpr int kKeys = D == 256 ? 64 : 128;
+  static constexpr int kStages = D == 64 ? 8 : 5;
+  static constexpr int kLag = D == 64 ? 3 : 1;               // loads in flight before one is waited for
+  static constexpr int kStageBytes = kKeys * D * 2;
+  static constexpr int kQBytes = kRows * D * 2;
+  static constexpr int kSoftWarps = 4 * kSlots;
+  static constexpr int kMmaWarp = kSoftWarps, kLoadWarp = kSoftWarps + 1;
+  static constexpr int kThreads = 32 * (kSoftWarps + 5);
+  static constexpr int kSmem = kSlots * kQBytes + kStages * kStageBytes + 1024 + 256;
+  static constexpr uint32_t kCols = 512;
+  static constexpr int kSCols = kKeys;                       // columns of a score buffer
+  static_assert(kSlots * (kBufs * kSCols + D) <= 512, "tensor memory");
+};
+// floats of a row tile's part: O as [D / 4][128 rows][4], then the rows' maxima and sums
+__host__ __device__ constexpr int64_t part_floats(int d) { return 128ll * d + 256; }
+}  // namespace pfx
+
+// shared memory descriptor of an operand whose contiguous dimension is not the product's: 64 columns (128 bytes, swizzled)
+// by 8 rows are a block; blocks along the columns lie `lbo` bytes apart, along the rows 1024
+__device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t saddr, uint32_t lbo) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(lbo >> 4) << 16;
+  d |= static_cast<uint64_t>(1024u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(2u) << 61;
+  return d;
+}
+__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+        "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+        "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+}
+// D(tmem) (+)= A(smem) * B(smem), 16-bit operands of one type
+__device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  mma_bf16(d_tmem, adesc, bdesc, idesc, accumulate);         // kind::f16: the descriptor names the type
+}
+// a wait of a whole warp: all lanes go on, or none does
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int where) {
+  return __all_sync(0xffffffffu, mbar_wait_short(bar, parity, abort_flag, where));
+}
+// four e4m3 values as two pairs of the type, exactly
+template <bool F16>
+__device__ __forceinline__ void widen_e4m3x4(uint32_t x, uint32_t& lo, uint32_t& hi) {
+  e4m3x4_to_f16(x, lo, hi);
+  if constexpr (!F16) {
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+    lo = bf16x2_bits(a.x, a.y);
+    hi = bf16x2_bits(b.x, b.y);
+  }
+}
+
+// The prefix that this call joins, and the first query row that holds it (-1: none, and then nothing is shared).
+__device__ __forceinline__ int prefix_leader(const PrefixArgs& a, int prefix, int* shared) {
+  if (threadIdx.x == 0) *shared = 0x7fffffff;
+  __syncthreads();
+  for (int b = threadIdx.x; b < a.own.B; b += blockDim.x) {
+    const int row = a.own.rows != nullptr ? __ldg(a.own.rows + b) : b;
+    if (row < 0 || row >= a.own.table_rows) continue;
+    const int n = min(__ldg(a.own.lens + row), a.own.table_width * a.own.page_size);
+    if (n >= prefix) {
+      atomicMin(shared, b);
+      break;
+    }
+  }
+  __syncthreads();
+  return *shared == 0x7fffffff ? -1 : *shared;
+}
+
+template <bool F16, bool FP8, int D, int PARTS>
+__global__ void __launch_bounds__(pfx::Cfg<D>::kThreads, 1) prefix_attention_kernel(const PrefixArgs a) {
+  using C = pfx::Cfg<D>;
+  constexpr int kKeys = C::kKeys, kStages = C::kStages, kSlots = C::kSlots, kBufs = C::kBufs;
+  extern __shared__ __align__(128) uint8_t smem_any[];
+  uint8_t* smem = smem_any + ((1024 - (smem_u32(smem_any) & 1023)) & 1023);
+  uint8_t* q_at = smem;
+  uint8_t* ring = smem + kSlots * C::kQBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + kStages * C::kStageBytes);
+  uint64_t* empty = full + kStages;
+  uint64_t* q_full = empty + kStages;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* s_full = q_empty + 1;                             // [kSlots * kBufs] scores are in tensor memory
+  uint64_t* p_full = s_full + 2;                              // [..] weights are
+  uint64_t* o_done = p_full + 2;                              // [kSlots] a product with the values is done
+  uint64_t* all_done = o_done + 2;
+  uint32_t* holder = reinterpret_cast<uint32_t*>(all_done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(holder + 1);
+  int* leader_at = reinterpret_cast<int*>(holder + 2);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const PagedAttnArgs& g = a.own;
+  grid_dep_launch();                                          // the rows' own tokens may be started beside this
+
+  if (tid == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 4);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(q_full, 4);
+    mbar_init(q_empty, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], 4);
+      mbar_init(&o_done[s], 1);
+    }
+    mbar_init(all_done, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == C::kMmaWarp) {
+    tmem_alloc(holder, C::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  const int prefix = max(0, min(prefix_of(g), g.table_width * g.page_size));
+  const int leader = prefix_leader(a, prefix, leader_at);     // and the barriers and the holder are written
+  tc_fence_after();
+  const uint32_t tmem = *holder;
+  const uint32_t o_col = tmem, s_col = tmem + kSlots * D;     // O of each slot, then the score buffers
+
+  // ---- this CTA: its row tiles, its team's run of key tiles ----
+  const int group = g.Hq / g.Hkv, rows = g.B * group, tiles = (rows + pfx::kRows - 1) / pfx::kRows;
+  const int team = blockIdx.x / a.members, tile0 = (blockIdx.x - team * a.members) * kSlots;
+  const bool pair = kSlots == 2 && tile0 + 1 < tiles;         // two row tiles, or one that both slots share
+  const int key_tiles = leader < 0 ? 0 : (prefix + kKeys - 1) / kKeys;
+  const int64_t units = static_cast<int64_t>(g.Hkv) * key_tiles;
+  const int64_t u0 = team * units / a.teams, u1 = (team + 1) * units / a.teams;
+  const int64_t padded = static_cast<int64_t>(a.members) * kSlots;
+
+  struct Segment {
+    int head, j0, n;
+  };
+  auto segment = [&](int64_t u) {
+    Segment s;
+    s.head = static_cast<int>(u / key_tiles);
+    s.j0 = static_cast<int>(u - static_cast<int64_t>(s.head) * key_tiles);
+    s.n = static_cast<int>(min(u1 - u, static_cast<int64_t>(key_tiles - s.j0)));
+    return s;
+  };
+  const int row_of_leader = leader < 0 ? 0 : g.rows != nullptr ? __ldg(g.rows + leader) : leader;
+  const int* table = g.table + row_of_leader * g.table_stride;
+  const int page_shift = 31 - __clz(g.page_size), page_mask = g.page_size - 1;
+
+  if (warp >= C::kLoadWarp) {
+    // ---- gathers: Q of a segment, then its keys and values, tile by tile ----
+    const int w = warp - C::kLoadWarp;
+    constexpr int kChunks = D / 8;                            // 16-byte chunks of a 16-bit row
+    int load = 0, landed = 0;                                 // ring loads issued, and handed over
+    uint32_t q_phase = 0;
+    bool ok = true;
+    auto place = [&](int rows_of, int r, int c) {             // in a tile of `rows_of` rows: 64 columns wide blocks, swizzled
+      return (c >> 3) * (rows_of * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+    };
+    auto hand_over = [&](uint64_t* bar) {                     // this warp's share has landed
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    for (int64_t u = u0; u < u1 && ok;) {
+      const Segment seg = segment(u);
+      if (u > u0) {
+        ok = warp_wait(q_empty, q_phase, abort_flag, pfx::kSite);
+        q_phase ^= 1u;
+        if (!ok) break;
+      }
+      // Q: 32 rows of each tile a warp
+      for (int s = 0; s < (pair ? 2 : 1); ++s) {
+        constexpr int kRowsAtOnce = 32 / kChunks > 0 ? 32 / kChunks : 1;
+        const uint32_t dst = smem_u32(q_at + s * C::kQBytes);
+        for (int r0 = 0; r0 < 32; r0 += kRowsAtOnce) {
+          const int r = 32 * w + r0 + lane / kChunks, c = lane % kChunks;
+          const int at = (tile0 + s) * pfx::kRows + r;
+          const bool valid = at < rows;
+          const int b = valid ? at / group : 0, h = valid ? at - b * group : 0;
+          const uint16_t* src = static_cast<const uint16_t*>(g.q) + b * g.q_sb + (seg.head * group + h) * g.q_sh;
+          cp_async16(dst + place(pfx::kRows, r, c), src + 8 * c, valid);
+        }
+      }
+      cp_async_commit();
+      cp_async_wait<0>();
+      hand_over(q_full);
+      const int64_t head_at = seg.head * g.head_stride;
+      constexpr int kPerWarp = kKeys / 4;                     // keys of a warp: 32 or 16
+      for (int j = seg.j0; j < seg.j0 + seg.n && ok; ++j) {
+        // lane r looks its key up
+        const int key = j * kKeys + w * kPerWarp + (lane & (kPerWarp - 1));
+        int page = -1;
+        if (key < prefix) page = __ldg(table + (key >> page_shift));
+        const bool there = page >= 0 && page < g.num_pages;
+        const uint32_t mask = __ballot_sync(0xffffffffu, there);
+        const int64_t off = there ? page * g.page_stride + head_at + (key & page_mask) * g.tok_stride : 0;
+        if constexpr (!FP8) {
+          for (int kv = 0; kv < 2 && ok; ++kv) {
+            const int stage = load % kStages;
+            if (load >= kStages && !(ok = warp_wait(&empty[stage], (load / kStages - 1) & 1, abort_flag, pfx::kSite + 1))) break;
+            const uint32_t dst = smem_u32(ring + stage * C::kStageBytes);
+            const uint16_t* base = static_cast<const uint16_t*>(kv ? g.v : g.k);
+            constexpr int kRowsAtOnce = 32 / kChunks > 0 ? 32 / kChunks : 1;
+            const int c = lane % kChunks;
+#pragma unroll 8
+            for (int r0 = 0; r0 < kPerWarp; r0 += kRowsAtOnce) {
+              const int r = r0 + lane / kChunks;
+              const int64_t o = __shfl_sync(0xffffffffu, off, r) + 8 * c;
+              cp_async16(dst + place(kKeys, kPerWarp * w + r, c), base + o, mask >> r & 1u);
+            }
+            cp_async_commit();
+            ++load;
+            if (load - landed > C::kLag) {
+              cp_async_wait<C::kLag>();
+              hand_over(&full[landed % kStages]);
+              ++landed;
+            }
+          }
+        } else {
+          // 16 codes a lane: both operands' rows are on their way before either is stored
+          constexpr int kLanes = D / 16, kAtOnce = 32 / kLanes, kLoads = kPerWarp / kAtOnce;
+          uint4 raw[2][kLoads];
+          const int c = lane % kLanes;
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+              const int r = i * kAtOnce + lane / kLanes;
+              const int64_t o = __shfl_sync(0xffffffffu, off, r) + 16 * c;
+              raw[kv][i] = mask >> r & 1u ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(kv ? g.v : g.k) + o))
+                                          : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            const int stage = load % kStages;
+            if (load >= kStages && !(ok = warp_wait(&empty[stage], (load / kStages - 1) & 1, abort_flag, pfx::kSite + 1))) break;
+            uint8_t* dst = ring + stage * C::kStageBytes;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+              const int r = kPerWarp * w + i * kAtOnce + lane / kLanes;
+              uint4 lo, hi;
+              widen_e4m3x4<F16>(raw[kv][i].x, lo.x, lo.y);
+              widen_e4m3x4<F16>(raw[kv][i].y, lo.z, lo.w);
+              widen_e4m3x4<F16>(raw[kv][i].z, hi.x, hi.y);
+              widen_e4m3x4<F16>(raw[kv][i].w, hi.z, hi.w);
+              *reinterpret_cast<uint4*>(dst + place(kKeys, r, 2 * c)) = lo;
+              *reinterpret_cast<uint4*>(dst + place(kKeys, r, 2 * c + 1)) = hi;
+            }
+            hand_over(&full[stage]);
+            ++load;
+            ++landed;
+          }
+        }
+      }
+      if constexpr (!FP8) {
+        cp_async_wait<0>();
+        for (; landed < load; ++landed) hand_over(&full[landed % kStages]);
+      }
+      u += seg.n;
+    }
+    cp_async_wait<0>();
+  } else if (warp == C::kMmaWarp) {
+    // ---- products, by one thread ----
+    if (elect_one()) {
+      constexpr uint32_t type = F16 ? 0u : (1u << 7) | (1u << 10);
+      constexpr uint32_t idesc_s = (1u << 4) | type | (static_cast<uint32_t>(kKeys >> 3) << 17) | (8u << 24);
+      constexpr uint32_t idesc_o = (1u << 4) | type | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) | (8u << 24);
+      int base = 0;                                           // ring loads before this segment
+      uint32_t q_phase = 0, p_phase[2] = {0, 0}, o_phase[2] = {0, 0};
+      bool ok = true;
+      for (int64_t u = u0; u < u1 && ok;) {
+        const Segment seg = segment(u);
+        const int jobs = pair ? 2 * seg.n : seg.n;            // job i: slot i & 1 (where there are two)
+        auto tile_of = [&](int i) { return pair ? i >> 1 : i; };
+        auto last_of_tile = [&](int i) { return !pair || (i & 1); };
+        auto scores = [&](int i) {
+          const int slot = kSlots == 2 ? i & 1 : 0, buf = kBufs == 2 ? i & 1 : slot;
+          const int l = base + 2 * tile_of(i), stage = l % kStages;
+          if (!mbar_wait_short(&full[stage], (l / kStages) & 1, abort_flag, pfx::kSite + 2)) return false;
+          tc_fence_after();
+          const uint64_t q = smem_desc_k_sw128(smem_u32(q_at + (pair ? slot : 0) * C::kQBytes));
+          const uint64_t k = smem_desc_k_sw128(smem_u32(ring + stage * C::kStageBytes));
+#pragma unroll
+          for (int x = 0; x < D / 16; ++x)
+            mma_f16_ss(s_col + buf * C::kSCols, q + ((x >> 2) * (pfx::kRows * 128) + (x & 3) * 32) / 16,
+                       k + ((x >> 2) * (kKeys * 128) + (x & 3) * 32) / 16, idesc_s, x != 0);
+          tc_commit(&s_full[buf]);
+          if (last_of_tile(i)) tc_commit(&empty[stage]);
+          if (i + 1 == jobs) tc_commit(q_empty);
+          return true;
+        };
+        ok = mbar_wait_short(q_full, q_phase, abort_flag, pfx::kSite + 3);
+        q_phase ^= 1u;
+        if (!ok) break;
+        const int ahead = kSlots == 2 ? 2 : 1;                // jobs whose scores come before a job's weights
+        for (int i = 0; i < min(ahead, jobs) && ok; ++i) ok = scores(i);
+        for (int i = 0; i < jobs && ok; ++i) {
+          const int slot = kSlots == 2 ? i & 1 : 0, buf = kBufs == 2 ? i & 1 : slot;
+          if (kBufs == 2 && i + 1 < jobs) {
+            // the other buffer's weights are consumed when the product before is done
+            if (i > 0) {
+              ok = mbar_wait_short(&o_done[0], o_phase[0], abort_flag, pfx::kSite + 4);
+              o_phase[0] ^= 1u;
+            }
+            ok = ok && scores(i + 1);
+            if (!ok) break;
+          } else if (kBufs == 2 && i > 0) {
+            ok = mbar_wait_short(&o_done[0], o_phase[0], abort_flag, pfx::kSite + 4);
+            o_phase[0] ^= 1u;
+            if (!ok) break;
+          }
+          const int l = base + 2 * tile_of(i) + 1, stage = l % kStages;
+          ok = mbar_wait_short(&full[stage], (l / kStages) & 1, abort_flag, pfx::kSite + 5) &&
+               mbar_wait_short(&p_full[buf], p_phase[buf], abort_flag, pfx::kSite + 6);
+          p_phase[buf] ^= 1u;
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t v = smem_u32(ring + stage * C::kStageBytes);
+          const bool first = kSlots == 2 ? i < 2 : i == 0;
+#pragma unroll
+          for (int x = 0; x < kKeys / 16; ++x) {
+            const uint64_t vd = smem_desc_mn_sw128(v + x * 2048, kKeys * 128);
+            const uint32_t p = s_col + buf * C::kSCols + 32 * (x >> 1) + 8 * (x & 1);
+            mma_f16_ts(o_col + slot * D, p, vd, idesc_o, !first || x != 0);
+            if constexpr (PARTS == 2) mma_f16_ts(o_col + slot * D, p + 16, vd, idesc_o, 1);
+          }
+          tc_commit(&o_done[slot]);
+          if (last_of_tile(i)) tc_commit(&empty[stage]);
+          if (kSlots == 2 && i + 2 < jobs) {
+            // this slot's scores take the place of the weights just used
+            ok = mbar_wait_short(&o_done[slot], o_phase[slot], abort_flag, pfx::kSite + 7) && scores(i + 2);
+            o_phase[slot] ^= 1u;
+          }
+        }
+        // the segment's last products: the next one's scores take the place of their weights
+        for (int i = max(0, jobs - kSlots); i < jobs && ok; ++i) {
+          const int slot = kSlots == 2 ? i & 1 : 0;
+          ok = mbar_wait_short(&o_done[slot], o_phase[slot], abort_flag, pfx::kSite + 4);
+          o_phase[slot] ^= 1u;
+        }
+        base += 2 * seg.n;
+        u += seg.n;
+      }
+      tc_commit(all_done);
+      mbar_wait_drain(all_done, 0, 50000000ull);
+    }
+    __syncwarp();
+  } else {
+    // ---- softmax: thread = row of the slot's tile ----
+    const int slot = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    constexpr float kLift = F16 ? 7.0f : 0.0f;                // f16 weights reach 2^15: up to 2^8 above the running maximum
+    constexpr float kSlackUp = 8.0f;
+    uint32_t s_phase[2] = {0, 0}, o_phase = 0;
+    bool ok = true;
+    for (int64_t u = u0; u < u1 && ok;) {
+      const Segment seg = segment(u);
+      const float mul = g.scale * 1.4426950408889634f * (FP8 && g.k_scale != nullptr ? __ldg(g.k_scale + seg.head) : 1.0f);
+      float m = -INFINITY, l = 0.0f;
+      const int step = kSlots == 2 && !pair ? 2 : 1;          // key tiles of this slot: first, first + step, ...
+      int done = 0;
+      for (int j = kSlots == 2 && !pair ? slot : 0; j < seg.n && ok; j += step, ++done) {
+        const int buf = kBufs == 2 ? done & 1 : slot;
+        const int key0 = (seg.j0 + j) * kKeys;
+        // which keys are there: looked up while the scores are on their way
+        int page[kKeys / 32];
+#pragma unroll
+        for (int x = 0; x < kKeys / 32; ++x) {
+          const int key = key0 + 32 * x + lane;
+          page[x] = key < prefix ? __ldg(table + (key >> page_shift)) : -1;
+        }
+        if (!(ok = warp_wait(&s_full[buf], s_phase[buf], abort_flag, pfx::kSite + 8))) break;
+        s_phase[buf] ^= 1u;
+        __syncwarp();
+        tc_fence_after();
+        uint32_t masks[kKeys / 32];
+        bool whole = true;
+#pragma unroll
+        for (int x = 0; x < kKeys / 32; ++x) {
+          masks[x] = __ballot_sync(0xffffffffu, page[x] >= 0 && page[x] < g.num_pages);
+          whole = whole && masks[x] == 0xffffffffu;
+        }
+        const uint32_t s_at = s_col + buf * C::kSCols + lanes;
+        float top = -INFINITY;
+        uint32_t v[32];
+#pragma unroll
+        for (int x = 0; x < kKeys / 32; ++x) {
+          tmem_ld_32x32b_x32(s_at + 32 * x, v);
+          tmem_wait_ld_dep(v);
+          if (whole) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(v[i]) * mul);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (masks[x] >> i & 1u) top = fmaxf(top, __uint_as_float(v[i]) * mul);
+          }
+        }
+        const bool raise = top > m + kSlackUp || (m == -INFINITY && top > m);
+        if (kBufs == 2 && done > 0) {                         // the product before still adds to O
+          ok = warp_wait(&o_done[slot], o_phase, abort_flag, pfx::kSite + 9);
+          o_phase ^= 1u;
+          if (!ok) break;
+          __syncwarp();
+          tc_fence_after();
+        }
+        if (__any_sync(0xffffffffu, raise)) {
+          const float to = raise ? top : m, f = raise ? exp2_fast(m - to) : 1.0f;
+          m = to;
+          l *= f;
+          if (done > 0) {
+#pragma unroll 1
+            for (int x = 0; x < D / 32; ++x) {
+              tmem_ld_32x32b_x32(o_col + slot * D + lanes + 32 * x, v);
+              tmem_wait_ld_dep(v);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+              tmem_st_x32(o_col + slot * D + lanes + 32 * x, v);
+            }
+          }
+        }
+        const float base = (m == -INFINITY ? 0.0f : m) - kLift;
+#pragma unroll
+        for (int x = 0; x < kKeys / 32; ++x) {
+          tmem_ld_32x32b_x32(s_at + 32 * x, v);
+          tmem_wait_ld_dep(v);
+          uint32_t p[32];                                     // the first part's pairs, then the second's
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float p0 = exp2_fast(fmaf(__uint_as_float(v[i]), mul, -base)), p1 = exp2_fast(fmaf(__uint_as_float(v[i + 1]), mul, -base));
+            if (!whole) {
+              p0 = masks[x] >> i & 1u ? p0 : 0.0f;
+              p1 = masks[x] >> (i + 1) & 1u ? p1 : 0.0f;
+            }
+            l += p0 + p1;
+            if constexpr (PARTS == 2) split16<F16>(p0, p1, p[i / 2], p[16 + i / 2]);
+            else p[i / 2] = narrow16<F16>(p0, p1);
+          }
+          if constexpr (PARTS == 2) tmem_st_x32(s_at + 32 * x, p);
+          else tmem_st_x16(s_at + 32 * x, reinterpret_cast<const uint32_t(&)[16]>(p));
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[buf]);
+      }
+      if (!ok) break;
+      // ---- this run's sums ----
+      if (done > 0) {
+        // the last product; earlier ones are done (their phases: one for every product of this slot)
+        if (kBufs == 1) {
+          const uint32_t last = (o_phase + static_cast<uint32_t>(done) - 1u) & 1u;
+          ok = warp_wait(&o_done[slot], last, abort_flag, pfx::kSite + 10);
+          o_phase = (o_phase + static_cast<uint32_t>(done)) & 1u;
+        } else {
+          ok = warp_wait(&o_done[slot], o_phase, abort_flag, pfx::kSite + 10);
+          o_phase ^= 1u;
+        }
+        if (!ok) break;
+        __syncwarp();
+        tc_fence_after();
+      }
+      float* part = a.parts + ((team + seg.head) * padded + tile0 + slot) * pfx::part_floats(D);
+      if (done > 0) {
+#pragma unroll 1
+        for (int x = 0; x < D / 32; ++x) {
+          uint32_t v[32];
+          tmem_ld_32x32b_x32(o_col + slot * D + lanes + 32 * x, v);
+          tmem_wait_ld_dep(v);
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            reinterpret_cast<uint4*>(part)[(8 * x + i / 4) * pfx::kRows + row] = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        }
+      }
+      part[128 * D + row] = m;
+      part[128 * D + 128 + row] = l;
+      tc_fence_before();
+      u += seg.n;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == C::kMmaWarp) tmem_dealloc(tmem, C::kCols);
+}
+
+// Joins a row's runs over the prefix, in their order, with its own tokens.  A block: 128 rows of a row tile, one head, 16
+// columns; thread = row.
+template <bool F16, int D>
+__global__ void __launch_bounds__(128) prefix_join_kernel(const PrefixArgs a) {
+  using C = pfx::Cfg<D>;
+  constexpr int kKeys = C::kKeys;
+  const PagedAttnArgs& g = a.own;
+  const int tile = blockIdx.x, head = blockIdx.y, d4 = blockIdx.z * 4, tid = threadIdx.x;
+  const int group = g.Hq / g.Hkv, rows = g.B * group, tiles = (rows + pfx::kRows - 1) / pfx::kRows;
+  grid_dep_wait();
+  const int at = tile * pfx::kRows + tid;
+  if (at >= rows) return;
+  const int b = at / group, h = head * group + at - b * group;
+  const int prefix = max(0, min(prefix_of(g), g.table_width * g.page_size));
+  const int row = g.rows != nullptr ? g.rows[b] : b;
+  const int n = row >= 0 && row < g.table_rows ? min(g.lens[row], g.table_width * g.page_size) : 0;
+  const bool joined = prefix > 0 && n >= prefix;
+  const int64_t own = static_cast<int64_t>(b) * g.Hq + h;
+  const float own_lse = g.lse[own] * 1.4426950408889634f;     // as a power of 2; -inf without tokens of its own
+  float top = own_lse, sum = 0.0f;
+  const int key_tiles = (prefix + kKeys - 1) / kKeys;
+  const int64_t units = static_cast<int64_t>(g.Hkv) * key_tiles, padded = static_cast<int64_t>(a.members) * C::kSlots;
+  const int subs = C::kSlots == 2 && tile + 1 == tiles && !(tile & 1) ? 2 : 1;
+  constexpr float kLift = F16 ? 7.0f : 0.0f;
+  auto each_part = [&](auto&& f) {
+    if (!joined) return;
+    for (int64_t x = static_cast<int64_t>(head) * key_tiles; x < static_cast<int64_t>(head + 1) * key_tiles;) {
+      const int64_t team = ((x + 1) * a.teams - 1) / units;
+      for (int s = 0; s < subs; ++s) f(a.parts + ((team + head) * padded + tile + s) * pfx::part_floats(D));
+      x = (team + 1) * units / a.teams;
+    }
+  };
+  each_part([&](const float* p) { top = fmaxf(top, p[128 * D + tid] - kLift); });
+  const float vs = g.cache_dtype == CQ_DT_FP8_E4M3 && g.v_scale != nullptr ? g.v_scale[head] : 1.0f;
+  float o[16];
+  const float f0 = own_lse == -INFINITY ? 0.0f : exp2f(own_lse - top);
+  sum = own_lse == -INFINITY ? 0.0f : f0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) o[i] = own_lse == -INFINITY ? 0.0f : g.out32[own * D + 4 * d4 + i] * f0;
+  each_part([&](const float* p) {
+    const float m = p[128 * D + tid], l = p[128 * D + 128 + tid];
+    if (l == 0.0f) return;                                    // a slot without a key tile, or keys that weigh nothing
+    const float f = m == -INFINITY ? 1.0f : exp2f(m - kLift - top);
+    sum += l * f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 v = reinterpret_cast<const float4*>(p)[(d4 + i) * pfx::kRows + tid];
+      o[4 * i] = fmaf(v.x * vs, f, o[4 * i]);
+      o[4 * i + 1] = fmaf(v.y * vs, f, o[4 * i + 1]);
+      o[4 * i + 2] = fmaf(v.z * vs, f, o[4 * i + 2]);
+      o[4 * i + 3] = fmaf(v.w * vs, f, o[4 * i + 3]);
+    }
+  });
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  uint32_t out[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) out[i] = narrow16<F16>(o[2 * i] * inv, o[2 * i + 1] * inv);
+  uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(g.out) + own * D + 4 * d4);
+  to[0] = make_uint4(out[0], out[1], out[2], out[3]);
+  to[1] = make_uint4(out[4], out[5], out[6], out[7]);
+  if (a.lse_out != nullptr && d4 == 0) a.lse_out[own] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) / 1.4426950408889634f;
+}
+
+namespace {
+int prefix_members(int64_t rows, int D) {
+  const int per = D == 256 ? pfx::kRows : 2 * pfx::kRows;
+  return static_cast<int>((rows + per - 1) / per);
+}
+int prefix_teams(int members) { return members < num_sms() ? num_sms() / members : 1; }
+}  // namespace
+
+// the runs' sums, the rows' own outputs and their logs, and the workspace of their kernel
+int64_t prefix_attention_workspace(int64_t batch, int Hq, int Hkv, int D, int64_t span) {
+  if (batch == 0) return 0;
+  const int members = prefix_members(batch * (Hq / Hkv), D);
+  const int64_t parts = static_cast<int64_t>(prefix_teams(members) + Hkv) * members * (D == 256 ? 1 : 2) * pfx::part_floats(D) * 4;
+  return parts + batch * Hq * (D + 4) * 4 + (paged_attention_workspace(batch, Hq, Hkv, D, span, 0, 0) + 255) / 256 * 256;
+}
+
+template <bool F16, bool FP8, int D, int PARTS>
+cudaError_t run_prefix(const PrefixArgs& a, cudaStream_t st) {
+  using C = pfx::Cfg<D>;
+  auto kern = prefix_attention_kernel<F16, FP8, D, PARTS>;
+  static unsigned long long devices = 0;
+  cudaError_t e = allow_shared(kern, C::kSmem, devices);
+  if (e != cudaSuccess) return e;
+  kern<<<static_cast<unsigned>(a.teams * a.members), C::kThreads, C::kSmem, st>>>(a);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  if ((e = launch_paged_attention(a.own, st)) != cudaSuccess) return e;
+  const int group = a.own.Hq / a.own.Hkv, tiles = (a.own.B * group + pfx::kRows - 1) / pfx::kRows;
+  return launch_early(prefix_join_kernel<F16, D>, dim3(tiles, a.own.Hkv, D / 16), 128, 0, st, a);
+}
+template <bool F16, bool FP8, int D>
+cudaError_t pick_prefix(const PrefixArgs& a, cudaStream_t st) {
+  return a.members == 1 ? run_prefix<F16, FP8, D, 2>(a, st) : run_prefix<F16, FP8, D, 1>(a, st);
+}
+template <bool F16, bool FP8>
+cudaError_t pick_prefix_dim(const PrefixArgs& a, cudaStream_t st) {
+  switch (a.own.D) {
+    case 64: return pick_prefix<F16, FP8, 64>(a, st);
+    case 128: return pick_prefix<F16, FP8, 128>(a, st);
+    default: return pick_prefix<F16, FP8, 256>(a, st);
+  }
+}
+
+// a.own: the whole call's arguments, its ws the whole workspace
+cudaError_t launch_prefix_attention(const PagedAttnArgs& call, cudaStream_t st) {
+  PrefixArgs a{};
+  a.own = call;
+  a.members = prefix_members(static_cast<int64_t>(call.B) * (call.Hq / call.Hkv), call.D);
+  a.teams = prefix_teams(a.members);
+  a.lse_out = call.lse;
+  a.parts = static_cast<float*>(call.ws);
+  float* next = a.parts + static_cast<int64_t>(a.teams + call.Hkv) * a.members * (call.D == 256 ? 1 : 2) * pfx::part_floats(call.D);
+  const int64_t heads = static_cast<int64_t>(call.B) * call.Hq;
+  a.own.out32 = next;
+  a.own.lse = next + heads * call.D;
+  a.own.ws = next + heads * (call.D + 4);
+  const bool fp8 = call.cache_dtype == CQ_DT_FP8_E4M3;
+  if (call.dtype == CQ_DT_F16) return fp8 ? pick_prefix_dim<true, true>(a, st) : pick_prefix_dim<true, false>(a, st);
+  return fp8 ? pick_prefix_dim<false, true>(a, st) : pick_prefix_dim<false, false>(a, st);
+}
+
+}  // namespace cq

@@ -42,6 +42,22 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                                          v_scale, out, return_lse)
 
 
+def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                     seq_lens: torch.Tensor, prefix: int | torch.Tensor, *, rows: torch.Tensor | None = None,
+                     scale: float | None = None, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                     out: torch.Tensor | None = None, return_lse: bool = False):
+    """``paged_attention`` of a batch whose rows begin with the same ``prefix`` tokens (an int, or one int32 on the device,
+    which a captured step reads anew): samples of one prompt, requests behind one instruction.  Their keys and values are
+    read once for all rows, not once for each.
+
+    Every row with ``prefix`` tokens or more must hold the same first ``prefix`` tokens, in whatever pages (those of the
+    first such row are read); a shorter row or an empty one is attended by itself.  Arguments and results are those of
+    ``paged_attention``.  A softmax weight enters the product with the prefix's values as two 16-bit parts where B *
+    q_heads / kv_heads is at most 256 (128 at D 256), else as one part, rounded to nearest."""
+    return _lib.decode().prefix_attention(q, k_cache, v_cache, block_table, seq_lens, prefix, rows, scale, k_scale, v_scale,
+                                          out, return_lse)
+
+
 def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
               block_table: torch.Tensor, rows: torch.Tensor, positions: torch.Tensor, *,
               k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> None:
@@ -210,6 +226,12 @@ class PagedKVCache:
     def attend(self, layer: int, q: torch.Tensor, rows: torch.Tensor | None = None, **kw) -> torch.Tensor:
         return paged_attention(q, self.k[layer], self.v[layer], self.block_table, self.seq_lens, rows=rows,
                                k_scale=self.k_scale, v_scale=self.v_scale, **kw)
+
+    def attend_prefix(self, layer: int, q: torch.Tensor, prefix: int | torch.Tensor, rows: torch.Tensor | None = None,
+                      **kw) -> torch.Tensor:
+        """``attend`` for rows whose first ``prefix`` tokens are the same."""
+        return prefix_attention(q, self.k[layer], self.v[layer], self.block_table, self.seq_lens, prefix, rows=rows,
+                                k_scale=self.k_scale, v_scale=self.v_scale, **kw)
 
     def check(self) -> None:
         check(self.k.device)

@@ -518,6 +518,26 @@ CQ_API int cq_paged_attention(const void* q, int64_t q_batch_stride, int64_t q_h
                               float* lse, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
+ * cq_prefix_attention: cq_paged_attention (without a window) for a batch whose rows begin with the same tokens: the keys and
+ * values of the first P tokens are read once for all rows, through the table of the first query row that has P tokens
+ * or more.  P is *prefix (int32, device memory) where that is not NULL, else prefix_len.  All rows with P tokens or more must
+ * hold the same first P tokens (in whatever pages); a shorter row, or one without tokens, is attended by itself.  Arguments
+ * and results as cq_paged_attention; a weight enters the product with the prefix's v as two 16-bit parts where batch * q_heads
+ * / kv_heads is at most 256 (128 at head_dim 256), else as one, rounded to nearest.
+ *   workspace of cq_prefix_attention_workspace_bytes (span = table_width * page_size), 256-byte aligned, of this call alone
+ */
+CQ_API int64_t cq_prefix_attention_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                                   int64_t span);
+CQ_API int cq_prefix_attention(const void* q, int64_t q_batch_stride, int64_t q_head_stride, int dtype, int64_t batch,
+                               int64_t q_heads, int64_t kv_heads, int64_t head_dim, const void* k_cache,
+                               const void* v_cache, int cache_dtype, int64_t num_pages, int64_t page_size,
+                               int64_t page_stride, int64_t head_stride, int64_t token_stride, const int32_t* block_table,
+                               int64_t table_rows, int64_t table_width, int64_t table_stride, const int32_t* rows,
+                               const int32_t* seq_lens, const int32_t* prefix, int64_t prefix_len, float scale,
+                               const float* k_scale, const float* v_scale, void* out, float* lse, void* workspace,
+                               int64_t workspace_bytes, void* stream);
+
+/*
  * cq_kv_append: the new keys and values of `tokens` tokens into the pages of their rows: token t goes to position
  * positions[t] of table row rows[t], in each of `layers` layers (k_new, v_new [layers, tokens, kv_heads, head_dim]
  * of `dtype` with strides in elements).  A token whose row, position or page is out of range is skipped, as the

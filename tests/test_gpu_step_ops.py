@@ -469,3 +469,248 @@ def test_sample_strides_streams_and_graphs(ops):
     torch.cuda.synchronize()
     assert torch.equal(held, ops.sample_tokens(x, u, top_p=0.9))
     assert bool((logs <= 0).all())
+
+
+# ----------------------------------------------------------------------------------------------------------
+# attention behind a shared prefix.  A score's fp32 error is at most err = (D + 16) 2^-23 scale sum |q| |k|; it and the
+# exponential (2^-20) enter numerator and denominator; a weight in two 16-bit parts is held to 2^-16 (2^-14 for its share of
+# the sums as elsewhere), in one part to u; f16 parts to 2^-32 of the running maximum beside that:
+# |o - exact| <= u |exact| + A (2 max err + 2^-14 [+ u]) + n 2^-32 max |v|, A = sum p |v| / sum p.
+# ----------------------------------------------------------------------------------------------------------
+
+def _prefix_problem(lens, prefix, hq, hk, d, page, dtype, cache, seed=0, holes=True):
+    """Rows of lens tokens; those with at least `prefix` of them share the first ones: whole pages, the last in copies."""
+    g = _gen(seed + d + prefix)
+    host = torch.Generator().manual_seed(seed)
+    b = len(lens)
+    width = max(1, -(-max(max(lens), 1) // page))
+    whole = prefix // page
+    joined = [n >= prefix for n in lens]
+    need = [max(0, -(-n // page) - (whole if j else 0)) for n, j in zip(lens, joined)]
+    pages = whole + sum(need) + 3
+    order = torch.randperm(pages, generator=host).int()
+    table = torch.full((b, width), -1, dtype=torch.int32)
+    used = whole
+    for r in range(b):
+        skip = whole if joined[r] else 0
+        table[r, :skip] = order[:skip]
+        table[r, skip: skip + need[r]] = order[used: used + need[r]]
+        used += need[r]
+    shape = (pages, hk, page, d)
+    k, v = (torch.randn(shape, generator=g, device="cuda") for _ in range(2))
+    scales = [None, None]
+    if cache == FP8:
+        k, v = k * 40, v * 40
+        scales = [0.02 + 0.02 * torch.rand(hk, generator=g, device="cuda") for _ in range(2)]
+    k, v = k.to(cache), v.to(cache)
+    first = next((r for r in range(b) if joined[r]), None)
+    for c in (k, v):
+        raw = c.view(torch.uint8) if cache == FP8 else c
+        if prefix % page and first is not None:
+            src = int(table[first, whole])
+            for r in range(b):
+                if joined[r]:
+                    raw[int(table[r, whole]), :, : prefix % page] = raw[src, :, : prefix % page].clone()
+        if holes:
+            nan = torch.tensor(float("nan"), device="cuda").to(cache)
+            nan = nan.view(torch.uint8) if cache == FP8 else nan
+            for r, n in enumerate(lens):
+                if n % page:
+                    raw[int(table[r, n // page]), :, n % page:] = nan
+    q = (1.5 * torch.randn(b, hq, d, generator=g, device="cuda")).to(dtype)
+    return q, k, v, table.cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda"), scales
+
+
+def _prefix_exact(q, k, v, table, lens, scales, scale=None, rows=None):
+    b, hq, d = q.shape
+    hk, page = k.shape[1], k.shape[2]
+    scale = d ** -0.5 if scale is None else scale
+    out, lse = torch.zeros(b, hq, d, dtype=torch.float64, device="cuda"), torch.full((b, hq), -math.inf, dtype=torch.float64, device="cuda")
+    slack = torch.zeros_like(out)
+    tail = torch.zeros(b, hq, 1, dtype=torch.float64, device="cuda")
+    for i in range(b):
+        r = i if rows is None else int(rows[i])
+        n = int(lens[r]) if 0 <= r < len(lens) else 0
+        at = torch.arange(n, device="cuda")
+        pages = table[r].long()[at // page] if n else at
+        at, pages = at[(pages >= 0) & (pages < len(k))], pages[(pages >= 0) & (pages < len(k))]
+        if not len(at):
+            continue
+        take = lambda c: (c.view(torch.uint8)[pages, :, at % page].view(FP8) if c.dtype == FP8 else c[pages, :, at % page]).double()  # noqa: E731
+        kk, vv = take(k), take(v)
+        if scales[0] is not None:
+            kk, vv = kk * scales[0].double().view(-1, 1), vv * scales[1].double().view(-1, 1)
+        kk, vv = (x.repeat_interleave(hq // hk, 1).transpose(0, 1) for x in (kk, vv))          # [hq, n, d]
+        qq = q[i].double().unsqueeze(1)
+        s = (qq @ kk.transpose(1, 2)).squeeze(1) * scale
+        err = (d + 16) * 2.0 ** -23 * abs(scale) * (qq.abs() @ kk.abs().transpose(1, 2)).squeeze(1).amax(-1)
+        p = torch.softmax(s, -1)
+        out[i], lse[i] = (p.unsqueeze(1) @ vv).squeeze(1), torch.logsumexp(s, -1)
+        slack[i] = (p.unsqueeze(1) @ vv.abs()).squeeze(1) * (2 * err + 2.0 ** -14).unsqueeze(-1)
+        tail[i] = n * 2.0 ** -32 * vv.abs().amax()
+        err_lse = err + 2.0 ** -19
+        assert bool((err_lse < 0.1).all())
+    share = slack / 2.0 ** -14                                          # at least A
+    return out, lse, slack, share, tail
+
+
+def _prefix_holds(kv, problem, prefix, rows=None, scale=None, **kw):
+    q, k, v, table, lens, scales = problem
+    got, lse = kv.prefix_attention(q, k, v, table, lens, prefix, rows=rows, scale=scale, k_scale=scales[0], v_scale=scales[1],
+                                   return_lse=True, **kw)
+    want, want_lse, slack, share, tail = _prefix_exact(q, k, v, table, lens, scales, scale, rows)
+    b, hq, d = q.shape
+    one_part = b * (hq // k.shape[1]) > (128 if d == 256 else 256)
+    u = U[q.dtype]
+    assert got.dtype == q.dtype and got.shape == q.shape
+    bound = u * want.abs() + slack * (1 + u) + (u * share if one_part else 0) + tail + 2.0 ** -25
+    over = ((got.double() - want).abs() - bound).max()
+    assert float(over) <= 0, float(over)
+    seen = ~torch.isinf(want_lse)
+    assert torch.equal(torch.isinf(lse), ~seen)
+    assert float((lse.double() - want_lse)[seen].abs().max() if seen.any() else 0.0) <= 2.0 ** -12
+    if want.numel() > 4000 and float(want.norm()) > 0:
+        once = float((want.to(q.dtype).double() - want).norm() / want.norm())
+        assert float((got.double() - want).norm() / want.norm()) <= (1.5 if one_part else 1.05) * once + 2.0 ** -14
+    return got
+
+
+@pytest.mark.parametrize("dtype,cache", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16),
+                                         (torch.bfloat16, FP8), (torch.float16, FP8)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("b,hq,hk,prefix,longest,page", [(1, 1, 1, 1, 1, 16), (2, 4, 1, 5, 3, 8), (4, 16, 2, 500, 60, 16),
+                                                         (3, 6, 3, 127, 40, 16), (3, 6, 3, 128, 0, 32), (5, 8, 4, 129, 200, 64),
+                                                         (40, 8, 2, 700, 30, 16), (33, 8, 1, 1111, 90, 16), (65, 12, 3, 300, 17, 128),
+                                                         (20, 56, 2, 2050, 5, 16), (70, 16, 1, 640, 9, 16), (2, 8, 8, 6000, 100, 16)])
+def test_prefix(kv, b, hq, hk, prefix, longest, page, d, dtype, cache):
+    lens = [prefix + (longest * i) // max(1, b - 1) for i in range(b)]
+    problem = _prefix_problem(lens, prefix, hq, hk, d, page, dtype, cache)
+    _prefix_holds(kv, problem, prefix)
+    _prefix_holds(kv, problem, torch.tensor([prefix], dtype=torch.int32, device="cuda"))
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("b,hq,hk", [(6, 8, 2), (50, 16, 2)])
+def test_prefix_of_uneven_rows(kv, b, hq, hk, d):
+    """Rows without the prefix, rows of nothing, prefixes of nothing and beyond every row."""
+    lens = [0, 400, 350, 3, 700, 349] + [350 + 7 * i for i in range(b - 6)]
+    problem = _prefix_problem(lens, 350, hq, hk, d, 16, torch.bfloat16, torch.bfloat16)
+    q, k, v, table, n, scales = problem
+    for prefix in (350, 349, 200, 17, 1, 0, 100000):
+        if prefix >= 350 or prefix == 0:
+            _prefix_holds(kv, problem, prefix)
+    lens = [260 + 7 * i for i in range(b)]
+    problem = _prefix_problem(lens, 260, hq, hk, d, 16, torch.bfloat16, torch.bfloat16)
+    for prefix in (260, 259, 128, 1):                                   # any shorter prefix is shared too
+        _prefix_holds(kv, problem, prefix)
+    rows = torch.arange(b, device="cuda", dtype=torch.int32).flip(0)
+    rows[1], rows[2], rows[3] = -1, b, rows[0]                          # no row, beyond the table, the same row twice
+    _prefix_holds(kv, problem, 260, rows=rows)
+    _prefix_holds(kv, problem, 260, scale=-0.02)
+    # a page that the table does not have, inside the prefix
+    holed = problem[3].clone()
+    holed[:, 3], holed[:, 9] = -1, len(problem[1])
+    _prefix_holds(kv, (*problem[:3], holed, *problem[4:]), 260)
+
+
+def test_prefix_agrees_with_one_row_at_a_time_and_again(kv):
+    problem = _prefix_problem([900 + i for i in range(48)], 900, 32, 8, 128, 16, torch.float16, torch.float16)
+    q, k, v, table, lens, _ = problem
+    got = _prefix_holds(kv, problem, 900)
+    plain = kv.paged_attention(q, k, v, table, lens)
+    assert float((got.double() - plain.double()).norm() / plain.double().norm()) <= 2.0 ** -11
+    for _ in range(4):
+        assert torch.equal(kv.prefix_attention(q, k, v, table, lens, 900), got)
+
+
+def test_prefix_large_scores(kv):
+    """Maxima that grow from tile to tile, one key that outweighs the rest, infinities and NaN in sight."""
+    lens = [1500 + i for i in range(20)]
+    for d in (64, 128, 256):
+        problem = _prefix_problem(lens, 1500, 8, 2, d, 16, torch.float16, torch.float16)
+        q, k, v, table, n, scales = problem
+        for j in range(1500):                                           # keys grow along the prefix
+            if j % 16 == 0:
+                k[int(table[0, j // 16])] *= 0.2 + 4 * j / 1500
+        if 1500 % 16:
+            src = int(table[0, 93])
+            for r in range(1, 20):
+                k[int(table[r, 93]), :, :12] = k[src, :, :12]
+        want, lse, slack, share, tail = _prefix_exact(*problem[:5], scales)
+        got = kv.prefix_attention(q, k, v, table, n, 1500)
+        assert float(((got.double() - want).abs() - U[torch.float16] * want.abs() - slack * 1.01 - tail - 2.0 ** -25).max()) <= 0
+        bad = v.clone()
+        bad[int(table[0, 5]), 0, 3, 7] = float("inf")
+        bad[int(table[0, 6]), 1, 4, 9] = float("nan")
+        got = kv.prefix_attention(q, k, bad, table, n, 1500)
+        off = ~torch.isfinite(got)
+        assert bool(off[:, :4, 7].all()) and bool(off[:, 4:, 9].all()) and int(off.sum()) == 20 * 8
+        worse = k.clone()
+        worse[int(table[0, 5]), 0, 3] = float("nan")
+        got = kv.prefix_attention(q, worse, v, table, n, 1500)
+        assert bool(got[:, :4].isnan().all()) and bool(torch.isfinite(got[:, 4:]).all())
+
+
+def test_prefix_strides_streams_graphs_and_workspaces(kv):
+    b, prefix = 12, 333
+    lens = [prefix + 5 * i for i in range(b)]
+    problem = _prefix_problem(lens, prefix, 8, 2, 64, 16, torch.bfloat16, torch.bfloat16)
+    q, k, v, table, n, scales = problem
+    want = _prefix_holds(kv, problem, prefix)
+    wide = torch.zeros(b, 11, 64, device="cuda", dtype=q.dtype)
+    wide[:, 1:9] = q
+    out = torch.full_like(q, 7.0)
+    assert kv.prefix_attention(wide[:, 1:9], k, v, table, n, prefix, out=out) is out and torch.equal(out, want)
+    head_last = k.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)  # [pages, page, heads, d] in memory
+    value_last = v.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)
+    assert torch.equal(kv.prefix_attention(q, head_last, value_last, table, n, prefix), want)
+    odd = torch.zeros(b, 8, 65, device="cuda", dtype=q.dtype)[..., 1:].copy_(q)
+    assert torch.equal(kv.prefix_attention(odd, k, v, table, n, prefix), want)
+    # two graphs and an eager call on two streams, each with its own workspace
+    shared = torch.tensor([prefix], dtype=torch.int32, device="cuda")
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = kv.prefix_attention(q, k, v, table, n, shared)
+        graphs.append((graph, held))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        graphs[0][0].replay()
+        with torch.cuda.stream(side):
+            graphs[1][0].replay()
+            mine = kv.prefix_attention(q, k, v, table, n, prefix)
+    torch.cuda.synchronize()
+    assert torch.equal(graphs[0][1], want) and torch.equal(graphs[1][1], want) and torch.equal(mine, want)
+    shared.fill_(200)                                                   # a captured step reads the prefix anew
+    graphs[0][0].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(graphs[0][1], kv.prefix_attention(q, k, v, table, n, 200))
+    empty = kv.prefix_attention(q[:0], k, v, table, n, prefix)
+    assert empty.shape == (0, 8, 64)
+    assert _status() == (0, 0)
+
+
+def test_prefix_offsets_past_32_bits(kv):
+    """Pages more than 2^32 bytes into a cache."""
+    pages, page, hk, d = 140_000, 16, 8, 128                            # 4.6 GB each
+    k = torch.zeros(pages, hk, page, d, dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros_like(k)
+    g = _gen(11)
+    ids = torch.tensor([pages - 1 - 5 * i for i in range(40)], dtype=torch.int32)
+    for p in ids.tolist():
+        k[p], v[p] = (torch.randn(hk, page, d, generator=g, device="cuda").bfloat16() for _ in range(2))
+    table = torch.full((3, 24), -1, dtype=torch.int32)
+    table[:, :20] = ids[:20]
+    for r in range(3):
+        table[r, 20:24] = ids[20 + 4 * r: 24 + 4 * r]
+    lens = torch.tensor([330, 384, 321], dtype=torch.int32, device="cuda")
+    q = torch.randn(3, 16, d, generator=g, device="cuda").bfloat16()
+    _prefix_holds(kv, (q, k, v, table.cuda(), lens, [None, None]), 320)
+
+
+def _status():
+    from comfy_quant_bench_b200 import _lib
+    torch.cuda.synchronize()
+    return _lib.take_device_status()
