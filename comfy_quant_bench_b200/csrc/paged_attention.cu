@@ -293,7 +293,10 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
     static_cast<pattn::Meta*>(a.ws)[blockIdx.x] = m;
   }
   it.v = row_view(a, it.b);
-  if (count == 0 && (!kCluster || it.v.units == 0)) return;
+  if (count == 0 && (!kCluster || it.v.units == 0)) {
+    if (a.out32 != nullptr) grid_dep_wait();
+    return;
+  }
 
   // ---- the warp's ring ----------------------------------------------------------------------
   uint8_t* my_ring = ring + warp * kStages * C::kStageBytes;
@@ -687,6 +690,9 @@ __global__ void __launch_bounds__(pattn::kWarps * 32, pattn::Cfg<D, FP8 ? 1 : 2,
     // a CTA's part stays until every rank has read it
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
+  // behind a shared prefix this grid may run beside the one before it: it ends after that, so that what waits for this one
+  // finds the results of both
+  if (a.out32 != nullptr) grid_dep_wait();
 }
 
 // Joins the parts of a row that several CTAs shared, in their order.  CTA (r, h): the segment whose first boundary
@@ -784,7 +790,7 @@ cudaError_t run_paged_attention(const PagedAttnArgs& a, cudaStream_t st) {
   const int group = a.Hq / a.Hkv, tiles = (group + 8 * NT - 1) / (8 * NT);
   const Deal deal = deal_units(a.B, a.Hq, a.Hkv, static_cast<int64_t>(a.table_width) * a.page_size, a.window, a.sinks);
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
@@ -797,6 +803,9 @@ cudaError_t run_paged_attention(const PagedAttnArgs& a, cudaStream_t st) {
     cfg.dynamicSmemBytes = C::kSmem;
     auto kern = paged_attention_kernel<F16, FP8, D, NT, true>;
     static unsigned long long devices = 0;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = a.out32 != nullptr ? 2 : 1;          // beside the kernel of the shared prefix
     const cudaError_t e = allow_shared(kern, C::kSmem, devices);
     return e != cudaSuccess ? e : cudaLaunchKernelEx(&cfg, kern, a, tiles, deal.mode, deal.cluster);
   }
@@ -809,8 +818,12 @@ cudaError_t run_paged_attention(const PagedAttnArgs& a, cudaStream_t st) {
   const int64_t most = deal.mode == pattn::kSegments ? deal.segs
                                                      : deal.segs * ((deal.units + pattn::kMinUnits - 1) / pattn::kMinUnits);
   if (most < grid) grid = most;
-  kern<<<static_cast<unsigned>(grid), pattn::kWarps * 32, C::kSmem, st>>>(a, tiles, deal.mode, 1);
-  e = cudaGetLastError();
+  if (a.out32 != nullptr) {                             // beside the kernel of the shared prefix
+    e = launch_early(kern, dim3(static_cast<unsigned>(grid)), pattn::kWarps * 32, C::kSmem, st, a, tiles, deal.mode, 1);
+  } else {
+    kern<<<static_cast<unsigned>(grid), pattn::kWarps * 32, C::kSmem, st>>>(a, tiles, deal.mode, 1);
+    e = cudaGetLastError();
+  }
   if (e != cudaSuccess || deal.mode != pattn::kRuns || grid == 1) return e;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;

@@ -16,6 +16,8 @@
 //
 // Weights enter P V in 16 bits: one part of the type (an error like that of rounding the output), or two parts, which adds
 // half to the product's work, where the batch has no more rows than one CTA takes and HBM is the limit.
+#include <type_traits>
+
 #include "decode_common.cuh"
 
 namespace cq {
@@ -32,15 +34,16 @@ struct Cfg {
   static constexpr int kLag = D == 64 ? 3 : 1;               // loads in flight before one is waited for
   static constexpr int kStageBytes = kKeys * D * 2;
   static constexpr int kQBytes = kRows * D * 2;
+  // warpgroups: softmax of each slot, gathers, products (one warp works)
   static constexpr int kSoftWarps = 4 * kSlots;
-  static constexpr int kMmaWarp = kSoftWarps, kLoadWarp = kSoftWarps + 1;
-  static constexpr int kThreads = 32 * (kSoftWarps + 5);
-  static constexpr int kSmem = kSlots * kQBytes + kStages * kStageBytes + 1024 + 256;
+  static constexpr int kLoadWarp = kSoftWarps, kMmaWarp = kSoftWarps + 4;
+  static constexpr int kThreads = 32 * (kSoftWarps + 8);
+  static constexpr int kSmem = kSlots * kQBytes + kStages * kStageBytes + 256;
   static constexpr uint32_t kCols = 512;
   static constexpr int kSCols = kKeys;                       // columns of a score buffer
   static_assert(kSlots * (kBufs * kSCols + D) <= 512, "tensor memory");
 };
-// floats of a row tile's part: O as [D / 4][128 rows][4], then the rows' maxima and sums
+// floats of a row tile's part: O as [D / 4][128 rows][4], then the rows' (maximum, sum)
 __host__ __device__ constexpr int64_t part_floats(int d) { return 128ll * d + 256; }
 }  // namespace pfx
 
@@ -69,9 +72,32 @@ __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[
 __device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   mma_bf16(d_tmem, adesc, bdesc, idesc, accumulate);         // kind::f16: the descriptor names the type
 }
+// mbar_wait_short all inline: a kernel that moves registers between its warps has room for no call
+__device__ __forceinline__ bool thread_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int where) {
+  unsigned long long since = 0;
+  for (uint32_t i = 1;; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    if (ok) return true;
+    if ((i & 255u) == 0) {
+      const unsigned long long now = globaltimer_ns();
+      if (since == 0) since = now;
+      if (*abort_flag) return false;
+      if (now - since > kWaitLimitNs) {
+        record_status(CQ_ERR_TIMEOUT, where);
+        *abort_flag = 1;
+        return false;
+      }
+    }
+  }
+}
 // a wait of a whole warp: all lanes go on, or none does
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int where) {
-  return __all_sync(0xffffffffu, mbar_wait_short(bar, parity, abort_flag, where));
+  return __all_sync(0xffffffffu, thread_wait(bar, parity, abort_flag, where));
 }
 // four e4m3 values as two pairs of the type, exactly
 template <bool F16>
@@ -105,8 +131,10 @@ template <bool F16, bool FP8, int D, int PARTS>
 __global__ void __launch_bounds__(pfx::Cfg<D>::kThreads, 1) prefix_attention_kernel(const PrefixArgs a) {
   using C = pfx::Cfg<D>;
   constexpr int kKeys = C::kKeys, kStages = C::kStages, kSlots = C::kSlots, kBufs = C::kBufs;
-  extern __shared__ __align__(128) uint8_t smem_any[];
-  uint8_t* smem = smem_any + ((1024 - (smem_u32(smem_any) & 1023)) & 1023);
+  // with two slots the gathers and products give registers to the softmax, whose threads hold a row of scores
+  constexpr int kSoftRegs = FP8 ? 168 : 184, kLoadRegs = FP8 ? 104 : 72, kMmaRegs = 72;
+  static_assert(2 * kSoftRegs + kLoadRegs + kMmaRegs <= 4 * 128, "the registers that 512 threads are launched with");
+  extern __shared__ __align__(1024) uint8_t smem[];           // the kernel has no other shared memory: it begins aligned
   uint8_t* q_at = smem;
   uint8_t* ring = smem + kSlots * C::kQBytes;
   uint64_t* full = reinterpret_cast<uint64_t*>(ring + kStages * C::kStageBytes);
@@ -114,8 +142,8 @@ __global__ void __launch_bounds__(pfx::Cfg<D>::kThreads, 1) prefix_attention_ker
   uint64_t* q_full = empty + kStages;
   uint64_t* q_empty = q_full + 1;
   uint64_t* s_full = q_empty + 1;                             // [kSlots * kBufs] scores are in tensor memory
-  uint64_t* p_full = s_full + 2;                              // [..] weights are
-  uint64_t* o_done = p_full + 2;                              // [kSlots] a product with the values is done
+  uint64_t* p_full = s_full + 2;                              // [..][2] half of the weights are
+  uint64_t* o_done = p_full + 4;                              // [kSlots] a product with the values is done
   uint64_t* all_done = o_done + 2;
   uint32_t* holder = reinterpret_cast<uint32_t*>(all_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(holder + 1);
@@ -133,7 +161,8 @@ __global__ void __launch_bounds__(pfx::Cfg<D>::kThreads, 1) prefix_attention_ker
     mbar_init(q_empty, 1);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 4);
+      mbar_init(&p_full[2 * s], 4);
+      mbar_init(&p_full[2 * s + 1], 4);
       mbar_init(&o_done[s], 1);
     }
     mbar_init(all_done, 1);
@@ -157,7 +186,8 @@ __global__ void __launch_bounds__(pfx::Cfg<D>::kThreads, 1) prefix_attention_ker
   const bool pair = kSlots == 2 && tile0 + 1 < tiles;         // two row tiles, or one that both slots share
   const int key_tiles = leader < 0 ? 0 : (prefix + kKeys - 1) / kKeys;
   const int64_t units = static_cast<int64_t>(g.Hkv) * key_tiles;
-  const int64_t u0 = team * units / a.teams, u1 = (team + 1) * units / a.teams;
+  const int64_t teams = min(static_cast<int64_t>(a.teams), units);     // each with a key tile or more
+  const int64_t u0 = team < teams ? team * units / teams : 0, u1 = team < teams ? (team + 1) * units / teams : 0;
   const int64_t padded = static_cast<int64_t>(a.members) * kSlots;
 
   struct Segment {
@@ -174,7 +204,97 @@ __global__ void __launch_bounds__(pfx::Cfg<D>::kThreads, 1) prefix_attention_ker
   const int* table = g.table + row_of_leader * g.table_stride;
   const int page_shift = 31 - __clz(g.page_size), page_mask = g.page_size - 1;
 
-  if (warp >= C::kLoadWarp) {
+  if (warp >= C::kMmaWarp) {
+    if constexpr (kSlots == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
+    // ---- products, by one thread ----
+    if (warp == C::kMmaWarp && elect_one()) {
+      constexpr uint32_t type = F16 ? 0u : (1u << 7) | (1u << 10);
+      constexpr uint32_t idesc_s = (1u << 4) | type | (static_cast<uint32_t>(kKeys >> 3) << 17) | (8u << 24);
+      constexpr uint32_t idesc_o = (1u << 4) | type | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) | (8u << 24);
+      int base = 0;                                           // ring loads before this segment
+      uint32_t q_phase = 0, p_phase[2] = {0, 0}, o_phase[2] = {0, 0};
+      bool ok = true;
+      for (int64_t u = u0; u < u1 && ok;) {
+        const Segment seg = segment(u);
+        const int jobs = pair ? 2 * seg.n : seg.n;            // job i: slot i & 1 (where there are two)
+        auto tile_of = [&](int i) { return pair ? i >> 1 : i; };
+        auto last_of_tile = [&](int i) { return !pair || (i & 1); };
+        auto scores = [&](int i) {
+          const int slot = kSlots == 2 ? i & 1 : 0, buf = kBufs == 2 ? i & 1 : slot;
+          const int l = base + 2 * tile_of(i), stage = l % kStages;
+          if (!thread_wait(&full[stage], (l / kStages) & 1, abort_flag, pfx::kSite + 2)) return false;
+          tc_fence_after();
+          const uint64_t q = smem_desc_k_sw128(smem_u32(q_at + (pair ? slot : 0) * C::kQBytes));
+          const uint64_t k = smem_desc_k_sw128(smem_u32(ring + stage * C::kStageBytes));
+#pragma unroll
+          for (int x = 0; x < D / 16; ++x)
+            mma_f16_ss(s_col + buf * C::kSCols, q + ((x >> 2) * (pfx::kRows * 128) + (x & 3) * 32) / 16,
+                       k + ((x >> 2) * (kKeys * 128) + (x & 3) * 32) / 16, idesc_s, x != 0);
+          tc_commit(&s_full[buf]);
+          if (last_of_tile(i)) tc_commit(&empty[stage]);
+          if (i + 1 == jobs) tc_commit(q_empty);
+          return true;
+        };
+        ok = thread_wait(q_full, q_phase, abort_flag, pfx::kSite + 3);
+        q_phase ^= 1u;
+        if (!ok) break;
+        const int ahead = kSlots == 2 ? 2 : 1;                // jobs whose scores come before a job's weights
+        for (int i = 0; i < min(ahead, jobs) && ok; ++i) ok = scores(i);
+        for (int i = 0; i < jobs && ok; ++i) {
+          const int slot = kSlots == 2 ? i & 1 : 0, buf = kBufs == 2 ? i & 1 : slot;
+          if (kBufs == 2 && i + 1 < jobs) {
+            // the other buffer's weights are consumed when the product before is done
+            if (i > 0) {
+              ok = thread_wait(&o_done[0], o_phase[0], abort_flag, pfx::kSite + 4);
+              o_phase[0] ^= 1u;
+            }
+            ok = ok && scores(i + 1);
+            if (!ok) break;
+          } else if (kBufs == 2 && i > 0) {
+            ok = thread_wait(&o_done[0], o_phase[0], abort_flag, pfx::kSite + 4);
+            o_phase[0] ^= 1u;
+            if (!ok) break;
+          }
+          const int l = base + 2 * tile_of(i) + 1, stage = l % kStages;
+          if (!(ok = thread_wait(&full[stage], (l / kStages) & 1, abort_flag, pfx::kSite + 5))) break;
+          const uint32_t v = smem_u32(ring + stage * C::kStageBytes);
+          const bool first = kSlots == 2 ? i < 2 : i == 0;
+#pragma unroll
+          for (int x = 0; x < kKeys / 16; ++x) {
+            if (x % (kKeys / 32) == 0) {
+              if (!(ok = thread_wait(&p_full[2 * buf + x / (kKeys / 32)], p_phase[buf], abort_flag, pfx::kSite + 6))) break;
+              tc_fence_after();
+            }
+            const uint64_t vd = smem_desc_mn_sw128(v + x * 2048, kKeys * 128);
+            const uint32_t p = s_col + buf * C::kSCols + 32 * (x >> 1) + 8 * (x & 1);
+            mma_f16_ts(o_col + slot * D, p, vd, idesc_o, !first || x != 0);
+            if constexpr (PARTS == 2) mma_f16_ts(o_col + slot * D, p + 16, vd, idesc_o, 1);
+          }
+          p_phase[buf] ^= 1u;
+          if (!ok) break;
+          tc_commit(&o_done[slot]);
+          if (last_of_tile(i)) tc_commit(&empty[stage]);
+          if (kSlots == 2 && i + 2 < jobs) {
+            // this slot's scores take the place of the weights just used
+            ok = thread_wait(&o_done[slot], o_phase[slot], abort_flag, pfx::kSite + 7) && scores(i + 2);
+            o_phase[slot] ^= 1u;
+          }
+        }
+        // the segment's last products: the next one's scores take the place of their weights
+        for (int i = max(0, jobs - kSlots); i < jobs && ok; ++i) {
+          const int slot = kSlots == 2 ? i & 1 : 0;
+          ok = thread_wait(&o_done[slot], o_phase[slot], abort_flag, pfx::kSite + 4);
+          o_phase[slot] ^= 1u;
+        }
+        base += 2 * seg.n;
+        u += seg.n;
+      }
+      tc_commit(all_done);
+      mbar_wait_drain(all_done, 0, 50000000ull);
+    }
+    __syncwarp();
+  } else if (warp >= C::kLoadWarp) {
+    if constexpr (kSlots == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
     // ---- gathers: Q of a segment, then its keys and values, tile by tile ----
     const int w = warp - C::kLoadWarp;
     constexpr int kChunks = D / 8;                            // 16-byte chunks of a 16-bit row
@@ -210,8 +330,11 @@ __global__ void __launch_bounds__(pfx::Cfg<D>::kThreads, 1) prefix_attention_ker
         }
       }
       cp_async_commit();
-      cp_async_wait<0>();
-      hand_over(q_full);
+      bool q_landed = false;
+      if constexpr (FP8) {
+        cp_async_wait<0>();
+        hand_over(q_full);
+      }
       const int64_t head_at = seg.head * g.head_stride;
       constexpr int kPerWarp = kKeys / 4;                     // keys of a warp: 32 or 16
       for (int j = seg.j0; j < seg.j0 + seg.n && ok; ++j) {
@@ -238,6 +361,11 @@ __global__ void __launch_bounds__(pfx::Cfg<D>::kThreads, 1) prefix_attention_ker
             }
             cp_async_commit();
             ++load;
+            if (!q_landed) {                                  // the first keys are on their way behind it
+              cp_async_wait<1>();
+              hand_over(q_full);
+              q_landed = true;
+            }
             if (load - landed > C::kLag) {
               cp_async_wait<C::kLag>();
               hand_over(&full[landed % kStages]);
@@ -287,94 +415,9 @@ __global__ void __launch_bounds__(pfx::Cfg<D>::kThreads, 1) prefix_attention_ker
       u += seg.n;
     }
     cp_async_wait<0>();
-  } else if (warp == C::kMmaWarp) {
-    // ---- products, by one thread ----
-    if (elect_one()) {
-      constexpr uint32_t type = F16 ? 0u : (1u << 7) | (1u << 10);
-      constexpr uint32_t idesc_s = (1u << 4) | type | (static_cast<uint32_t>(kKeys >> 3) << 17) | (8u << 24);
-      constexpr uint32_t idesc_o = (1u << 4) | type | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) | (8u << 24);
-      int base = 0;                                           // ring loads before this segment
-      uint32_t q_phase = 0, p_phase[2] = {0, 0}, o_phase[2] = {0, 0};
-      bool ok = true;
-      for (int64_t u = u0; u < u1 && ok;) {
-        const Segment seg = segment(u);
-        const int jobs = pair ? 2 * seg.n : seg.n;            // job i: slot i & 1 (where there are two)
-        auto tile_of = [&](int i) { return pair ? i >> 1 : i; };
-        auto last_of_tile = [&](int i) { return !pair || (i & 1); };
-        auto scores = [&](int i) {
-          const int slot = kSlots == 2 ? i & 1 : 0, buf = kBufs == 2 ? i & 1 : slot;
-          const int l = base + 2 * tile_of(i), stage = l % kStages;
-          if (!mbar_wait_short(&full[stage], (l / kStages) & 1, abort_flag, pfx::kSite + 2)) return false;
-          tc_fence_after();
-          const uint64_t q = smem_desc_k_sw128(smem_u32(q_at + (pair ? slot : 0) * C::kQBytes));
-          const uint64_t k = smem_desc_k_sw128(smem_u32(ring + stage * C::kStageBytes));
-#pragma unroll
-          for (int x = 0; x < D / 16; ++x)
-            mma_f16_ss(s_col + buf * C::kSCols, q + ((x >> 2) * (pfx::kRows * 128) + (x & 3) * 32) / 16,
-                       k + ((x >> 2) * (kKeys * 128) + (x & 3) * 32) / 16, idesc_s, x != 0);
-          tc_commit(&s_full[buf]);
-          if (last_of_tile(i)) tc_commit(&empty[stage]);
-          if (i + 1 == jobs) tc_commit(q_empty);
-          return true;
-        };
-        ok = mbar_wait_short(q_full, q_phase, abort_flag, pfx::kSite + 3);
-        q_phase ^= 1u;
-        if (!ok) break;
-        const int ahead = kSlots == 2 ? 2 : 1;                // jobs whose scores come before a job's weights
-        for (int i = 0; i < min(ahead, jobs) && ok; ++i) ok = scores(i);
-        for (int i = 0; i < jobs && ok; ++i) {
-          const int slot = kSlots == 2 ? i & 1 : 0, buf = kBufs == 2 ? i & 1 : slot;
-          if (kBufs == 2 && i + 1 < jobs) {
-            // the other buffer's weights are consumed when the product before is done
-            if (i > 0) {
-              ok = mbar_wait_short(&o_done[0], o_phase[0], abort_flag, pfx::kSite + 4);
-              o_phase[0] ^= 1u;
-            }
-            ok = ok && scores(i + 1);
-            if (!ok) break;
-          } else if (kBufs == 2 && i > 0) {
-            ok = mbar_wait_short(&o_done[0], o_phase[0], abort_flag, pfx::kSite + 4);
-            o_phase[0] ^= 1u;
-            if (!ok) break;
-          }
-          const int l = base + 2 * tile_of(i) + 1, stage = l % kStages;
-          ok = mbar_wait_short(&full[stage], (l / kStages) & 1, abort_flag, pfx::kSite + 5) &&
-               mbar_wait_short(&p_full[buf], p_phase[buf], abort_flag, pfx::kSite + 6);
-          p_phase[buf] ^= 1u;
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t v = smem_u32(ring + stage * C::kStageBytes);
-          const bool first = kSlots == 2 ? i < 2 : i == 0;
-#pragma unroll
-          for (int x = 0; x < kKeys / 16; ++x) {
-            const uint64_t vd = smem_desc_mn_sw128(v + x * 2048, kKeys * 128);
-            const uint32_t p = s_col + buf * C::kSCols + 32 * (x >> 1) + 8 * (x & 1);
-            mma_f16_ts(o_col + slot * D, p, vd, idesc_o, !first || x != 0);
-            if constexpr (PARTS == 2) mma_f16_ts(o_col + slot * D, p + 16, vd, idesc_o, 1);
-          }
-          tc_commit(&o_done[slot]);
-          if (last_of_tile(i)) tc_commit(&empty[stage]);
-          if (kSlots == 2 && i + 2 < jobs) {
-            // this slot's scores take the place of the weights just used
-            ok = mbar_wait_short(&o_done[slot], o_phase[slot], abort_flag, pfx::kSite + 7) && scores(i + 2);
-            o_phase[slot] ^= 1u;
-          }
-        }
-        // the segment's last products: the next one's scores take the place of their weights
-        for (int i = max(0, jobs - kSlots); i < jobs && ok; ++i) {
-          const int slot = kSlots == 2 ? i & 1 : 0;
-          ok = mbar_wait_short(&o_done[slot], o_phase[slot], abort_flag, pfx::kSite + 4);
-          o_phase[slot] ^= 1u;
-        }
-        base += 2 * seg.n;
-        u += seg.n;
-      }
-      tc_commit(all_done);
-      mbar_wait_drain(all_done, 0, 50000000ull);
-    }
-    __syncwarp();
   } else {
     // ---- softmax: thread = row of the slot's tile ----
+    if constexpr (kSlots == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
     const int slot = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     constexpr float kLift = F16 ? 7.0f : 0.0f;                // f16 weights reach 2^15: up to 2^8 above the running maximum
@@ -387,19 +430,20 @@ __global__ void __launch_bounds__(pfx::Cfg<D>::kThreads, 1) prefix_attention_ker
       float m = -INFINITY, l = 0.0f;
       const int step = kSlots == 2 && !pair ? 2 : 1;          // key tiles of this slot: first, first + step, ...
       int done = 0;
-      for (int j = kSlots == 2 && !pair ? slot : 0; j < seg.n && ok; j += step, ++done) {
-        const int buf = kBufs == 2 ? done & 1 : slot;
-        const int key0 = (seg.j0 + j) * kKeys;
-        // which keys are there: looked up while the scores are on their way
-        int page[kKeys / 32];
+      // which keys of a tile are there: looked up a tile ahead
+      int page[kKeys / 32];
+      auto look_up = [&](int j) {
 #pragma unroll
         for (int x = 0; x < kKeys / 32; ++x) {
-          const int key = key0 + 32 * x + lane;
-          page[x] = key < prefix ? __ldg(table + (key >> page_shift)) : -1;
+          const int key = (seg.j0 + j) * kKeys + 32 * x + lane;
+          page[x] = j < seg.n && key < prefix ? __ldg(table + (key >> page_shift)) : -1;
         }
+      };
+      look_up(kSlots == 2 && !pair ? slot : 0);
+      for (int j = kSlots == 2 && !pair ? slot : 0; j < seg.n && ok; j += step, ++done) {
+        const int buf = kBufs == 2 ? done & 1 : slot;
         if (!(ok = warp_wait(&s_full[buf], s_phase[buf], abort_flag, pfx::kSite + 8))) break;
         s_phase[buf] ^= 1u;
-        __syncwarp();
         tc_fence_after();
         uint32_t masks[kKeys / 32];
         bool whole = true;
@@ -408,28 +452,33 @@ __global__ void __launch_bounds__(pfx::Cfg<D>::kThreads, 1) prefix_attention_ker
           masks[x] = __ballot_sync(0xffffffffu, page[x] >= 0 && page[x] < g.num_pages);
           whole = whole && masks[x] == 0xffffffffu;
         }
+        look_up(j + step);
         const uint32_t s_at = s_col + buf * C::kSCols + lanes;
-        float top = -INFINITY;
-        uint32_t v[32];
+        // half a row of scores; the largest, NaN where one is
+        uint32_t v[kKeys / 32][32];
 #pragma unroll
-        for (int x = 0; x < kKeys / 32; ++x) {
-          tmem_ld_32x32b_x32(s_at + 32 * x, v);
-          tmem_wait_ld_dep(v);
-          if (whole) {
+        for (int x = 0; x < kKeys / 32; ++x) tmem_ld_32x32b_x32(s_at + 32 * x, v[x]);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(v[i]) * mul);
-          } else {
+        for (int x = 0; x < kKeys / 32; ++x) tmem_wait_ld_dep(v[x]);
+        float top = -INFINITY, top2 = -INFINITY;
+        auto largest = [&](auto whole_tile, float sign) {     // a negative scale turns the order around
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (masks[x] >> i & 1u) top = fmaxf(top, __uint_as_float(v[i]) * mul);
-          }
-        }
+          for (int x = 0; x < kKeys / 32; ++x)
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float s0 = __uint_as_float(v[x][i]) * sign, s1 = __uint_as_float(v[x][i + 1]) * sign;
+              if (whole_tile || masks[x] >> i & 1u) top = fmaxf(top, s0);
+              if (whole_tile || masks[x] >> (i + 1) & 1u) top2 = fmaxf(top2, s1);
+            }
+        };
+        if (whole && mul >= 0.0f) largest(std::true_type{}, 1.0f);
+        else largest(std::false_type{}, mul < 0.0f ? -1.0f : 1.0f);
+        top = fmaxf(top, top2);
+        top = top == -INFINITY ? top : top * fabsf(mul);
         const bool raise = top > m + kSlackUp || (m == -INFINITY && top > m);
         if (kBufs == 2 && done > 0) {                         // the product before still adds to O
-          ok = warp_wait(&o_done[slot], o_phase, abort_flag, pfx::kSite + 9);
+          if (!(ok = warp_wait(&o_done[slot], o_phase, abort_flag, pfx::kSite + 9))) break;
           o_phase ^= 1u;
-          if (!ok) break;
-          __syncwarp();
           tc_fence_after();
         }
         if (__any_sync(0xffffffffu, raise)) {
@@ -438,70 +487,79 @@ __global__ void __launch_bounds__(pfx::Cfg<D>::kThreads, 1) prefix_attention_ker
           l *= f;
           if (done > 0) {
 #pragma unroll 1
-            for (int x = 0; x < D / 32; ++x) {
-              tmem_ld_32x32b_x32(o_col + slot * D + lanes + 32 * x, v);
-              tmem_wait_ld_dep(v);
+            for (int x = 0; x < D / 16; ++x) {
+              uint32_t o[16];
+              const uint32_t at = o_col + slot * D + lanes + 16 * x;
+              tmem_ld_x16(at, o);
+              tmem_wait_ld_x16(o);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-              tmem_st_x32(o_col + slot * D + lanes + 32 * x, v);
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tmem_st_x16(at, o);
             }
           }
         }
         const float base = (m == -INFINITY ? 0.0f : m) - kLift;
+        float2 sums[2] = {};
+        auto weights = [&](auto whole_tile) {
 #pragma unroll
-        for (int x = 0; x < kKeys / 32; ++x) {
-          tmem_ld_32x32b_x32(s_at + 32 * x, v);
-          tmem_wait_ld_dep(v);
-          uint32_t p[32];                                     // the first part's pairs, then the second's
+          for (int x = 0; x < kKeys / 32; ++x) {
+            uint32_t p[PARTS == 2 ? 32 : 16];                 // the first part's pairs, then the second's
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            float p0 = exp2_fast(fmaf(__uint_as_float(v[i]), mul, -base)), p1 = exp2_fast(fmaf(__uint_as_float(v[i + 1]), mul, -base));
-            if (!whole) {
-              p0 = masks[x] >> i & 1u ? p0 : 0.0f;
-              p1 = masks[x] >> (i + 1) & 1u ? p1 : 0.0f;
+            for (int i = 0; i < 32; i += 2) {
+              const float2 y = fma2(make_float2(__uint_as_float(v[x][i]), __uint_as_float(v[x][i + 1])), make_float2(mul, mul), make_float2(-base, -base));
+              float2 w = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+              if (!whole_tile) {
+                w.x = masks[x] >> i & 1u ? w.x : 0.0f;
+                w.y = masks[x] >> (i + 1) & 1u ? w.y : 0.0f;
+              }
+              sums[i / 2 & 1] = fma2(w, make_float2(1.0f, 1.0f), sums[i / 2 & 1]);
+              p[i / 2] = narrow16<F16>(w.x, w.y);
+              if constexpr (PARTS == 2) {
+                const float2 rest = fma2(widen16<F16>(p[i / 2]), make_float2(-1.0f, -1.0f), w);
+                p[16 + i / 2] = narrow16<F16>(rest.x, rest.y);
+              }
             }
-            l += p0 + p1;
-            if constexpr (PARTS == 2) split16<F16>(p0, p1, p[i / 2], p[16 + i / 2]);
-            else p[i / 2] = narrow16<F16>(p0, p1);
+            if constexpr (PARTS == 2) tmem_st_x32(s_at + 32 * x, p);
+            else tmem_st_x16(s_at + 32 * x, p);
+            if ((x + 1) % (kKeys / 64) == 0) {                // a half: the product may begin with it
+              tmem_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&p_full[2 * buf + x / (kKeys / 64)]);
+            }
           }
-          if constexpr (PARTS == 2) tmem_st_x32(s_at + 32 * x, p);
-          else tmem_st_x16(s_at + 32 * x, reinterpret_cast<const uint32_t(&)[16]>(p));
-        }
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[buf]);
+        };
+        if (whole) weights(std::true_type{});
+        else weights(std::false_type{});
+        l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
       }
-      if (!ok) break;
       // ---- this run's sums ----
+      if (!ok) break;
       if (done > 0) {
         // the last product; earlier ones are done (their phases: one for every product of this slot)
         if (kBufs == 1) {
-          const uint32_t last = (o_phase + static_cast<uint32_t>(done) - 1u) & 1u;
-          ok = warp_wait(&o_done[slot], last, abort_flag, pfx::kSite + 10);
+          ok = warp_wait(&o_done[slot], (o_phase + static_cast<uint32_t>(done) - 1u) & 1u, abort_flag, pfx::kSite + 10);
           o_phase = (o_phase + static_cast<uint32_t>(done)) & 1u;
         } else {
           ok = warp_wait(&o_done[slot], o_phase, abort_flag, pfx::kSite + 10);
           o_phase ^= 1u;
         }
         if (!ok) break;
-        __syncwarp();
         tc_fence_after();
       }
       float* part = a.parts + ((team + seg.head) * padded + tile0 + slot) * pfx::part_floats(D);
       if (done > 0) {
 #pragma unroll 1
-        for (int x = 0; x < D / 32; ++x) {
-          uint32_t v[32];
-          tmem_ld_32x32b_x32(o_col + slot * D + lanes + 32 * x, v);
-          tmem_wait_ld_dep(v);
+        for (int x = 0; x < D / 16; ++x) {
+          uint32_t o[16];
+          tmem_ld_x16(o_col + slot * D + lanes + 16 * x, o);
+          tmem_wait_ld_x16(o);
 #pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            reinterpret_cast<uint4*>(part)[(8 * x + i / 4) * pfx::kRows + row] = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+          for (int i = 0; i < 16; i += 4)
+            reinterpret_cast<uint4*>(part)[(4 * x + i / 4) * pfx::kRows + row] = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
         }
       }
-      part[128 * D + row] = m;
-      part[128 * D + 128 + row] = l;
+      reinterpret_cast<float2*>(part + 128 * D)[row] = make_float2(m, l);
       tc_fence_before();
       u += seg.n;
     }
@@ -511,67 +569,90 @@ __global__ void __launch_bounds__(pfx::Cfg<D>::kThreads, 1) prefix_attention_ker
   if (warp == C::kMmaWarp) tmem_dealloc(tmem, C::kCols);
 }
 
-// Joins a row's runs over the prefix, in their order, with its own tokens.  A block: 128 rows of a row tile, one head, 16
-// columns; thread = row.
+// Joins a row's runs over the prefix, in their order, with its own tokens.  A block: 128 rows of a row tile, one head, eight
+// columns; thread = row.  What the runs left is in L2: eight runs' loads are in flight at a time.
 template <bool F16, int D>
 __global__ void __launch_bounds__(128) prefix_join_kernel(const PrefixArgs a) {
   using C = pfx::Cfg<D>;
-  constexpr int kKeys = C::kKeys;
+  constexpr int kKeys = C::kKeys, kAtOnce = 8;
   const PagedAttnArgs& g = a.own;
-  const int tile = blockIdx.x, head = blockIdx.y, d4 = blockIdx.z * 4, tid = threadIdx.x;
+  const int tile = blockIdx.x, head = blockIdx.y, d4 = blockIdx.z * 2, tid = threadIdx.x;
   const int group = g.Hq / g.Hkv, rows = g.B * group, tiles = (rows + pfx::kRows - 1) / pfx::kRows;
-  grid_dep_wait();
-  const int at = tile * pfx::kRows + tid;
-  if (at >= rows) return;
-  const int b = at / group, h = head * group + at - b * group;
   const int prefix = max(0, min(prefix_of(g), g.table_width * g.page_size));
-  const int row = g.rows != nullptr ? g.rows[b] : b;
-  const int n = row >= 0 && row < g.table_rows ? min(g.lens[row], g.table_width * g.page_size) : 0;
-  const bool joined = prefix > 0 && n >= prefix;
-  const int64_t own = static_cast<int64_t>(b) * g.Hq + h;
-  const float own_lse = g.lse[own] * 1.4426950408889634f;     // as a power of 2; -inf without tokens of its own
-  float top = own_lse, sum = 0.0f;
   const int key_tiles = (prefix + kKeys - 1) / kKeys;
   const int64_t units = static_cast<int64_t>(g.Hkv) * key_tiles, padded = static_cast<int64_t>(a.members) * C::kSlots;
   const int subs = C::kSlots == 2 && tile + 1 == tiles && !(tile & 1) ? 2 : 1;
-  constexpr float kLift = F16 ? 7.0f : 0.0f;
-  auto each_part = [&](auto&& f) {
-    if (!joined) return;
-    for (int64_t x = static_cast<int64_t>(head) * key_tiles; x < static_cast<int64_t>(head + 1) * key_tiles;) {
-      const int64_t team = ((x + 1) * a.teams - 1) / units;
-      for (int s = 0; s < subs; ++s) f(a.parts + ((team + head) * padded + tile + s) * pfx::part_floats(D));
-      x = (team + 1) * units / a.teams;
-    }
-  };
-  each_part([&](const float* p) { top = fmaxf(top, p[128 * D + tid] - kLift); });
+  const int at = tile * pfx::kRows + tid;
+  const bool live = at < rows;
+  const int b = live ? at / group : 0, h = head * group + (live ? at - b * group : 0);
+  const int row = g.rows != nullptr ? g.rows[b] : b;
+  const int n = row >= 0 && row < g.table_rows ? min(g.lens[row], g.table_width * g.page_size) : 0;
+  int parts = 0;
+  const float* first = a.parts;
+  if (live && prefix > 0 && n >= prefix) {                    // the row has the prefix: the teams with a run over this head
+    const int64_t teams = min(static_cast<int64_t>(a.teams), units);
+    const int64_t t0 = ((static_cast<int64_t>(head) * key_tiles + 1) * teams - 1) / units;
+    const int64_t t1 = (static_cast<int64_t>(head + 1) * key_tiles * teams - 1) / units;
+    parts = static_cast<int>(t1 - t0 + 1) * subs;
+    first += ((t0 + head) * padded + tile) * pfx::part_floats(D);
+  }
+  const int64_t stride = padded * pfx::part_floats(D);
+  grid_dep_wait();
+  const int64_t own = static_cast<int64_t>(b) * g.Hq + h;
   const float vs = g.cache_dtype == CQ_DT_FP8_E4M3 && g.v_scale != nullptr ? g.v_scale[head] : 1.0f;
-  float o[16];
-  const float f0 = own_lse == -INFINITY ? 0.0f : exp2f(own_lse - top);
-  sum = own_lse == -INFINITY ? 0.0f : f0;
+  constexpr float kLift = F16 ? 7.0f : 0.0f;
+  // the running maximum is of what the weights were raised by, a power of 2; own tokens first (-inf: none)
+  float top = live ? g.lse[own] * 1.4426950408889634f + kLift : -INFINITY;
+  const bool has_own = top != -INFINITY;
+  float sum = has_own ? 1.0f : 0.0f, o[8];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) o[i] = own_lse == -INFINITY ? 0.0f : g.out32[own * D + 4 * d4 + i] * f0;
-  each_part([&](const float* p) {
-    const float m = p[128 * D + tid], l = p[128 * D + 128 + tid];
-    if (l == 0.0f) return;                                    // a slot without a key tile, or keys that weigh nothing
-    const float f = m == -INFINITY ? 1.0f : exp2f(m - kLift - top);
-    sum += l * f;
+  for (int i = 0; i < 2; ++i) {
+    const float4 v = has_own ? *reinterpret_cast<const float4*>(g.out32 + own * D + 4 * (d4 + i)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    o[4 * i] = v.x, o[4 * i + 1] = v.y, o[4 * i + 2] = v.z, o[4 * i + 3] = v.w;
+  }
+  for (int i0 = 0; i0 < parts; i0 += kAtOnce) {
+    float2 ml[kAtOnce];
+    float4 v[kAtOnce][2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float4 v = reinterpret_cast<const float4*>(p)[(d4 + i) * pfx::kRows + tid];
-      o[4 * i] = fmaf(v.x * vs, f, o[4 * i]);
-      o[4 * i + 1] = fmaf(v.y * vs, f, o[4 * i + 1]);
-      o[4 * i + 2] = fmaf(v.z * vs, f, o[4 * i + 2]);
-      o[4 * i + 3] = fmaf(v.w * vs, f, o[4 * i + 3]);
+    for (int j = 0; j < kAtOnce; ++j) {
+      const int i = min(i0 + j, parts - 1);
+      const float* p = first + (subs == 2 ? i >> 1 : i) * stride + (subs == 2 && (i & 1) ? pfx::part_floats(D) : 0);
+      ml[j] = reinterpret_cast<const float2*>(p + 128 * D)[tid];
+      v[j][0] = reinterpret_cast<const float4*>(p)[d4 * pfx::kRows + tid];
+      v[j][1] = reinterpret_cast<const float4*>(p)[(d4 + 1) * pfx::kRows + tid];
     }
-  });
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  uint32_t out[8];
+    float most = top;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) out[i] = narrow16<F16>(o[2 * i] * inv, o[2 * i + 1] * inv);
-  uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(g.out) + own * D + 4 * d4);
-  to[0] = make_uint4(out[0], out[1], out[2], out[3]);
-  to[1] = make_uint4(out[4], out[5], out[6], out[7]);
-  if (a.lse_out != nullptr && d4 == 0) a.lse_out[own] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) / 1.4426950408889634f;
+    for (int j = 0; j < kAtOnce; ++j)
+      if (i0 + j < parts) most = fmaxf(most, ml[j].x);
+    const float down = top == -INFINITY ? 1.0f : exp2f(top - most);   // -inf so far: what is there weighs nothing, or is NaN
+    sum *= down;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) o[x] *= down;
+    top = most;
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      if (i0 + j >= parts || ml[j].y == 0.0f) continue;       // a slot without a key tile, or keys that weigh nothing
+      const float f = ml[j].x == -INFINITY ? 1.0f : exp2f(ml[j].x - top);
+      sum = fmaf(ml[j].y, f, sum);
+      const float fv = f * vs;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        o[4 * i] = fmaf(v[j][i].x, fv, o[4 * i]);
+        o[4 * i + 1] = fmaf(v[j][i].y, fv, o[4 * i + 1]);
+        o[4 * i + 2] = fmaf(v[j][i].z, fv, o[4 * i + 2]);
+        o[4 * i + 3] = fmaf(v[j][i].w, fv, o[4 * i + 3]);
+      }
+    }
+  }
+  if (!live) return;
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  uint32_t out[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out[i] = narrow16<F16>(o[2 * i] * inv, o[2 * i + 1] * inv);
+  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(g.out) + own * D + 4 * d4) = make_uint4(out[0], out[1], out[2], out[3]);
+  if (a.lse_out != nullptr && d4 == 0)
+    a.lse_out[own] = sum == 0.0f ? -INFINITY : (top - kLift + log2f(sum)) / 1.4426950408889634f;
 }
 
 namespace {
@@ -601,7 +682,7 @@ cudaError_t run_prefix(const PrefixArgs& a, cudaStream_t st) {
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   if ((e = launch_paged_attention(a.own, st)) != cudaSuccess) return e;
   const int group = a.own.Hq / a.own.Hkv, tiles = (a.own.B * group + pfx::kRows - 1) / pfx::kRows;
-  return launch_early(prefix_join_kernel<F16, D>, dim3(tiles, a.own.Hkv, D / 16), 128, 0, st, a);
+  return launch_early(prefix_join_kernel<F16, D>, dim3(tiles, a.own.Hkv, D / 8), 128, 0, st, a);
 }
 template <bool F16, bool FP8, int D>
 cudaError_t pick_prefix(const PrefixArgs& a, cudaStream_t st) {

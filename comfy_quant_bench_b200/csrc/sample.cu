@@ -20,6 +20,7 @@ namespace samp {
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kList = 1024;                    // tokens of a border bin that are ranked; more are halved
+constexpr int kFew = kThreads;                 // candidates that one CTA can finish alone, one a thread
 constexpr int kMaxCluster = 8;
 constexpr int kFixed = 44;                     // fractional bits of a weight
 constexpr float kReach = 31.2f;                // weights below e^-31.2 < 2^-45 round to 0
@@ -40,7 +41,8 @@ struct Shared {
   uint32_t total[kBins];                       // the row's
   uint32_t warp_counts[kWarps];
   float extremes[2][kMaxCluster];
-  int list_n;
+  int list_n;                                  // of rank 0: candidates that the ranks have reserved places for
+  int list_at, pushed;                         // this CTA's first place, and places used
   int found[4];
   u64 found_sum;
 };
@@ -72,6 +74,10 @@ __device__ __forceinline__ uint32_t logit_order(float l) {
   return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
 }
 
+__device__ __forceinline__ float logit_of_order(uint32_t order) {
+  return __uint_as_float(order ^ (order >> 31 ? 0x80000000u : 0xffffffffu));
+}
+
 template <int TYPE>                            // CQ_DT_BF16, CQ_DT_F16, CQ_DT_F32
 struct Sampler {
   using u64 = samp::u64;
@@ -91,6 +97,27 @@ struct Sampler {
     if constexpr (TYPE == CQ_DT_F32) l = reinterpret_cast<const float*>(data)[e];
     else l = widen16<TYPE == CQ_DT_F16>(reinterpret_cast<const uint16_t*>(data)[e]).x;
     return l;
+  }
+  // f(logit, element) for this thread's share of the CTA's elements, 16 bytes at a time; all elements exist (those outside
+  // the row are -inf)
+  template <typename F>
+  __device__ __forceinline__ void each(F&& f) const {
+    constexpr int kPer = 16 / kSize;
+#pragma unroll 2
+    for (int w = tid; w < count / kPer; w += samp::kThreads) {
+      const uint4 v = reinterpret_cast<const uint4*>(data)[w];
+      const uint32_t* u = &v.x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (TYPE == CQ_DT_F32) {
+          f(__uint_as_float(u[j]), w * kPer + j);
+        } else {
+          const float2 l = widen16<TYPE == CQ_DT_F16>(u[j]);
+          f(l.x, w * kPer + 2 * j);
+          f(l.y, w * kPer + 2 * j + 1);
+        }
+      }
+    }
   }
   // the bin of a logit, -1 where its weight is 0 (or it is NaN)
   __device__ __forceinline__ int bin(float l) const {
@@ -120,6 +147,12 @@ struct Sampler {
   }
   __device__ __forceinline__ uint32_t there(const void* mine, int r) const { return mapa_shared(smem_u32(mine), r); }
 
+  // rank 0's count of listed tokens, increased; the count before
+  __device__ __forceinline__ int add_at_first(int n) const {
+    int before;
+    asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(before) : "r"(there(&s.list_n, 0)), "r"(n) : "memory");
+    return before;
+  }
   // the sum over the CTA's threads, in every thread
   __device__ __forceinline__ u64 block_sum(u64 v) {
 #pragma unroll
@@ -157,20 +190,17 @@ struct Sampler {
     if (n <= samp::kList) {
       if (tid == 0) s.list_n = 0;
       cluster_sync_all();                                              // lists are empty, and what they held is read
-      for (int e = first + lane; e < first + span; e += 32) {
-        const float l = logit(e);
-        if (bin(l) != b) continue;
+      each([&](float l, int e) {
+        if (bin(l) != b) return;
         const u64 c = composite(l, e);
-        if (c < from) continue;
-        const uint32_t at = there(&s.list_n, 0);
-        int place;
-        asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(place) : "r"(at) : "memory");
+        if (c < from) return;
+        const int place = add_at_first(1);
         const u64 w = WEIGHTS ? weight_of(exponent(l)) : 1;
         for (int r = 0; r < ranks; ++r) {
           st_cluster_u64(there(&s.list[place], r), c);
           st_cluster_u64(there(&s.weight[place], r), w);
         }
-      }
+      });
       cluster_sync_all();
       const int held = static_cast<int>(ld_cluster_u32(there(&s.list_n, 0)));
       u64 best = 0;
@@ -197,16 +227,60 @@ struct Sampler {
     while (lo < hi) {
       const u64 mid = lo + (hi - lo) / 2 + 1;
       u64 sum = 0;
-      for (int e = first + lane; e < first + span; e += 32) {
-        const float l = logit(e);
+      each([&](float l, int e) {
         if (bin(l) == b && composite(l, e) >= mid) sum += WEIGHTS ? weight_of(exponent(l)) : 1;
-      }
+      });
       if (above + cluster_sum(sum) >= target) lo = mid;
       else hi = mid - 1;
     }
     return lo;
   }
 };
+
+// The token from a list of n <= kFew candidates: every token that can stay is among them.  `total`: what top-p refers to
+// where top-k does not cut (else the sum of those that top-k keeps).  One CTA, one candidate a thread.
+template <int TYPE>
+__device__ void finish_from_list(const SampleArgs& a, Sampler<TYPE>& s, int64_t row, int n, int top_k, bool cut_p, float top_p,
+                                 double floor_y, unsigned long long total) {
+  using u64 = samp::u64;
+  const int i = s.tid;
+  const bool mine = i < n;
+  const u64 c = mine ? s.s.list[i] : 0, w = mine ? s.s.weight[i] : 0;
+  u64 above = 0;
+  int before = 0;
+  if (i < (n + 31 & ~31)) {
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const bool over = s.s.list[j] > c;
+      above += over ? s.s.weight[j] : 0;
+      before += over;
+    }
+  }
+  bool stays = mine && (top_k == 0 || before < top_k);
+  if (top_k != 0) total = s.block_sum(stays ? w : 0);
+  if (cut_p) {
+    const double wanted = ceil(static_cast<double>(fmaxf(top_p, 0.0f)) * static_cast<double>(total));
+    const u64 target = wanted >= 9.2e18 ? total : static_cast<u64>(wanted);
+    stays = stays && (above < target || before == 0);
+  }
+  const double y = mine ? s.exponent(logit_of_order(static_cast<uint32_t>(c >> 32))) : -100.0;
+  stays = stays && y >= floor_y;
+  const u64 kept = stays ? w : 0, sum = s.block_sum(kept);
+  s.s.weight[i] = kept;                                                // everyone has read them: block_sum waits
+  __syncthreads();
+  const double at = static_cast<double>(a.uniform[row]) * static_cast<double>(sum);
+  u64 goal = !(at > 0.0) ? 0 : at >= 9.2e18 ? sum - 1 : static_cast<u64>(at);
+  goal = goal > sum - 1 ? sum - 1 : goal;
+  if (kept == 0) return;
+  u64 through = 0;                                                     // of the tokens up to this one's index: the low half is reversed
+#pragma unroll 4
+  for (int j = 0; j < n; ++j) through += static_cast<uint32_t>(s.s.list[j]) >= static_cast<uint32_t>(c) ? s.s.weight[j] : 0;
+  if (through > goal && through - kept <= goal) {
+    a.tokens[row] = static_cast<long long>(0xffffffffu - static_cast<uint32_t>(c));
+    if (a.logprobs != nullptr)
+      a.logprobs[row] = static_cast<float>(y * 0.693147180559945309417 - log(static_cast<double>(sum) * 5.6843418860808015e-14));   // 2^-44
+  }
+}
 
 template <int TYPE>
 __global__ void __launch_bounds__(samp::kThreads, 2) sample_kernel(const SampleArgs a, const int ranks) {
@@ -220,6 +294,7 @@ __global__ void __launch_bounds__(samp::kThreads, 2) sample_kernel(const SampleA
   const int64_t row = blockIdx.x / ranks;
   grid_dep_launch();
   if (tid < 64) sh.power[tid] = exp2(tid / 64.0);
+  if (tid == 0) sh.list_n = 0;
   for (int i = tid; i < samp::kBins; i += samp::kThreads) sh.hist[i] = 0;
   grid_dep_wait();
 
@@ -332,20 +407,47 @@ __global__ void __launch_bounds__(samp::kThreads, 2) sample_kernel(const SampleA
   u64 cut = 0;                                                         // what lies at or above it stays
   if (cut_k || cut_p) {
     // ---- tokens by bins, over the whole row in every CTA ----
-    for (int e = s.first + s.lane; e < s.first + s.span; e += 32) {
-      const int b = s.bin(s.logit(e));
+    s.each([&](float l, int) {
+      const int b = s.bin(l);
       if (b >= 0) atomicAdd(&sh.hist[b], 1u);
-    }
+    });
     cluster_sync_all();
     const int per = samp::kBins / ranks;
     for (int i = rank * per + tid; i < (rank + 1) * per; i += samp::kThreads) {
       uint32_t sum = 0;
-      for (int r = 0; r < ranks; ++r) sum += ld_cluster_u32(s.there(&sh.hist[i], r));
-      for (int r = 0; r < ranks; ++r) st_cluster_u32(s.there(&sh.total[i], r), sum);
+#pragma unroll
+      for (int r = 0; r < samp::kMaxCluster; ++r) sum += r < ranks ? ld_cluster_u32(s.there(&sh.hist[i], r)) : 0;
+#pragma unroll
+      for (int r = 0; r < samp::kMaxCluster; ++r)
+        if (r < ranks) st_cluster_u32(s.there(&sh.total[i], r), sum);
     }
     cluster_sync_all();
   }
   constexpr int kEach = samp::kBins / samp::kThreads;                  // bins of a thread in a scan
+  const double floor_y = min_p > 0.0f ? log2(static_cast<double>(fminf(min_p, 1.0f))) : -100.0;
+  // the tokens of the bins up to `last`, with their weights, into rank 0's list; with `sum` the weights of all tokens too.
+  // A CTA's places are reserved by what its own bins count.
+  auto list_up_to = [&](int last, u64* sum) {
+    uint32_t mine = 0;
+    for (int b = tid; b <= last; b += samp::kThreads) mine += sh.hist[b];
+    const int n = static_cast<int>(s.block_sum(mine));
+    if (tid == 0) {
+      sh.pushed = 0;
+      sh.list_at = s.add_at_first(n);
+    }
+    __syncthreads();
+    s.each([&](float l, int e) {
+      const int b = s.bin(l);
+      if (b < 0 || (sum == nullptr && b > last)) return;
+      const u64 w = s.weight_of(s.exponent(l));
+      if (sum != nullptr) *sum += w;
+      if (b > last) return;
+      const int place = sh.list_at + atomicAdd(&sh.pushed, 1);
+      st_cluster_u64(s.there(&sh.list[place], 0), s.composite(l, e));
+      st_cluster_u64(s.there(&sh.weight[place], 0), w);
+    });
+    if (sum == nullptr) cluster_sync_all();
+  };
   if (cut_k) {
     // ---- the bin in which the k-th token lies ----
     uint32_t mine = 0;
@@ -374,7 +476,12 @@ __global__ void __launch_bounds__(samp::kThreads, 2) sample_kernel(const SampleA
     __syncthreads();
     const int b = sh.found[0];
     if (b >= 0) {
-      const int above = sh.found[1];
+      const int above = sh.found[1], n = above + static_cast<int>(sh.total[b]);
+      if (n <= samp::kFew) {
+        list_up_to(b, nullptr);
+        if (rank == 0) finish_from_list<TYPE>(a, s, row, n, top_k, cut_p, top_p, floor_y, 0);
+        return;
+      }
       cut = s.template cut_in_bin<false>(b, 0, above, top_k, sh.total[b]);
     }
   }
@@ -383,7 +490,7 @@ __global__ void __launch_bounds__(samp::kThreads, 2) sample_kernel(const SampleA
     // bin that the bounds allow; sums of the bins before are exact, and those of the allowed bins each ----
     // top-k's cut ends the bins; its own one is counted whole in the upper bounds and not at all in the lower
     const double step = s.inv_width > 0.0f ? s.by / static_cast<double>(s.inv_width) : 0.0;
-    const float ratio = static_cast<float>(exp2(step * 1.001));        // of a bin's bounds (1.001: fp32 bins)
+    const float ratio = exp2f(static_cast<float>(step) * 1.001f);      // of a bin's bounds (1.001: fp32 bins)
     const float stepf = static_cast<float>(step);
     const int last = cut != 0 ? sh.found[0] : samp::kBins - 1;         // no token below this bin
     float mine = 0.0f;
@@ -427,19 +534,34 @@ __global__ void __launch_bounds__(samp::kThreads, 2) sample_kernel(const SampleA
       }
       before += up;
     }
-    for (int i = tid; i < samp::kBins; i += samp::kThreads) sh.wsum[i] = 0;
     __syncthreads();
     const int lo = sh.found[2], hi = sh.found[3];
     u64 above = 0, sum = 0;
-    for (int e = s.first + s.lane; e < s.first + s.span; e += 32) {
-      const float l = s.logit(e);
+    if (cut == 0) {
+      // few tokens up to the last bin that the border can lie in: one CTA finishes from a list of them
+      uint32_t upto = 0;
+      for (int b = tid; b <= hi; b += samp::kThreads) upto += sh.total[b];
+      const int n = static_cast<int>(s.block_sum(upto));
+      if (n <= samp::kFew) {
+        list_up_to(hi, &sum);
+        const u64(*all)[2] = s.exchange(s.block_sum(sum), 0);
+        if (rank != 0) return;
+        u64 whole_sum = 0;
+        for (int r = 0; r < ranks; ++r) whole_sum += all[r][0];
+        finish_from_list<TYPE>(a, s, row, n, 0, true, top_p, floor_y, whole_sum);
+        return;
+      }
+    }
+    for (int i = tid; i < samp::kBins; i += samp::kThreads) sh.wsum[i] = 0;
+    __syncthreads();
+    s.each([&](float l, int e) {
       const int b = s.bin(l);
-      if (b < 0 || s.composite(l, e) < cut) continue;
+      if (b < 0 || s.composite(l, e) < cut) return;
       const u64 w = s.weight_of(s.exponent(l));
       sum += w;
       if (b < lo) above += w;
       else if (b <= hi) atomicAdd(&sh.wsum[b], w);
-    }
+    });
     const u64 my_sum = s.block_sum(sum), my_above = s.block_sum(above);
     const u64(*all)[2] = s.exchange(my_sum, my_above);
     u64 total = 0;
@@ -495,7 +617,6 @@ __global__ void __launch_bounds__(samp::kThreads, 2) sample_kernel(const SampleA
   }
 
   // ---- what stays: sums by warps, then the token ----
-  const double floor_y = min_p > 0.0f ? log2(static_cast<double>(fminf(min_p, 1.0f))) : -100.0;
   auto kept = [&](int e, double& y) {
     const float l = s.logit(e);
     if (s.bin(l) < 0 || s.composite(l, e) < cut) return static_cast<u64>(0);
