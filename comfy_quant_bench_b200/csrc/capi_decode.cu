@@ -124,10 +124,10 @@ int cq_prefix_attention(const void* q, int64_t q_batch_stride, int64_t q_head_st
       !valid_head_dim(head_dim) || kv_heads > 65535 || !fits_int(prefix_len))
     return CQ_ERR_SHAPE;
   if (batch == 0) return CQ_OK;
-  if (workspace_bytes < cq_prefix_attention_workspace_bytes(batch, q_heads, kv_heads, head_dim, table_width * page_size))
-    return CQ_ERR_SHAPE;
+  const int64_t need = cq_prefix_attention_workspace_bytes(batch, q_heads, kv_heads, head_dim, table_width * page_size);
+  if (workspace_bytes < need) return CQ_ERR_SHAPE;
   if (q == nullptr || k_cache == nullptr || v_cache == nullptr || seq_lens == nullptr || out == nullptr ||
-      (block_table == nullptr && table_width > 0) || workspace == nullptr)
+      (block_table == nullptr && table_width > 0) || (workspace == nullptr && need > 0))
     return CQ_ERR_ARG;
   const int vec = cache_dtype == CQ_DT_FP8_E4M3 ? 16 : 8;      // elements of a 16-byte access
   if (!aligned(q, 16) || q_batch_stride % 8 != 0 || q_head_stride % 8 != 0 || !aligned(k_cache, 16) ||

@@ -331,7 +331,7 @@ py::object attention(const Tensor& q_arg, const Tensor& k_cache, const Tensor& v
   const float factor = static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(d)));
   if (shared) {
     const int64_t bytes = cq_prefix_attention_workspace_bytes(b, hq, hk, d, width * page);
-    ws = bytes_like(q, bytes);
+    if (bytes > 0) ws = bytes_like(q, bytes);
     check_status("cq_prefix_attention",
                  cq_prefix_attention(q.data_ptr(), q.stride(0), q.stride(1), dtype_code(dt), b, hq, hk, d, k_cache.data_ptr(),
                                      v_cache.data_ptr(), dtype_code(ct), pages, page, k_cache.stride(0), k_cache.stride(1),

@@ -144,7 +144,8 @@ __global__ void __launch_bounds__(pfx::Cfg<D>::kThreads, 1) prefix_attention_ker
   uint64_t* s_full = q_empty + 1;                             // [kSlots * kBufs] scores are in tensor memory
   uint64_t* p_full = s_full + 2;                              // [..][2] half of the weights are
   uint64_t* o_done = p_full + 4;                              // [kSlots] a product with the values is done
-  uint64_t* all_done = o_done + 2;
+  uint64_t* run_done = o_done + 2;                            // [kSlots] a run's last product is done
+  uint64_t* all_done = run_done + 2;
   uint32_t* holder = reinterpret_cast<uint32_t*>(all_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(holder + 1);
   int* leader_at = reinterpret_cast<int*>(holder + 2);
@@ -164,6 +165,7 @@ __global__ void __launch_bounds__(pfx::Cfg<D>::kThreads, 1) prefix_attention_ker
       mbar_init(&p_full[2 * s], 4);
       mbar_init(&p_full[2 * s + 1], 4);
       mbar_init(&o_done[s], 1);
+      mbar_init(&run_done[s], 1);
     }
     mbar_init(all_done, 1);
     *abort_flag = 0;
@@ -273,6 +275,7 @@ __global__ void __launch_bounds__(pfx::Cfg<D>::kThreads, 1) prefix_attention_ker
           p_phase[buf] ^= 1u;
           if (!ok) break;
           tc_commit(&o_done[slot]);
+          if (i + kSlots >= jobs) tc_commit(&run_done[slot]);
           if (last_of_tile(i)) tc_commit(&empty[stage]);
           if (kSlots == 2 && i + 2 < jobs) {
             // this slot's scores take the place of the weights just used
@@ -337,14 +340,69 @@ __global__ void __launch_bounds__(pfx::Cfg<D>::kThreads, 1) prefix_attention_ker
       }
       const int64_t head_at = seg.head * g.head_stride;
       constexpr int kPerWarp = kKeys / 4;                     // keys of a warp: 32 or 16
-      for (int j = seg.j0; j < seg.j0 + seg.n && ok; ++j) {
-        // lane r looks its key up
+      // lane r looks its key of a tile up
+      struct Keys {
+        int64_t off;
+        uint32_t mask;
+      };
+      auto look_up = [&](int j) {
         const int key = j * kKeys + w * kPerWarp + (lane & (kPerWarp - 1));
         int page = -1;
-        if (key < prefix) page = __ldg(table + (key >> page_shift));
+        if (j < seg.j0 + seg.n && key < prefix) page = __ldg(table + (key >> page_shift));
         const bool there = page >= 0 && page < g.num_pages;
-        const uint32_t mask = __ballot_sync(0xffffffffu, there);
-        const int64_t off = there ? page * g.page_stride + head_at + (key & page_mask) * g.tok_stride : 0;
+        return Keys{there ? page * g.page_stride + head_at + (key & page_mask) * g.tok_stride : 0, __ballot_sync(0xffffffffu, there)};
+      };
+      if constexpr (FP8) {
+        // 16 codes a lane, through registers: an operand's next rows are on their way while the other's are widened
+        constexpr int kLanes = D / 16, kAtOnce = 32 / kLanes, kLoads = kPerWarp / kAtOnce;
+        uint4 raw[2][kLoads];
+        const int c = lane % kLanes;
+        auto fetch = [&](int kv, const Keys& keys) {
+#pragma unroll
+          for (int i = 0; i < kLoads; ++i) {
+            const int r = i * kAtOnce + lane / kLanes;
+            const int64_t o = __shfl_sync(0xffffffffu, keys.off, r) + 16 * c;
+            uint4& x = raw[kv][i];
+            x = make_uint4(0, 0, 0, 0);
+            if (keys.mask >> r & 1u)
+              asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                           : "l"(static_cast<const uint8_t*>(kv ? g.v : g.k) + o));
+          }
+        };
+        auto store = [&](int kv) {
+          const int stage = load % kStages;
+          if (load >= kStages && !(ok = warp_wait(&empty[stage], (load / kStages - 1) & 1, abort_flag, pfx::kSite + 1))) return;
+          uint8_t* dst = ring + stage * C::kStageBytes;
+#pragma unroll
+          for (int i = 0; i < kLoads; ++i) {
+            const int r = kPerWarp * w + i * kAtOnce + lane / kLanes;
+            uint4 lo, hi;
+            widen_e4m3x4<F16>(raw[kv][i].x, lo.x, lo.y);
+            widen_e4m3x4<F16>(raw[kv][i].y, lo.z, lo.w);
+            widen_e4m3x4<F16>(raw[kv][i].z, hi.x, hi.y);
+            widen_e4m3x4<F16>(raw[kv][i].w, hi.z, hi.w);
+            *reinterpret_cast<uint4*>(dst + place(kKeys, r, 2 * c)) = lo;
+            *reinterpret_cast<uint4*>(dst + place(kKeys, r, 2 * c + 1)) = hi;
+          }
+          hand_over(&full[stage]);
+          ++load;
+        };
+        Keys next = look_up(seg.j0);
+        fetch(0, next);
+        fetch(1, next);
+        next = look_up(seg.j0 + 1);
+        for (int j = seg.j0; j < seg.j0 + seg.n; ++j) {
+          store(0);
+          if (!ok) break;
+          fetch(0, next);
+          store(1);
+          if (!ok) break;
+          fetch(1, next);
+          next = look_up(j + 2);
+        }
+      }
+      for (int j = seg.j0; !FP8 && j < seg.j0 + seg.n && ok; ++j) {
+        const Keys keys = look_up(j);
         if constexpr (!FP8) {
           for (int kv = 0; kv < 2 && ok; ++kv) {
             const int stage = load % kStages;
@@ -356,8 +414,8 @@ __global__ void __launch_bounds__(pfx::Cfg<D>::kThreads, 1) prefix_attention_ker
 #pragma unroll 8
             for (int r0 = 0; r0 < kPerWarp; r0 += kRowsAtOnce) {
               const int r = r0 + lane / kChunks;
-              const int64_t o = __shfl_sync(0xffffffffu, off, r) + 8 * c;
-              cp_async16(dst + place(kKeys, kPerWarp * w + r, c), base + o, mask >> r & 1u);
+              const int64_t o = __shfl_sync(0xffffffffu, keys.off, r) + 8 * c;
+              cp_async16(dst + place(kKeys, kPerWarp * w + r, c), base + o, keys.mask >> r & 1u);
             }
             cp_async_commit();
             ++load;
@@ -371,40 +429,6 @@ __global__ void __launch_bounds__(pfx::Cfg<D>::kThreads, 1) prefix_attention_ker
               hand_over(&full[landed % kStages]);
               ++landed;
             }
-          }
-        } else {
-          // 16 codes a lane: both operands' rows are on their way before either is stored
-          constexpr int kLanes = D / 16, kAtOnce = 32 / kLanes, kLoads = kPerWarp / kAtOnce;
-          uint4 raw[2][kLoads];
-          const int c = lane % kLanes;
-#pragma unroll
-          for (int kv = 0; kv < 2; ++kv)
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-              const int r = i * kAtOnce + lane / kLanes;
-              const int64_t o = __shfl_sync(0xffffffffu, off, r) + 16 * c;
-              raw[kv][i] = mask >> r & 1u ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(kv ? g.v : g.k) + o))
-                                          : make_uint4(0, 0, 0, 0);
-            }
-#pragma unroll
-          for (int kv = 0; kv < 2; ++kv) {
-            const int stage = load % kStages;
-            if (load >= kStages && !(ok = warp_wait(&empty[stage], (load / kStages - 1) & 1, abort_flag, pfx::kSite + 1))) break;
-            uint8_t* dst = ring + stage * C::kStageBytes;
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-              const int r = kPerWarp * w + i * kAtOnce + lane / kLanes;
-              uint4 lo, hi;
-              widen_e4m3x4<F16>(raw[kv][i].x, lo.x, lo.y);
-              widen_e4m3x4<F16>(raw[kv][i].y, lo.z, lo.w);
-              widen_e4m3x4<F16>(raw[kv][i].z, hi.x, hi.y);
-              widen_e4m3x4<F16>(raw[kv][i].w, hi.z, hi.w);
-              *reinterpret_cast<uint4*>(dst + place(kKeys, r, 2 * c)) = lo;
-              *reinterpret_cast<uint4*>(dst + place(kKeys, r, 2 * c + 1)) = hi;
-            }
-            hand_over(&full[stage]);
-            ++load;
-            ++landed;
           }
         }
       }
@@ -422,7 +446,7 @@ __global__ void __launch_bounds__(pfx::Cfg<D>::kThreads, 1) prefix_attention_ker
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     constexpr float kLift = F16 ? 7.0f : 0.0f;                // f16 weights reach 2^15: up to 2^8 above the running maximum
     constexpr float kSlackUp = 8.0f;
-    uint32_t s_phase[2] = {0, 0}, o_phase = 0;
+    uint32_t s_phase[2] = {0, 0}, o_phase = 0, run_phase = 0;   // o_phase: products of earlier runs
     bool ok = true;
     for (int64_t u = u0; u < u1 && ok;) {
       const Segment seg = segment(u);
@@ -476,17 +500,19 @@ __global__ void __launch_bounds__(pfx::Cfg<D>::kThreads, 1) prefix_attention_ker
         top = fmaxf(top, top2);
         top = top == -INFINITY ? top : top * fabsf(mul);
         const bool raise = top > m + kSlackUp || (m == -INFINITY && top > m);
-        if (kBufs == 2 && done > 0) {                         // the product before still adds to O
-          if (!(ok = warp_wait(&o_done[slot], o_phase, abort_flag, pfx::kSite + 9))) break;
-          o_phase ^= 1u;
-          tc_fence_after();
-        }
         if (__any_sync(0xffffffffu, raise)) {
           const float to = raise ? top : m, f = raise ? exp2_fast(m - to) : 1.0f;
           m = to;
           l *= f;
           if (done > 0) {
-#pragma unroll 1
+            // with two buffers the product before may still add to O; those before it are done, since one of them was the
+            // last use of this buffer.  With one, these scores came after the product
+            if (kBufs == 2) {
+              ok = warp_wait(&o_done[slot], (o_phase + static_cast<uint32_t>(done) - 1u) & 1u, abort_flag, pfx::kSite + 9);
+              if (!ok) break;
+              tc_fence_after();
+            }
+#pragma unroll 2
             for (int x = 0; x < D / 16; ++x) {
               uint32_t o[16];
               const uint32_t at = o_col + slot * D + lanes + 16 * x;
@@ -536,14 +562,9 @@ __global__ void __launch_bounds__(pfx::Cfg<D>::kThreads, 1) prefix_attention_ker
       // ---- this run's sums ----
       if (!ok) break;
       if (done > 0) {
-        // the last product; earlier ones are done (their phases: one for every product of this slot)
-        if (kBufs == 1) {
-          ok = warp_wait(&o_done[slot], (o_phase + static_cast<uint32_t>(done) - 1u) & 1u, abort_flag, pfx::kSite + 10);
-          o_phase = (o_phase + static_cast<uint32_t>(done)) & 1u;
-        } else {
-          ok = warp_wait(&o_done[slot], o_phase, abort_flag, pfx::kSite + 10);
-          o_phase ^= 1u;
-        }
+        ok = warp_wait(&run_done[slot], run_phase, abort_flag, pfx::kSite + 10);
+        run_phase ^= 1u;
+        o_phase += static_cast<uint32_t>(done);
         if (!ok) break;
         tc_fence_after();
       }
@@ -663,9 +684,19 @@ int prefix_members(int64_t rows, int D) {
 int prefix_teams(int members) { return members < num_sms() ? num_sms() / members : 1; }
 }  // namespace
 
+// Sharing pays from about 128 MB of keys and values that the rows would read one by one (by the table's width, since
+// lengths are on the device): four launches and the split of the rows' sums cost 14 to 20 us, and reading runs at 5 to 6
+// TB/s.  Us one by one and shared: 16 rows of 8 heads of 128 behind 1000 tokens (70 MB) 15 and 22, 32 rows (139 MB) 22
+// and 22, 16 rows behind 4000 (266 MB) 38 and 36, 64 rows behind 1000 (279 MB) 40 and 27; 8-bit codes of 256: 139 MB 28
+// and 26; heads of 64: 133 MB 31 and 31.
+bool prefix_pays(int64_t batch, int Hkv, int D, int64_t span, int size) {
+  return static_cast<double>(batch) * Hkv * static_cast<double>(span) * D * 2 * size > 134217728.0;
+}
+
 // the runs' sums, the rows' own outputs and their logs, and the workspace of their kernel
 int64_t prefix_attention_workspace(int64_t batch, int Hq, int Hkv, int D, int64_t span) {
   if (batch == 0) return 0;
+  if (!prefix_pays(batch, Hkv, D, span, 2)) return paged_attention_workspace(batch, Hq, Hkv, D, span, 0, 0);
   const int members = prefix_members(batch * (Hq / Hkv), D);
   const int64_t parts = static_cast<int64_t>(prefix_teams(members) + Hkv) * members * (D == 256 ? 1 : 2) * pfx::part_floats(D) * 4;
   return parts + batch * Hq * (D + 4) * 4 + (paged_attention_workspace(batch, Hq, Hkv, D, span, 0, 0) + 255) / 256 * 256;
@@ -699,6 +730,13 @@ cudaError_t pick_prefix_dim(const PrefixArgs& a, cudaStream_t st) {
 
 // a.own: the whole call's arguments, its ws the whole workspace
 cudaError_t launch_prefix_attention(const PagedAttnArgs& call, cudaStream_t st) {
+  if (!prefix_pays(call.B, call.Hkv, call.D, static_cast<int64_t>(call.table_width) * call.page_size,
+                   call.cache_dtype == CQ_DT_FP8_E4M3 ? 1 : 2)) {
+    PagedAttnArgs each = call;                                // every row through its own table
+    each.prefix = nullptr;
+    each.prefix_len = 0;
+    return launch_paged_attention(each, st);
+  }
   PrefixArgs a{};
   a.own = call;
   a.members = prefix_members(static_cast<int64_t>(call.B) * (call.Hq / call.Hkv), call.D);

@@ -50,10 +50,11 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     which a captured step reads anew): samples of one prompt, requests behind one instruction.  Their keys and values are
     read once for all rows, not once for each.
 
-    Every row with ``prefix`` tokens or more must hold the same first ``prefix`` tokens, in whatever pages (those of the
-    first such row are read); a shorter row or an empty one is attended by itself.  Arguments and results are those of
-    ``paged_attention``.  A softmax weight enters the product with the prefix's values as two 16-bit parts where B *
-    q_heads / kv_heads is at most 256 (128 at D 256), else as one part, rounded to nearest."""
+    Every row with ``prefix`` tokens or more must hold the same first ``prefix`` tokens, in pages of its own table, whichever
+    they are (those of the first such row are read); a shorter row or an empty one is attended by itself.  Where the rows'
+    keys and values come to 128 MB or less by the table's width, sharing does not pay and every row is read through its
+    own table.  Arguments and results are those of ``paged_attention``.  A softmax weight enters the product with shared values as two 16-bit parts where B * q_heads
+    / kv_heads is at most 256 (128 at D 256), else as one part, rounded to nearest."""
     return _lib.decode().prefix_attention(q, k_cache, v_cache, block_table, seq_lens, prefix, rows, scale, k_scale, v_scale,
                                           out, return_lse)
 

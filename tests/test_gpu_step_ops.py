@@ -478,7 +478,13 @@ def test_sample_strides_streams_and_graphs(ops):
 # |o - exact| <= u |exact| + A (2 max err + 2^-14 [+ u]) + n 2^-32 max |v|, A = sum p |v| / sum p.
 # ----------------------------------------------------------------------------------------------------------
 
-def _prefix_problem(lens, prefix, hq, hk, d, page, dtype, cache, seed=0, holes=True):
+def _wide(table, hk, d, page, size):
+    """The table with columns of no pages, so many that the call shares the prefix however few tokens the rows hold."""
+    width = -(-((1 << 27) + 1) // (len(table) * hk * d * 2 * size * page))
+    return torch.cat([table, table.new_full((len(table), max(0, width - table.shape[1])), -1)], dim=1)
+
+
+def _prefix_problem(lens, prefix, hq, hk, d, page, dtype, cache, seed=0, holes=True, wide=True):
     """Rows of lens tokens; those with at least `prefix` of them share the first ones: whole pages, the last in copies."""
     g = _gen(seed + d + prefix)
     host = torch.Generator().manual_seed(seed)
@@ -518,6 +524,8 @@ def _prefix_problem(lens, prefix, hq, hk, d, page, dtype, cache, seed=0, holes=T
                 if n % page:
                     raw[int(table[r, n // page]), :, n % page:] = nan
     q = (1.5 * torch.randn(b, hq, d, generator=g, device="cuda")).to(dtype)
+    if wide:
+        table = _wide(table, hk, d, page, k.element_size())
     return q, k, v, table.cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda"), scales
 
 
@@ -584,6 +592,8 @@ def _prefix_holds(kv, problem, prefix, rows=None, scale=None, **kw):
                                                          (20, 56, 2, 2050, 5, 16), (70, 16, 1, 640, 9, 16), (2, 8, 8, 6000, 100, 16)])
 def test_prefix(kv, b, hq, hk, prefix, longest, page, d, dtype, cache):
     lens = [prefix + (longest * i) // max(1, b - 1) for i in range(b)]
+    problem = _prefix_problem(lens, prefix, hq, hk, d, page, dtype, cache, wide=False)
+    _prefix_holds(kv, problem, prefix)                                  # every row by itself
     problem = _prefix_problem(lens, prefix, hq, hk, d, page, dtype, cache)
     _prefix_holds(kv, problem, prefix)
     _prefix_holds(kv, problem, torch.tensor([prefix], dtype=torch.int32, device="cuda"))
@@ -707,6 +717,7 @@ def test_prefix_offsets_past_32_bits(kv):
         table[r, 20:24] = ids[20 + 4 * r: 24 + 4 * r]
     lens = torch.tensor([330, 384, 321], dtype=torch.int32, device="cuda")
     q = torch.randn(3, 16, d, generator=g, device="cuda").bfloat16()
+    table = _wide(table, hk, d, page, 2)
     _prefix_holds(kv, (q, k, v, table.cuda(), lens, [None, None]), 320)
 
 
