@@ -33,6 +33,7 @@ struct Shared {
       u64 list[kList], weight[kList];          // a border bin's tokens
     };
   };
+  u64 other[kFew];
   u64 warp_sums[2][kWarps];
   u64 slots[2][kMaxCluster][2];                // what the cluster's CTAs tell one another
   u64 best[kWarps];
@@ -165,6 +166,24 @@ struct Sampler {
     for (int w = 0; w < samp::kWarps; ++w) v += s.warp_sums[0][w];
     return v;
   }
+  // the sum over the threads up to this one; `total`: over all
+  __device__ __forceinline__ u64 block_scan(u64 v, u64& total) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    __syncthreads();
+    if (lane == 31) s.warp_sums[0][warp] = v;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < samp::kWarps; ++w) {
+      if (w == warp) v += total;
+      total += s.warp_sums[0][w];
+    }
+    return v;
+  }
   // two values of each CTA, in every CTA, by rank, in s.slots[parity] after the call (until the call after the next)
   __device__ __forceinline__ const u64 (*exchange(u64 a, u64 b))[2] {
     parity ^= 1;
@@ -237,48 +256,67 @@ struct Sampler {
   }
 };
 
+// One key a thread, n of them (the others' keys are 0), sorted by the first threads, largest first: bitonic, within a warp by
+// shuffles.
+__device__ __forceinline__ unsigned long long sort_keys(unsigned long long key, int n, unsigned long long* box) {
+  const int i = threadIdx.x;
+  int size = 32;
+  while (size < n) size *= 2;
+  for (int k = 2; k <= size; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      unsigned long long other;
+      if (j >= 32) {
+        __syncthreads();
+        box[i] = key;
+        __syncthreads();
+        other = box[i ^ j];
+      } else {
+        other = __shfl_xor_sync(0xffffffffu, key, j);
+      }
+      const bool larger = ((i & j) == 0) == ((i & k) == 0);
+      key = (other > key) == larger ? other : key;
+    }
+  return key;
+}
+
 // The token from a list of n <= kFew candidates: every token that can stay is among them.  `total`: what top-p refers to
 // where top-k does not cut (else the sum of those that top-k keeps).  One CTA, one candidate a thread.
 template <int TYPE>
 __device__ void finish_from_list(const SampleArgs& a, Sampler<TYPE>& s, int64_t row, int n, int top_k, bool cut_p, float top_p,
-                                 double floor_y, unsigned long long total) {
+                                 double floor_y, unsigned long long total, double uniform) {
   using u64 = samp::u64;
   const int i = s.tid;
-  const bool mine = i < n;
-  const u64 c = mine ? s.s.list[i] : 0, w = mine ? s.s.weight[i] : 0;
-  u64 above = 0;
-  int before = 0;
-  if (i < (n + 31 & ~31)) {
-#pragma unroll 4
-    for (int j = 0; j < n; ++j) {
-      const bool over = s.s.list[j] > c;
-      above += over ? s.s.weight[j] : 0;
-      before += over;
-    }
-  }
-  bool stays = mine && (top_k == 0 || before < top_k);
-  if (top_k != 0) total = s.block_sum(stays ? w : 0);
+  // in order: the rank is the thread's number
+  const u64 c = sort_keys(i < n ? s.s.list[i] : 0, n, s.s.weight);
+  const bool mine = i < n && (top_k == 0 || i < top_k);
+  const double y = mine ? s.exponent(logit_of_order(static_cast<uint32_t>(c >> 32))) : -100.0;
+  const u64 w = s.weight_of(y);
+  u64 sum;
+  const u64 through = s.block_scan(w, sum);
+  if (top_k != 0) total = sum;
+  bool stays = mine && y >= floor_y;
   if (cut_p) {
     const double wanted = ceil(static_cast<double>(fmaxf(top_p, 0.0f)) * static_cast<double>(total));
     const u64 target = wanted >= 9.2e18 ? total : static_cast<u64>(wanted);
-    stays = stays && (above < target || before == 0);
+    stays = stays && (through - w < target || i == 0);
   }
-  const double y = mine ? s.exponent(logit_of_order(static_cast<uint32_t>(c >> 32))) : -100.0;
-  stays = stays && y >= floor_y;
-  const u64 kept = stays ? w : 0, sum = s.block_sum(kept);
-  s.s.weight[i] = kept;                                                // everyone has read them: block_sum waits
+  // what stays, by index: the composite's low half is the index reversed
   __syncthreads();
-  const double at = static_cast<double>(a.uniform[row]) * static_cast<double>(sum);
+  s.s.weight[i] = stays ? w : 0;
+  s.s.list[i] = c;
+  const u64 by_index = sort_keys(stays ? c << 32 | static_cast<uint32_t>(i) : 0, n, s.s.other);
+  const int from = static_cast<int>(by_index & 0xffffffffu);
+  __syncthreads();
+  const u64 kept = by_index != 0 ? s.s.weight[from] : 0;
+  const u64 upto = s.block_scan(kept, sum);
+  const double at = uniform * static_cast<double>(sum);
   u64 goal = !(at > 0.0) ? 0 : at >= 9.2e18 ? sum - 1 : static_cast<u64>(at);
   goal = goal > sum - 1 ? sum - 1 : goal;
-  if (kept == 0) return;
-  u64 through = 0;                                                     // of the tokens up to this one's index: the low half is reversed
-#pragma unroll 4
-  for (int j = 0; j < n; ++j) through += static_cast<uint32_t>(s.s.list[j]) >= static_cast<uint32_t>(c) ? s.s.weight[j] : 0;
-  if (through > goal && through - kept <= goal) {
-    a.tokens[row] = static_cast<long long>(0xffffffffu - static_cast<uint32_t>(c));
+  if (upto > goal && upto - kept <= goal) {
+    a.tokens[row] = static_cast<long long>(0xffffffffu - static_cast<uint32_t>(by_index >> 32));
     if (a.logprobs != nullptr)
-      a.logprobs[row] = static_cast<float>(y * 0.693147180559945309417 - log(static_cast<double>(sum) * 5.6843418860808015e-14));   // 2^-44
+      a.logprobs[row] = static_cast<float>(s.exponent(logit_of_order(static_cast<uint32_t>(s.s.list[from] >> 32))) * 0.693147180559945309417 -
+                                           log(static_cast<double>(sum) * 5.6843418860808015e-14));   // 2^-44
   }
 }
 
@@ -297,6 +335,12 @@ __global__ void __launch_bounds__(samp::kThreads, 2) sample_kernel(const SampleA
   if (tid == 0) sh.list_n = 0;
   for (int i = tid; i < samp::kBins; i += samp::kThreads) sh.hist[i] = 0;
   grid_dep_wait();
+
+  const float temperature = a.temperatures != nullptr ? a.temperatures[row] : a.temperature;
+  const int top_k = a.top_ks != nullptr ? a.top_ks[row] : a.top_k;
+  const float top_p = a.top_ps != nullptr ? a.top_ps[row] : a.top_p;
+  const float min_p = a.min_ps != nullptr ? a.min_ps[row] : a.min_p;
+  const double uniform = static_cast<double>(a.uniform[row]);
 
   // ---- this CTA's share of the row's 16-byte words; elements outside the row become -inf ----
   const uintptr_t begin = reinterpret_cast<uintptr_t>(a.logits) + row * a.ld * kSize, end = begin + static_cast<int64_t>(a.vocab) * kSize;
@@ -371,10 +415,6 @@ __global__ void __launch_bounds__(samp::kThreads, 2) sample_kernel(const SampleA
       least = fminf(least, __uint_as_float(static_cast<uint32_t>(all[r][1])));
     }
   }
-  const float temperature = a.temperatures != nullptr ? a.temperatures[row] : a.temperature;
-  const int top_k = a.top_ks != nullptr ? a.top_ks[row] : a.top_k;
-  const float top_p = a.top_ps != nullptr ? a.top_ps[row] : a.top_p;
-  const float min_p = a.min_ps != nullptr ? a.min_ps[row] : a.min_p;
   s.top = most;
   if (most == -INFINITY) {                                             // nothing to choose from
     if (rank == 0 && tid == 0) {
@@ -425,7 +465,7 @@ __global__ void __launch_bounds__(samp::kThreads, 2) sample_kernel(const SampleA
   }
   constexpr int kEach = samp::kBins / samp::kThreads;                  // bins of a thread in a scan
   const double floor_y = min_p > 0.0f ? log2(static_cast<double>(fminf(min_p, 1.0f))) : -100.0;
-  // the tokens of the bins up to `last`, with their weights, into rank 0's list; with `sum` the weights of all tokens too.
+  // the tokens of the bins up to `last` into rank 0's list; with `sum` the weights of all tokens are added up, too.
   // A CTA's places are reserved by what its own bins count.
   auto list_up_to = [&](int last, u64* sum) {
     uint32_t mine = 0;
@@ -439,12 +479,9 @@ __global__ void __launch_bounds__(samp::kThreads, 2) sample_kernel(const SampleA
     s.each([&](float l, int e) {
       const int b = s.bin(l);
       if (b < 0 || (sum == nullptr && b > last)) return;
-      const u64 w = s.weight_of(s.exponent(l));
-      if (sum != nullptr) *sum += w;
+      if (sum != nullptr) *sum += s.weight_of(s.exponent(l));
       if (b > last) return;
-      const int place = sh.list_at + atomicAdd(&sh.pushed, 1);
-      st_cluster_u64(s.there(&sh.list[place], 0), s.composite(l, e));
-      st_cluster_u64(s.there(&sh.weight[place], 0), w);
+      st_cluster_u64(s.there(&sh.list[sh.list_at + atomicAdd(&sh.pushed, 1)], 0), s.composite(l, e));
     });
     if (sum == nullptr) cluster_sync_all();
   };
@@ -479,7 +516,7 @@ __global__ void __launch_bounds__(samp::kThreads, 2) sample_kernel(const SampleA
       const int above = sh.found[1], n = above + static_cast<int>(sh.total[b]);
       if (n <= samp::kFew) {
         list_up_to(b, nullptr);
-        if (rank == 0) finish_from_list<TYPE>(a, s, row, n, top_k, cut_p, top_p, floor_y, 0);
+        if (rank == 0) finish_from_list<TYPE>(a, s, row, n, top_k, cut_p, top_p, floor_y, 0, uniform);
         return;
       }
       cut = s.template cut_in_bin<false>(b, 0, above, top_k, sh.total[b]);
@@ -489,15 +526,15 @@ __global__ void __launch_bounds__(samp::kThreads, 2) sample_kernel(const SampleA
     // ---- bounds of the sums from the counts: a token of bin b weighs 2^-(b + 1) width .. 2^-b width; the border lies in a
     // bin that the bounds allow; sums of the bins before are exact, and those of the allowed bins each ----
     // top-k's cut ends the bins; its own one is counted whole in the upper bounds and not at all in the lower
-    const double step = s.inv_width > 0.0f ? s.by / static_cast<double>(s.inv_width) : 0.0;
-    const float ratio = exp2f(static_cast<float>(step) * 1.001f);      // of a bin's bounds (1.001: fp32 bins)
-    const float stepf = static_cast<float>(step);
+    const float step = s.inv_width > 0.0f ? static_cast<float>(s.by) / s.inv_width : 0.0f;   // a bin's width, as a power of 2
+    const float ratio = exp2f(step * 1.001f);                          // of a bin's bounds (1.001: fp32 bins)
     const int last = cut != 0 ? sh.found[0] : samp::kBins - 1;         // no token below this bin
-    float mine = 0.0f;
+    float up[kEach], mine = 0.0f;                                      // upper bounds
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
       const int b = tid * kEach + j;
-      mine += b <= last ? sh.total[b] * exp2f(-stepf * b) : 0.0f;      // upper bound
+      up[j] = b <= last ? sh.total[b] * exp2f(-step * b) : 0.0f;
+      mine += up[j];
     }
     float before = mine;
 #pragma unroll
@@ -520,19 +557,18 @@ __global__ void __launch_bounds__(samp::kThreads, 2) sample_kernel(const SampleA
       whole += fbox[w];
     }
     // exact sum before a bin in [before / ratio, before], the row's in [whole / ratio - its border bin's, whole]
-    const float border = cut != 0 ? sh.total[last] * exp2f(-stepf * last) : 0.0f;
+    const float border = cut != 0 ? sh.total[last] * exp2f(-step * last) : 0.0f;
     const float p = fmaxf(top_p, 0.0f), slack = 1.0f + 1e-3f;
     const float least_target = p * fmaxf(whole - border, 0.0f) / (ratio * slack), most_target = p * whole * slack;
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
       const int b = tid * kEach + j;
-      const float up = b <= last ? sh.total[b] * exp2f(-stepf * b) : 0.0f;
       // bin b can hold the border unless all of it is surely kept, or all of it surely dropped
-      if (up > 0.0f && (before + up) * slack >= least_target && before / (ratio * slack) <= most_target) {
+      if (up[j] > 0.0f && (before + up[j]) * slack >= least_target && before <= most_target * (ratio * slack)) {
         atomicMin(&sh.found[2], b);
         atomicMax(&sh.found[3], b);
       }
-      before += up;
+      before += up[j];
     }
     __syncthreads();
     const int lo = sh.found[2], hi = sh.found[3];
@@ -548,7 +584,7 @@ __global__ void __launch_bounds__(samp::kThreads, 2) sample_kernel(const SampleA
         if (rank != 0) return;
         u64 whole_sum = 0;
         for (int r = 0; r < ranks; ++r) whole_sum += all[r][0];
-        finish_from_list<TYPE>(a, s, row, n, 0, true, top_p, floor_y, whole_sum);
+        finish_from_list<TYPE>(a, s, row, n, 0, true, top_p, floor_y, whole_sum, uniform);
         return;
       }
     }
@@ -642,8 +678,7 @@ __global__ void __launch_bounds__(samp::kThreads, 2) sample_kernel(const SampleA
     if (r < rank) before += all[r][0];
     total += all[r][0];
   }
-  const double u = static_cast<double>(a.uniform[row]);
-  const double at = u > 0.0 ? u * static_cast<double>(total) : 0.0;    // NaN: the first
+  const double at = uniform > 0.0 ? uniform * static_cast<double>(total) : 0.0;   // NaN: the first
   u64 goal = at >= 9.2e18 ? total - 1 : static_cast<u64>(at);
   goal = goal > total - 1 ? total - 1 : goal;
   if (goal < before || goal >= before + sum) return;                   // another warp's
