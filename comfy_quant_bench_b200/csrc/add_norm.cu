@@ -29,11 +29,15 @@ template <int OUT>
 __device__ __forceinline__ float scaled(float p, const Coder& c) {
   return c.tiny ? (c.most > 0.0f ? __fdiv_rn(p, c.most) * c.by : 0.0f) : p * c.by;
 }
+// the nearest code in 64 bits: rare, and out of the way of the others
+__device__ __noinline__ int int8_code_exactly(float p, float most) {
+  return static_cast<int>(rint(static_cast<double>(p) * 127.0 / static_cast<double>(most)));
+}
 __device__ __forceinline__ uint32_t int8_code(float p, const Coder& c) {
   const float t = scaled<kNormInt8>(p, c), k = rintf(t);
   int code = static_cast<int>(k);
-  // t is off by 2^-22 of at most 127: only within 2^-14 of a border can the nearest code be another one
-  if (fabsf(fabsf(t - k) - 0.5f) < 6.2e-5f) code = static_cast<int>(rint(static_cast<double>(p) * 127.0 / static_cast<double>(c.most)));
+  // t is off by 2^-23 of itself, 1.52e-5 at most: only that near to a border can the nearest code be another one
+  if (fabsf(t - k) > 0.5f - 1.6e-5f) code = int8_code_exactly(p, c.most);
   return static_cast<uint32_t>(code) & 0xffu;
 }
 __device__ __forceinline__ uint32_t e4m3_pair(float a, float b) {
@@ -83,14 +87,14 @@ __global__ void __launch_bounds__(WARP ? 256 : CHUNKS < 4 ? 512 : 1024) add_norm
 #pragma unroll
   for (int i = 0; i < CHUNKS; ++i) {
     const int c = tid + i * team;
-    h[i] = c < eights ? *reinterpret_cast<const uint4*>(x + 8 * c) : make_uint4(0, 0, 0, 0);
+    h[i] = c < eights ? __ldcs(reinterpret_cast<const uint4*>(x + 8 * c)) : make_uint4(0, 0, 0, 0);
   }
   if (a.residual != nullptr) {
     uint4 add[CHUNKS];
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
       const int c = tid + i * team;
-      add[i] = c < eights ? *reinterpret_cast<const uint4*>(r + 8 * c) : make_uint4(0, 0, 0, 0);
+      add[i] = c < eights ? __ldcs(reinterpret_cast<const uint4*>(r + 8 * c)) : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
@@ -171,19 +175,23 @@ __global__ void __launch_bounds__(WARP ? 256 : CHUNKS < 4 ? 512 : 1024) add_norm
   }
 }
 
-// Other widths: element by element, a row a block; the row's sum h goes through shared memory.
-template <bool F16, int OUT>
+// Other widths: element by element, a row a warp or a block; a thread leaves its elements of h in shared memory meanwhile.
+template <bool F16, int OUT, bool WARP>
 __global__ void __launch_bounds__(256) add_norm_odd_kernel(const AddNormArgs a) {
-  extern __shared__ uint16_t row_h[];
+  extern __shared__ uint16_t rows_h[];
   __shared__ float red[64];
-  const int64_t row = blockIdx.x;
+  const int team = WARP ? 32 : blockDim.x, tid = WARP ? threadIdx.x & 31 : threadIdx.x;
+  const int64_t row = WARP ? blockIdx.x * static_cast<int64_t>(blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+  uint16_t* row_h = rows_h + (WARP ? (threadIdx.x >> 5) * a.width : 0);
   grid_dep_launch();
   grid_dep_wait();
+  if (WARP && row >= a.rows) return;
   const uint16_t* x = static_cast<const uint16_t*>(a.x) + row * a.ldx;
   const uint16_t* r = static_cast<const uint16_t*>(a.residual) + row * a.ldr;
   const uint16_t* w = static_cast<const uint16_t*>(a.weight);
   float sum = 0.0f, most = 0.0f;
-  for (int c = threadIdx.x; c < a.width; c += blockDim.x) {
+#pragma unroll 4
+  for (int c = tid; c < a.width; c += team) {
     uint32_t h = x[c];
     if (a.residual != nullptr) h = narrow16<F16>(widen16<F16>(h).x + widen16<F16>(r[c]).x, 0.0f) & 0xffffu;
     row_h[c] = static_cast<uint16_t>(h);
@@ -192,11 +200,12 @@ __global__ void __launch_bounds__(256) add_norm_odd_kernel(const AddNormArgs a) 
     sum = fmaf(f, f, sum);
     most = fmaxf(most, fabsf(f * widen16<F16>(w[c]).x));
   }
-  row_reduce<false>(sum, most, red);
+  row_reduce<WARP>(sum, most, red);
   const float inv = rsqrtf(sum / static_cast<float>(a.width) + a.eps);
   const Coder by = coder<OUT>(most);
-  if (OUT != kNormSame && threadIdx.x == 0) a.scale[row] = most * inv / (OUT == kNormInt8 ? 127.0f : 448.0f);
-  for (int c = threadIdx.x; c < a.width; c += blockDim.x) {
+  if (OUT != kNormSame && tid == 0) a.scale[row] = most * inv / (OUT == kNormInt8 ? 127.0f : 448.0f);
+#pragma unroll 4
+  for (int c = tid; c < a.width; c += team) {
     const float p = widen16<F16>(row_h[c]).x * widen16<F16>(w[c]).x;
     const int64_t to = row * a.width + c;
     if constexpr (OUT == kNormSame) static_cast<uint16_t*>(a.out)[to] = static_cast<uint16_t>(narrow16<F16>(p * inv, 0.0f));
@@ -225,17 +234,20 @@ cudaError_t run_add_norm(const AddNormArgs& a, cudaStream_t st) {
 template <bool F16>
 cudaError_t pick_add_norm(const AddNormArgs& a, cudaStream_t st) {
   if (a.width % 8 != 0) {
-    const dim3 grid(static_cast<unsigned>(a.rows));
-    const int threads = a.width <= 256 ? (a.width + 31) / 32 * 32 : 256, bytes = 2 * a.width;
-    static unsigned long long devices[3] = {0, 0, 0};
+    // a warp a row where there are many short ones: 518289 rows of 123 take 235 us, and 763 with a block each; 65536 of 999
+    // 158 and 259; but 777 of 1001 13 us, and 6.5 with a block each
+    const bool warp = a.width <= 1024 && a.rows >= 4736;
+    const dim3 grid(static_cast<unsigned>(warp ? (a.rows + 7) / 8 : a.rows));
+    const int bytes = 2 * a.width * (warp ? 8 : 1);
+    static unsigned long long devices[6] = {};
     auto launch = [&](auto kernel, unsigned long long& d) {
       const cudaError_t e = allow_shared(kernel, 2 * kNormMaxWidth, d);
-      return e != cudaSuccess ? e : launch_early(kernel, grid, threads, bytes, st, a);
+      return e != cudaSuccess ? e : launch_early(kernel, grid, 256, bytes, st, a);
     };
     switch (a.out_kind) {
-      case kNormSame: return launch(add_norm_odd_kernel<F16, kNormSame>, devices[0]);
-      case kNormInt8: return launch(add_norm_odd_kernel<F16, kNormInt8>, devices[1]);
-      default: return launch(add_norm_odd_kernel<F16, kNormFp8>, devices[2]);
+      case kNormSame: return warp ? launch(add_norm_odd_kernel<F16, kNormSame, true>, devices[0]) : launch(add_norm_odd_kernel<F16, kNormSame, false>, devices[1]);
+      case kNormInt8: return warp ? launch(add_norm_odd_kernel<F16, kNormInt8, true>, devices[2]) : launch(add_norm_odd_kernel<F16, kNormInt8, false>, devices[3]);
+      default: return warp ? launch(add_norm_odd_kernel<F16, kNormFp8, true>, devices[4]) : launch(add_norm_odd_kernel<F16, kNormFp8, false>, devices[5]);
     }
   }
   switch (a.out_kind) {

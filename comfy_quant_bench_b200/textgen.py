@@ -7,13 +7,16 @@ sequence and step.  With x the residual stream [tokens, hidden] (bf16), a block 
     x = x + Wo attention(q, cache of k and v)
     y = RMSNorm(x) * w2;  x = x + Wd (silu(Wg y) * Wu y)
 
-Every linear is ``ops.w4a16_linear``; keys and values live in a ``kvcache.PagedKVCache`` and a step's attention reads them
-there.  Every second block may see only a window and the first few tokens (``window``, ``sinks``).  Weights are random:
-the module shows how the operators go together, and ``python -m comfy_quant_bench_b200.textgen`` times a step.
+Every linear is ``ops.w4a16_linear``, every addition to the stream and the norm after it ``ops.add_rmsnorm``; the heads'
+norms, the rotary embedding and the cache's append are ``kvcache.append_rotated``.  Keys and values live in a
+``kvcache.PagedKVCache`` and a step's attention reads them there.  Every second block may see only a window and the first
+few tokens (``window``, ``sinks``).  Weights are random: the module shows how the operators go together, and
+``python -m comfy_quant_bench_b200.textgen`` times a step.
 
 ``generate`` writes several continuations of one prompt: the prompt's row is forked, its pages are shared, and a row's
-last page is copied when the row first writes to it.  A step works on device state alone, so ``capture`` turns it into one
-CUDA graph.
+last page is copied when the row first writes to it; attention reads the prompt once for all of them
+(``kvcache.prefix_attention``), and ``ops.sample_tokens`` chooses the tokens.  A step works on device state alone, so
+``capture`` turns it into one CUDA graph.
 """
 from __future__ import annotations
 
@@ -40,6 +43,9 @@ class TextConfig:
     window: int = 0              # > 0: every second block sees this many tokens and the first `sinks`
     sinks: int = 0
     rope_base: float = 10000.0
+    rope_scaling: str | None = None      # kvcache.rope_table's, with its factor and original context
+    rope_factor: float = 1.0
+    rope_original: int = 0
     max_tokens: int = 2048
     rows: int = 16
     pages: int = 1024
@@ -86,31 +92,24 @@ class TextModel:
         scale = torch.full((cfg.kv_heads,), 0.02, device=device) if cfg.cache_dtype == torch.float8_e4m3fn else None
         self.cache = kvcache.PagedKVCache(cfg.layers, cfg.pages, cfg.kv_heads, cfg.head_dim, cfg.rows, cfg.max_tokens,
                                           cfg.page_size, cfg.cache_dtype, device, scale, scale)
-        inv = cfg.rope_base ** (-torch.arange(0, cfg.head_dim, 2, device=device, dtype=torch.float32) / cfg.head_dim)
         room = self.cache.block_table.shape[1] * cfg.page_size               # max_tokens up to whole pages: any position
-        angle = torch.outer(torch.arange(room, device=device, dtype=torch.float32), inv)
-        self.rope = torch.stack([angle.cos(), angle.sin()], dim=-1)          # [tokens, D/2, 2]
-
-    def _heads(self, x: torch.Tensor, weight: torch.Tensor, rope: torch.Tensor) -> torch.Tensor:
-        """RMSNorm and rotary embedding of each head of x [tokens, heads, D]."""
-        t, h, d = x.shape
-        each = rope.unsqueeze(1).expand(t, h, d // 2, 2).reshape(t * h, d // 2, 2)
-        return ops.rmsnorm_rope_rows(x.reshape(t * h, d), weight, each, d).view(t, h, d)
+        self.rope = kvcache.rope_table(room, cfg.head_dim, base=cfg.rope_base, scaling=cfg.rope_scaling, factor=cfg.rope_factor,
+                                       original=cfg.rope_original, device=device)      # [tokens, D/2, 2]
 
     def _forward(self, tokens, rows, positions, attention) -> torch.Tensor:
         """Logits [tokens, vocab] (bf16); ``attention(layer, block, q)`` after the tokens' keys and values are cached."""
         c = self.cfg
-        x = self.embed[tokens]
-        rope = self.rope[positions.clamp(min=0)]
+        out, x = self.embed[tokens], None                        # what the last linear gave, and the stream before it
         for layer, b in enumerate(self.blocks):
-            y = b.qkv(ops.rmsnorm_rope_rows(x, b.norm1)).view(len(tokens), c.heads + 2 * c.kv_heads, c.head_dim)
+            y, x = ops.add_rmsnorm(out, b.norm1, x)
+            y = b.qkv(y).view(len(tokens), c.heads + 2 * c.kv_heads, c.head_dim)
             q, k, v = y.split((c.heads, c.kv_heads, c.kv_heads), dim=1)
-            q, k = self._heads(q, b.norm_q, rope), self._heads(k, b.norm_k, rope)
-            self.cache.append(layer, k, v, rows, positions)
-            x = x + b.out(attention(layer, b, q, k, v).reshape(len(tokens), c.heads * c.head_dim))
-            gate, up = b.up(ops.rmsnorm_rope_rows(x, b.norm2)).chunk(2, dim=-1)
-            x = x + b.down(F.silu(gate) * up)
-        return self.head(ops.rmsnorm_rope_rows(x, self.norm))
+            q, k = self.cache.append_rotated(layer, q, k, v, rows, positions, self.rope, interleaved=True, q_norm=b.norm_q,
+                                             k_norm=b.norm_k, return_k=True)
+            y, x = ops.add_rmsnorm(b.out(attention(layer, b, q, k, v).reshape(len(tokens), c.heads * c.head_dim)), b.norm2, x)
+            gate, up = b.up(y).chunk(2, dim=-1)
+            out = b.down(F.silu(gate) * up)
+        return self.head(ops.add_rmsnorm(out, self.norm, x)[0])
 
     def prompt(self, tokens: torch.Tensor, row: int) -> torch.Tensor:
         """A prompt [tokens] into the empty cache row; logits [tokens, vocab]."""
@@ -131,34 +130,40 @@ class TextModel:
 
         return self._forward(tokens, where.expand(n).contiguous(), positions, attention)
 
-    def step(self, tokens: torch.Tensor, rows: torch.Tensor, positions: torch.Tensor | None = None) -> torch.Tensor:
+    def step(self, tokens: torch.Tensor, rows: torch.Tensor, positions: torch.Tensor | None = None,
+             prefix: int | torch.Tensor | None = None) -> torch.Tensor:
         """One token for each of the cache rows (int32): logits [rows, vocab].  ``positions``: where the tokens go, if
-        they are reserved already."""
+        they are reserved already.  ``prefix``: the rows' first so many tokens are the same (an int, or one int32 on the
+        device)."""
         if positions is None:
             positions = self.cache.reserve(rows, 1)
 
         def attention(layer, b, q, k, v):
-            return self.cache.attend(layer, q, rows, window=b.window, sinks=b.sinks)
+            if prefix is None or b.window:
+                return self.cache.attend(layer, q, rows, window=b.window, sinks=b.sinks)
+            return self.cache.attend_prefix(layer, q, prefix, rows)
 
         return self._forward(tokens, rows, positions, attention)
 
-    def capture(self, rows: torch.Tensor):
+    def capture(self, rows: torch.Tensor, prefix: int | torch.Tensor | None = None):
         """A step of these rows as one CUDA graph: (tokens to fill in, graph, logits)."""
         tokens = torch.zeros(len(rows), dtype=torch.long, device=self.device)
         start = self.cache.seq_lens[rows.long()].clone()         # warm-up: written at the rows' ends, nothing reserved
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
-            self.step(tokens, rows, torch.full_like(start, -1))
+            self.step(tokens, rows, torch.full_like(start, -1), prefix)
         torch.cuda.current_stream().wait_stream(side)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
-            logits = self.step(tokens, rows)
+            logits = self.step(tokens, rows, None, prefix)
         return tokens, graph, logits
 
-    def generate(self, prompt: torch.Tensor, samples: int, steps: int, uniform: torch.Tensor | None = None) -> torch.Tensor:
+    def generate(self, prompt: torch.Tensor, samples: int, steps: int, uniform: torch.Tensor | None = None,
+                 **sampling) -> torch.Tensor:
         """``samples`` continuations of ``steps`` tokens of one prompt: [samples, steps].  ``uniform`` [steps, samples] in
-        [0, 1) chooses the tokens (inverse distribution function); without it each is the likeliest."""
+        [0, 1) chooses the tokens (``ops.sample_tokens``, with its temperature, top_k, top_p and min_p); without it each is
+        the likeliest."""
         if samples + 1 > self.cfg.rows:
             raise ValueError(f"{samples} samples and the prompt need {samples + 1} cache rows, there are {self.cfg.rows}")
         rows = torch.arange(1, samples + 1, dtype=torch.int32, device=self.device)
@@ -168,13 +173,9 @@ class TextModel:
         positions = self.cache.branch(torch.zeros_like(rows), rows, 1)
         out = []
         for i in range(steps):
-            if uniform is None:
-                out.append(logits.argmax(-1))
-            else:
-                total = logits.float().softmax(-1).cumsum(-1)
-                out.append(torch.searchsorted(total, uniform[i].view(-1, 1) * total[:, -1:]).squeeze(1).clamp(max=self.cfg.vocab - 1))
+            out.append(logits.argmax(-1) if uniform is None else ops.sample_tokens(logits, uniform[i], **sampling))
             if i + 1 < steps:
-                logits = self.step(out[-1], rows, positions)
+                logits = self.step(out[-1], rows, positions, len(prompt))
                 positions = None
         self.cache.check()
         return torch.stack(out, dim=1)
@@ -193,7 +194,7 @@ def main() -> None:
     prompt = torch.randint(0, cfg.vocab, (a.prompt,), generator=g, device="cuda")
     tokens = model.generate(prompt, a.samples, 4)
     rows = torch.arange(1, a.samples + 1, dtype=torch.int32, device="cuda")
-    fill, graph, _ = model.capture(rows)
+    fill, graph, _ = model.capture(rows, a.prompt)
     fill.copy_(tokens[:, -1])
     torch.cuda.synchronize()
     t = time.perf_counter()

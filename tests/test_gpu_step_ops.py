@@ -725,3 +725,58 @@ def _status():
     from comfy_quant_bench_b200 import _lib
     torch.cuda.synchronize()
     return _lib.take_device_status()
+
+
+# ----------------------------------------------------------------------------------------------------------
+# the operators together, in the small language model of ``textgen``.  Both ways of attending a shared prompt lie within the
+# bound that test_gpu_textgen derives for a model's logits (2.3e-2 of relative L2 for two blocks), so they differ by twice it.
+# ----------------------------------------------------------------------------------------------------------
+
+def _model(**kw):
+    from comfy_quant_bench_b200 import textgen
+    base = dict(vocab=500, hidden=256, layers=2, heads=8, kv_heads=2, head_dim=64, ffn=512, group_size=64, max_tokens=160, rows=6,
+                pages=80, page_size=16)
+    return textgen.TextModel(textgen.TextConfig(**{**base, **kw}))
+
+
+@pytest.mark.parametrize("kw", [{}, {"max_tokens": 70000}, {"max_tokens": 70000, "window": 24, "sinks": 3}])
+def test_steps_behind_a_shared_prompt(kv, kw):
+    """Rows forked from one prompt; with room for 70000 tokens a row its tokens are attended once for all rows."""
+    g = _gen(5)
+    prompt, tokens = torch.randint(0, 500, (37,), generator=g, device="cuda"), torch.randint(0, 500, (12, 5), generator=g, device="cuda")
+    models = [_model(**kw) for _ in range(3)]
+    rows = torch.arange(1, 6, dtype=torch.int32, device="cuda")
+    for m in models:
+        m.prompt(prompt, 0)
+        m.cache.branch(torch.zeros_like(rows), rows, 0)
+    shared = torch.tensor([37], dtype=torch.int32, device="cuda")
+    fill, graph, held = models[2].capture(rows, shared)
+    for i in range(12):
+        alone, together = models[0].step(tokens[i], rows), models[1].step(tokens[i], rows, None, 37)
+        assert float((alone.float() - together.float()).norm() / alone.float().norm()) <= 4.6e-2
+        fill.copy_(tokens[i])
+        graph.replay()
+        assert torch.equal(held, together)
+    for m in models:
+        m.cache.check()
+    assert _status() == (0, 0)
+
+
+def test_generate_with_filters(ops):
+    m = _model()
+    prompt = torch.arange(33, device="cuda")
+    u = torch.rand(10, 3, generator=_gen(1), device="cuda")
+    greedy = m.generate(prompt, 3, 10)
+    assert torch.equal(m.generate(prompt, 3, 10, u, top_k=1), greedy)
+    assert torch.equal(m.generate(prompt, 3, 10, u, temperature=0.0), greedy)
+    assert torch.equal(m.generate(prompt, 3, 10, u, min_p=1.0), greedy)
+    some = m.generate(prompt, 3, 10, u, temperature=0.7, top_k=50, top_p=0.9, min_p=0.01)
+    assert some.shape == (3, 10) and torch.equal(m.generate(prompt, 3, 10, u, temperature=0.7, top_k=50, top_p=0.9, min_p=0.01), some)
+
+
+def test_a_long_context_model_steps(ops):
+    m = _model(rope_scaling="parts", rope_factor=4.0, rope_original=40, cache_dtype=FP8)
+    logits = m.prompt(torch.arange(100, device="cuda"), 0)
+    step = m.step(torch.tensor([3], device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda"))
+    assert bool(torch.isfinite(logits).all()) and bool(torch.isfinite(step).all())
+    m.cache.check()

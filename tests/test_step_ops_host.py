@@ -111,3 +111,74 @@ def test_tables_of_angles():
                 dict(rot_dim=64, scaling="parts", factor=2.0)):
         with pytest.raises(ValueError):
             kvcache.rope_table(4, device="cpu", **bad)
+
+
+def test_prefix_attention_argument_checks_need_no_device(lib):
+    from comfy_quant_bench_b200 import _lib as L
+    size = lib.cq_prefix_attention_workspace_bytes
+    assert size(4, 8, 2, 128, 100, ) == 0 and size(0, 8, 2, 128, 1 << 20) == 0          # read row by row, whole
+    assert size(64, 32, 8, 128, 16000) > 64 * 32 * 132 * 4
+    assert size(2, 8, 3, 128, 64) == -1 and size(2, 8, 2, 96, 64) == -1 and size(-1, 8, 2, 64, 64) == -1
+
+    def call(q=VP, dt=0, b=64, hq=32, hk=8, d=128, cdt=0, pages=10, page=16, st=128, width=1000, ts=1000, lens=VP, prefix=VP, n=0,
+             out=VP, ws=VP, wsn=1 << 40):
+        return lib.cq_prefix_attention(q, 4096, 128, dt, b, hq, hk, d, VP, VP, cdt, pages, page, 16384, 2048, st, VP, 64, width, ts,
+                                       None, lens, prefix, n, 1.0, None, None, out, None, ws, wsn, None)
+    assert call(dt=2) == L.CQ_ERR_ARG and call(cdt=1) == L.CQ_ERR_ARG and call(q=None) == L.CQ_ERR_ARG
+    assert call(lens=None) == L.CQ_ERR_ARG and call(out=None) == L.CQ_ERR_ARG and call(ws=None) == L.CQ_ERR_ARG
+    assert call(page=12) == L.CQ_ERR_SHAPE and call(hq=30) == L.CQ_ERR_SHAPE and call(d=96) == L.CQ_ERR_SHAPE
+    assert call(n=-1) == L.CQ_ERR_SHAPE and call(n=1 << 31) == L.CQ_ERR_SHAPE and call(wsn=1024) == L.CQ_ERR_SHAPE
+    assert call(b=65536) == L.CQ_ERR_SHAPE and call(ts=999) == L.CQ_ERR_SHAPE
+    assert call(q=ctypes.c_void_p(264)) == L.CQ_ERR_ALIGN and call(st=129) == L.CQ_ERR_ALIGN
+    assert call(prefix=ctypes.c_void_p(258)) == L.CQ_ERR_ALIGN and call(ws=ctypes.c_void_p(128)) == L.CQ_ERR_ALIGN
+    assert call(b=0, q=None, lens=None, out=None, ws=None) == L.CQ_OK
+
+
+def test_sample_argument_checks_need_no_device(lib):
+    from comfy_quant_bench_b200 import _lib as L
+
+    def call(x=VP, ld=100, dt=3, rows=2, vocab=100, u=VP, k=0, tokens=VP, logs=None, ts=None):
+        return lib.cq_sample(x, ld, dt, rows, vocab, u, ts, 1.0, None, k, None, 1.0, None, 0.0, tokens, logs, None)
+    assert call(dt=2) == L.CQ_ERR_ARG and call(dt=4) == L.CQ_ERR_ARG and call(x=None) == L.CQ_ERR_ARG
+    assert call(u=None) == L.CQ_ERR_ARG and call(tokens=None) == L.CQ_ERR_ARG
+    assert call(rows=-1) == L.CQ_ERR_SHAPE and call(vocab=0) == L.CQ_ERR_SHAPE and call(vocab=327681, ld=400000) == L.CQ_ERR_SHAPE
+    assert call(ld=99) == L.CQ_ERR_SHAPE and call(k=-1) == L.CQ_ERR_SHAPE
+    assert call(x=ctypes.c_void_p(258)) == L.CQ_ERR_ALIGN and call(tokens=ctypes.c_void_p(260)) == L.CQ_ERR_ALIGN
+    assert call(ts=ctypes.c_void_p(258)) == L.CQ_ERR_ALIGN
+    assert call(rows=0, x=None, u=None, tokens=None) == L.CQ_OK
+
+
+def test_more_refusals_say_what_is_wrong():
+    from comfy_quant_bench_b200 import kvcache, ops
+    k, n = torch.zeros(6, 2, 16, 64, dtype=BF), torch.zeros(2, dtype=torch.int32)
+    t, q = torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, 4, 64, dtype=BF)
+    x, u = torch.zeros(3, 50), torch.zeros(3)
+
+    def attend(prefix=5, q=q, **kw):
+        return kvcache.prefix_attention(q, k, k, t, n, prefix, **kw)
+
+    def sample(x=x, u=u, **kw):
+        return ops.sample_tokens(x, u, **kw)
+    for says, call in (("must not be negative, got -1", lambda: attend(-1)),
+                       ("int32 tensor of one element", lambda: attend(n)),
+                       ("int32 tensor of one element", lambda: attend(torch.zeros(1, dtype=torch.int64))),
+                       ("multiple of kv_heads", lambda: attend(q=q[:, :3])),
+                       ("64, 128 or 256", lambda: attend(q=q[..., :32])),
+                       ("rows must have 2 entries", lambda: attend(rows=n[:1])),
+                       (r"f32 \[rows, vocab\]", lambda: sample(x=x.double())),
+                       (r"f32 \[rows, vocab\]", lambda: sample(x=x[0])),
+                       ("1 to 327680, got 0", lambda: sample(x=x[:, :0])),
+                       (r"uniform must be f32 \[3\]", lambda: sample(u=u[:2])),
+                       (r"uniform must be f32 \[3\]", lambda: sample(u=u.double())),
+                       ("temperature is out of range", lambda: sample(temperature=-1.0)),
+                       ("temperature is out of range", lambda: sample(temperature=float("nan"))),
+                       ("top_k is out of range", lambda: sample(top_k=-3)),
+                       ("top_p is out of range", lambda: sample(top_p=1.5)),
+                       ("min_p is out of range", lambda: sample(min_p=-0.1)),
+                       (r"top_p must be a number or Float \[3\]", lambda: sample(top_p=u[:1])),
+                       (r"top_k must be a number or Int \[3\]", lambda: sample(top_k=u))):
+        with pytest.raises(ValueError, match=says):
+            call()
+    for call in (attend, sample):
+        with pytest.raises(ValueError, match="CUDA"):
+            call()
