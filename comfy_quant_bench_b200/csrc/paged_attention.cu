@@ -18,6 +18,9 @@
 // the warps' running maxima, sums and outputs are joined in the stages they have just consumed.  All orders are fixed,
 // so equal calls give equal bits.
 //
+// Behind a shared prefix (prefix_attention.cu) a row that holds it sees only its own tokens, and its output stays fp32 with
+// the log of its sum, for that file's join.
+//
 // Softmax statistics, scores and outputs are fp32.  The weights p enter the second product as two parts of the cache's
 // 16-bit type, p = hi + lo, since one part alone would add up to as much error as rounding the output does.  f16 parts
 // hold 2^15 p, and the sum is taken over the same: without it a weight of 2^-25 of the largest, which a long tail behind
