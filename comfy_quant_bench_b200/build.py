@@ -72,7 +72,6 @@ def build(verbose: bool = False, force: bool = False) -> str:
     if force or needs_build():
         _run([nvcc_path(), "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
               "--expt-relaxed-constexpr", "-shared", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
-              "--split-compile", "0",                     # the kernels are optimised on all cores: 4.5 min -> 2
               "-Xptxas", "-v" if verbose else "-O3", "-o", LIB + ".tmp", os.path.join(SRC, "libcq.cu")], LIB, verbose)
     if force or _stale(BIND, [BIND_SRC, HEADER]):
         _build_bind(verbose)
