@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(pfx::Cfg<D>::kThreads, 1) prefix_attention_ker
         }
         look_up(j + step);
         const uint32_t s_at = s_col + buf * C::kSCols + lanes;
-        // half a row of scores; the largest, NaN where one is
+        // a row of scores; NaN is passed over here and shows in the weights
         uint32_t v[kKeys / 32][32];
 #pragma unroll
         for (int x = 0; x < kKeys / 32; ++x) tmem_ld_32x32b_x32(s_at + 32 * x, v[x]);
