@@ -54,8 +54,11 @@ struct Shared {
 };
 }  // namespace samp
 
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_arrive();
+  cluster_wait();
 }
 __device__ __forceinline__ void st_cluster_u64(uint32_t addr, unsigned long long v) {
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
@@ -344,6 +347,8 @@ __global__ void __launch_bounds__(samp::kThreads, 2) sample_kernel(const SampleA
   if (tid < 64) sh.power[tid] = exp2(tid / 64.0);
   if (tid == 0) sh.list_n = 0;
   for (int i = tid; i < samp::kBins; i += samp::kThreads) sh.hist[i] = 0;
+  __syncwarp();
+  cluster_arrive();                                                    // this CTA has started; waited for before the first store to another
   grid_dep_wait();
 
   const float temperature = a.temperatures != nullptr ? a.temperatures[row] : a.temperature;
@@ -418,6 +423,7 @@ __global__ void __launch_bounds__(samp::kThreads, 2) sample_kernel(const SampleA
     least = fminf(least, box[samp::kWarps + w]);
   }
   __syncthreads();
+  cluster_wait();                                                      // all CTAs of the cluster run: their memory may be written
   {
     const u64(*all)[2] = s.exchange(__float_as_uint(most), __float_as_uint(least));
     for (int r = 0; r < ranks; ++r) {

@@ -182,3 +182,19 @@ def test_more_refusals_say_what_is_wrong():
     for call in (attend, sample):
         with pytest.raises(ValueError, match="CUDA"):
             call()
+
+
+def test_sampling_waits_for_its_cluster_before_it_writes_to_it():
+    """Another CTA's shared memory may be touched once that CTA runs: every CTA arrives at the cluster's barrier as it starts
+    and waits there, on every path, before its first store to another (whose help, ``exchange``, is the first to use one)."""
+    import os
+    import re
+
+    from comfy_quant_bench_b200 import build
+    source = open(os.path.join(build.SRC, "sample.cu")).read()
+    body = source[source.index("sample_kernel(const SampleArgs"):]
+    body = body[:body.index("\nnamespace {")]
+    before = re.split(r"exchange\(|there\(|cluster_sum\(|add_at_first\(|cut_in_bin<|list_up_to", body)[0]
+    assert before.count("cluster_arrive()") == 1 and before.count("cluster_wait()") == 1
+    assert before.index("cluster_arrive()") < before.index("grid_dep_wait()") < before.index("cluster_wait()")
+    assert "return;" not in before and "cluster_sync_all()" not in before
