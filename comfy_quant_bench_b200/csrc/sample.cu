@@ -457,7 +457,8 @@ __global__ void __launch_bounds__(samp::kThreads, 2) sample_kernel(const SampleA
   }
   s.by = 1.4426950408889634074 / static_cast<double>(temperature);
   s.range = fminf(fminf(samp::kReach * temperature, most - least), 3e38f);
-  s.inv_width = s.range > 0.0f ? samp::kBins / s.range : 0.0f;
+  // finite where the reach is next to nothing (temperatures below 7e-37): bins are then wider than they have to be
+  s.inv_width = s.range > 0.0f ? fminf(samp::kBins / s.range, 1e38f) : 0.0f;
   const bool cut_k = top_k > 0 && top_k < a.vocab, cut_p = top_p < 1.0f;
 
   u64 cut = 0;                                                         // what lies at or above it stays
@@ -542,8 +543,9 @@ __global__ void __launch_bounds__(samp::kThreads, 2) sample_kernel(const SampleA
     // ---- bounds of the sums from the counts: a token of bin b weighs 2^-(b + 1) width .. 2^-b width; the border lies in a
     // bin that the bounds allow; sums of the bins before are exact, and those of the allowed bins each ----
     // top-k's cut ends the bins; its own one is counted whole in the upper bounds and not at all in the lower
-    const float step = s.inv_width > 0.0f ? static_cast<float>(s.by) / s.inv_width : 0.0f;   // a bin's width, as a power of 2
-    const float ratio = exp2f(step * 1.001f);                          // of a bin's bounds (1.001: fp32 bins)
+    const float step = s.inv_width > 0.0f ? static_cast<float>(s.by / s.inv_width) : 0.0f;   // a bin's width, as a power of 2
+    // of a bin's bounds (1.001: fp32 bins); what is in a bin weighs 2^-46 at least, however wide the bin
+    const float ratio = exp2f(fminf(step * 1.001f, 46.0f));
     const int last = cut != 0 ? sh.found[0] : samp::kBins - 1;         // no token below this bin
     float up[kEach], mine = 0.0f;                                      // upper bounds
 #pragma unroll

@@ -780,3 +780,22 @@ def test_a_long_context_model_steps(ops):
     step = m.step(torch.tensor([3], device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda"))
     assert bool(torch.isfinite(logits).all()) and bool(torch.isfinite(step).all())
     m.cache.check()
+
+
+@pytest.mark.parametrize("t", [2.0 ** -149, 1e-44, 1e-40, 4e-39, 5e-39, 2.0 ** -126, 1e-37, 3e-37, 6.6e-37, 7e-37, 1e-36, 1e-30])
+@pytest.mark.parametrize("vocab", [9, 700, 5000])
+def test_sample_temperatures_next_to_nothing(ops, vocab, t):
+    """Temperatures down to the smallest subnormal: the definition holds, for logits that differ by far more than the
+    temperature (the largest, or those equal to it, share the row) and for some that differ by a few times it."""
+    t = float(torch.tensor(t, dtype=torch.float32))
+    x, u = _logits(6, vocab, torch.float32)
+    x[1, 3::4] = x[1].max() + 1                                        # several at the maximum
+    x[2] = -7.0                                                        # all of them
+    g = torch.Generator().manual_seed(vocab)
+    fine = torch.randn(6, vocab, generator=g, dtype=torch.float64) * 6 * t
+    fine = torch.round(fine * 2.0 ** 149) * 2.0 ** -149                # multiples of the smallest number: f32 holds them
+    for logits in (x, fine.float().cuda()):
+        for k, p, m in ((0, 1.0, 0.0), (0, 0.9, 0.0), (0, 0.4, 0.05), (4, 1.0, 0.0), (5, 0.7, 0.0), (vocab - 1, 0.95, 0.0), (0, 0.0, 0.0)):
+            tokens = _sample_holds(ops, logits, u, t, k, p, m)
+            each = torch.full((6,), t, device="cuda")
+            assert torch.equal(ops.sample_tokens(logits, u, temperature=each, top_k=k, top_p=p, min_p=m), tokens)
