@@ -5,8 +5,9 @@
 //   order of the indexes, whose running sum exceeds u times the sum.
 //
 // The choice has to be the one of exact arithmetic, so weights are integers, round(2^44 weight): sums are exact, in any
-// order, and equal calls give equal bits.  2^x comes in 64 bits from a table of 2^(j/64) and a polynomial of degree four in
-// the rest, |rest| <= 1/128 (Taylor, 4e-14).  A token whose weight rounds to 0 can neither be chosen nor count.
+// order, and equal calls give equal bits.  2^x comes in 64 bits from a table of 2^(j/64) and a polynomial of degree five in
+// the rest, |rest| <= 1/128 (Taylor: the next term is 4e-17, a thousandth of 2^-44; of degree four it would be 4e-14, more
+// than half of it).  A token whose weight rounds to 0 can neither be chosen nor count.
 //
 // A cluster of CTAs takes a row and keeps it in shared memory: one read of the logits.  A cut (of top-k, of top-p) is an
 // element's composite, its logit's order in the high half and its index, reversed, in the low: what lies at or above it
@@ -144,7 +145,8 @@ struct Sampler {
     const int k = static_cast<int>(__double2loint(t));
     const double f = fma(t - magic, -1.0 / 64.0, y);
     constexpr double l2 = 0.693147180559945309417;
-    double p = fma(f, l2 * l2 * l2 * l2 / 24.0, l2 * l2 * l2 / 6.0);
+    double p = fma(f, l2 * l2 * l2 * l2 * l2 / 120.0, l2 * l2 * l2 * l2 / 24.0);
+    p = fma(f, p, l2 * l2 * l2 / 6.0);
     p = fma(f, p, l2 * l2 / 2.0);
     p = fma(f, p, l2);
     p = fma(f, p, 1.0) * s.power[k & 63];

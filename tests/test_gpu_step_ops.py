@@ -9,7 +9,10 @@ Bounds.  u is half a step of the output type relative to the value (2^-8 bf16, 2
 * Rotation: each of the two products and their sum is fp32, the norm before it as above:
   |y - exact| <= u |exact| + ((D / 32 + 28) 2^-24) (|a| + |b|) for the pair (a, b) turned.
 """
+import decimal
+import fractions
 import math
+import random
 
 import pytest
 import torch
@@ -799,3 +802,36 @@ def test_sample_temperatures_next_to_nothing(ops, vocab, t):
             tokens = _sample_holds(ops, logits, u, t, k, p, m)
             each = torch.full((6,), t, device="cuda")
             assert torch.equal(ops.sample_tokens(logits, u, temperature=each, top_k=k, top_p=p, min_p=m), tokens)
+
+
+def _weights_next_to_a_choice(n):
+    """[(logit, temperature, u, token)] of two tokens, the first with a logit below 0, the second with 0.  With w the first
+    one's weight and W = round(2^44 w) it is chosen where W exceeds u (W + 2^44), that is where W > 2^44 u / (1 - u).  The
+    quotient of logit and temperature, a fraction of two integers below 2^24, puts W next to that border, on one of its
+    sides: a weight that is off by one unit more than its rounding is chosen wrongly."""
+    decimal.getcontext().prec = 50
+    rng, one, cases = random.Random(1), decimal.Decimal(2) ** 44, []
+    while len(cases) < n:
+        share = 2.0 ** (-(2 * rng.randrange(40) + 1 + rng.uniform(-0.06, 0.06)) / 128)    # halfway between table entries
+        u = math.floor(share / (1 + share) * 2 ** 25) / 2 ** 25                           # an f32
+        border = decimal.Decimal(u) / (1 - decimal.Decimal(u)) * one
+        aim = math.floor(border) + rng.randrange(2) + decimal.Decimal(rng.uniform(-0.3, 0.3))
+        x = fractions.Fraction(-(aim / one).ln()).limit_denominator((1 << 24) - 1)
+        exact = one * (decimal.Decimal(-x.numerator) / decimal.Decimal(x.denominator)).exp()
+        held = int(exact.to_integral_value())
+        if x.numerator < 1 << 24 and abs(exact - held) <= decimal.Decimal("0.45") and decimal.Decimal("0.01") <= abs(held - border) <= 1:
+            cases.append((-x.numerator * 2.0 ** -24, x.denominator * 2.0 ** -24, u, 0 if held > border else 1))
+    return cases
+
+
+def test_sample_weights_are_right_to_their_rounding(ops):
+    cases = _weights_next_to_a_choice(600)
+    x, t, u, want = (torch.tensor(c) for c in zip(*cases))
+    assert 200 < int(want.sum()) < 400
+    logits = torch.stack([x, torch.zeros_like(x)], dim=1).cuda()
+    for width in (2, 3000):                                            # alone, and where eight CTAs hold the row
+        row = torch.full((len(cases), width), float("-inf"), device="cuda")
+        row[:, 0], row[:, -1] = logits[:, 0], logits[:, 1]
+        for p in (1.0, 0.999):
+            got = ops.sample_tokens(row, u.cuda(), temperature=t.cuda(), top_p=p)
+            assert torch.equal((got > 0).long().cpu(), want), (width, p, int(((got > 0).long().cpu() != want).sum()))
