@@ -4,48 +4,92 @@
 //
 // and y rounded once to the type, or in 8 bits: with p = h w and P the largest |p| of the row (or of a group of 32, 64 or
 // 128 columns), code = round(top p / P), scale = P / (top sqrt(mean(h^2) + eps)), top = 127 (int8) or 448 (e4m3).  The
-// root cancels in the code, and p is exact in fp32 (16-bit factors), so an int8 code is a function of exact values: next
-// to a border between two codes it is decided in 64 bits.
+// root cancels in the code, and p is exact in fp32 (16-bit factors), so a code is a function of exact values: the nearest
+// one of the exact quotient.
 //
 // Bound by reading x, r and writing h, y once: a row stays in registers between its sums and its outputs.  One reduction
 // serves both the sum of squares and the maximum.
 //
 // Measured on a B200 (device time): 16384 rows of 4096, bf16 in and out: 82 us, 6.6 TB/s, HBM's rate; 100000 rows of 512 to
-// e4m3: 57 us, 6.3 TB/s; 8192 rows of 8192 to e4m3 in groups of 128: 88 us, 5.4 TB/s, and to int8: 111 us, 4.2 TB/s, bound by
+// e4m3: 56 us, 6.4 TB/s; 8192 rows of 8192 to e4m3 in groups of 128: 85 us, 5.5 TB/s, and to int8: 107 us, 4.4 TB/s, bound by
 // the conversions (an SM's integer and conversion pipes); one row of 4096: 2.3 us, launch and latency.
 #include "decode_common.cuh"
 
 namespace cq {
 
-// Codes of p against the largest P: `by` is top / P, or 0 where P is 0.
+// int8 codes of p against the largest P: `by` is 127 / P, or 0 where P is 0.
 struct Coder {
   float most, by;
-  bool tiny;                                   // top / P would overflow: the quotient first
+  bool tiny;                                   // 127 / P would overflow: the quotient first
 };
-template <int OUT>
 __device__ __forceinline__ Coder coder(float most) {
-  constexpr float top = OUT == kNormInt8 ? 127.0f : 448.0f;
   Coder c{most, 0.0f, most < 1e-30f};
-  if (most > 0.0f) c.by = c.tiny ? top : __fdiv_rn(top, most);
+  if (most > 0.0f) c.by = c.tiny ? 127.0f : __fdiv_rn(127.0f, most);
   return c;
-}
-template <int OUT>
-__device__ __forceinline__ float scaled(float p, const Coder& c) {
-  return c.tiny ? (c.most > 0.0f ? __fdiv_rn(p, c.most) * c.by : 0.0f) : p * c.by;
 }
 // the nearest code in 64 bits: rare, and out of the way of the others
 __device__ __noinline__ int int8_code_exactly(float p, float most) {
   return static_cast<int>(rint(static_cast<double>(p) * 127.0 / static_cast<double>(most)));
 }
 __device__ __forceinline__ uint32_t int8_code(float p, const Coder& c) {
-  const float t = scaled<kNormInt8>(p, c), k = rintf(t);
+  const float t = c.tiny ? (c.most > 0.0f ? __fdiv_rn(p, c.most) * c.by : 0.0f) : p * c.by, k = rintf(t);
   int code = static_cast<int>(k);
   // t is off by 2^-23 of itself, 1.52e-5 at most: only that near to a border can the nearest code be another one
   if (fabsf(t - k) > 0.5f - 1.6e-5f) code = int8_code_exactly(p, c.most);
   return static_cast<uint32_t>(code) & 0xffu;
 }
-__device__ __forceinline__ uint32_t e4m3_pair(float a, float b) {
-  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+
+// e4m3 codes of the quotients 448 p / P.  A border b between two codes has five bits, so 448 p - b P is 0 or, where p has bf16
+// factors, 2^-21 of either at least: 448 p is exact then, and a step of Newton's method, t + (448 p - t P) / P, rounds the
+// quotient to fp32 but for 2^-45 of itself, to the quotient's side of b or to b with it.  f16 factors have more digits: t is off
+// by 2^-23, and near a border the sign of 448 p - b P, exact in two parts, decides.  (Bits that tell where a border is
+// near, for bf16 too: 101 us in the first 8-bit case above, since many quotients of 8-bit numbers lie on one.)
+struct Quotients {
+  float wide, most, inv;                       // 448 and P, times a power of 2 that keeps the products in range, and 1 / P
+};
+template <bool F16>
+__device__ __forceinline__ Quotients quotients(float most) {
+  const float scale = F16 ? 1.0f : most > 1e30f ? 0x1p-40f : most < 1e-20f ? 0x1p60f : 1.0f;
+  const bool some = most > 0.0f && most < INFINITY;                    // else every finite p has code 0
+  return {448.0f * scale, some ? most * scale : 0.0f, some ? __frcp_rn(most * scale) : 0.0f};
+}
+__device__ __forceinline__ uint32_t e4m3_pair(float2 t) { return __nv_cvt_float2_to_fp8x2(t, __NV_SATFINITE, __NV_E4M3); }
+// four bits are kept from 2^-6 on, and a border has 1000... behind them: the bits that follow are moved to the top, and those of
+// a value that may lie on the other side of a border are at most kNear
+constexpr uint32_t kNear = 6u << 12;
+__device__ __forceinline__ uint32_t from_border(float t) { return (__float_as_uint(t) << 12) + (3u << 12) - (0x80000u << 12); }
+// t on its quotient's side of the border between two codes, or on it.  Below 2^-6 a code is a multiple of 2^-9, as from there
+// to 2^-5: the bits are those of t moved up (short of 2^-6, so that the sum does not round to 2^-5)
+__device__ __forceinline__ float settled(float t, float p, float most) {
+  const float up = fabsf(t) < 0x1.fffffp-7f ? 0x1p-6f : 0.0f;
+  const float border = __uint_as_float((__float_as_uint(fabsf(t) + up) & 0xfff00000u) | 0x80000u) - up;
+  const float size = fabsf(p), wide = 448.0f * size, d = fmaf(-border, most, wide) + fmaf(448.0f, size, -wide);
+  return copysignf(d == 0.0f ? border : fmaf(border, copysignf(0x1p-20f, d), border), p);
+}
+// N = 2 or 8 values; two codes to a uint32
+template <bool F16, int N>
+__device__ __forceinline__ void e4m3_codes(const float (&p)[N], const Quotients& c, uint32_t (&code)[N / 2]) {
+  const float2 none = make_float2(0.0f, 0.0f), inv = make_float2(c.inv, c.inv);
+  float2 t[N / 2];
+  uint32_t from = 0xffffffffu;
+  float least = 1.0f;
+#pragma unroll
+  for (int j = 0; j < N / 2; ++j) {
+    const float2 wide = fma2(make_float2(p[2 * j], p[2 * j + 1]), make_float2(c.wide, c.wide), none);
+    t[j] = fma2(wide, inv, none);
+    if constexpr (F16) {
+      from = min(from, min(from_border(t[j].x), from_border(t[j].y)));
+      least = fminf(least, fminf(fabsf(t[j].x), fabsf(t[j].y)));
+    } else {
+      t[j] = fma2(fma2(t[j], make_float2(-c.most, -c.most), wide), inv, t[j]);
+    }
+  }
+  if (F16 && (from <= kNear || least < 0x1p-6f) && c.most > 0.0f) {
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) t[j] = make_float2(settled(t[j].x, p[2 * j], c.most), settled(t[j].y, p[2 * j + 1], c.most));
+  }
+#pragma unroll
+  for (int j = 0; j < N / 2; ++j) code[j] = e4m3_pair(t[j]);
 }
 
 // The sum and the maximum over a row's threads: a warp, or a block of whole warps.
@@ -161,20 +205,18 @@ __global__ void __launch_bounds__(WARP ? 256 : CHUNKS < 4 ? 512 : 1024) add_norm
         if (c < eights && (8 * c & (a.group - 1)) == 0) a.scale[8 * c / a.group * a.rows + row] = top * inv / kTop;
       }
       if (c >= eights) continue;
-      const Coder by = coder<OUT>(top);
       uint2 q;
       if constexpr (OUT == kNormInt8) {
+        const Coder by = coder(top);
         uint32_t b[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) b[j] = int8_code(p[j], by);
         q.x = b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24;
         q.y = b[4] | b[5] << 8 | b[6] << 16 | b[7] << 24;
       } else {
-        float t[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) t[j] = scaled<OUT>(p[j], by);
-        q.x = e4m3_pair(t[0], t[1]) | e4m3_pair(t[2], t[3]) << 16;
-        q.y = e4m3_pair(t[4], t[5]) | e4m3_pair(t[6], t[7]) << 16;
+        uint32_t codes[4];
+        e4m3_codes<F16>(p, quotients<F16>(top), codes);
+        q = make_uint2(codes[0] | codes[1] << 16, codes[2] | codes[3] << 16);
       }
       *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.out) + row * a.width + 8 * c) = q;
     }
@@ -208,7 +250,8 @@ __global__ void __launch_bounds__(256) add_norm_odd_kernel(const AddNormArgs a) 
   }
   row_reduce<WARP>(sum, most, red);
   const float inv = rsqrtf(sum / static_cast<float>(a.width) + a.eps);
-  const Coder by = coder<OUT>(most);
+  const Coder by = coder(most);
+  const Quotients per = quotients<F16>(most);
   if (OUT != kNormSame && tid == 0) a.scale[row] = most * inv / (OUT == kNormInt8 ? 127.0f : 448.0f);
 #pragma unroll 4
   for (int c = tid; c < a.width; c += team) {
@@ -216,7 +259,12 @@ __global__ void __launch_bounds__(256) add_norm_odd_kernel(const AddNormArgs a) 
     const int64_t to = row * a.width + c;
     if constexpr (OUT == kNormSame) static_cast<uint16_t*>(a.out)[to] = static_cast<uint16_t>(narrow16<F16>(p * inv, 0.0f));
     else if constexpr (OUT == kNormInt8) static_cast<uint8_t*>(a.out)[to] = static_cast<uint8_t>(int8_code(p, by));
-    else static_cast<uint8_t*>(a.out)[to] = static_cast<uint8_t>(e4m3_pair(scaled<OUT>(p, by), 0.0f));
+    else {
+      const float twice[2] = {p, p};
+      uint32_t code[1];
+      e4m3_codes<F16>(twice, per, code);
+      static_cast<uint8_t*>(a.out)[to] = static_cast<uint8_t>(code[0]);
+    }
   }
 }
 

@@ -835,3 +835,62 @@ def test_sample_weights_are_right_to_their_rounding(ops):
         for p in (1.0, 0.999):
             got = ops.sample_tokens(row, u.cuda(), temperature=t.cuda(), top_p=p)
             assert torch.equal((got > 0).long().cpu(), want), (width, p, int(((got > 0).long().cpu() != want).sum()))
+
+
+def _nearest_e4m3(q):
+    """The e4m3 value nearest to q (64 bits, at most 448), halves to the even one: multiples of 2^(e - 3) in [2^e, 2^(e + 1)),
+    of 2^-9 below 2^-6."""
+    step = torch.exp2((torch.frexp(q)[1].double() - 4).clamp(min=-9))
+    return torch.round(q / step) * step
+
+
+def _e4m3_codes_hold(ops, x, r, w, group):
+    q, scale, h = ops.add_rmsnorm(x, w, r, quant="fp8", group_size=group)
+    m, c = x.shape
+    p = (h.double() * w.double()).view(m, -1, group or c)
+    most = p.abs().amax(-1, keepdim=True)
+    want = _nearest_e4m3(p * 448.0 / torch.where(most == 0, 1.0, most)).view(m, c)
+    assert torch.equal(q.double(), want), int((q.double() != want).sum())
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("m,c,group", [(4096, 4096, 0), (4096, 4096, 32), (16384, 512, 128), (5000, 1001, 0), (700, 2049, 0), (5000, 520, 0)])
+def test_norm_e4m3_codes_are_the_nearest(ops, m, c, group, dtype):
+    """A code is the nearest one of the exact quotient 448 p / P (products p of 16-bit numbers), halves to the even one."""
+    x, r, w = _norm_problem(m, c, dtype)
+    _e4m3_codes_hold(ops, x, r, w, group)
+    _e4m3_codes_hold(ops, x, None, torch.ones_like(w), group)           # products of few digits: many on a border
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_norm_e4m3_codes_on_borders(ops, dtype):
+    """Quotients on borders: P = 2^a 7 gives 448 p / P = p 2^(6 - a), and other P quotients next to them; subnormal codes too."""
+    p = torch.cat([(2 * torch.arange(8, 16) + 1) * 2.0 ** e for e in range(-7, 4)] + [(2 * torch.arange(0, 8) + 1) * 2.0 ** -10 / 2.0 ** 2])
+    p = p[p < 100]
+    for top in (112.0, 111.0, 113.0, 127.5, 119.0, 448.0, 224.0):
+        x = torch.cat([p, -p, torch.tensor([top, 0.0])]).cuda().to(dtype)
+        for c in (x.numel(), (x.numel() + 7) // 8 * 8):
+            row = torch.zeros(2, c, dtype=dtype, device="cuda")
+            row[0, : x.numel()], row[1, -x.numel():] = x, x.flip(0)
+            for weight in (1.0, 1.5, 2.0 ** -100 if dtype == torch.bfloat16 else 2.0 ** -10):
+                _e4m3_codes_hold(ops, row, None, torch.full((c,), weight, device="cuda").to(dtype), 0)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("quant", ["int8", "fp8"])
+@pytest.mark.parametrize("c,group", [(512, 0), (512, 64), (509, 0)])
+def test_norm_codes_beside_an_infinity_and_of_extreme_rows(ops, c, group, quant, dtype):
+    """p / P is 0 beside an infinite P; rows near the ends of the type's range have the codes of their quotients."""
+    x = torch.randn(6, c, generator=_gen(c), device="cuda")
+    x[0, 5], x[1, 6] = float("inf"), float("-inf")
+    ends = [1e30, 3e38, 1e-25, 1e-35] if dtype == torch.bfloat16 else [60.0, 15000.0, 1e-3, 1e-4]
+    for i, size in enumerate(ends):
+        x[2 + i] *= size / x[2 + i].abs().max()
+    x, w = x.to(dtype), torch.ones(c, device="cuda", dtype=dtype)
+    q, scale, _ = ops.add_rmsnorm(x, w, quant=quant, group_size=group)
+    assert not q[0, : group or c].float()[torch.arange(group or c, device="cuda") != 5].any()
+    assert not q[1, : group or c].float()[torch.arange(group or c, device="cuda") != 6].any()
+    p = x[2:].double().view(4, -1, group or c)
+    quotient = (p * (127.0 if quant == "int8" else 448.0) / p.abs().amax(-1, keepdim=True)).view(4, c)
+    want = quotient.round() if quant == "int8" else _nearest_e4m3(quotient)
+    assert torch.equal(q[2:].double(), want)
