@@ -8,7 +8,7 @@
 // keys (64 at D 256), S, P and O in tensor memory.  A CTA holds two row tiles (one at D 256) against the same keys; where
 // there is one row tile only, its two tile slots take every other key tile.  Four warps a slot turn S into P in place, a row
 // a thread; one thread issues the products; four warps gather keys and values from their pages (8-bit caches are widened on
-// the way, which is exact).  A row's maximum is only raised when a score exceeds it by 2^8, since raising it rewrites O.
+// the way, which is exact).  A row's maximum is only raised when a score exceeds it by 2^8 (f16: 2), since raising it rewrites O.
 //
 // Work: teams of CTAs, a CTA for each pair of row tiles, take equal runs of key tiles, through as many key-value heads as
 // that covers; the team's CTAs read the same keys at the same time, from L2.  Every run leaves its sums (fp32) in the
@@ -53,6 +53,12 @@ struct Cfg {
   static constexpr int kSCols = kKeys;                       // columns of a score buffer
   static_assert(kSlots * (kBufs * kSCols + D) <= 512, "tensor memory");
 };
+// weights are raised by 2^lift, and the running maximum once a score exceeds it by 2^slack.  bf16 parts have fp32's range; f16
+// parts reach 2^15 and hold 2^-25, so 2^-39 of the running maximum: a long tail behind one strong key keeps its values
+template <bool F16>
+__host__ __device__ constexpr float lift() { return F16 ? 14.0f : 0.0f; }
+template <bool F16>
+__host__ __device__ constexpr float slack() { return F16 ? 1.0f : 8.0f; }
 // floats of a row tile's part: O as [D / 4][128 rows][4], then the rows' (maximum, sum)
 __host__ __device__ constexpr int64_t part_floats(int d) { return 128ll * d + 256; }
 }  // namespace pfx
@@ -454,8 +460,7 @@ __global__ void __launch_bounds__(pfx::Cfg<D>::kThreads, 1) prefix_attention_ker
     if constexpr (kSlots == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
     const int slot = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    constexpr float kLift = F16 ? 7.0f : 0.0f;                // f16 weights reach 2^15: up to 2^8 above the running maximum
-    constexpr float kSlackUp = 8.0f;
+    constexpr float kLift = pfx::lift<F16>(), kSlackUp = pfx::slack<F16>();
     uint32_t s_phase[2] = {0, 0}, o_phase = 0, run_phase = 0;   // o_phase: products of earlier runs
     bool ok = true;
     for (int64_t u = u0; u < u1 && ok;) {
@@ -631,7 +636,7 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const PrefixArgs a) {
   grid_dep_wait();
   const int64_t own = static_cast<int64_t>(b) * g.Hq + h;
   const float vs = g.cache_dtype == CQ_DT_FP8_E4M3 && g.v_scale != nullptr ? g.v_scale[head] : 1.0f;
-  constexpr float kLift = F16 ? 7.0f : 0.0f;
+  constexpr float kLift = pfx::lift<F16>();
   // the running maximum is of what the weights were raised by, a power of 2; own tokens first (-inf: none)
   float top = live ? g.lse[own] * 1.4426950408889634f + kLift : -INFINITY;
   const bool has_own = top != -INFINITY;

@@ -894,3 +894,23 @@ def test_norm_codes_beside_an_infinity_and_of_extreme_rows(ops, c, group, quant,
     quotient = (p * (127.0 if quant == "int8" else 448.0) / p.abs().amax(-1, keepdim=True)).view(4, c)
     want = quotient.round() if quant == "int8" else _nearest_e4m3(quotient)
     assert torch.equal(q[2:].double(), want)
+
+
+@pytest.mark.parametrize("cache", [torch.float16, FP8])
+@pytest.mark.parametrize("b,hq,hk,d,prefix", [(40, 8, 8, 128, 2096), (33, 24, 8, 64, 4000), (17, 8, 8, 256, 2000), (64, 64, 8, 128, 1104)])
+def test_prefix_keeps_a_tail_behind_one_strong_key(kv, b, hq, hk, d, prefix, cache):
+    """f16 weights of e^-18 (2^-26) of the largest, whose own value is 0: all that is left is the tail.  A part of a weight holds
+    2^-25 of 2^14, 2^-39 of the running maximum, so 2^-13 of such a weight; one part rounds it by 2^-11 besides."""
+    lens = [prefix + i % 5 for i in range(b)]
+    q, k, v, table, n, scales = _prefix_problem(lens, prefix, hq, hk, d, 16, torch.float16, cache, holes=False, wide=False)
+    q.zero_(), k.view(torch.uint8).zero_()
+    q[..., 0] = 1.0
+    at = int(table[0, 0])
+    k[at, :, 0, 0] = 18.0
+    v.copy_((600 + 200 * torch.rand(v.shape, generator=_gen(d), device="cuda")).clamp(max=448 if cache == FP8 else 1000).to(cache))
+    v[at, :, 0] = 0.0
+    scales = [None if s is None else torch.ones_like(s) for s in scales]
+    got = kv.prefix_attention(q, k, v, table, n, prefix, scale=1.0, k_scale=scales[0], v_scale=scales[1])
+    want = _prefix_exact(q, k, v, table, n, scales, 1.0)[0]
+    assert float(want.min()) > 2.0 ** -8
+    assert float(((got.double() - want).abs() / want).max()) <= 2 * 2.0 ** -11 + 2.0 ** -13 + 2.0 ** -14
