@@ -141,7 +141,7 @@ int cq_prefix_attention(const void* q, int64_t q_batch_stride, int64_t q_head_st
                             workspace, static_cast<int>(batch), static_cast<int>(q_heads),
                             static_cast<int>(kv_heads), static_cast<int>(head_dim), static_cast<int>(num_pages),
                             static_cast<int>(page_size), static_cast<int>(table_rows), static_cast<int>(table_width),
-                            dtype, cache_dtype, 0, 0, scale, prefix, static_cast<int>(prefix_len), nullptr};
+                            dtype, cache_dtype, 0, 0, scale, prefix, static_cast<int>(prefix_len), 0, nullptr};
   return cuda_status(cq::launch_prefix_attention(a, static_cast<cudaStream_t>(stream)));
 }
 

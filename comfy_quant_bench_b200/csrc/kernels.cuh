@@ -176,10 +176,10 @@ struct PagedAttnArgs {
   void* ws;
   int B, Hq, Hkv, D, num_pages, page_size, table_rows, table_width, dtype, cache_dtype, window, sinks;
   float scale;
-  // attention behind a shared prefix: rows that hold its `prefix_len` (or *prefix) tokens see only what comes after them, and
-  // the outputs go to out32 in fp32 (out32 null: neither)
+  // attention behind a shared prefix: rows that hold its `prefix_len` (or *prefix) tokens see only what comes after them, where
+  // those are `share_from` or more, and the outputs go to out32 in fp32 (out32 null: neither)
   const int* prefix;
-  int prefix_len;
+  int prefix_len, share_from;
   float* out32;               // [B, Hq, D]
 };
 // the call's own arguments (own.out32, own.lse and own.ws point into its workspace), and how it is dealt out

@@ -124,7 +124,11 @@ __device__ __forceinline__ int swz(int r, int c) {
 struct RowView {
   int row, n, vis, nsink, units;
 };
-__device__ __forceinline__ int prefix_of(const PagedAttnArgs& a) { return a.prefix != nullptr ? __ldg(a.prefix) : a.prefix_len; }
+// the tokens that this call reads once for all rows: none where that would not pay
+__device__ __forceinline__ int prefix_of(const PagedAttnArgs& a) {
+  const int n = min(a.prefix != nullptr ? __ldg(a.prefix) : a.prefix_len, a.table_width * a.page_size);
+  return n >= a.share_from ? n : 0;
+}
 __device__ __forceinline__ RowView row_view(const PagedAttnArgs& a, int b) {
   RowView v;
   v.row = a.rows != nullptr ? __ldg(a.rows + b) : b;
@@ -138,7 +142,7 @@ __device__ __forceinline__ RowView row_view(const PagedAttnArgs& a, int b) {
     v.vis = a.window + v.nsink;
   }
   if (a.out32 != nullptr) {                             // behind a shared prefix, where the row holds it
-    const int prefix = max(0, min(prefix_of(a), a.table_width * a.page_size));
+    const int prefix = prefix_of(a);
     if (n >= prefix) v.vis = n - prefix;
   }
   v.units = (v.vis + pattn::kUnit - 1) / pattn::kUnit;

@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(pfx::Cfg<D>::kThreads, 1) prefix_attention_ker
     tmem_relinquish();
   }
   tc_fence_before();
-  const int prefix = max(0, min(prefix_of(g), g.table_width * g.page_size));
+  const int prefix = prefix_of(g);
   const int leader = prefix_leader(a, prefix, leader_at);     // and the barriers and the holder are written
   tc_fence_after();
   const uint32_t tmem = *holder;
@@ -614,7 +614,7 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const PrefixArgs a) {
   const PagedAttnArgs& g = a.own;
   const int tile = blockIdx.x, head = blockIdx.y, d4 = blockIdx.z * 2, tid = threadIdx.x;
   const int group = g.Hq / g.Hkv, rows = g.B * group, tiles = (rows + pfx::kRows - 1) / pfx::kRows;
-  const int prefix = max(0, min(prefix_of(g), g.table_width * g.page_size));
+  const int prefix = prefix_of(g);
   const int key_tiles = (prefix + kKeys - 1) / kKeys;
   const int64_t units = static_cast<int64_t>(g.Hkv) * key_tiles, padded = static_cast<int64_t>(a.members) * C::kSlots;
   const int subs = C::kSlots == 2 && tile + 1 == tiles && !(tile & 1) ? 2 : 1;
@@ -699,19 +699,19 @@ int prefix_members(int64_t rows, int D) {
 int prefix_teams(int members) { return members < num_sms() ? num_sms() / members : 1; }
 }  // namespace
 
-// Sharing pays from about 128 MB of keys and values that the rows would read one by one (by the table's width, since
-// lengths are on the device): four launches and the split of the rows' sums cost 14 to 20 us, and reading runs at 5 to 6
-// TB/s.  Us one by one and shared: 16 rows of 8 heads of 128 behind 1000 tokens (70 MB) 15 and 22, 32 rows (139 MB) 22
-// and 22, 16 rows behind 4000 (266 MB) 38 and 36, 64 rows behind 1000 (279 MB) 40 and 27; 8-bit codes of 256: 139 MB 28
-// and 26; heads of 64: 133 MB 31 and 31.
-bool prefix_pays(int64_t batch, int Hkv, int D, int64_t span, int size) {
-  return static_cast<double>(batch) * Hkv * static_cast<double>(span) * D * 2 * size > 134217728.0;
+// Sharing pays from about 128 MB of shared keys and values that the rows would read one by one: four launches and the split
+// of the rows' sums cost 14 to 20 us, and reading runs at 5 to 6 TB/s.  Us one by one and shared: 16 rows of 8 heads of 128
+// behind 1000 tokens (70 MB) 15 and 22, 32 rows (139 MB) 22 and 22, 16 rows behind 4000 (266 MB) 38 and 36, 64 rows behind
+// 1000 (279 MB) 40 and 27; 8-bit codes of 256: 139 MB 28 and 26; heads of 64: 133 MB 31 and 31.  So many tokens they are; a
+// prefix on the device that has fewer is left to the rows' own kernel, whose results are those of a call that shares nothing.
+int64_t prefix_share_from(int64_t batch, int Hkv, int D, int size) {
+  return 134217728 / (batch * Hkv * D * 2 * size) + 1;
 }
 
 // the runs' sums, the rows' own outputs and their logs, and the workspace of their kernel
 int64_t prefix_attention_workspace(int64_t batch, int Hq, int Hkv, int D, int64_t span) {
   if (batch == 0) return 0;
-  if (!prefix_pays(batch, Hkv, D, span, 2)) return paged_attention_workspace(batch, Hq, Hkv, D, span, 0, 0);
+  if (span < prefix_share_from(batch, Hkv, D, 2)) return paged_attention_workspace(batch, Hq, Hkv, D, span, 0, 0);
   const int members = prefix_members(batch * (Hq / Hkv), D);
   const int64_t parts = static_cast<int64_t>(prefix_teams(members) + Hkv) * members * (D == 256 ? 1 : 2) * pfx::part_floats(D) * 4;
   return parts + batch * Hq * (D + 4) * 4 + (paged_attention_workspace(batch, Hq, Hkv, D, span, 0, 0) + 255) / 256 * 256;
@@ -745,15 +745,13 @@ cudaError_t pick_prefix_dim(const PrefixArgs& a, cudaStream_t st) {
 
 // a.own: the whole call's arguments, its ws the whole workspace
 cudaError_t launch_prefix_attention(const PagedAttnArgs& call, cudaStream_t st) {
-  if (!prefix_pays(call.B, call.Hkv, call.D, static_cast<int64_t>(call.table_width) * call.page_size,
-                   call.cache_dtype == CQ_DT_FP8_E4M3 ? 1 : 2)) {
-    PagedAttnArgs each = call;                                // every row through its own table
-    each.prefix = nullptr;
-    each.prefix_len = 0;
-    return launch_paged_attention(each, st);
-  }
+  const int64_t span = static_cast<int64_t>(call.table_width) * call.page_size;
+  const int64_t from = prefix_share_from(call.B, call.Hkv, call.D, call.cache_dtype == CQ_DT_FP8_E4M3 ? 1 : 2);
+  if ((call.prefix != nullptr || call.prefix_len > span ? span : call.prefix_len) < from)
+    return launch_paged_attention(call, st);                  // every row through its own table
   PrefixArgs a{};
   a.own = call;
+  a.own.share_from = static_cast<int>(from);                  // at most the span
   a.members = prefix_members(static_cast<int64_t>(call.B) * (call.Hq / call.Hkv), call.D);
   a.teams = prefix_teams(a.members);
   a.lse_out = call.lse;

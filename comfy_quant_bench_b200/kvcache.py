@@ -51,9 +51,9 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     read once for all rows, not once for each.
 
     Every row with ``prefix`` tokens or more must hold the same first ``prefix`` tokens, in pages of its own table, whichever
-    they are (those of the first such row are read); a shorter row or an empty one is attended by itself.  Where the rows'
-    keys and values come to 128 MB or less by the table's width, sharing does not pay and every row is read through its
-    own table.  Arguments and results are those of ``paged_attention``.  A softmax weight enters the product with shared values as two 16-bit parts where B * q_heads
+    they are (those of the first such row are read); a shorter row or an empty one is attended by itself.  Where the shared
+    keys and values, once for each row, come to 128 MB or less, sharing does not pay and every row is read through its own
+    table, as by ``paged_attention``.  Arguments and results are those of ``paged_attention``.  A softmax weight enters the product with shared values as two 16-bit parts where B * q_heads
     / kv_heads is at most 256 (128 at D 256), else as one part, rounded to nearest."""
     return _lib.decode().prefix_attention(q, k_cache, v_cache, block_table, seq_lens, prefix, rows, scale, k_scale, v_scale,
                                           out, return_lse)

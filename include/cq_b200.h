@@ -522,7 +522,7 @@ CQ_API int cq_paged_attention(const void* q, int64_t q_batch_stride, int64_t q_h
  * values of the first P tokens are read once for all rows, through the table of the first query row that has P tokens
  * or more.  P is *prefix (int32, device memory) where that is not NULL, else prefix_len.  All rows with P tokens or more must
  * hold the same first P tokens (in pages of their own tables, whichever they are); a shorter row, or one without tokens, is
- * attended by itself.  Where the rows' keys and values are at most 128 MB by the table's width (batch * kv_heads * span *
+ * attended by itself.  Where the P tokens' keys and values, once for each row, are at most 128 MB (batch * kv_heads * P *
  * head_dim * 2 elements), sharing does not pay and every row is read through its own table.  Arguments and results as
  * cq_paged_attention; a weight enters the product with a shared v as two 16-bit parts where batch * q_heads / kv_heads is at
  * most 256 (128 at head_dim 256), else as one, rounded to nearest.

@@ -914,3 +914,172 @@ def test_prefix_keeps_a_tail_behind_one_strong_key(kv, b, hq, hk, d, prefix, cac
     want = _prefix_exact(q, k, v, table, n, scales, 1.0)[0]
     assert float(want.min()) > 2.0 ** -8
     assert float(((got.double() - want).abs() / want).max()) <= 2 * 2.0 ** -11 + 2.0 ** -13 + 2.0 ** -14
+
+
+# ----------------------------------------------------------------------------------------------------------
+# where sharing pays: more than 128 MB of shared keys and values that the rows would read one by one.  Fewer, and the results
+# are those of the rows' own kernel, bit for bit, however wide the table.
+# ----------------------------------------------------------------------------------------------------------
+
+def _rows_that_pay(hk, d, prefix, cache):
+    return (1 << 27) // (hk * prefix * d * 2 * (1 if cache == FP8 else 2)) + 1
+
+
+@pytest.mark.parametrize("cache", [torch.bfloat16, torch.float16, FP8])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("b,hq,hk,prefix", [(6, 8, 2, 333), (33, 16, 4, 60), (3, 5, 1, 1), (12, 8, 8, 0)])
+def test_prefix_short_in_a_wide_table(kv, b, hq, hk, prefix, d, cache):
+    lens = [prefix + 3 * i for i in range(b)]
+    dtype = torch.float16 if cache == FP8 else cache
+    problem = _prefix_problem(lens, prefix, hq, hk, d, 16, dtype, cache)
+    q, k, v, table, n, scales = problem
+    kw = dict(k_scale=scales[0], v_scale=scales[1], return_lse=True)
+    want, log = kv.paged_attention(q, k, v, table, n, **kw)
+    got, same = kv.prefix_attention(q, k, v, table, n, prefix, **kw)
+    assert torch.equal(got, want) and torch.equal(same, log)
+    shared = torch.tensor([prefix], dtype=torch.int32, device="cuda")
+    assert torch.equal(_prefix_holds(kv, problem, shared), want)
+    shared.fill_(-5)
+    assert torch.equal(_prefix_holds(kv, problem, shared), want)
+
+
+_COMBINED = [[(torch.bfloat16, torch.bfloat16), (torch.float16, FP8)], [(torch.float16, torch.float16), (torch.bfloat16, FP8)]]
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("case", list(enumerate([(8, 8, 1111, 60, 16), (8, 1, 5000, 33, 16), (16, 2, 700, 30, 16), (6, 3, 2049, 40, 64),
+                                            (56, 8, 640, 17, 128), (12, 12, 129, 5, 32), (64, 8, 127, 9, 16), (8, 8, 6000, 100, 16),
+                                            (2, 1, 60000, 3, 16), (64, 64, 6, 2, 8), (32, 8, 1024, 0, 16)])), ids=lambda c: str(c[1]))
+def test_prefix_where_sharing_pays(kv, case, d):
+    i, (hq, hk, prefix, longest, page) = case
+    for dtype, cache in _COMBINED[(i + d // 128) % 2]:
+        b = _rows_that_pay(hk, d, prefix, cache)
+        lens = [prefix + (longest * r) // max(1, b - 1) for r in range(b)]
+        problem = _prefix_problem(lens, prefix, hq, hk, d, page, dtype, cache, wide=False)
+        got = _prefix_holds(kv, problem, prefix)
+        q, k, v, table, n, scales = problem
+        shared = torch.tensor([prefix], dtype=torch.int32, device="cuda")
+        for again in (prefix, shared):
+            assert torch.equal(kv.prefix_attention(q, k, v, table, n, again, k_scale=scales[0], v_scale=scales[1]), got)
+        assert _status() == (0, 0)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("hq", [8, 40])
+def test_prefix_of_uneven_rows_where_sharing_pays(kv, hq, d):
+    """Rows without the prefix, rows of nothing, prefixes of nothing and beyond every row, holes in the table."""
+    b = _rows_that_pay(8, d, 300, torch.bfloat16) + 6
+    lens = [0, 400, 350, 3, 700, 349] + [350 + 7 * (i % 20) for i in range(b - 6)]
+    problem = _prefix_problem(lens, 350, hq, 8, d, 16, torch.bfloat16, torch.bfloat16, wide=False)
+    for prefix in (350, 0, 100000):
+        _prefix_holds(kv, problem, prefix)
+    lens = [360 + 7 * (i % 20) for i in range(b)]
+    problem = _prefix_problem(lens, 360, hq, 8, d, 16, torch.bfloat16, torch.bfloat16, wide=False)
+    for prefix in (360, 359, 321):                                      # any shorter prefix is shared too
+        _prefix_holds(kv, problem, prefix)
+    rows = torch.arange(b, device="cuda", dtype=torch.int32).flip(0)
+    rows[1], rows[2], rows[3] = -1, b, rows[0]                          # no row, beyond the table, the same row twice
+    _prefix_holds(kv, problem, 360, rows=rows)
+    _prefix_holds(kv, problem, 360, scale=-0.02)
+    holed = problem[3].clone()
+    holed[:, 3], holed[:, 9] = -1, len(problem[1])                      # pages that the table does not have, inside the prefix
+    _prefix_holds(kv, (*problem[:3], holed, *problem[4:]), 360)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_prefix_large_scores_where_sharing_pays(kv, d):
+    """Maxima that grow from tile to tile, infinities and NaN in sight."""
+    b = _rows_that_pay(8, d, 1500, torch.float16)
+    problem = _prefix_problem([1500 + i % 9 for i in range(b)], 1500, 16, 8, d, 16, torch.float16, torch.float16, wide=False)
+    q, k, v, table, n, scales = problem
+    for j in range(0, 1500, 16):                                        # keys grow along the prefix
+        k[int(table[0, j // 16])] *= 0.2 + 4 * j / 1500
+    src = int(table[0, 93])
+    for r in range(1, b):
+        k[int(table[r, 93]), :, :12] = k[src, :, :12]
+    want, lse, slack, share, tail = _prefix_exact(*problem[:5], scales)
+    one_part = 2 * b > (128 if d == 256 else 256)
+    got = kv.prefix_attention(q, k, v, table, n, 1500)
+    u = U[torch.float16]
+    assert float(((got.double() - want).abs() - u * want.abs() - slack * 1.01 - (u * share if one_part else 0) - tail - 2.0 ** -25).max()) <= 0
+    bad = v.clone()
+    bad[int(table[0, 5]), 0, 3, 7] = float("inf")
+    bad[int(table[0, 6]), 1, 4, 9] = float("nan")
+    off = ~torch.isfinite(kv.prefix_attention(q, k, bad, table, n, 1500))
+    assert bool(off[:, :2, 7].all()) and bool(off[:, 2:4, 9].all()) and int(off.sum()) == b * 4
+    worse = k.clone()
+    worse[int(table[0, 5]), 0, 3] = float("nan")
+    got = kv.prefix_attention(q, worse, v, table, n, 1500)
+    assert bool(got[:, :2].isnan().all()) and bool(torch.isfinite(got[:, 2:]).all())
+
+
+def test_prefix_strides_streams_and_graphs_where_sharing_pays(kv):
+    b = _rows_that_pay(8, 64, 950, torch.bfloat16)
+    problem = _prefix_problem([1000 + i % 30 for i in range(b)], 1000, 16, 8, 64, 16, torch.bfloat16, torch.bfloat16, wide=False)
+    q, k, v, table, n, _ = problem
+    want = _prefix_holds(kv, problem, 1000)
+    wide = torch.zeros(b, 19, 64, device="cuda", dtype=q.dtype)
+    wide[:, 1:17] = q
+    out = torch.full_like(q, 7.0)
+    assert kv.prefix_attention(wide[:, 1:17], k, v, table, n, 1000, out=out) is out and torch.equal(out, want)
+    head_last, value_last = (c.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3) for c in (k, v))
+    assert torch.equal(kv.prefix_attention(q, head_last, value_last, table, n, 1000), want)
+    shared = torch.tensor([1000], dtype=torch.int32, device="cuda")
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = kv.prefix_attention(q, k, v, table, n, shared)
+        graphs.append((graph, held))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        graphs[0][0].replay()
+        with torch.cuda.stream(side):
+            graphs[1][0].replay()
+            mine = kv.prefix_attention(q, k, v, table, n, 1000)
+    torch.cuda.synchronize()
+    assert torch.equal(graphs[0][1], want) and torch.equal(graphs[1][1], want) and torch.equal(mine, want)
+    for prefix in (960, 20, 0, 1000):                                   # a captured step reads the prefix anew, and what pays
+        shared.fill_(prefix)
+        graphs[0][0].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(graphs[0][1], kv.prefix_attention(q, k, v, table, n, prefix))
+    assert _status() == (0, 0)
+
+
+def test_prefix_offsets_past_32_bits_where_sharing_pays(kv):
+    pages, page, hk, d = 140_000, 16, 8, 128                            # 4.6 GB each
+    k = torch.zeros(pages, hk, page, d, dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros_like(k)
+    b = _rows_that_pay(hk, d, 320, torch.bfloat16)
+    ids = torch.tensor([pages - 1 - 5 * i for i in range(20 + 4 * b)], dtype=torch.int32)
+    g = _gen(11)
+    for c in (k, v):
+        c[ids.long().cuda()] = torch.randn(len(ids), hk, page, d, generator=g, device="cuda").bfloat16()
+    table = torch.cat([ids[:20].expand(b, 20), ids[20:].view(b, 4)], dim=1).cuda()
+    lens = torch.tensor([320 + i % 65 for i in range(b)], dtype=torch.int32, device="cuda")
+    q = torch.randn(b, 16, d, generator=g, device="cuda").bfloat16()
+    _prefix_holds(kv, (q, k, v, table, lens, [None, None]), 320)
+
+
+def test_steps_behind_a_shared_prompt_where_sharing_pays(kv):
+    """40 rows forked from a prompt of 500 tokens, eight heads of 256: its tokens are attended once for all rows."""
+    g = _gen(6)
+    prompt, tokens = torch.randint(0, 500, (500,), generator=g, device="cuda"), torch.randint(0, 500, (4, 40), generator=g, device="cuda")
+    models = [_model(heads=8, kv_heads=8, head_dim=256, rows=41, pages=200, max_tokens=520) for _ in range(3)]
+    rows = torch.arange(1, 41, dtype=torch.int32, device="cuda")
+    for m in models:
+        m.prompt(prompt, 0)
+        m.cache.branch(torch.zeros_like(rows), rows, 0)
+    shared = torch.tensor([500], dtype=torch.int32, device="cuda")
+    fill, graph, held = models[2].capture(rows, shared)
+    for i in range(4):
+        alone, together = models[0].step(tokens[i], rows), models[1].step(tokens[i], rows, None, 500)
+        assert float((alone.float() - together.float()).norm() / alone.float().norm()) <= 4.6e-2
+        fill.copy_(tokens[i])
+        graph.replay()
+        assert torch.equal(held, together)
+    for m in models:
+        m.cache.check()
+    assert _status() == (0, 0)
