@@ -122,6 +122,9 @@ SIGNATURES = {
     "cq_prefix_attention": (_int, [_vp, _i64, _i64, _int, _i64, _i64, _i64, _i64, _vp, _vp, _int, _i64, _i64, _i64, _i64,
                                    _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _f32, _vp, _vp, _vp, _vp, _vp, _i64,
                                    _vp]),
+    "cq_prefix_attention_parts": (_int, [_vp, _i64, _i64, _int, _i64, _i64, _i64, _i64, _vp, _vp, _int, _i64, _i64, _i64,
+                                         _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _int, _f32, _vp, _vp, _vp,
+                                         _vp, _vp, _i64, _vp]),
     "cq_kv_append": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _int, _i64, _i64, _i64, _i64, _vp, _vp, _int,
                             _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
     "cq_kv_append_rotated": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _int, _i64, _i64, _i64, _i64, _vp,

@@ -111,14 +111,15 @@ int64_t cq_prefix_attention_workspace_bytes(int64_t batch, int64_t q_heads, int6
                                         span);
 }
 
-int cq_prefix_attention(const void* q, int64_t q_batch_stride, int64_t q_head_stride, int dtype, int64_t batch,
-                        int64_t q_heads, int64_t kv_heads, int64_t head_dim, const void* k_cache, const void* v_cache,
-                        int cache_dtype, int64_t num_pages, int64_t page_size, int64_t page_stride, int64_t head_stride,
-                        int64_t token_stride, const int32_t* block_table, int64_t table_rows, int64_t table_width,
-                        int64_t table_stride, const int32_t* rows, const int32_t* seq_lens, const int32_t* prefix,
-                        int64_t prefix_len, float scale, const float* k_scale, const float* v_scale, void* out, float* lse,
-                        void* workspace, int64_t workspace_bytes, void* stream) {
+int cq_prefix_attention_parts(const void* q, int64_t q_batch_stride, int64_t q_head_stride, int dtype, int64_t batch,
+                              int64_t q_heads, int64_t kv_heads, int64_t head_dim, const void* k_cache, const void* v_cache,
+                              int cache_dtype, int64_t num_pages, int64_t page_size, int64_t page_stride, int64_t head_stride,
+                              int64_t token_stride, const int32_t* block_table, int64_t table_rows, int64_t table_width,
+                              int64_t table_stride, const int32_t* rows, const int32_t* seq_lens, const int32_t* prefix,
+                              int64_t prefix_len, int weight_parts, float scale, const float* k_scale, const float* v_scale,
+                              void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
   if (!valid16(dtype) || (cache_dtype != dtype && cache_dtype != CQ_DT_FP8_E4M3)) return CQ_ERR_ARG;
+  if (weight_parts < 0 || weight_parts > 2) return CQ_ERR_ARG;
   if (int rc = check_tables(table_rows, table_width, table_stride, num_pages, page_size)) return rc;
   if (!fits_int(batch) || batch > 65535 || q_heads < 1 || kv_heads < 1 || q_heads > 4096 || q_heads % kv_heads != 0 ||
       !valid_head_dim(head_dim) || kv_heads > 65535 || !fits_int(prefix_len))
@@ -142,7 +143,20 @@ int cq_prefix_attention(const void* q, int64_t q_batch_stride, int64_t q_head_st
                             static_cast<int>(kv_heads), static_cast<int>(head_dim), static_cast<int>(num_pages),
                             static_cast<int>(page_size), static_cast<int>(table_rows), static_cast<int>(table_width),
                             dtype, cache_dtype, 0, 0, scale, prefix, static_cast<int>(prefix_len), 0, nullptr};
-  return cuda_status(cq::launch_prefix_attention(a, static_cast<cudaStream_t>(stream)));
+  return cuda_status(cq::launch_prefix_attention(a, weight_parts, static_cast<cudaStream_t>(stream)));
+}
+
+int cq_prefix_attention(const void* q, int64_t q_batch_stride, int64_t q_head_stride, int dtype, int64_t batch,
+                        int64_t q_heads, int64_t kv_heads, int64_t head_dim, const void* k_cache, const void* v_cache,
+                        int cache_dtype, int64_t num_pages, int64_t page_size, int64_t page_stride, int64_t head_stride,
+                        int64_t token_stride, const int32_t* block_table, int64_t table_rows, int64_t table_width,
+                        int64_t table_stride, const int32_t* rows, const int32_t* seq_lens, const int32_t* prefix,
+                        int64_t prefix_len, float scale, const float* k_scale, const float* v_scale, void* out, float* lse,
+                        void* workspace, int64_t workspace_bytes, void* stream) {
+  return cq_prefix_attention_parts(q, q_batch_stride, q_head_stride, dtype, batch, q_heads, kv_heads, head_dim, k_cache, v_cache,
+                                   cache_dtype, num_pages, page_size, page_stride, head_stride, token_stride, block_table,
+                                   table_rows, table_width, table_stride, rows, seq_lens, prefix, prefix_len, 0, scale, k_scale,
+                                   v_scale, out, lse, workspace, workspace_bytes, stream);
 }
 
 int64_t cq_pages_workspace_bytes(int64_t num_pages, int64_t reserved_rows) {

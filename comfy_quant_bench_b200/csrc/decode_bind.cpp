@@ -276,8 +276,8 @@ int64_t row_stride(const Tensor& table) { return table.size(0) > 1 ? table.strid
 using Prefix = std::variant<Tensor, int64_t>;   // tokens that all rows share
 
 py::object attention(const Tensor& q_arg, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table_arg,
-                     const Tensor& lens, const Prefix* shared, const Opt& rows, std::optional<double> scale, int64_t window,
-                     int64_t sinks, const Opt& k_scale, const Opt& v_scale, const Opt& out_arg, bool return_lse) {
+                     const Tensor& lens, const Prefix* shared, int64_t weight_parts, const Opt& rows, std::optional<double> scale,
+                     int64_t window, int64_t sinks, const Opt& k_scale, const Opt& v_scale, const Opt& out_arg, bool return_lse) {
   const at::ScalarType dt = q_arg.scalar_type(), ct = k_cache.scalar_type();
   if (q_arg.dim() != 3 || !half_type(dt)) refuse("q must be bf16 or f16 [B, q_heads, D]");
   const int64_t b = q_arg.size(0), hq = q_arg.size(1), d = q_arg.size(2);
@@ -333,12 +333,13 @@ py::object attention(const Tensor& q_arg, const Tensor& k_cache, const Tensor& v
     const int64_t bytes = cq_prefix_attention_workspace_bytes(b, hq, hk, d, width * page);
     if (bytes > 0) ws = bytes_like(q, bytes);
     check_status("cq_prefix_attention",
-                 cq_prefix_attention(q.data_ptr(), q.stride(0), q.stride(1), dtype_code(dt), b, hq, hk, d, k_cache.data_ptr(),
-                                     v_cache.data_ptr(), dtype_code(ct), pages, page, k_cache.stride(0), k_cache.stride(1),
-                                     k_cache.stride(2), static_cast<const int32_t*>(table.data_ptr()), table_rows, width,
-                                     row_stride(table), ptr<const int32_t>(rows), static_cast<const int32_t*>(lens.data_ptr()),
-                                     ptr<const int32_t>(prefix), prefix_len, factor, ks, vs, out.data_ptr(), ptr<float>(lse),
-                                     ptr(ws), bytes, stream_of(index)));
+                 cq_prefix_attention_parts(q.data_ptr(), q.stride(0), q.stride(1), dtype_code(dt), b, hq, hk, d, k_cache.data_ptr(),
+                                           v_cache.data_ptr(), dtype_code(ct), pages, page, k_cache.stride(0),
+                                           k_cache.stride(1), k_cache.stride(2), static_cast<const int32_t*>(table.data_ptr()),
+                                           table_rows, width, row_stride(table), ptr<const int32_t>(rows),
+                                           static_cast<const int32_t*>(lens.data_ptr()), ptr<const int32_t>(prefix),
+                                           prefix_len, static_cast<int>(weight_parts), factor, ks, vs, out.data_ptr(),
+                                           ptr<float>(lse), ptr(ws), bytes, stream_of(index)));
     if (return_lse) return py::make_tuple(out, *lse);
     return py::cast(out);
   }
@@ -357,12 +358,14 @@ py::object attention(const Tensor& q_arg, const Tensor& k_cache, const Tensor& v
 py::object paged_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table, const Tensor& lens,
                            const Opt& rows, std::optional<double> scale, int64_t window, int64_t sinks, const Opt& k_scale,
                            const Opt& v_scale, const Opt& out, bool return_lse) {
-  return attention(q, k_cache, v_cache, table, lens, nullptr, rows, scale, window, sinks, k_scale, v_scale, out, return_lse);
+  return attention(q, k_cache, v_cache, table, lens, nullptr, 0, rows, scale, window, sinks, k_scale, v_scale, out, return_lse);
 }
 py::object prefix_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table,
                             const Tensor& lens, const Prefix& prefix, const Opt& rows, std::optional<double> scale,
-                            const Opt& k_scale, const Opt& v_scale, const Opt& out, bool return_lse) {
-  return attention(q, k_cache, v_cache, table, lens, &prefix, rows, scale, 0, 0, k_scale, v_scale, out, return_lse);
+                            const Opt& k_scale, const Opt& v_scale, const Opt& out, bool return_lse,
+                            std::optional<int64_t> weight_parts) {
+  if (weight_parts && *weight_parts != 1 && *weight_parts != 2) refuse("weight_parts must be None, 1 or 2, got ", *weight_parts);
+  return attention(q, k_cache, v_cache, table, lens, &prefix, weight_parts.value_or(0), rows, scale, 0, 0, k_scale, v_scale, out, return_lse);
 }
 
 // x, or a contiguous copy where its rows are not 16-byte aligned

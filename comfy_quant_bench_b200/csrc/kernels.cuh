@@ -191,7 +191,8 @@ struct PrefixArgs {
 };
 // span: keys a table row can hold
 int64_t prefix_attention_workspace(int64_t batch, int Hq, int Hkv, int D, int64_t span);
-cudaError_t launch_prefix_attention(const PagedAttnArgs& a, cudaStream_t st);
+// weight_parts: 16-bit parts of a weight, 1 or 2, or 0: by the rows
+cudaError_t launch_prefix_attention(const PagedAttnArgs& a, int weight_parts, cudaStream_t st);
 // span: keys a table row can hold; 0 bytes where no row is split
 int64_t paged_attention_workspace(int64_t batch, int Hq, int Hkv, int D, int64_t span, int64_t window, int64_t sinks);
 cudaError_t launch_paged_attention(const PagedAttnArgs& a, cudaStream_t st);

@@ -14,9 +14,11 @@
 // that covers; the team's CTAs read the same keys at the same time, from L2.  Every run leaves its sums (fp32) in the
 // workspace, the row's own tokens go through the kernel of paged_attention.cu, and a last kernel joins them in a fixed order.
 //
-// Weights enter P V in 16 bits: one part of the type, which errs about as much as rounding the output does (relative L2 error
-// of 256 rows behind 30011 tokens: 2.3e-3, where rounding the exact result costs 1.7e-3), or two parts, which adds half to the
-// products, where the batch has no more rows than one CTA takes (64 rows behind 16003 tokens: 52 us with the join, 46 with one).
+// Weights enter P V in 16 bits: in two parts of the type, as in paged_attention.cu, or in one, which errs about as much as
+// rounding the output does.  256 rows of 64 heads behind 30011 tokens: 358 us a call with one part and a relative L2 error of
+// 2.3e-3, 433 us with two and 1.7e-3, what rounding the exact result costs; two parts add half to the products.  The caller
+// chooses; without a choice two where the batch has no more rows than one CTA takes (64 rows behind 16003 tokens: 52 us with
+// the join, 46 with one part), else one.
 //
 // Measured on a B200 (device time of the prefix's kernel): 256 rows of 64 heads on 8 of 128 behind 30011 tokens: 284 us, 890
 // TFLOP/s.  Bound by the chain from scores to weights to product to scores: with 128 x 128 tiles a slot's maximum, exponentials
@@ -731,20 +733,21 @@ cudaError_t run_prefix(const PrefixArgs& a, cudaStream_t st) {
   return launch_early(prefix_join_kernel<F16, D>, dim3(tiles, a.own.Hkv, D / 8), 128, 0, st, a);
 }
 template <bool F16, bool FP8, int D>
-cudaError_t pick_prefix(const PrefixArgs& a, cudaStream_t st) {
-  return a.members == 1 ? run_prefix<F16, FP8, D, 2>(a, st) : run_prefix<F16, FP8, D, 1>(a, st);
+cudaError_t pick_prefix(const PrefixArgs& a, int weight_parts, cudaStream_t st) {
+  const bool two = weight_parts == 0 ? a.members == 1 : weight_parts == 2;
+  return two ? run_prefix<F16, FP8, D, 2>(a, st) : run_prefix<F16, FP8, D, 1>(a, st);
 }
 template <bool F16, bool FP8>
-cudaError_t pick_prefix_dim(const PrefixArgs& a, cudaStream_t st) {
+cudaError_t pick_prefix_dim(const PrefixArgs& a, int weight_parts, cudaStream_t st) {
   switch (a.own.D) {
-    case 64: return pick_prefix<F16, FP8, 64>(a, st);
-    case 128: return pick_prefix<F16, FP8, 128>(a, st);
-    default: return pick_prefix<F16, FP8, 256>(a, st);
+    case 64: return pick_prefix<F16, FP8, 64>(a, weight_parts, st);
+    case 128: return pick_prefix<F16, FP8, 128>(a, weight_parts, st);
+    default: return pick_prefix<F16, FP8, 256>(a, weight_parts, st);
   }
 }
 
 // a.own: the whole call's arguments, its ws the whole workspace
-cudaError_t launch_prefix_attention(const PagedAttnArgs& call, cudaStream_t st) {
+cudaError_t launch_prefix_attention(const PagedAttnArgs& call, int weight_parts, cudaStream_t st) {
   const int64_t span = static_cast<int64_t>(call.table_width) * call.page_size;
   const int64_t from = prefix_share_from(call.B, call.Hkv, call.D, call.cache_dtype == CQ_DT_FP8_E4M3 ? 1 : 2);
   if ((call.prefix != nullptr || call.prefix_len > span ? span : call.prefix_len) < from)
@@ -762,8 +765,9 @@ cudaError_t launch_prefix_attention(const PagedAttnArgs& call, cudaStream_t st) 
   a.own.lse = next + heads * call.D;
   a.own.ws = next + heads * (call.D + 4);
   const bool fp8 = call.cache_dtype == CQ_DT_FP8_E4M3;
-  if (call.dtype == CQ_DT_F16) return fp8 ? pick_prefix_dim<true, true>(a, st) : pick_prefix_dim<true, false>(a, st);
-  return fp8 ? pick_prefix_dim<false, true>(a, st) : pick_prefix_dim<false, false>(a, st);
+  if (call.dtype == CQ_DT_F16)
+    return fp8 ? pick_prefix_dim<true, true>(a, weight_parts, st) : pick_prefix_dim<true, false>(a, weight_parts, st);
+  return fp8 ? pick_prefix_dim<false, true>(a, weight_parts, st) : pick_prefix_dim<false, false>(a, weight_parts, st);
 }
 
 }  // namespace cq

@@ -45,7 +45,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                      seq_lens: torch.Tensor, prefix: int | torch.Tensor, *, rows: torch.Tensor | None = None,
                      scale: float | None = None, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
-                     out: torch.Tensor | None = None, return_lse: bool = False):
+                     out: torch.Tensor | None = None, return_lse: bool = False, weight_parts: int | None = None):
     """``paged_attention`` of a batch whose rows begin with the same ``prefix`` tokens (an int, or one int32 on the device,
     which a captured step reads anew): samples of one prompt, requests behind one instruction.  Their keys and values are
     read once for all rows, not once for each.
@@ -53,10 +53,13 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     Every row with ``prefix`` tokens or more must hold the same first ``prefix`` tokens, in pages of its own table, whichever
     they are (those of the first such row are read); a shorter row or an empty one is attended by itself.  Where the shared
     keys and values, once for each row, come to 128 MB or less, sharing does not pay and every row is read through its own
-    table, as by ``paged_attention``.  Arguments and results are those of ``paged_attention``.  A softmax weight enters the product with shared values as two 16-bit parts where B * q_heads
-    / kv_heads is at most 256 (128 at D 256), else as one part, rounded to nearest."""
+    table, as by ``paged_attention``.  Other arguments and results are those of ``paged_attention``.
+
+    ``weight_parts``: the 16-bit parts in which a softmax weight enters the product with shared values.  2 is as
+    ``paged_attention`` has it; 1 is faster for large batches and errs about as much as rounding the result does.  None: 2
+    where B * q_heads / kv_heads is at most 256 (128 at D 256), else 1."""
     return _lib.decode().prefix_attention(q, k_cache, v_cache, block_table, seq_lens, prefix, rows, scale, k_scale, v_scale,
-                                          out, return_lse)
+                                          out, return_lse, weight_parts)
 
 
 def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,

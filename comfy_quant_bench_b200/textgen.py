@@ -141,7 +141,7 @@ class TextModel:
         def attention(layer, b, q, k, v):
             if prefix is None or b.window:
                 return self.cache.attend(layer, q, rows, window=b.window, sinks=b.sinks)
-            return self.cache.attend_prefix(layer, q, prefix, rows)
+            return self.cache.attend_prefix(layer, q, prefix, rows, weight_parts=2)      # as exact as ``attend``
 
         return self._forward(tokens, rows, positions, attention)
 

@@ -525,8 +525,10 @@ CQ_API int cq_paged_attention(const void* q, int64_t q_batch_stride, int64_t q_h
  * attended by itself.  Where the P tokens' keys and values, once for each row, are at most 128 MB (batch * kv_heads * P *
  * head_dim * 2 elements), sharing does not pay and every row is read through its own table.  Arguments and results as
  * cq_paged_attention; a weight enters the product with a shared v as two 16-bit parts where batch * q_heads / kv_heads is at
- * most 256 (128 at head_dim 256), else as one, rounded to nearest.
- *   workspace (0 bytes where no row is split) of cq_prefix_attention_workspace_bytes (span = table_width * page_size), 256-byte aligned, of this call alone
+ * most 256 (128 at head_dim 256), else as one, rounded to nearest (cq_prefix_attention_parts: as `weight_parts`, 1 or 2, says
+ * for every batch; 0: as cq_prefix_attention).
+ *   workspace (0 bytes where no row is split) of cq_prefix_attention_workspace_bytes (span = table_width * page_size),
+ *             256-byte aligned, of this call alone
  */
 CQ_API int64_t cq_prefix_attention_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                                                    int64_t span);
@@ -538,6 +540,15 @@ CQ_API int cq_prefix_attention(const void* q, int64_t q_batch_stride, int64_t q_
                                const int32_t* seq_lens, const int32_t* prefix, int64_t prefix_len, float scale,
                                const float* k_scale, const float* v_scale, void* out, float* lse, void* workspace,
                                int64_t workspace_bytes, void* stream);
+CQ_API int cq_prefix_attention_parts(const void* q, int64_t q_batch_stride, int64_t q_head_stride, int dtype, int64_t batch,
+                                     int64_t q_heads, int64_t kv_heads, int64_t head_dim, const void* k_cache,
+                                     const void* v_cache, int cache_dtype, int64_t num_pages, int64_t page_size,
+                                     int64_t page_stride, int64_t head_stride, int64_t token_stride, const int32_t* block_table,
+                                     int64_t table_rows, int64_t table_width, int64_t table_stride, const int32_t* rows,
+                                     const int32_t* seq_lens, const int32_t* prefix, int64_t prefix_len,
+                                     int weight_parts, float scale,
+                                     const float* k_scale, const float* v_scale, void* out, float* lse, void* workspace,
+                                     int64_t workspace_bytes, void* stream);
 
 /*
  * cq_kv_append: the new keys and values of `tokens` tokens into the pages of their rows: token t goes to position

@@ -1083,3 +1083,44 @@ def test_steps_behind_a_shared_prompt_where_sharing_pays(kv):
     for m in models:
         m.cache.check()
     assert _status() == (0, 0)
+
+
+@pytest.mark.parametrize("dtype,cache", [(torch.bfloat16, torch.bfloat16), (torch.float16, FP8)])
+@pytest.mark.parametrize("b,hq,hk,d,prefix", [(300, 32, 8, 64, 600), (130, 8, 4, 256, 700), (100, 64, 8, 128, 1000), (20, 8, 8, 128, 2000)])
+def test_prefix_weights_in_one_part_or_two(kv, b, hq, hk, d, prefix, dtype, cache):
+    """Two parts: the bound of paged attention, whatever the batch; one: u of the weights besides."""
+    problem = _prefix_problem([prefix + i % 7 for i in range(b)], prefix, hq, hk, d, 16, dtype, cache, wide=False)
+    q, k, v, table, n, scales = problem
+    want, _, slack, share, tail = _prefix_exact(q, k, v, table, n, scales)
+    u = U[dtype]
+    once = float((want.to(dtype).double() - want).norm() / want.norm())
+    got = {}
+    for parts in (1, 2, None):
+        got[parts] = kv.prefix_attention(q, k, v, table, n, prefix, k_scale=scales[0], v_scale=scales[1], weight_parts=parts)
+        one = parts == 1 or (parts is None and b * (hq // hk) > (128 if d == 256 else 256))
+        off = (got[parts].double() - want).abs()
+        assert float((off - u * want.abs() - slack * (1 + u) - (u * share if one else 0) - tail - 2.0 ** -25).max()) <= 0
+        assert float(off.norm() / want.norm()) <= (1.5 if one else 1.05) * once + 2.0 ** -14
+    assert torch.equal(got[1], got[2]) == (b < _rows_that_pay(hk, d, prefix, cache))    # 20 rows in 8 bits: 82 MB, read row by row
+    assert torch.equal(got[None], got[1 if b * (hq // hk) > (128 if d == 256 else 256) else 2])
+
+
+def test_a_step_behind_a_shared_prompt_is_as_exact_as_alone(kv, monkeypatch):
+    """The model's attention behind a prompt holds the bound of attention row by row: weights in two parts."""
+    held = []
+    whole = kv.prefix_attention
+
+    def recorded(q, k, v, table, lens, prefix, rows=None, **kw):
+        out = whole(q, k, v, table, lens, prefix, rows=rows, **kw)
+        held.append((q.clone(), out.clone(), kv.paged_attention(q, k, v, table, lens, rows=rows)))
+        return out
+    monkeypatch.setattr(kv, "prefix_attention", recorded)
+    m = _model(heads=32, kv_heads=4, head_dim=128, rows=41, pages=400, max_tokens=2010)
+    m.prompt(torch.randint(0, 500, (2000,), generator=_gen(8), device="cuda"), 0)
+    rows = torch.arange(1, 41, dtype=torch.int32, device="cuda")
+    m.cache.branch(torch.zeros_like(rows), rows, 0)
+    m.step(torch.arange(40, device="cuda"), rows, None, 2000)
+    assert len(held) == 2
+    # each holds 2^-14: two results 2^-13 apart round to neighbours, 2^-7 apart, in 2^-6 of the cases: 2^-10 in the square mean
+    for q, got, want in held:
+        assert float((got.double() - want.double()).norm() / want.double().norm()) <= 2.0 ** -10

@@ -198,3 +198,20 @@ def test_sampling_waits_for_its_cluster_before_it_writes_to_it():
     assert before.count("cluster_arrive()") == 1 and before.count("cluster_wait()") == 1
     assert before.index("cluster_arrive()") < before.index("grid_dep_wait()") < before.index("cluster_wait()")
     assert "return;" not in before and "cluster_sync_all()" not in before
+
+
+def test_weight_parts_are_checked(lib):
+    from comfy_quant_bench_b200 import _lib as L
+    from comfy_quant_bench_b200 import kvcache
+
+    def call(parts, dt=0, ws=VP):
+        return lib.cq_prefix_attention_parts(VP, 4096, 128, dt, 64, 32, 8, 128, VP, VP, 0, 10, 16, 16384, 2048, 128, VP, 64, 1000,
+                                             1000, None, VP, VP, 0, parts, 1.0, None, None, VP, None, ws, 1 << 40, None)
+    assert call(3) == L.CQ_ERR_ARG and call(-1) == L.CQ_ERR_ARG and call(2, dt=2) == L.CQ_ERR_ARG and call(1, ws=None) == L.CQ_ERR_ARG
+    k, n = torch.zeros(6, 2, 16, 64, dtype=BF), torch.zeros(2, dtype=torch.int32)
+    t, q = torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, 4, 64, dtype=BF)
+    for parts in (0, 3, -1):
+        with pytest.raises(ValueError, match="weight_parts must be None, 1 or 2, got"):
+            kvcache.prefix_attention(q, k, k, t, n, 5, weight_parts=parts)
+    with pytest.raises(ValueError, match="CUDA"):
+        kvcache.prefix_attention(q, k, k, t, n, 5, weight_parts=2)
