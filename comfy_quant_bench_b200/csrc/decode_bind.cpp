@@ -201,6 +201,7 @@ Opt row_param(const Each& p, int64_t n, at::ScalarType type, const char* name, d
   }
   one = std::get<double>(p);
   if (!(one >= least && one <= most)) refuse(name, " is out of range: ", std::to_string(one));
+  if (type == at::kInt && one != std::floor(one)) refuse(name, " must be a whole number, got ", std::to_string(one));
   return std::nullopt;
 }
 

@@ -215,3 +215,14 @@ def test_weight_parts_are_checked(lib):
             kvcache.prefix_attention(q, k, k, t, n, 5, weight_parts=parts)
     with pytest.raises(ValueError, match="CUDA"):
         kvcache.prefix_attention(q, k, k, t, n, 5, weight_parts=2)
+
+
+def test_a_fraction_of_a_token_is_refused():
+    from comfy_quant_bench_b200 import ops
+    x, u = torch.zeros(3, 50), torch.zeros(3)
+    for k in (0.5, 2.5, 49.999):
+        with pytest.raises(ValueError, match="top_k must be a whole number, got"):
+            ops.sample_tokens(x, u, top_k=k)
+    for k in (3, 3.0, True):
+        with pytest.raises(ValueError, match="CUDA"):
+            ops.sample_tokens(x, u, top_k=k)
