@@ -164,6 +164,8 @@ class TextModel:
         """``samples`` continuations of ``steps`` tokens of one prompt: [samples, steps].  ``uniform`` [steps, samples] in
         [0, 1) chooses the tokens (``ops.sample_tokens``, with its temperature, top_k, top_p and min_p); without it each is
         the likeliest."""
+        if uniform is None and sampling:
+            raise ValueError(f"{', '.join(sampling)} without uniform numbers: the likeliest tokens are not sampled")
         if samples + 1 > self.cfg.rows:
             raise ValueError(f"{samples} samples and the prompt need {samples + 1} cache rows, there are {self.cfg.rows}")
         rows = torch.arange(1, samples + 1, dtype=torch.int32, device=self.device)

@@ -226,3 +226,11 @@ def test_a_fraction_of_a_token_is_refused():
     for k in (3, 3.0, True):
         with pytest.raises(ValueError, match="CUDA"):
             ops.sample_tokens(x, u, top_k=k)
+
+
+def test_sampling_arguments_without_numbers_to_sample_by_are_refused():
+    from comfy_quant_bench_b200 import textgen
+    model = object.__new__(textgen.TextModel)                            # refused before anything is looked at
+    for kw in (dict(temperature=0.7), dict(top_k=5, top_p=0.9), dict(temprature=0.7)):
+        with pytest.raises(ValueError, match=f"{next(iter(kw))}.* without uniform numbers"):
+            model.generate(torch.zeros(3, dtype=torch.long), 2, 4, **kw)
