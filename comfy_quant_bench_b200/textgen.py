@@ -159,10 +159,18 @@ class TextModel:
             logits = self.step(tokens, rows, None, prefix)
         return tokens, graph, logits
 
+    def _choose(self, logits: torch.Tensor, uniform: torch.Tensor, sampling: dict) -> torch.Tensor:
+        """The next tokens of logits [rows, vocab] by a number for each row, or one for all."""
+        uniform = uniform.reshape(-1).float().expand(len(logits))
+        if self.cfg.vocab <= 327680 or sampling:
+            return ops.sample_tokens(logits, uniform, **sampling)
+        total = logits.float().softmax(-1).cumsum(-1)            # more tokens than ``sample_tokens`` takes
+        return torch.searchsorted(total, uniform.view(-1, 1) * total[:, -1:]).squeeze(1).clamp(max=self.cfg.vocab - 1)
+
     def generate(self, prompt: torch.Tensor, samples: int, steps: int, uniform: torch.Tensor | None = None,
                  **sampling) -> torch.Tensor:
-        """``samples`` continuations of ``steps`` tokens of one prompt: [samples, steps].  ``uniform`` [steps, samples] in
-        [0, 1) chooses the tokens (``ops.sample_tokens``, with its temperature, top_k, top_p and min_p); without it each is
+        """``samples`` continuations of ``steps`` tokens of one prompt: [samples, steps].  ``uniform`` [steps, samples] (or one
+        number a step) in [0, 1) chooses the tokens (``ops.sample_tokens``, with its temperature, top_k, top_p and min_p); without it each is
         the likeliest."""
         if uniform is None and sampling:
             raise ValueError(f"{', '.join(sampling)} without uniform numbers: the likeliest tokens are not sampled")
@@ -175,7 +183,7 @@ class TextModel:
         positions = self.cache.branch(torch.zeros_like(rows), rows, 1)
         out = []
         for i in range(steps):
-            out.append(logits.argmax(-1) if uniform is None else ops.sample_tokens(logits, uniform[i], **sampling))
+            out.append(logits.argmax(-1) if uniform is None else self._choose(logits, uniform[i], sampling))
             if i + 1 < steps:
                 logits = self.step(out[-1], rows, positions, len(prompt))
                 positions = None

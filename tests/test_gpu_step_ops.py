@@ -1124,3 +1124,28 @@ def test_a_step_behind_a_shared_prompt_is_as_exact_as_alone(kv, monkeypatch):
     # each holds 2^-14: two results 2^-13 apart round to neighbours, 2^-7 apart, in 2^-6 of the cases: 2^-10 in the square mean
     for q, got, want in held:
         assert float((got.double() - want.double()).norm() / want.double().norm()) <= 2.0 ** -10
+
+
+def test_generate_takes_numbers_of_any_type_and_one_for_all_rows(ops):
+    m = _model()
+    prompt, u = torch.arange(33, device="cuda"), torch.randint(0, 128, (6, 3), generator=_gen(2), device="cuda") / 128
+    want = m.generate(prompt, 3, 6, u)
+    for same in (u.bfloat16(), u.half(), u.double(), u.unsqueeze(-1)):   # exact in all of them
+        assert torch.equal(m.generate(prompt, 3, 6, same), want)
+    one = m.generate(prompt, 3, 6, u[:, :1].expand(6, 3))
+    assert torch.equal(m.generate(prompt, 3, 6, u[:, :1]), one) and torch.equal(m.generate(prompt, 3, 6, u[:, 0]), one)
+    assert torch.equal(m.generate(prompt, 3, 6, torch.zeros(6, 3, dtype=torch.long, device="cuda")), m.generate(prompt, 3, 6, 0 * u))
+
+
+def test_generate_with_more_tokens_than_the_sampler_takes(ops):
+    m = _model(vocab=327744)
+    u = torch.rand(3, 2, generator=_gen(3), device="cuda")
+    got = m.generate(torch.arange(20, device="cuda"), 2, 3, u)
+    assert got.shape == (2, 3) and int(got.min()) >= 0 and int(got.max()) < 327744
+    logits = m.prompt(torch.arange(20, device="cuda"), 5)[-1].double().softmax(-1).cumsum(0)
+    for r in range(2):                                                   # a cumulative sum in f32: off by 2^-24 a token at most
+        at = int(got[r, 0])
+        off = 327744 * 2.0 ** -24
+        assert float(logits[at - 1] if at else 0.0) <= float(u[0, r]) + off and float(logits[at]) >= float(u[0, r]) - off
+    with pytest.raises(ValueError, match="327680"):
+        m.generate(torch.arange(20, device="cuda"), 2, 3, u, top_k=5)
