@@ -74,7 +74,8 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
 
 
 def rope_table(positions: int, rot_dim: int, *, base: float = 10000.0, scaling: str | None = None, factor: float = 1.0,
-               original: int = 0, fast: float = 32.0, slow: float = 1.0, device="cuda") -> torch.Tensor:
+               original: int = 0, fast: float = 32.0, slow: float = 1.0, blend: str = "turns", size: float | None = None,
+               device="cuda") -> torch.Tensor:
     """Angles of rotary positions: f32 [positions, rot_dim / 2, 2] = (cos, sin) of p * base ** (-2i / rot_dim), computed in
     64 bits.  ``scaling`` stretches a model's context by ``factor``:
 
@@ -82,8 +83,11 @@ def rope_table(positions: int, rot_dim: int, *, base: float = 10000.0, scaling: 
     * "base": the base grows to base * factor ** (rot_dim / (rot_dim - 2)), so that the slowest pair is divided by the
       factor and the fastest stays;
     * "parts": with ``original`` the context that the model was trained on, pairs that turn more than ``fast`` times in it
-      stay, those that turn less than ``slow`` times are divided by the factor, a linear blend between; cos and sin are
-      multiplied by 0.1 ln(factor) + 1."""
+      stay, those that turn less than ``slow`` times are divided by the factor, between them an angle is a blend of both:
+      linear in the pair's turns, or, with ``blend`` "pairs", in the pair's index, between the indexes that turn ``fast`` and
+      ``slow`` times, rounded outward to whole ones.  Checkpoints differ in this: it has to be theirs.
+
+    cos and sin are multiplied by ``size``; None: by 0.1 ln(factor) + 1 with "parts", else by 1."""
     if rot_dim < 2 or rot_dim % 2:
         raise ValueError(f"rot_dim must be even, got {rot_dim}")
     if scaling not in (None, "linear", "base", "parts"):
@@ -92,17 +96,28 @@ def rope_table(positions: int, rot_dim: int, *, base: float = 10000.0, scaling: 
         raise ValueError(f"factor must be at least 1, got {factor}")
     if scaling == "parts" and (original < 1 or not fast > slow):
         raise ValueError("scaling 'parts' needs original > 0 and fast > slow")
+    if blend not in ("turns", "pairs"):
+        raise ValueError(f"blend must be 'turns' or 'pairs', got {blend!r}")
+    if size is not None and not 0 < size < math.inf:
+        raise ValueError(f"size must be above 0, got {size}")
     if scaling == "base" and rot_dim > 2:
         base = base * factor ** (rot_dim / (rot_dim - 2))
     inv = base ** (-torch.arange(0, rot_dim, 2, device=device, dtype=torch.float64) / rot_dim)
-    size = 1.0
     if scaling == "linear":
         inv = inv / factor
     elif scaling == "parts":
-        turns = original * inv / (2 * math.pi)
-        kept = ((turns - slow) / (fast - slow)).clamp(0, 1)
+        if blend == "turns":
+            turns = original * inv / (2 * math.pi)
+            kept = ((turns - slow) / (fast - slow)).clamp(0, 1)
+        else:
+            # original * base ** (-2i / rot_dim) = 2 pi n: pair i turns n times
+            first, last = (rot_dim * math.log(original / (2 * math.pi * n)) / (2 * math.log(base)) for n in (fast, slow))
+            first, last = max(math.floor(first), 0), min(math.ceil(last), rot_dim - 1)
+            pair = torch.arange(rot_dim // 2, device=device, dtype=torch.float64)
+            kept = 1 - ((pair - first) / max(last - first, 1e-3)).clamp(0, 1) if last >= 0 else 0 * pair
         inv = inv * kept + inv / factor * (1 - kept)
-        size = 0.1 * math.log(factor) + 1
+    if size is None:
+        size = 0.1 * math.log(factor) + 1 if scaling == "parts" else 1.0
     angle = torch.outer(torch.arange(positions, device=device, dtype=torch.float64), inv)
     return (size * torch.stack([angle.cos(), angle.sin()], dim=-1)).float()
 

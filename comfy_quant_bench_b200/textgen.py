@@ -43,9 +43,13 @@ class TextConfig:
     window: int = 0              # > 0: every second block sees this many tokens and the first `sinks`
     sinks: int = 0
     rope_base: float = 10000.0
-    rope_scaling: str | None = None      # kvcache.rope_table's, with its factor and original context
+    rope_scaling: str | None = None      # kvcache.rope_table's, with its factor, original context and so on
     rope_factor: float = 1.0
     rope_original: int = 0
+    rope_fast: float = 32.0
+    rope_slow: float = 1.0
+    rope_blend: str = "turns"
+    rope_size: float | None = None
     max_tokens: int = 2048
     rows: int = 16
     pages: int = 1024
@@ -94,7 +98,8 @@ class TextModel:
                                           cfg.page_size, cfg.cache_dtype, device, scale, scale)
         room = self.cache.block_table.shape[1] * cfg.page_size               # max_tokens up to whole pages: any position
         self.rope = kvcache.rope_table(room, cfg.head_dim, base=cfg.rope_base, scaling=cfg.rope_scaling, factor=cfg.rope_factor,
-                                       original=cfg.rope_original, device=device)      # [tokens, D/2, 2]
+                                       original=cfg.rope_original, fast=cfg.rope_fast, slow=cfg.rope_slow,
+                                       blend=cfg.rope_blend, size=cfg.rope_size, device=device)      # [tokens, D/2, 2]
 
     def _forward(self, tokens, rows, positions, attention) -> torch.Tensor:
         """Logits [tokens, vocab] (bf16); ``attention(layer, block, q)`` after the tokens' keys and values are cached."""

@@ -234,3 +234,39 @@ def test_sampling_arguments_without_numbers_to_sample_by_are_refused():
     for kw in (dict(temperature=0.7), dict(top_k=5, top_p=0.9), dict(temprature=0.7)):
         with pytest.raises(ValueError, match=f"{next(iter(kw))}.* without uniform numbers"):
             model.generate(torch.zeros(3, dtype=torch.long), 2, 4, **kw)
+
+
+@pytest.mark.parametrize("rot,base,factor,original,fast,slow", [(128, 500000.0, 8.0, 8192, 4.0, 1.0), (64, 10000.0, 16.0, 4096, 32.0, 1.0),
+                                                                (128, 10000.0, 4.0, 32768, 32.0, 1.0), (16, 100.0, 2.0, 40, 1.01, 1.0), (32, 10000.0, 2.0, 5, 4.0, 2.0)])
+@pytest.mark.parametrize("blend", ["turns", "pairs"])
+@pytest.mark.parametrize("size", [None, 1.0, 1.25])
+def test_tables_stretched_by_parts(rot, base, factor, original, fast, slow, blend, size):
+    """Every angle against the formula: with a size of 1 and fast 4, slow 1, too, and with the blend over the pairs' indexes."""
+    from comfy_quant_bench_b200 import kvcache
+    table = kvcache.rope_table(3000, rot, base=base, scaling="parts", factor=factor, original=original, fast=fast, slow=slow,
+                               blend=blend, size=size, device="cpu")
+    at = [rot * math.log(original / (2 * math.pi * n)) / (2 * math.log(base)) for n in (fast, slow)]
+    first, last = max(math.floor(at[0]), 0), min(math.ceil(at[1]), rot - 1)
+    times = (0.1 * math.log(factor) + 1) if size is None else size
+    for i in range(rot // 2):
+        angle = base ** (-2 * i / rot)
+        if blend == "turns":
+            kept = min(1.0, max(0.0, (original * angle / (2 * math.pi) - slow) / (fast - slow)))
+        else:
+            kept = 0.0 if last < 0 or i >= last > first else 1.0 if i <= first else 1 - (i - first) / (last - first)
+        angle = angle * kept + angle / factor * (1 - kept)
+        for p in (0, 1, 777, 2999):
+            assert abs(float(table[p, i, 0]) - times * math.cos(p * angle)) <= times * 2.0 ** -24 + 1e-9
+            assert abs(float(table[p, i, 1]) - times * math.sin(p * angle)) <= times * 2.0 ** -24 + 1e-9
+
+
+def test_the_size_of_turned_columns_and_blends_are_checked():
+    from comfy_quant_bench_b200 import kvcache
+    plain = kvcache.rope_table(50, 32, device="cpu")
+    for scaling in (None, "linear", "base"):
+        kw = dict(scaling=scaling, factor=2.0 if scaling else 1.0, device="cpu")
+        assert float((kvcache.rope_table(50, 32, size=1.5, **kw) - 1.5 * kvcache.rope_table(50, 32, **kw)).abs().max()) <= 1.5 * 2.0 ** -23
+    assert torch.equal(kvcache.rope_table(50, 32, size=1.0, device="cpu"), plain)
+    for bad in (dict(size=0.0), dict(size=-1.0), dict(size=float("nan")), dict(size=float("inf")), dict(blend="pair")):
+        with pytest.raises(ValueError):
+            kvcache.rope_table(4, 32, device="cpu", **bad)
