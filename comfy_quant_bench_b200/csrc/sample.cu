@@ -47,7 +47,6 @@ struct Shared {
   uint32_t hist[kBins];                        // this CTA's
   uint32_t total[kBins];                       // the row's
   uint32_t warp_counts[kWarps];
-  float extremes[2][kMaxCluster];
   int list_n;                                  // of rank 0: candidates that the ranks have reserved places for
   int list_at, pushed;                         // this CTA's first place, and places used
   int found[4];
@@ -97,7 +96,7 @@ struct Sampler {
   int rank, ranks, tid, lane, warp;
   int first, span;                             // this warp's elements: [first, first + span)
   int index0;                                  // row index of element 0; may be negative (before the row's first)
-  int vocab, count;                            // count: elements held
+  int count;                                   // elements held
   float top, range, inv_width;
   double by;                                   // log2(e) / T
   int parity;
@@ -402,7 +401,6 @@ __global__ void __launch_bounds__(samp::kThreads, 2) sample_kernel(const SampleA
   }
   S s{sh, data, rank, ranks, tid, tid & 31, tid >> 5};
   s.count = (w1 - w0) * kPer;
-  s.vocab = a.vocab;
   s.index0 = static_cast<int>((static_cast<int64_t>(word0 + w0 << 4) - static_cast<int64_t>(begin)) / kSize);
   s.parity = 0;
   const int per_warp = ((s.count + samp::kWarps - 1) / samp::kWarps + 31) & ~31;
