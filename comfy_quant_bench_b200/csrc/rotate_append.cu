@@ -178,8 +178,8 @@ __global__ void __launch_bounds__(AHEAD == 1 ? 1024 : rota::kThreads) rotate_app
 namespace {
 template <bool F16, bool FP8, bool NORM>
 cudaError_t run_rotate(const RotateArgs& a, int items, cudaStream_t st) {
-  // few tokens: all heads of a token at once; many: two heads a thread on their way together
-  if (a.T <= 2 * 148) return launch_early(rotate_append_kernel<F16, FP8, NORM, 1>, dim3(a.T), items < 1024 ? items : 1024, 0, st, a);
+  // two tokens an SM or fewer: all heads of a token at once; more: two heads a thread on their way together
+  if (a.T <= 2 * num_sms()) return launch_early(rotate_append_kernel<F16, FP8, NORM, 1>, dim3(a.T), items < 1024 ? items : 1024, 0, st, a);
   const int threads = (items + 1) / 2 + 31 & ~31;
   return launch_early(rotate_append_kernel<F16, FP8, NORM, 2>, dim3(a.T), threads < rota::kThreads ? threads : rota::kThreads, 0, st, a);
 }
