@@ -1149,3 +1149,29 @@ def test_generate_with_more_tokens_than_the_sampler_takes(ops):
         assert float(logits[at - 1] if at else 0.0) <= float(u[0, r]) + off and float(logits[at]) >= float(u[0, r]) - off
     with pytest.raises(ValueError, match="327680"):
         m.generate(torch.arange(20, device="cuda"), 2, 3, u, top_k=5)
+
+
+@pytest.mark.parametrize("off", [0, 1, 3])
+def test_sample_the_largest_vocabulary(ops, off):
+    """327680 tokens in f32: a CTA's share and the helpers come to 202 KB, and sums of equal logits to 2^62.3."""
+    n = 327680
+    x, u = _logits(3, n, torch.float32)
+    x[1] = -2.0
+    x[2] = torch.where(torch.arange(n, device="cuda") % 3 == 0, 1.0, -8.0)
+    u = torch.tensor([float(u[0]), 0.75, 0.3125], device="cuda")
+    wide = torch.full((3, n + 5), 60000.0, device="cuda")               # neighbours are not read
+    wide[:, off:off + n] = x
+    for k, p, m in ((0, 1.0, 0.0), (0, 0.9, 0.0), (50, 0.8, 0.05), (n // 2, 0.5, 0.0), (n - 1, 1.0, 0.0), (0, 0.25, 0.5)):
+        _sample_holds(ops, wide[:, off:off + n], u, 0.9, k, p, m)
+
+
+@pytest.mark.parametrize("t", [3, 400])
+@pytest.mark.parametrize("cache", ["own", "fp8"])
+@pytest.mark.parametrize("which", [0, 1])
+def test_rotated_append_norm_of_queries_or_keys_alone(kv, which, cache, t):
+    dtype = torch.bfloat16
+    rope = kv.rope_table(64, 64)
+    problem = list(_rotate_problem(t, 6, 2, 128, 64, dtype, FP8 if cache == "fp8" else dtype))
+    problem[6] = [w if i == which else None for i, w in enumerate(problem[6])]
+    for interleaved in (False, True):
+        _rotate_holds(kv, problem, 6, 2, 64, interleaved, rope)
