@@ -1,5 +1,6 @@
 // extern "C" entry points of the decode-side operators (declared in include/cq_b200.h): the W4A16 linear, the paged
-// key-value cache, the residual norm, rotated appends, attention behind a shared prefix and sampling.  Argument checks on the host, then kernel launches on the caller's stream.
+// key-value cache, the residual norm, rotated appends, attention behind a shared prefix and sampling.  Argument checks on
+// the host, then kernel launches on the caller's stream.
 #include <cstdint>
 #include <initializer_list>
 

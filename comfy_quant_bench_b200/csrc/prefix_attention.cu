@@ -13,6 +13,8 @@
 // Work: teams of CTAs, a CTA for each pair of row tiles, take equal runs of key tiles, through as many key-value heads as
 // that covers; the team's CTAs read the same keys at the same time, from L2.  Every run leaves its sums (fp32) in the
 // workspace, the row's own tokens go through the kernel of paged_attention.cu, and a last kernel joins them in a fixed order.
+// The second kernel is launched early, but a CTA of the first leaves no room for one of it on an SM (225 KB of shared memory): it
+// begins on the SMs that are done.
 //
 // Weights enter P V in 16 bits: in two parts of the type, as in paged_attention.cu, or in one, which errs about as much as
 // rounding the output does.  256 rows of 64 heads behind 30011 tokens: 358 us a call with one part and a relative L2 error of
@@ -20,13 +22,13 @@
 // chooses; without a choice two where the batch has no more rows than one CTA takes (64 rows behind 16003 tokens: 52 us with
 // the join, 46 with one part), else one.
 //
-// Measured on a B200 (device time of the prefix's kernel): 256 rows of 64 heads on 8 of 128 behind 30011 tokens: 284 us, 890
-// TFLOP/s.  Bound by the chain from scores to weights to product to scores: with 128 x 128 tiles a slot's maximum, exponentials
+// Measured on a B200 (device time of the prefix's kernel): 256 rows of 64 heads on 8 of 128 behind 30011 tokens: 284 to 290
+// us, 870 to 890 TFLOP/s.  Bound by the chain from scores to weights to product to scores: with 128 x 128 tiles a slot's maximum, exponentials
 // and conversions take about 2400 cycles, the two products 1300, and two slots hide each other's only in part (a pair of
 // tiles takes 4200; the exponential unit and the tensor pipe are both busy for 2000 to 2600 of them).  Measured and left: a
 // quarter of the exponentials as polynomials (no change), two threads a row (no change), tiles of 64 keys with the scores double
-// buffered (342 us against 274 in the same run: products of 64 columns wait for shared memory).  64 rows behind 16003 tokens: 47
-// us, half of it the start and end of a run; 40 rows of 16 heads on 4 of 256 behind 20000 tokens in 8 bits: 72 us, bound by the
+// buffered (342 us against 274 in the same run: products of 64 columns wait for shared memory).  64 rows behind 16003 tokens: 45
+// us, half of it the start and end of a run; 40 rows of 16 heads on 4 of 256 behind 20000 tokens in 8 bits: 67 us, bound by the
 // gathers, which hold one operand in flight at a time.
 #include <type_traits>
 
@@ -169,7 +171,7 @@ __global__ void __launch_bounds__(pfx::Cfg<D>::kThreads, 1) prefix_attention_ker
   int* leader_at = reinterpret_cast<int*>(holder + 2);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const PagedAttnArgs& g = a.own;
-  grid_dep_launch();                                          // the rows' own tokens may be started beside this
+  grid_dep_launch();                                          // the rows' own tokens are started where this is done
 
   if (tid == 0) {
     for (int s = 0; s < kStages; ++s) {

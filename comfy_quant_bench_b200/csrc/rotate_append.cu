@@ -10,8 +10,8 @@
 // first heads are on their way; blocks that stay for several tokens keep fewer loads in flight (139 us).
 //
 // Bound by reading and writing each head once.  Measured on a B200 (device time): 16001 tokens, 32 query and 8 key-value heads
-// of 128, f16, half of each turned: 84 us, 4.7 TB/s; 64 tokens with norms into an 8-bit cache: 6.2 us, one token 4.2 us,
-// launch and the chain of position, page and angle.
+// of 128, f16, half of each turned: 82 to 85 us, 4.7 TB/s; all of each, with norms, bf16: 101 us, 4.0 TB/s, and into an 8-bit cache
+// 113 us, 3.3 TB/s; 64 tokens with norms into an 8-bit cache: 5.8 us, one token 3.7 us, launch and the chain of position, page and angle.
 #include "decode_common.cuh"
 
 namespace cq {

@@ -15,8 +15,9 @@
 // the border's few tokens are ranked one against another; a bin with more of them (equal logits) is halved instead.  Where no
 // more than 512 tokens can stay, one CTA takes them over, sorts them in registers and finishes, and the others leave.
 //
-// Measured on a B200 (device time): 128 rows of 128257 f32 logits, top-k 200, top-p and min-p: 85 us, 0.8 TB/s; one row of
-// 32000 with top-p: about 12 us.  Bound by the chain of a row's steps (load, maximum, counts, candidates, sort: four waits
+// Measured on a B200, calls in a row: 128 rows of 128257 f32 logits, top-k 200, top-p and min-p: 86 us, 0.8 TB/s; one row of
+// 32000 bf16 logits with top-p 0.9: 15 to 20 us by the box (27 alone and cold); 128 rows of 32000 bf16: 49 us with all filters,
+// 93 with top-p alone, 35 with none, 18 for the likeliest token.  Bound by the chain of a row's steps (load, maximum, counts, candidates, sort: four waits
 // for the cluster of about 0.5 us each among them), of which an SM holds two CTAs at a time.
 #include "decode_common.cuh"
 
@@ -726,8 +727,9 @@ namespace {
 template <int TYPE>
 cudaError_t run_sample(const SampleArgs& a, cudaStream_t st) {
   constexpr int kSize = TYPE == CQ_DT_F32 ? 4 : 2;
-  // a CTA for each 2048 tokens, up to a cluster of eight: one row of 32000 takes 15 us on eight, 20 on four, 38 on two and 66
-  // on one; on sixteen it takes 20 again, and 128 rows of 128257 136 us instead of 85
+  // a CTA for each 2048 tokens, up to a cluster of eight: one row of 32000 with top-p takes 20 us on eight, 28 on four, 39 on
+  // two and 68 on one, 128 rows of 128257 204 us on eight and 253 on four (sixteen were slower at both).  Not the best for many
+  // rows of fewer tokens: 32 rows of 32000 take 27 us on eight and 36 on four, but 128 rows 95 on eight, 70 on four and 58 on two
   int ranks = 1;
   while (ranks < samp::kMaxCluster && ranks * 2048 < a.vocab) ranks *= 2;
   const int words = (a.vocab * kSize + 15) / 16 + 1;

@@ -47,8 +47,8 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
                      scale: float | None = None, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
                      out: torch.Tensor | None = None, return_lse: bool = False, weight_parts: int | None = None):
     """``paged_attention`` of a batch whose rows begin with the same ``prefix`` tokens (an int, or one int32 on the device,
-    which a captured step reads anew): samples of one prompt, requests behind one instruction.  Their keys and values are
-    read once for all rows, not once for each.
+    which a captured step reads anew), one new token a row: samples of one prompt, or requests behind one instruction, once
+    they are in the cache.  The shared keys and values are read once for all rows, not once for each.
 
     Every row with ``prefix`` tokens or more must hold the same first ``prefix`` tokens, in pages of its own table, whichever
     they are (those of the first such row are read); a shorter row or an empty one is attended by itself.  Where the shared

@@ -783,9 +783,10 @@ def add_rmsnorm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | 
     f16), and y = h * weight / sqrt(mean(h^2) + eps) over the last dimension (1 to 32768), in fp32, rounded once.
 
     Returns (y, h).  With ``quant`` "int8" or "fp8" (e4m3), (codes, scale, h): y ~ codes * scale with f32 scales [rows]
-    (rows: the leading dimensions flattened), or [C / group_size, rows] for groups of 32, 64 or 128 columns; they feed
-    the int8 GEMMs (``gemm_rowcol``) without another pass.  A code is round(127 p / P) (448 for fp8), p = h * weight, P
-    its largest magnitude in the row or group; int8 codes are the nearest-even ones of the exact quotient.
+    (rows: the leading dimensions flattened), or [C / group_size, rows] for groups of 32, 64 or 128 columns.  int8 codes
+    with a scale a row feed ``gemm_rowcol`` without another pass; no linear here takes the other forms.  A code is round(127
+    p / P) (448 for fp8), p = h * weight, P its largest magnitude in the row or group: the nearest one of the exact
+    quotient, halves to the even one.
 
     ``out_residual`` (contiguous; may be x or residual itself) takes h; without a residual h is x.  A row with a NaN
     gives NaN, as scale too; a row of zeros zero codes and scales.  The weight is taken in x's type."""
@@ -800,7 +801,8 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.
     With weights exp((l - max) / temperature): the first ``top_k`` tokens, by logit and then by index, stay (0: all); of
     those the shortest head whose sum reaches ``top_p`` times theirs; of those the ones with a weight of at least ``min_p``
     (of the largest).  The token is the first, by index, whose running sum exceeds uniform times the sum of what stays.
-    Each of the four is a number, or a tensor [rows] (f32; top_k int32).  Temperature 0: the likeliest, lowest index first.
+    Each of the four is a number, or a tensor [rows] (f32; top_k int32, a whole number).  Temperature 0: the likeliest,
+    lowest index first; above 0, however little, tokens of one logit share.
 
     Weights are held to 2^-45 of the largest and added without rounding, so equal calls give equal tokens.  NaN logits
     count as -inf; tokens at +inf share the row among them.  A row without a logit above -inf gives -1.  With

@@ -633,7 +633,9 @@ CQ_API int cq_pages_compact(const int32_t* block_table, int64_t table_rows, int6
  *   out_kind CQ_NORM_SAME: out [rows, width] of `dtype`, y rounded once.  CQ_NORM_INT8 / CQ_NORM_FP8: out int8 / e4m3
  *            codes round(top p / P) with p = h * weight, P its largest magnitude in the row (group == 0) or in each group of
  *            32, 64 or 128 columns, top 127 / 448; scale f32 [rows] or [width / group, rows] = P / (top sqrt(mean(h^2) +
- *            eps)).  int8 codes round to nearest even of the exact quotient.  Zero rows have zero codes and scales.
+ *            eps)).  Codes are the nearest ones of the exact quotient, halves to the even one.  Zero rows have zero codes
+ *            and scales.  int8 codes with a scale a row are what cq_gemm_rowcol takes; the other forms have no
+ *            consumer in this library.
  * width 1 to 32768.  Widths that are a multiple of 8 need 16-byte aligned bases and row strides that are multiples of 8.
  * A row with a NaN gives NaN (scales NaN); one with an infinity what the formula gives (its scale NaN).
  */
