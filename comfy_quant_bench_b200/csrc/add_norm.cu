@@ -92,13 +92,19 @@ __device__ __forceinline__ void e4m3_codes(const float (&p)[N], const Quotients&
   for (int j = 0; j < N / 2; ++j) code[j] = e4m3_pair(t[j]);
 }
 
+// the larger one, or NaN where either is
+__device__ __forceinline__ float larger(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
 // The sum and the maximum over a row's threads: a warp, or a block of whole warps.
 template <bool WARP>
 __device__ __forceinline__ void row_reduce(float& sum, float& most, float* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    most = larger(most, __shfl_xor_sync(0xffffffffu, most, o));
   }
   if constexpr (!WARP) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
@@ -112,7 +118,7 @@ __device__ __forceinline__ void row_reduce(float& sum, float& most, float* red) 
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      most = larger(most, __shfl_xor_sync(0xffffffffu, most, o));
     }
   }
 }
@@ -168,7 +174,7 @@ __global__ void __launch_bounds__(WARP ? 256 : CHUNKS < 4 ? 512 : 1024) add_norm
       const float2 f = widen16<F16>(u[j]), g = widen16<F16>(v[j]);
       sum = fmaf(f.x, f.x, sum);
       sum = fmaf(f.y, f.y, sum);
-      if (kMost) most = fmaxf(most, fmaxf(fabsf(f.x * g.x), fabsf(f.y * g.y)));
+      if (kMost) most = larger(most, larger(fabsf(f.x * g.x), fabsf(f.y * g.y)));
     }
     if (c < eights && a.h_out != nullptr) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.h_out) + row * a.ldh + 8 * c) = h[i];
   }
@@ -200,8 +206,8 @@ __global__ void __launch_bounds__(WARP ? 256 : CHUNKS < 4 ? 512 : 1024) add_norm
       if constexpr (GROUPS) {
         top = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(p[j]));
-        for (int o = 1; o < a.group >> 3; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        for (int j = 0; j < 8; ++j) top = larger(top, fabsf(p[j]));
+        for (int o = 1; o < a.group >> 3; o <<= 1) top = larger(top, __shfl_xor_sync(0xffffffffu, top, o));
         if (c < eights && (8 * c & (a.group - 1)) == 0) a.scale[8 * c / a.group * a.rows + row] = top * inv / kTop;
       }
       if (c >= eights) continue;
@@ -246,7 +252,7 @@ __global__ void __launch_bounds__(256) add_norm_odd_kernel(const AddNormArgs a) 
     if (a.h_out != nullptr) static_cast<uint16_t*>(a.h_out)[row * a.ldh + c] = static_cast<uint16_t>(h);
     const float f = widen16<F16>(h).x;
     sum = fmaf(f, f, sum);
-    most = fmaxf(most, fabsf(f * widen16<F16>(w[c]).x));
+    most = larger(most, fabsf(f * widen16<F16>(w[c]).x));
   }
   row_reduce<WARP>(sum, most, red);
   const float inv = rsqrtf(sum / static_cast<float>(a.width) + a.eps);

@@ -1175,3 +1175,25 @@ def test_rotated_append_norm_of_queries_or_keys_alone(kv, which, cache, t):
     problem[6] = [w if i == which else None for i, w in enumerate(problem[6])]
     for interleaved in (False, True):
         _rotate_holds(kv, problem, 6, 2, 64, interleaved, rope)
+
+
+@pytest.mark.parametrize("quant", ["int8", "fp8"])
+@pytest.mark.parametrize("c,group", [(256, 0), (2048, 0), (2048, 64), (255, 0), (2049, 0)])
+def test_norm_products_that_are_no_numbers_show_in_the_scale(ops, c, group, quant):
+    """P of products with a NaN is NaN, though the row has none: a NaN weight, or an infinity times a weight of 0."""
+    x = torch.randn(5, c, generator=_gen(c), device="cuda").bfloat16()
+    w = torch.ones(c, device="cuda").bfloat16()
+    plain = ops.add_rmsnorm(x, w, quant=quant, group_size=group)
+    hurt = w.clone()
+    hurt[c - 7] = float("nan")
+    _, scale, _ = ops.add_rmsnorm(x, hurt, quant=quant, group_size=group)
+    if group:
+        assert bool(scale[-1].isnan().all()) and torch.equal(scale[:-1], plain[1][:-1])
+    else:
+        assert bool(scale.isnan().all())
+    x[3, 9] = float("inf")
+    hurt = w.clone()
+    hurt[9] = 0.0
+    _, scale, _ = ops.add_rmsnorm(x, hurt, quant=quant, group_size=group)
+    assert bool(scale[..., 3][:1].isnan().all() if group else scale[3].isnan())
+    assert bool(torch.isfinite(scale[..., [0, 1, 2, 4]]).all())
