@@ -294,8 +294,8 @@ cudaError_t run_add_norm(const AddNormArgs& a, cudaStream_t st) {
 template <bool F16>
 cudaError_t pick_add_norm(const AddNormArgs& a, cudaStream_t st) {
   if (a.width % 8 != 0) {
-    // a warp a row where the rows give every SM 32 short ones or more: 518289 rows of 123 take 235 us, and 763 with a block each; 65536 of 999
-    // 158 and 259; but 777 of 1001 13 us, and 6.5 with a block each
+    // a warp a row where the rows give every SM 32 short ones or more: 518289 rows of 123 take 235 us, and 763 with a block
+    // each; 65536 of 999 158 and 259; but 777 of 1001 13 us, and 6.5 with a block each
     const bool warp = a.width <= 1024 && a.rows >= 32 * num_sms();
     const dim3 grid(static_cast<unsigned>(warp ? (a.rows + 7) / 8 : a.rows));
     const int bytes = 2 * a.width * (warp ? 8 : 1);

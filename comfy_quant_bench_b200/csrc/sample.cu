@@ -16,9 +16,10 @@
 // more than 512 tokens can stay, one CTA takes them over, sorts them in registers and finishes, and the others leave.
 //
 // Measured on a B200, calls in a row: 128 rows of 128257 f32 logits, top-k 200, top-p and min-p: 86 us, 0.8 TB/s; one row of
-// 32000 bf16 logits with top-p 0.9: 15 to 20 us by the box (27 alone and cold); 128 rows of 32000 bf16: 49 us with all filters,
-// 93 with top-p alone, 35 with none, 18 for the likeliest token.  Bound by the chain of a row's steps (load, maximum, counts, candidates, sort: four waits
-// for the cluster of about 0.5 us each among them), of which an SM holds two CTAs at a time.
+// 32000 bf16 logits with top-p 0.9: 15 to 20 us by the box (27 alone and cold); 128 rows of 32000 bf16: 49 us with all
+// filters, 93 with top-p alone, 35 with none, 18 for the likeliest token.  Bound by the chain of a row's steps (load, maximum,
+// counts, candidates, sort: four waits for the cluster of about 0.5 us each among them), of which an SM holds two CTAs at a
+// time.
 #include "decode_common.cuh"
 
 namespace cq {
@@ -350,7 +351,7 @@ __global__ void __launch_bounds__(samp::kThreads, 2) sample_kernel(const SampleA
   if (tid == 0) sh.list_n = 0;
   for (int i = tid; i < samp::kBins; i += samp::kThreads) sh.hist[i] = 0;
   __syncwarp();
-  cluster_arrive();                                                    // this CTA has started; waited for before the first store to another
+  cluster_arrive();                                                    // this CTA runs: waited for below
   grid_dep_wait();
 
   const float temperature = a.temperatures != nullptr ? a.temperatures[row] : a.temperature;
@@ -424,7 +425,7 @@ __global__ void __launch_bounds__(samp::kThreads, 2) sample_kernel(const SampleA
     least = fminf(least, box[samp::kWarps + w]);
   }
   __syncthreads();
-  cluster_wait();                                                      // all CTAs of the cluster run: their memory may be written
+  cluster_wait();                                                      // all of them run: their memory may be written
   {
     const u64(*all)[2] = s.exchange(__float_as_uint(most), __float_as_uint(least));
     for (int r = 0; r < ranks; ++r) {
